@@ -16,6 +16,7 @@ from .train import RNG, Config, TrainableTransformer, initWeights, train
 from .checkpoint import load_checkpoint, save_checkpoint
 from .infer import (KVCache, PagedKVCache, QuantLinear, Transformer, attentionDecode, attentionNaive,
                     flashAttention)
+from .kv4 import (QuantKVCache, beamStep, cacheReorder, kv4Attention, kv4Evict, kv4Put, kv4Values)
 
 
 def set_precision(mode: str) -> None:
@@ -32,5 +33,6 @@ __all__ = [
     "crossEntropyMean", "embedLookup", "matmulT", "ropeRows", "rmsNorm", "sliceCols",
     "swigluRows", "weightedSum", "RNG", "Config", "TrainableTransformer", "initWeights", "train",
     "set_precision", "QuantLinear", "KVCache", "PagedKVCache", "Transformer", "attentionDecode",
-    "attentionNaive", "flashAttention",
+    "attentionNaive", "flashAttention", "QuantKVCache", "kv4Put", "kv4Values", "kv4Attention", "kv4Evict",
+    "beamStep", "cacheReorder",
 ]

@@ -62,6 +62,19 @@ class AdamSched(C.Structure):
                 ("total_steps", C.c_double)]
 
 
+class Kv4(C.Structure):
+    """fcu_kv4."""
+    _fields_ = [("k", C.c_void_p), ("v", C.c_void_p), ("kg", C.c_void_p), ("vg", C.c_void_p),
+                ("weight", C.c_void_p), ("pos", C.c_void_p), ("table", C.c_void_p),
+                ("layers", C.c_int64), ("blocks", C.c_int64), ("n_kv", C.c_int), ("dH", C.c_int),
+                ("block_size", C.c_int), ("max_blocks", C.c_int)]
+
+
+class CacheArray(C.Structure):
+    """fcu_cache_array."""
+    _fields_ = [("base", C.c_void_p), ("heads", C.c_int64), ("unit", C.c_int64)]
+
+
 _P = C.c_void_p
 _I64 = C.c_int64
 _INT = C.c_int
@@ -133,6 +146,16 @@ _SIGS = {
     "fcu_dequantize_rows": (_INT, [_P, _INT, _P, _I64, _I64, _P, _I64, _P]),
     "fcu_decode_rope_kv": (_INT, [_P, _P, _I64, _INT, _INT, _INT, _INT, _D, _P, _P, _P, _I64, _P, _INT, _INT]),
     "fcu_attn_decode": (_INT, [_P, _P, _I64, _P, _P, _I64, _P, _INT, _INT, _P, _INT, _INT, _INT, _INT, _D, _P]),
+    "fcu_kv4_row_bytes": (_INT, [_INT]),
+    "fcu_kv4_put": (_INT, [_P, _P, _I64, _INT, _INT, _INT, _D, _P, _P, C.POINTER(Kv4)]),
+    "fcu_kv4_values": (_INT, [_P, C.POINTER(Kv4), _P, _INT, _INT, _P, _P]),
+    "fcu_kv4_attn_work": (_I64, [_P, C.POINTER(Kv4), _INT, _INT]),
+    "fcu_kv4_attn": (_INT, [_P, _P, _I64, C.POINTER(Kv4), _P, _INT, _INT, _D, _P, _P, _I64]),
+    "fcu_kv4_evict_work": (_I64, [_P, C.POINTER(Kv4), _INT]),
+    "fcu_kv4_evict": (_INT, [_P, C.POINTER(Kv4), _P, _INT, _INT, _INT, _P, _P, _I64]),
+    "fcu_beam_work": (_I64, [_P, _INT, _INT, _I64]),
+    "fcu_beam_step": (_INT, [_P, _P, _I64, _P, _P, _INT, _INT, _I64, _INT, _P, _P, _P, _P, _P, _I64]),
+    "fcu_cache_reorder": (_INT, [_P, C.POINTER(CacheArray), _INT, _I64, _I64, _P, _INT, _INT, _P, _P, _INT, _INT]),
     "fcu_comm_unique_id": (_INT, [_P]),
     "fcu_comm_init": (_INT, [_INT, _P, _INT, _INT, _D, C.POINTER(_P)]),
     "fcu_comm_destroy": (_INT, [_P]),

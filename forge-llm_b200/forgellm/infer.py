@@ -130,6 +130,16 @@ class KVCache:
     def bytes(self) -> int:
         return 2 * self.k.numel() * 4
 
+    def reorder(self, parents) -> None:
+        """After a beam-search selection: parents [B, W] (B * W == batch), beam w
+        of search b continues beam parents[b, w] (kv4.cacheReorder)."""
+        from .kv4 import _reorder
+        t = getattr(self, "_table_host", None)
+        if t is not None and np.unique(t).size < t.size:
+            raise ValueError("a cache whose sequences share blocks cannot be reordered")
+        shape = (self.nLayers, -1, 1, self.block_size, self.kvDim)
+        _reorder(self, [self.k.view(shape), self.v.view(shape)], parents, np.full(self.batch, self.len, np.int32))
+
 
 class PagedKVCache(KVCache):
     """Block-allocated KV cache (attention.js:157-187): blocks of blockSize
@@ -255,7 +265,8 @@ class Transformer:
                                      logits=z(B, c.vocabSize),
                                      ids=torch.empty(B, dtype=torch.int32, device=dev),
                                      pos=torch.empty(B, dtype=torch.int32, device=dev),
-                                     lens=torch.empty(B, dtype=torch.int32, device=dev))
+                                     lens=torch.empty(B, dtype=torch.int32, device=dev),
+                                     slots=torch.empty(B, dtype=torch.int32, device=dev))
         return b
 
     def forward(self, token: int, pos: int, cache: KVCache, graph: bool = False) -> torch.Tensor:
@@ -274,12 +285,20 @@ class Transformer:
         if B > cache.batch:
             raise ValueError(f"{B} sequences for a cache of {cache.batch}")
         bf = self._buffers(B)
-        host = np.array([list(tokens), list(positions), [p + 1 for p in positions]], np.int32)
+        # the cache row of each token: its position, but for a cache that evicts
+        q4 = hasattr(cache, "slotOf")
+        slots = [cache.slotOf(p, b) for b, p in enumerate(positions)] if q4 else list(positions)
+        host = np.array([list(tokens), list(positions), [s + 1 for s in slots], slots], np.int32)
         dev_host = torch.from_numpy(host)
         bf["ids"].copy_(dev_host[0])
         bf["pos"].copy_(dev_host[1])
         bf["lens"].copy_(dev_host[2])
-        cache.len = max(cache.len, max(positions) + 1)
+        if q4:
+            bf["slots"].copy_(dev_host[3])
+            for b, s in enumerate(slots):
+                cache._used(b, s)
+        else:
+            cache.len = max(cache.len, max(positions) + 1)
         if not graph:
             return self._step(B, cache)
         from ._lib import lib
@@ -307,6 +326,42 @@ class Transformer:
         graphs[key] = (graph_, scr.value, cache.k)
         return out
 
+    def beamSearch(self, prompt, beams: int, maxNew: int, cache: KVCache, eosId: int | None = None,
+                   budget: int | None = None, recent: int = 0, graph: bool = False):
+        """Beam search from `prompt` (token ids) for up to maxNew tokens: a list
+        of (tokens, score), best first; tokens end with eosId (the config's
+        unless given) where the beam ended.  cache: an unused one of batch
+        `beams`, of any kind; with `budget` (a QuantKVCache made with track=True)
+        every sequence is evicted down to that many slots after each token."""
+        from .kv4 import beamStep
+        c = self.cfg
+        eos = c.eosId if eosId is None else int(eosId)
+        ids = [int(t) for t in prompt]
+        if not ids or maxNew < 1 or cache.batch != beams or cache.len:
+            raise ValueError(f"beamSearch: {len(ids)} prompt tokens, maxNew {maxNew}, {beams} beams on "
+                             f"{'a used' if cache.len else 'a'} cache of {cache.batch}")
+        for p, t in enumerate(ids):
+            logits = self.forward(t, p, cache, graph=graph)
+            if budget is not None:
+                cache.evict(budget, recent)
+        cache.reorder(np.zeros((1, beams), np.int64))    # every beam starts from the prompt's rows
+        logits = logits.expand(beams, -1).contiguous()
+        # until the beams differ only the first one counts
+        scores = torch.from_numpy(np.array([0.0] + [-math.inf] * (beams - 1), np.float32)).to(logits.device)
+        done = torch.zeros(beams, dtype=torch.bool, device=logits.device)
+        texts = [[] for _ in range(beams)]
+        for i in range(maxNew):
+            scores, tokens, parents, done = beamStep(logits, scores.view(-1), done.view(-1), beams, eos)
+            tok, par, end = tokens[0].tolist(), parents[0].tolist(), done[0].tolist()
+            texts = [texts[p] + ([] if texts[p][-1:] == [eos] else [t]) for p, t in zip(par, tok)]
+            if all(end) or i == maxNew - 1:
+                break
+            cache.reorder(np.array([par]))
+            logits = self.forwardBatch(tok, [len(ids) + i] * beams, cache, graph=graph)
+            if budget is not None:
+                cache.evict(budget, recent)
+        return list(zip(texts, scores[0].tolist()))
+
     def _step(self, B: int, cache: KVCache) -> torch.Tensor:
         """The launches of one decode step on the step's device buffers."""
         c = self.cfg
@@ -317,17 +372,32 @@ class Transformer:
         self.tokEmb.rows(bf["ids"], out=x)
         table = cache.table.data_ptr() if cache.table is not None else None
         rows = cache.rows_per_layer()
+        q4 = hasattr(cache, "slotOf")
+        if q4:
+            from . import kv4
+            qkv, qh = q[:, :c.qkvOut], q[:, :c.nHeads * dH].view(B, c.nHeads, dH)
+            lens, table4 = bf["lens"], cache.table[:B] if cache.table is not None else None
+            blocks = cache.k.shape[1] if table4 is not None else B * cache.max_blocks
         for l, L in enumerate(self.layers):
             call("fcu_rmsnorm_fwd", h, x.data_ptr(), L["ln1"].data_ptr(), B, D, float(c.normEps), xb.data_ptr(),
                  inv.data_ptr())
             L["wqkv"].forward(xb, out=q)
-            kc = cache.k.data_ptr() + 4 * l * rows * c.kvDim
-            vc = cache.v.data_ptr() + 4 * l * rows * c.kvDim
-            call("fcu_decode_rope_kv", h, q.data_ptr(), c.qkvOut, B, c.nHeads, c.nKvHeads, dH, float(c.ropeTheta),
-                 bf["pos"].data_ptr(), kc, vc, c.kvDim, table, cache.max_blocks, cache.block_size)
-            call("fcu_attn_decode", h, q.data_ptr(), c.qkvOut, kc, vc, c.kvDim, table, cache.max_blocks,
-                 cache.block_size, bf["lens"].data_ptr(), B, c.nHeads, c.nKvHeads, dH, 1 / math.sqrt(dH),
-                 att.data_ptr())
+            if q4:
+                arrays = [x[l, :blocks] for x in (cache.k, cache.kg, cache.v, cache.vg)]
+                weight, pos = ((cache.weight[l, :blocks], cache.pos[l, :blocks]) if cache.weight is not None
+                               else (None, None))
+                kv4.kv4Put(qkv, c.nHeads, bf["pos"], bf["slots"], *arrays, theta=float(c.ropeTheta), table=table4,
+                           weight=weight, pos=pos)
+                kv4.kv4Attention(qh, *arrays, lens, table=table4, weight=weight, out=att)
+            else:
+                kc = cache.k.data_ptr() + 4 * l * rows * c.kvDim
+                vc = cache.v.data_ptr() + 4 * l * rows * c.kvDim
+                call("fcu_decode_rope_kv", h, q.data_ptr(), c.qkvOut, B, c.nHeads, c.nKvHeads, dH,
+                     float(c.ropeTheta), bf["pos"].data_ptr(), kc, vc, c.kvDim, table, cache.max_blocks,
+                     cache.block_size)
+                call("fcu_attn_decode", h, q.data_ptr(), c.qkvOut, kc, vc, c.kvDim, table, cache.max_blocks,
+                     cache.block_size, bf["lens"].data_ptr(), B, c.nHeads, c.nKvHeads, dH, 1 / math.sqrt(dH),
+                     att.data_ptr())
             L["wo"].forward(att, out=xb2)
             call("fcu_add_fwd", h, x.data_ptr(), xb2.data_ptr(), B * D, x.data_ptr())
             call("fcu_rmsnorm_fwd", h, x.data_ptr(), L["ln2"].data_ptr(), B, D, float(c.normEps), xb.data_ptr(),

@@ -1,0 +1,378 @@
+"""Generation over a 4-bit KV cache: quantized writes and values, attention,
+eviction by accumulated attention weight, beam-search selection and the
+reordering of caches after it (libforgecu's fcu_kv4_*, fcu_beam_step and
+fcu_cache_reorder; the layouts and the arithmetic are in include/forgecu.h).
+
+The functions take the arrays of one cache layer: codes `k`, `v` uint8
+[blocks, nKV, blockSize, rowBytes], grids `kg`, `vg` bf16 [blocks, nKV,
+blockSize, 2] (step, base) and, where they are kept, `weight` fp32 and `pos`
+int32 [blocks, nKV, blockSize].  `table` (int32 [B, maxBlocks]) maps a
+sequence's blocks to the arrays'; without one, sequence b owns the b-th equal
+share of them.  `QuantKVCache` holds such arrays for every layer.  The forge-llm
+reference has no counterpart: its caches are fp32 and it samples one sequence.
+
+All tensors are on the current CUDA device and every call runs on its current
+stream.  A call that finds them anywhere else, or of another type, shape or
+stride than it takes, raises ValueError before anything is launched.
+"""
+from __future__ import annotations
+
+import ctypes as C
+import math
+
+import numpy as np
+import torch
+
+from ._lib import CacheArray, Kv4, call, lib
+from .autograd import ctx, device
+from .infer import KVCache, _dev_f32
+
+_U8, _BF, _F32, _I32 = torch.uint8, torch.bfloat16, torch.float32, torch.int32
+
+
+def _need(ok, what: str) -> None:
+    if not ok:
+        raise ValueError(what)
+
+
+def _check(name: str, t, dtype, shape=None) -> None:
+    """t is a contiguous tensor of `dtype` (and `shape`) on the current device."""
+    if not isinstance(t, torch.Tensor) or t.dtype != dtype:
+        raise ValueError(f"{name}: a {dtype} tensor is needed, got "
+                         f"{t.dtype if isinstance(t, torch.Tensor) else type(t).__name__}")
+    if not t.is_cuda or t.device.index != torch.cuda.current_device():
+        raise ValueError(f"{name} is on {t.device}, not on the current CUDA device")
+    if shape is not None and tuple(t.shape) != shape:
+        raise ValueError(f"{name}: shape {tuple(t.shape)}, {shape} is needed")
+    if not t.is_contiguous():
+        raise ValueError(f"{name} is not contiguous")
+
+
+def _cache(k, kg, v, vg, dHead, B, table, weight=None, pos=None, layers=False) -> Kv4:
+    """The C-ABI's view of one layer's arrays (five dimensions: of all layers)."""
+    _check("k", k, _U8)
+    _need(k.ndim == (5 if layers else 4), f"k: {k.ndim} dimensions")
+    rb = lib().fcu_kv4_row_bytes(int(dHead))
+    _need(rb > 0, f"head dim {dHead}: even, 2 to 256")
+    _need(k.shape[-1] == rb, f"k: rows of {k.shape[-1]} bytes, head dim {dHead} has {rb}")
+    lead = tuple(k.shape[:-1])
+    _check("v", v, _U8, tuple(k.shape))
+    _check("kg", kg, _BF, (*lead, 2))
+    _check("vg", vg, _BF, (*lead, 2))
+    if weight is not None:
+        _check("weight", weight, _F32, lead)
+    if pos is not None:
+        _check("pos", pos, _I32, lead)
+    L, (blocks, nKV, bs) = (lead[0] if layers else 1), lead[-3:]
+    if table is not None:
+        _need(table.ndim == 2 and table.shape[0] == B, f"table: shape {tuple(table.shape)} for {B} sequences")
+        _check("table", table, _I32)
+        mb = table.shape[1]
+    else:
+        _need(blocks % max(B, 1) == 0, f"{blocks} blocks do not divide among {B} sequences")
+        mb = blocks // max(B, 1)
+    return Kv4(k.data_ptr(), v.data_ptr(), kg.data_ptr(), vg.data_ptr(),
+               weight.data_ptr() if weight is not None else None, pos.data_ptr() if pos is not None else None,
+               table.data_ptr() if table is not None else None, L, blocks, nKV, int(dHead), bs, mb)
+
+
+def _work(nbytes: int) -> torch.Tensor | None:
+    """A call's workspace.  The allocator hands it out again only to work queued
+    behind the call on the same stream (in a capture: from the graph's pool)."""
+    return torch.empty(nbytes, dtype=_U8, device=device()) if nbytes > 0 else None
+
+
+def _rows(name: str, t, cols_min: int) -> int:
+    """Row stride of a two-dimensional fp32 tensor with unit column stride."""
+    if not isinstance(t, torch.Tensor) or t.dtype != _F32 or t.ndim != 2:
+        raise ValueError(f"{name}: a two-dimensional float32 tensor is needed")
+    if not t.is_cuda or t.device.index != torch.cuda.current_device():
+        raise ValueError(f"{name} is on {t.device}, not on the current CUDA device")
+    if t.shape[1] < cols_min or (t.shape[1] > 1 and t.stride(1) != 1):
+        raise ValueError(f"{name}: shape {tuple(t.shape)} with strides {t.stride()}")
+    return t.stride(0) if t.shape[0] > 1 else t.shape[1]
+
+
+def kv4Put(qkv, nHeads: int, positions, slots, k, kg, v, vg, T: int = 1, theta: float = 10000.0, table=None,
+           weight=None, pos=None) -> None:
+    """T new tokens of each of B sequences: qkv [B * T, (nHeads + 2 nKV) dHead]
+    fp32 (rows may be strided), token t of sequence b at position positions[b] + t
+    and slot slots[b] + t (int32 [B]).  The q heads are rotated in place, k and v
+    go to the cache in 4 bits; their columns of qkv stay as they are.  theta 0:
+    the rows carry their rotation already.  A token whose slot is outside the
+    cache, or whose position is negative, changes nothing."""
+    _check("positions", positions, _I32)
+    B = positions.numel()
+    _check("slots", slots, _I32)
+    _need(slots.numel() == B, f"{slots.numel()} slots for {B} sequences")
+    _need(T >= 1 and nHeads >= 0 and theta >= 0, f"T={T}, nHeads={nHeads}, theta={theta}")
+    _need(k.ndim == 4, f"k: {k.ndim} dimensions")
+    heads = nHeads + 2 * k.shape[1]
+    ld = _rows("qkv", qkv, 1)
+    _need(qkv.shape[0] == B * T and qkv.shape[1] % heads == 0,
+          f"qkv: shape {tuple(qkv.shape)} for {B} x {T} tokens of {heads} heads")
+    _need(qkv.shape[0] < 2 or ld >= qkv.shape[1], "qkv: its rows overlap")
+    c = _cache(k, kg, v, vg, qkv.shape[1] // heads, B, table, weight, pos)
+    call("fcu_kv4_put", ctx().handle, qkv.data_ptr(), ld, B, T, nHeads, float(theta), positions.data_ptr(),
+         slots.data_ptr(), c)
+
+
+def kv4Values(k, kg, v, vg, dHead: int, start, T: int, table=None):
+    """(K, V) fp32 [B, T, nKV, dHead]: the values of slots start[b] .. start[b] + T
+    (start int32 [B]).  A slot outside the cache gives NaN."""
+    _check("start", start, _I32)
+    B = start.numel()
+    _need(T >= 0, f"T={T}")
+    c = _cache(k, kg, v, vg, dHead, B, table)
+    out = torch.empty(2, B, T, c.n_kv, dHead, dtype=_F32, device=k.device)
+    K, V = out[0], out[1]
+    call("fcu_kv4_values", ctx().handle, c, start.data_ptr(), B, T, K.data_ptr(), V.data_ptr())
+    return K, V
+
+
+def kv4Attention(q, k, kg, v, vg, lens, scale: float | None = None, table=None, weight=None, out=None):
+    """[B, nHeads, dHead]: attention of q [B, nHeads, dHead] fp32 (the sequences
+    may be strided) over the first lens[b] slots of each sequence (int32 [B];
+    0 gives zeros), grouped heads as in attentionDecode.  scale: 1 / sqrt(dHead)
+    unless given.  With `weight`, every slot's attention weight, summed over its
+    kv head's q heads, is added to it."""
+    _need(isinstance(q, torch.Tensor) and q.dtype == _F32 and q.ndim == 3, "q: a float32 [B, nHeads, dHead] is needed")
+    B, nH, dH = q.shape
+    _need(q.is_cuda and q.device.index == torch.cuda.current_device(), f"q is on {q.device}, not on the current CUDA device")
+    _need((dH == 1 or q.stride(2) == 1) and (nH == 1 or q.stride(1) == dH) and (B == 1 or q.stride(0) >= nH * dH),
+          f"q: strides {q.stride()}")
+    _check("lens", lens, _I32, (B,))
+    c = _cache(k, kg, v, vg, dH, B, table, weight)
+    if out is None:
+        out = torch.empty((B, nH, dH), dtype=_F32, device=q.device)
+    else:
+        _check("out", out, _F32)
+        _need(out.numel() == q.numel(), f"out: shape {tuple(out.shape)}")
+    h = ctx().handle
+    nbytes = lib().fcu_kv4_attn_work(h, c, B, nH)
+    work = _work(nbytes)
+    call("fcu_kv4_attn", h, q.data_ptr(), q.stride(0) if B > 1 else nH * dH, c, lens.data_ptr(), B, nH,
+         1 / math.sqrt(dH) if scale is None else float(scale), out.data_ptr(),
+         work.data_ptr() if work is not None else None, max(nbytes, 0))
+    return out
+
+
+def kv4Evict(k, kg, v, vg, weight, pos, lens, budget: int, recent: int, table=None, newLens=None):
+    """Cuts every head of every layer (arrays with a leading layer dimension)
+    of sequences longer than `budget` down to it: the slots of the `recent`
+    newest positions and those of largest weight stay (ties: the lowest slot),
+    moved into the freed slots.  Returns the new lengths, min(lens, budget)."""
+    _check("lens", lens, _I32)
+    B = lens.numel()
+    _need(weight is not None and pos is not None, "eviction goes by `weight` and `pos`")
+    _need(budget >= 1 and 0 <= recent <= budget, f"budget {budget}, recent {recent}")
+    _need(k.ndim == 5, f"k: {k.ndim} dimensions")
+    rb = k.shape[-1]
+    c = _cache(k, kg, v, vg, 2 * rb, B, table, weight, pos, layers=True)
+    if newLens is None:
+        newLens = torch.empty_like(lens)
+    else:
+        _check("newLens", newLens, _I32, tuple(lens.shape))
+    h = ctx().handle
+    nbytes = lib().fcu_kv4_evict_work(h, c, B)
+    work = _work(nbytes)
+    call("fcu_kv4_evict", h, c, lens.data_ptr(), B, budget, recent, newLens.data_ptr(),
+         work.data_ptr() if work is not None else None, max(nbytes, 0))
+    return newLens
+
+
+def beamStep(logits, scores, done, beams: int, eos: int):
+    """One beam-search selection: logits [B * beams, V] fp32 (rows may be
+    strided), scores fp32 and done bool [B * beams].  Returns (scores, tokens,
+    parents, done), [B, beams] each, best first: score + log softmax(logits) over
+    all beams and tokens of a sequence, ties to the lowest (beam, token); a beam
+    that is done goes on as (eos, its score)."""
+    ld = _rows("logits", logits, 1)
+    R, V = logits.shape
+    _need(R < 2 or ld >= V, "logits: its rows overlap")
+    _need(1 <= beams <= 32 and R % beams == 0, f"{R} rows for searches of {beams} beams (1 to 32)")
+    _need(0 <= eos < V, f"eos {eos} outside the vocabulary of {V}")
+    _check("scores", scores, _F32)
+    _check("done", done, torch.bool)
+    _need(scores.numel() == R and done.numel() == R, f"{scores.numel()} scores, {done.numel()} done for {R} rows")
+    B = R // beams
+    dev = logits.device
+    outScores = torch.empty((B, beams), dtype=_F32, device=dev)
+    tokens, parents = torch.empty((2, B, beams), dtype=_I32, device=dev).unbind(0)
+    outDone = torch.empty((B, beams), dtype=torch.bool, device=dev)
+    h = ctx().handle
+    nbytes = lib().fcu_beam_work(h, B, beams, V)
+    work = _work(nbytes)
+    call("fcu_beam_step", h, logits.data_ptr(), ld, scores.data_ptr(), done.data_ptr(), B, beams, V, eos,
+         outScores.data_ptr(), tokens.data_ptr(), parents.data_ptr(), outDone.data_ptr(),
+         work.data_ptr() if work is not None else None, max(nbytes, 0))
+    return outScores, tokens, parents, outDone
+
+
+def cacheReorder(arrays, parents, lens, table=None) -> None:
+    """The caches of B searches of W beams follow a selection, in place: beam w
+    of sequence b (cache sequence b * W + w) takes over slots [0, lens[source])
+    of its source b * W + parents[b, w].  arrays: up to 8 tensors [layers, blocks,
+    heads, blockSize, ...] whose slots hold a multiple of 4 bytes (an fp32 cache
+    has one head: its rows); parents int32 [B, W]; lens int32 [B * W]."""
+    _check("parents", parents, _I32)
+    _need(parents.ndim == 2 and parents.shape[1] <= 32, f"parents: shape {tuple(parents.shape)} (at most 32 beams)")
+    B, W = parents.shape
+    _check("lens", lens, _I32)
+    _need(lens.numel() == B * W, f"{lens.numel()} lengths for {B} x {W} beams")
+    _need(1 <= len(arrays) <= 8, f"{len(arrays)} arrays (1 to 8)")
+    L, blocks, bs = arrays[0].shape[0], arrays[0].shape[1], arrays[0].shape[3]
+    spec = (CacheArray * len(arrays))()
+    for i, t in enumerate(arrays):
+        _check(f"arrays[{i}]", t, t.dtype)
+        _need(t.ndim >= 4 and (t.shape[0], t.shape[1], t.shape[3]) == (L, blocks, bs),
+              f"arrays[{i}]: shape {tuple(t.shape)} beside {tuple(arrays[0].shape)}")
+        spec[i] = CacheArray(t.data_ptr(), t.shape[2], math.prod(t.shape[4:]) * t.element_size())
+    if table is not None:
+        _need(table.ndim == 2 and table.shape[0] == B * W, f"table: shape {tuple(table.shape)} for {B * W} beams")
+        _check("table", table, _I32)
+        mb = table.shape[1]
+    else:
+        _need(W > 0 and blocks % max(B * W, 1) == 0, f"{blocks} blocks do not divide among {B * W} beams")
+        mb = blocks // max(B * W, 1)
+    call("fcu_cache_reorder", ctx().handle, spec, len(arrays), L, blocks,
+         table.data_ptr() if table is not None else None, bs, mb, parents.data_ptr(), lens.data_ptr(), B, W)
+
+
+class QuantKVCache(KVCache):
+    """KVCache / PagedKVCache holding 4-bit rows (blockSize given: paged, with
+    `table` and `physBlocks` as in PagedKVCache).  Transformer.forward and
+    forwardBatch take it in their place.  track=True keeps every slot's attention
+    weight and position, which evict() goes by; after an eviction a position no
+    longer names its slot: sequence b's next token goes to slot lens[b]."""
+
+    def __init__(self, nLayers: int, maxSeq: int, nKvHeads: int, dHead: int, batch: int = 1,
+                 blockSize: int | None = None, table=None, physBlocks: int | None = None, track: bool = False):
+        rb = lib().fcu_kv4_row_bytes(int(dHead))
+        _need(rb > 0, f"head dim {dHead}: even, 2 to 256")
+        self.nLayers, self.maxSeq, self.batch = nLayers, maxSeq, batch
+        self.nKvHeads, self.dHead, self.kvDim = nKvHeads, dHead, nKvHeads * dHead
+        self.block_size = maxSeq if blockSize is None else blockSize
+        self.max_blocks = -(-maxSeq // self.block_size)
+        phys = physBlocks if physBlocks is not None else batch * self.max_blocks
+        dev = device()
+        lead = (nLayers, phys, nKvHeads, self.block_size)
+        self.k = torch.zeros(*lead, rb, dtype=_U8, device=dev)
+        self.v = torch.zeros_like(self.k)
+        self.kg = torch.zeros(*lead, 2, dtype=_BF, device=dev)
+        self.vg = torch.zeros_like(self.kg)
+        self.weight = torch.zeros(lead, dtype=_F32, device=dev) if track else None
+        self.pos = torch.zeros(lead, dtype=_I32, device=dev) if track else None
+        self.table, self._table_host = None, None
+        if table is not None:
+            t = np.ascontiguousarray(table, np.int32).reshape(batch, self.max_blocks)
+            if t.min() < 0 or t.max() >= phys:
+                raise ValueError("QuantKVCache: block table entry outside the physical blocks")
+            self._table_host, self.table = t, torch.from_numpy(t).to(dev)
+        elif phys != batch * self.max_blocks:
+            raise ValueError(f"QuantKVCache: {phys} physical blocks need a block table")
+        self.reset()
+
+    def reset(self) -> None:
+        self.len = 0
+        self.lens = np.zeros(self.batch, np.int32)       # slots in use
+        self.dropped = np.zeros(self.batch, np.int32)    # tokens evicted so far
+
+    def slotOf(self, pos: int, seq: int = 0) -> int:
+        """The slot that position `pos` of a sequence is written to: its next one
+        or, while nothing was evicted, any."""
+        s = int(pos) - int(self.dropped[seq])
+        if s < 0 or s >= self.max_blocks * self.block_size:
+            raise ValueError(f"QuantKVCache: no slot for position {pos} ({self.dropped[seq]} tokens evicted, "
+                             f"{self.max_blocks * self.block_size} slots)")
+        if self.dropped[seq] and s < self.lens[seq]:
+            raise ValueError(f"QuantKVCache: position {pos} may have been evicted")
+        return s
+
+    def _used(self, seq: int, slot: int) -> None:
+        self.lens[seq] = max(self.lens[seq], slot + 1)
+        self.len = max(self.len, int(self.lens[seq]))
+
+    def _layer(self, l: int, seq: int | None = None):
+        """Arrays and table of layer l (of one sequence: its own table row)."""
+        if seq is None:
+            return (self.k[l], self.kg[l], self.v[l], self.vg[l]), self.table
+        if self.table is not None:
+            return (self.k[l], self.kg[l], self.v[l], self.vg[l]), self.table[seq:seq + 1]
+        a, b = seq * self.max_blocks, (seq + 1) * self.max_blocks
+        return (self.k[l, a:b], self.kg[l, a:b], self.v[l, a:b], self.vg[l, a:b]), None
+
+    def rows_per_layer(self) -> int:
+        return self.k.shape[1] * self.block_size
+
+    def put(self, layer: int, pos: int, k, v, seq: int = 0) -> None:
+        slot = self.slotOf(pos, seq)
+        row = torch.cat([_dev_f32(k).reshape(1, -1), _dev_f32(v).reshape(1, -1)], 1)
+        at = torch.tensor([[pos], [slot]], dtype=_I32, device=row.device)
+        arrays, table = self._layer(layer, seq)
+        w = p = None
+        if self.weight is not None:
+            a, b = (seq * self.max_blocks, (seq + 1) * self.max_blocks) if table is None else (0, self.k.shape[1])
+            w, p = self.weight[layer, a:b], self.pos[layer, a:b]
+        kv4Put(row, 0, at[0], at[1], *arrays, theta=0.0, table=table, weight=w, pos=p)
+        self._used(seq, slot)
+
+    def _view(self, layer: int, start: int, n: int, seq: int):
+        arrays, table = self._layer(layer, seq)
+        K, V = kv4Values(*arrays, self.dHead, torch.tensor([start], dtype=_I32, device=self.k.device), n, table=table)
+        return K.reshape(n, self.kvDim), V.reshape(n, self.kvDim)
+
+    def kView(self, layer: int, upto: int, seq: int = 0) -> torch.Tensor:
+        """The values of the first `upto` slots (a copy)."""
+        return self._view(layer, 0, upto, seq)[0]
+
+    def vView(self, layer: int, upto: int, seq: int = 0) -> torch.Tensor:
+        return self._view(layer, 0, upto, seq)[1]
+
+    def sliceK(self, layer: int, pos: int, seq: int = 0) -> torch.Tensor:
+        return self._view(layer, pos, 1, seq)[0][0]
+
+    def sliceV(self, layer: int, pos: int, seq: int = 0) -> torch.Tensor:
+        return self._view(layer, pos, 1, seq)[1][0]
+
+    def _own_blocks(self) -> None:
+        t = self._table_host
+        if t is not None and np.unique(t).size < t.size:
+            raise ValueError("QuantKVCache: sequences that share blocks cannot be evicted from or reordered")
+
+    def evict(self, budget: int, recent: int) -> None:
+        """kv4Evict of every layer and sequence."""
+        _need(self.weight is not None, "QuantKVCache: made without track=True")
+        _need(budget >= 1 and 0 <= recent <= budget, f"budget {budget}, recent {recent}")
+        self._own_blocks()
+        if self.lens.max(initial=0) <= budget:
+            return
+        lens = torch.from_numpy(self.lens.copy()).to(self.k.device)
+        kv4Evict(self.k, self.kg, self.v, self.vg, self.weight, self.pos, lens, budget, recent, table=self.table)
+        new = np.minimum(self.lens, budget).astype(np.int32)
+        self.dropped += self.lens - new
+        self.lens, self.len = new, int(new.max())
+
+    def reorder(self, parents) -> None:
+        """cacheReorder for searches of parents.shape[1] beams over all `batch`
+        sequences (parents: a host or device int array [B, W])."""
+        self._own_blocks()
+        _reorder(self, [t for t in (self.k, self.kg, self.v, self.vg, self.weight, self.pos) if t is not None],
+                 parents, self.lens)
+        p = np.asarray(parents.cpu() if isinstance(parents, torch.Tensor) else parents)
+        src = (np.arange(p.shape[0])[:, None] * p.shape[1] + p).reshape(-1)
+        self.lens, self.dropped = self.lens[src].copy(), self.dropped[src].copy()
+        self.len = int(self.lens.max(initial=0))
+
+    def bytes(self) -> int:
+        return sum(t.numel() * t.element_size() for t in (self.k, self.v, self.kg, self.vg, self.weight, self.pos)
+                   if t is not None)
+
+
+def _reorder(cache, arrays, parents, lens) -> None:
+    p = parents if isinstance(parents, torch.Tensor) else torch.as_tensor(np.asarray(parents))
+    _need(p.ndim == 2 and p.numel() == cache.batch, f"parents: shape {tuple(p.shape)} for a cache of {cache.batch}")
+    if not p.is_cuda and p.numel():
+        _need(int(p.min()) >= 0 and int(p.max()) < p.shape[1], "parents outside their search's beams")
+    lens = torch.from_numpy(np.ascontiguousarray(lens, np.int32)).to(cache.k.device)
+    cacheReorder(arrays, p.to(device=cache.k.device, dtype=_I32).contiguous(), lens, table=cache.table)

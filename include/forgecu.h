@@ -463,6 +463,123 @@ int fcu_attn_decode(fcu_ctx *ctx, const float *q, int64_t ld_q, const float *k_c
                     int64_t row_stride, const int32_t *block_table, int max_blocks, int block_size,
                     const int32_t *seq_lens, int B, int nH, int nKV, int dH, double scale, float *out);
 
+/* ---------------------------------------------------------------- 4-bit KV cache */
+/* No counterpart in the reference, whose caches hold fp32: a cache of 4-bit
+ * codes, 4.5 bits per value at head dim 64 with its grids (32 in KVCache).
+ *
+ * A row (one kv head of one slot) holds dH values as codes c in 0..15 on a
+ * grid of its own, x^ = base + step * c in fp32, with
+ *   base = bf16(min x),  step = bf16(fp32(max(0, max x - base) / 15)),
+ *   c = clamp(rint((x - base) / step), 0, 15)  (0 where step is 0),
+ * differences and quotients in double, ties to even.  A row holding a NaN or
+ * a magnitude of 2^127 or more is stored as NaN.
+ *
+ * Arrays of one layer (layers back to back):
+ *   k, v     codes  [blocks, nKV, block_size, fcu_kv4_row_bytes(dH)], element
+ *            e in nibble e & 1 of byte e / 2; 16-byte aligned
+ *   kg, vg   grids  [blocks, nKV, block_size, 2] bf16: step, base
+ *   weight   fp32   [blocks, nKV, block_size]: attention weight each slot has
+ *            received (may be NULL: not kept)
+ *   pos      int32  [blocks, nKV, block_size]: the position a slot holds (may
+ *            be NULL: not kept)
+ * Slot j of sequence b lives in block table[b * max_blocks + j / block_size]
+ * (table NULL: block b * max_blocks + j / block_size) at j % block_size.  A
+ * table entry outside [0, blocks) is never followed: attention over such a
+ * block and values of its slots are NaN, writes to it are dropped, and
+ * fcu_kv4_evict leaves the whole sequence as it is. */
+typedef struct {
+  void *k, *v, *kg, *vg;
+  float *weight;
+  int32_t *pos;
+  const int32_t *table;
+  int64_t layers;     /* layers the arrays hold; only fcu_kv4_evict walks more than the first */
+  int64_t blocks;     /* blocks per layer */
+  int n_kv, dH;       /* kv heads; values per head: even, at most 256 */
+  int block_size, max_blocks;
+} fcu_kv4;
+
+/* Bytes of one row's codes: dH padded to 32, 64, 96, 128, 192 or 256 elements
+ * (the padding's codes are 0), two to a byte; -1 for a dH the cache does not
+ * take (odd, below 2 or above 256).  Host function. */
+int fcu_kv4_row_bytes(int dH);
+/* For each of B sequences, T new tokens: row b * T + t of qkv ([q heads | k
+ * heads | v heads], dH each, rows ld_qkv floats apart) stands at position
+ * positions[b] + t and goes to slot slots[b] + t (both device).  The q heads
+ * are rotated in place and the k heads on the way as fcu_decode_rope_kv
+ * rotates them (theta 0: not at all), then k and v are quantized into the
+ * slot; its weight becomes 0 and its pos the position where those are kept.
+ * The k and v columns of qkv stay as they are.  A token whose slot is outside
+ * [0, max_blocks * block_size), in a bad block, or whose position is negative,
+ * leaves everything untouched. */
+int fcu_kv4_put(fcu_ctx *ctx, float *qkv, int64_t ld_qkv, int B, int T, int nH, double theta,
+                const int32_t *positions, const int32_t *slots, const fcu_kv4 *cache);
+/* K[b, t, h, :], V[b, t, h, :] (fp32 [B, T, nKV, dH]; either may be NULL) =
+ * the values of slot start[b] + t of head h.  A slot outside the sequence's
+ * capacity gives NaN. */
+int fcu_kv4_values(fcu_ctx *ctx, const fcu_kv4 *cache, const int32_t *start, int B, int T, float *K, float *V);
+/* Bytes of workspace fcu_kv4_attn needs for B sequences of nH q heads (it
+ * depends on whether the cache keeps weights); 0 if none, -1 for arguments
+ * that fcu_kv4_attn would refuse. */
+int64_t fcu_kv4_attn_work(fcu_ctx *ctx, const fcu_kv4 *cache, int B, int nH);
+/* out[b, h, :] = sum_j p_j v^_j over slots j < seq_lens[b] (device; clamped to
+ * the capacity), p = softmax_j(scale * q_bh . k^_j), kv head h / (nH / nKV):
+ * fcu_attn_decode over the 4-bit cache.  A length of 0 gives zeros.  q rows are
+ * ld_q floats apart, out is [B, nH * dH].  Where the cache keeps weights, the
+ * slot's weight grows by its p summed over the q heads of its kv head.
+ * nH / nKV <= 16.  `work` is the caller's (fcu_kv4_attn_work bytes, 16-byte
+ * aligned) and may be reused once the call's work on the stream is done. */
+int fcu_kv4_attn(fcu_ctx *ctx, const float *q, int64_t ld_q, const fcu_kv4 *cache, const int32_t *seq_lens, int B,
+                 int nH, double scale, float *out, void *work, int64_t work_bytes);
+/* Bytes of workspace fcu_kv4_evict needs; 0 if none. */
+int64_t fcu_kv4_evict_work(fcu_ctx *ctx, const fcu_kv4 *cache, int B);
+/* Every (layer, sequence, kv head) of more than `budget` slots is cut down to
+ * `budget`.  Slots whose pos is among the newest `recent` positions (pos >
+ * max pos - recent) stay, then those of largest weight, ties to the lowest
+ * slot, a NaN weight last.  The kept slots at or past `budget` move, in slot
+ * order, into the freed slots below it, in slot order (codes, grids, weight and
+ * pos); everything else stays where it is, so the slots are in no order of
+ * position afterwards: attention does not depend on it.  new_lens[b] =
+ * min(seq_lens[b], budget), not the buffer seq_lens is in.  The cache keeps
+ * weight and pos; 1 <= budget, 0 <= recent <= budget.  No two sequences may
+ * share a block. */
+int fcu_kv4_evict(fcu_ctx *ctx, const fcu_kv4 *cache, const int32_t *seq_lens, int B, int budget, int recent,
+                  int32_t *new_lens, void *work, int64_t work_bytes);
+
+/* ---------------------------------------------------------------- beam search */
+/* Bytes of workspace fcu_beam_step needs. */
+int64_t fcu_beam_work(fcu_ctx *ctx, int B, int W, int64_t V);
+/* One selection of a search with W beams in each of B sequences.  Row b * W + w
+ * of logits ([V] floats, rows ld floats apart) belongs to beam w of sequence b,
+ * whose score is scores[b * W + w]; done (bytes, 0 or 1) marks the beams that
+ * have ended.  Candidate (w, token) of a sequence scores
+ *   scores[w] + logits[w][token] - log sum exp logits[w]
+ * in double; a beam that has ended offers (w, eos) at scores[w] alone; whatever
+ * is not finite counts as -inf.  The W best, by score and then by lowest
+ * w * V + token, give out_scores, tokens, parents (= w) and out_done (ended
+ * before, or token is eos), [B, W] each, best first; none of them may be an
+ * input's buffer.  1 <= W <= 32.  logits may hold -inf (a banned token); a NaN
+ * or +inf makes all of its row's candidates -inf. */
+int fcu_beam_step(fcu_ctx *ctx, const float *logits, int64_t ld, const float *scores, const uint8_t *done, int B,
+                  int W, int64_t V, int eos, float *out_scores, int32_t *tokens, int32_t *parents,
+                  uint8_t *out_done, void *work, int64_t work_bytes);
+/* One array of a cache for fcu_cache_reorder: [layers, blocks, heads,
+ * block_size, unit bytes] (KVCache: heads 1, unit = row bytes); unit a multiple
+ * of 4, base 16-byte aligned. */
+typedef struct {
+  void *base;
+  int64_t heads, unit;
+} fcu_cache_array;
+/* The caches of B * W beams (sequence b's beam w is cache sequence b * W + w)
+ * follow a selection, in place: in every array and layer, slots
+ * [0, lens[src]) of beam w become those of src = b * W + parents[b * W + w] as
+ * they were before the call; slots past that stay.  A parent outside [0, W)
+ * leaves its beam as it is, and so does a block outside [0, blocks).  Slots map
+ * to blocks as in fcu_kv4; no two beams may share a block.  1 <= W <= 32, at
+ * most 8 arrays. */
+int fcu_cache_reorder(fcu_ctx *ctx, const fcu_cache_array *arrays, int n_arrays, int64_t layers, int64_t blocks,
+                      const int32_t *table, int block_size, int max_blocks, const int32_t *parents,
+                      const int32_t *lens, int B, int W);
+
 /* ---------------------------------------------------------------- data-parallel exchange */
 /* NCCL over NVLink / NVSwitch, one communicator per GPU.  The reference has no
  * counterpart (it trains on one CPU thread); this is the exchange a
