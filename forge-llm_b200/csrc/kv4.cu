@@ -42,6 +42,10 @@ int view(const char *who, const fcu_kv4 *in, int64_t B, bool need_values, Cache 
   out->bs = in->block_size;
   out->mb = in->max_blocks;
   out->cap = cap;
+  // the smallest 2^s >= bs; mul = floor(2^32 (2^s - bs) / bs) + 1 (Granlund and Montgomery's multiplier for division)
+  out->div_shift = 0;
+  while (((int64_t)1 << out->div_shift) < out->bs) out->div_shift++;
+  out->div_mul = (uint32_t)(((((uint64_t)1 << out->div_shift) - out->bs) << 32) / out->bs + 1);
   return FCU_OK;
 }
 

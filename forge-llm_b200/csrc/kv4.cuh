@@ -36,7 +36,13 @@ struct Cache {
   int nKV, dH, rb;           // rb: bytes of a row's codes
   int bs, mb;                // slots per block, blocks per sequence
   int64_t cap;               // slots per sequence
+  uint32_t div_mul;          // j / bs = (umulhi(div_mul, j) + j) >> div_shift for j < 2^31
+  int div_shift;
 };
+
+__device__ __forceinline__ int64_t block_index(const Cache &c, int64_t j) {
+  return (__umulhi(c.div_mul, (uint32_t)j) + (uint32_t)j) >> c.div_shift;
+}
 
 // Physical block of logical block i of sequence b; -1 if the table names a
 // block the cache does not have (its slots are then never touched).
@@ -48,7 +54,7 @@ __device__ __forceinline__ int64_t block_of(const Cache &c, int64_t b, int64_t i
 
 // Row index of slot j of head h of sequence b in layer 0; -1 for a bad block.
 __device__ __forceinline__ int64_t row_of(const Cache &c, int64_t b, int h, int64_t j) {
-  const int64_t i = c.mb == 1 ? 0 : (int64_t)((uint32_t)j / (uint32_t)c.bs);
+  const int64_t i = block_index(c, j);
   const int64_t p = block_of(c, b, i);
   return p < 0 ? -1 : (p * c.nKV + h) * c.bs + (j - i * c.bs);
 }

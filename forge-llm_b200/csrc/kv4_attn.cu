@@ -8,15 +8,15 @@
 // reading the cache: a slot of one kv head is 2 (dH / 2 + 4) bytes, and every
 // q head of the group uses it while it is on the chip.
 //
-// Both products run on mma.sync m16n8k16 with fp16 operands and fp32 sums.
-// The codes are exact in fp16 without a conversion: a nibble in the low byte
-// of a 16-bit half IS the subnormal c 2^-24 (or 16 c 2^-24), so two ANDs on a
-// word give four operands.  The other operand carries 22 bits, x = hi + lo, in
-// rows r and r + 8 of the same instruction (heads 0..7 and their remainders),
-// whose sums are added in fp32; a power of two keeps it in fp16's range.  (An
-// M = 128 tcgen05 tile would want the codes expanded to 16 bits in shared
-// memory first, four times the traffic of the codes themselves; from registers
-// the legacy pipe is fast enough, one m16n8k16 per 36 bytes of cache.)
+// Both products run on mma.sync m16n8k16 with the codes as the 16-row operand,
+// fp16 operands and fp32 sums.  The codes are exact in fp16 without a
+// conversion: a nibble in the low byte of a 16-bit half IS the subnormal
+// c 2^-24 (or 16 c 2^-24), so two ANDs on a word give four operands.  The other
+// operand carries 22 bits, x = hi + lo, in columns 2i and 2i + 1 (four heads to
+// an 8-column tile), whose sums one thread holds side by side and adds in fp32;
+// a power of two keeps x in fp16's range.  (A tcgen05 tile would want the codes
+// expanded to 16 bits in shared memory first, four times the traffic of the
+// codes themselves; fed from registers the legacy pipe is fast enough.)
 //
 // Work is cut by tiles of slots, not by sequence: the tiles of all (sequence,
 // kv head) segments in a row are dealt in equal runs to as many CTAs as the GPU
@@ -33,22 +33,35 @@ namespace {
 
 constexpr int kThreads = 128;
 constexpr int kWarps = kThreads / 32;
-constexpr int kStages = 2;
-constexpr int kHeads = 8;              // q heads of one CTA (rows of the mma tile, twice)
+constexpr int kKBufs = 2;      // k tiles on chip, one of them on its way
 constexpr float kLog2e = 1.4426950408889634f;
 
-// W: a row is W 16-byte units (dP = 32 W elements).
-template <int W>
+// W: a row is W 16-byte units (dP = 32 W elements).  G: tiles of four q heads.
+template <int W, int G>
 struct Cfg {
-  static constexpr int kTile = W <= 4 ? 64 : 32;                  // slots of one warp's step
+  static constexpr int kTile = W <= 2 ? 128 : W <= 4 ? 64 : 32;        // slots of one warp's step
   static constexpr int kRow = 16 * W;
-  static constexpr int kGridStride = kTile / 4 + 4;               // words; slots 4i + t of column t
+  static constexpr int kGridStride = kTile / 8 + (kTile > 32 ? 4 : 0);   // words of the grids of slots x, x + 8, ...
+  static constexpr int kGrids = 4 * 8 * kGridStride;
   static constexpr int kCodes = kTile * kRow;
-  static constexpr int kStage = 2 * kCodes + 2 * 16 * kGridStride;
-  static constexpr int kCtas = W <= 2 ? 4 : W <= 4 ? 3 : 2;       // per SM, by registers
-  static constexpr int kRing = kWarps * kStages * kStage;
-  static constexpr int kMerge = kWarps * kHeads * (32 * W + 2) * 4;   // the warps' o, m, l at a segment's end
+  static constexpr int kPart = kCodes + kGrids;                   // a tile's k or v
+  static constexpr int kHeads = 4 * G;
+  static constexpr int kRing = kWarps * (kKBufs + 1) * kPart;
+  static constexpr int kMerge = kWarps * kHeads * (32 * W + 4) * 4;   // the warps' o, m, l at a segment's end
   static constexpr int kSmem = kRing > kMerge ? kRing : kMerge;
+  // resident per SM: by registers, and by shared memory (228 KB, 1 KB and the
+  // static arrays of each CTA aside)
+  static constexpr int kByRegs = G == 1 ? (W <= 3 ? 4 : 3) : (W <= 4 ? 3 : 2);
+  static constexpr int kBySmem = 228 * 1024 / (kSmem + 3 * 1024);
+  static constexpr int kCtas = kByRegs < kBySmem ? kByRegs : kBySmem;
+};
+constexpr int kMaxHeads = 8;           // q heads of one CTA
+
+// What run c leaves for the merge: the segment that begins in it and is cut by
+// its end (pieces 0: none).
+struct Cut {
+  int pieces, heads;
+  int64_t bh;            // b * nH + the first head
 };
 
 struct AttnArgs {
@@ -59,10 +72,12 @@ struct AttnArgs {
   int B, nH, g;          // g: q heads per kv head
   int gs, hg;            // q heads of one segment, segments per kv head
   int ctas;              // runs (CTAs of the main kernel)
+  int vec;               // q rows and heads start on 16 bytes
   float scale;
   float *out;
-  float *part;           // [ctas][2][kHeads][dH + 2]: o, then m (log2 units) and l
-  float2 *ml;            // [B, nH] final m and l, where weights are kept
+  float *part;           // [ctas][2][kMaxHeads][dH + 2]: o, then m (log2 units) and l
+  Cut *cuts;             // [ctas]
+  float2 *ml;            // [B, nH] where weights are kept: m and l, or of a cut segment (its run's bits, -pieces)
   float *scores;         // [B, nH, cap] in log2 units, where weights are kept
 };
 
@@ -160,20 +175,34 @@ __device__ __forceinline__ float ex2(float x) {
   return y;
 }
 
+// c += a b, and the same from zero
 __device__ __forceinline__ void mma(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-  asm volatile(
+  asm(
       "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
       : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
+__device__ __forceinline__ void mma0(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm(
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+      : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.f));
+}
 
-// (x, y) as fp16 pairs, hi and the remainders
-__device__ __forceinline__ void split(float x, float y, uint32_t *hi, uint32_t *lo) {
-  const __half2 h = __floats2half2_rn(x, y);
-  const float2 f = __half22float2(h);
-  const __half2 l = __floats2half2_rn(x - f.x, y - f.y);
-  *hi = *reinterpret_cast<const uint32_t *>(&h);
-  *lo = *reinterpret_cast<const uint32_t *>(&l);
+// x as (hi, lo) fp16: its first 11 bits, which fp16 holds, and the rest rounded
+// to 11 (2^-22 of x at most is lost; below fp16's normal range 2^-25)
+__device__ __forceinline__ uint32_t split(float x) {
+  const float h = __uint_as_float(__float_as_uint(x) & 0xffffe000u);
+  const __half2 p = __floats2half2_rn(h, x - h);
+  return *reinterpret_cast<const uint32_t *>(&p);
+}
+
+// The 8 x 8 matrix of 16-bit elements whose row `lane / 4` the warp holds in
+// pairs, transposed.
+__device__ __forceinline__ uint32_t transpose8(uint32_t x) {
+  uint32_t y;
+  asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+  return y;
 }
 
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void *src, bool on) {
@@ -183,65 +212,98 @@ __device__ __forceinline__ void cp_async4(uint32_t dst, const void *src, bool on
   asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(on ? 4 : 0));
 }
 
-// Starts the copies of one tile (slots j0 .. j0 + cnt of head h of sequence b)
-// into a warp's stage.  Slots past cnt are zero; those of a bad block have NaN
-// grids.
+// Shared memory keeps the 16-byte piece c of slot x's row at c ^ swizzle(x), so
+// that one piece of eight neighbouring slots lies in all 32 banks, which is what
+// ldmatrix reads at a time (odd W: their rows are 4 banks times an odd number
+// apart as they are).
 template <int W>
-__device__ __forceinline__ void issue(const Cache &c, int64_t b, int h, int64_t j0, int cnt, uint8_t *stage) {
-  using C = Cfg<W>;
+__device__ __forceinline__ int swizzle(int x) {
+  if constexpr (W == 8) return x & 7;
+  else if constexpr (W == 4) return (x >> 1) & 3;
+  else if constexpr (W % 2 == 0) return (x >> 2) & 1;
+  else return 0;
+}
+// Where a tile's slot x keeps its grid: those of slots x, x + 8, ... are neighbours.
+template <class C>
+__device__ __forceinline__ uint32_t grid_at(int x) {
+  return 4 * ((x & 7) * C::kGridStride + (x >> 3));
+}
+
+// Starts the copies of one tile's k or v (slots j0 .. j0 + cnt of head h of
+// sequence b) into shared memory.  Slots past cnt are zero; those of a bad block
+// have NaN grids.
+template <class C, int W>
+__device__ __forceinline__ void issue(const Cache &c, const uint8_t *codes, const uint32_t *grids, int64_t b, int h,
+                                      int j0, int cnt, uint8_t *part) {
   const int lane = threadIdx.x & 31;
-  const uint32_t k_s = (uint32_t)__cvta_generic_to_shared(stage), v_s = k_s + C::kCodes;
-  const uint32_t kg_s = v_s + C::kCodes, vg_s = kg_s + 16 * C::kGridStride;
-  const int64_t blk = c.mb == 1 ? 0 : (int64_t)((uint32_t)j0 / (uint32_t)c.bs);
-  const int off = (int)(j0 - blk * c.bs);
-  if (off + cnt <= c.bs) {
-    // one block: the tile's rows are contiguous
-    const int64_t p = block_of(c, b, blk);
-    const bool ok = p >= 0;
-    const int64_t row = ok ? (p * c.nKV + h) * c.bs + off : 0;
-    const uint8_t *ks = c.k + row * C::kRow, *vs = c.v + row * C::kRow;
+  const uint32_t code_s = (uint32_t)__cvta_generic_to_shared(part), grid_s = code_s + C::kCodes;
+  const int blk = (int)block_index(c, j0), off = j0 - blk * c.bs;
+  const int64_t p = block_of(c, b, blk);
+  if (cnt == C::kTile && off + C::kTile <= c.bs && p >= 0) {
+    // a full tile inside one block: its rows are contiguous
+    const int64_t row = (p * c.nKV + h) * c.bs + off;
+    const uint8_t *src = codes + row * C::kRow + 16 * lane;
 #pragma unroll
     for (int i = 0; i < C::kTile * W / 32; i++) {
       const int x = i * 32 + lane;
-      const bool on = ok && x / W < cnt;
-      cp_async16(k_s + 16 * x, on ? ks + 16 * x : c.k, on);
-      cp_async16(v_s + 16 * x, on ? vs + 16 * x : c.v, on);
+      cp_async16(code_s + 16 * (W % 2 == 0 ? x - x % W + (x % W ^ swizzle<W>(x / W)) : x), src + 512 * i, true);
     }
+    const uint32_t *g = grids + row + lane;
+#pragma unroll
+    for (int i = 0; i < C::kTile / 32; i++) cp_async4(grid_s + grid_at<C>(lane) + 16 * i, g + 32 * i, true);
+  } else {
+    int64_t rows[C::kTile / 32];        // of slots lane and lane + 32
 #pragma unroll
     for (int i = 0; i < C::kTile / 32; i++) {
       const int x = i * 32 + lane;
-      const uint32_t at = 4 * ((x & 3) * C::kGridStride + (x >> 2));
-      const bool on = ok && x < cnt;
-      if (ok || x >= cnt) {
-        cp_async4(kg_s + at, on ? c.kg + row + x : c.kg, on);
-        cp_async4(vg_s + at, on ? c.vg + row + x : c.vg, on);
-      } else {
-        *reinterpret_cast<uint32_t *>(stage + 2 * C::kCodes + at) = kNanGrid;
-        *reinterpret_cast<uint32_t *>(stage + 2 * C::kCodes + 16 * C::kGridStride + at) = kNanGrid;
-      }
+      rows[i] = x < cnt ? row_of(c, b, h, j0 + x) : -1;
+      const uint32_t at = grid_at<C>(x);
+      if (rows[i] >= 0 || x >= cnt) cp_async4(grid_s + at, rows[i] >= 0 ? grids + rows[i] : grids, rows[i] >= 0);
+      else *reinterpret_cast<uint32_t *>(part + C::kCodes + at) = kNanGrid;
     }
-  } else {
-#pragma unroll 1
+#pragma unroll
     for (int i = 0; i < C::kTile * W / 32; i++) {
       const int x = i * 32 + lane, j = x / W;
-      const int64_t row = j < cnt ? row_of(c, b, h, j0 + j) : -1;
-      const int64_t at = row * C::kRow + 16 * (x - j * W);
-      cp_async16(k_s + 16 * x, row >= 0 ? c.k + at : c.k, row >= 0);
-      cp_async16(v_s + 16 * x, row >= 0 ? c.v + at : c.v, row >= 0);
-    }
-#pragma unroll 1
-    for (int x = lane; x < C::kTile; x += 32) {
-      const uint32_t at = 4 * ((x & 3) * C::kGridStride + (x >> 2));
-      const int64_t row = x < cnt ? row_of(c, b, h, j0 + x) : -1;
-      if (row >= 0 || x >= cnt) {
-        cp_async4(kg_s + at, row >= 0 ? c.kg + row : c.kg, row >= 0);
-        cp_async4(vg_s + at, row >= 0 ? c.vg + row : c.vg, row >= 0);
-      } else {
-        *reinterpret_cast<uint32_t *>(stage + 2 * C::kCodes + at) = kNanGrid;
-        *reinterpret_cast<uint32_t *>(stage + 2 * C::kCodes + 16 * C::kGridStride + at) = kNanGrid;
+      // the warp's pieces x are of slots that at most two of the rows[] hold
+      constexpr int kLast = C::kTile / 32 - 1;
+      const int lo = i * 32 / W / 32, hi = (i * 32 + 31) / W / 32;
+      int64_t row = __shfl_sync(0xffffffffu, rows[lo < kLast ? lo : kLast], j & 31);
+      if (hi != lo) {
+        const int64_t up = __shfl_sync(0xffffffffu, rows[hi < kLast ? hi : kLast], j & 31);
+        if (j >= 32 * hi) row = up;
       }
+      cp_async16(code_s + 16 * (W % 2 == 0 ? x - x % W + (x % W ^ swizzle<W>(j)) : x),
+                 row >= 0 ? codes + row * C::kRow + 16 * (x - j * W) : codes, row >= 0);
     }
   }
+}
+
+// 8 x 8 matrices of 16-bit elements, as they lie or transposed: lane i gives row
+// i % 8 of matrix i / 8.
+template <bool T>
+__device__ __forceinline__ void ldsm4(uint32_t p, uint32_t &a, uint32_t &b, uint32_t &c, uint32_t &d) {
+  if constexpr (T)
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
+                 : "=r"(a), "=r"(b), "=r"(c), "=r"(d) : "r"(p) : "memory");
+  else
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
+                 : "=r"(a), "=r"(b), "=r"(c), "=r"(d) : "r"(p) : "memory");
+}
+template <bool T>
+__device__ __forceinline__ void ldsm2(uint32_t p, uint32_t &a, uint32_t &b) {
+  if constexpr (T)
+    asm volatile("ldmatrix.sync.aligned.m8n8.x2.trans.shared.b16 {%0,%1}, [%2];" : "=r"(a), "=r"(b) : "r"(p) : "memory");
+  else
+    asm volatile("ldmatrix.sync.aligned.m8n8.x2.shared.b16 {%0,%1}, [%2];" : "=r"(a), "=r"(b) : "r"(p) : "memory");
+}
+// The rows of slots 16 k .. 16 k + 16 of a tile: w[e][c] of thread (r, t) is word
+// t of piece c of slot 16 k + 8 e + r, or (T) unit r of piece c of slots 2t and
+// 2t + 1 of those eight.  off: lane's place for pieces 2c and 2c + 1.
+template <int W, bool T>
+__device__ __forceinline__ void rows16(uint32_t codes, const uint32_t (&off)[(W + 1) / 2], int k, uint32_t (&w)[2][W]) {
+#pragma unroll
+  for (int c = 0; c + 1 < W; c += 2) ldsm4<T>(codes + off[c / 2] + 16 * k * 16 * W, w[0][c], w[1][c], w[0][c + 1], w[1][c + 1]);
+  if constexpr (W % 2) ldsm2<T>(codes + off[W / 2] + 16 * k * 16 * W, w[0][W - 1], w[1][W - 1]);
 }
 
 // N words from shared memory at an address aligned to 4 N bytes' largest power of two
@@ -265,19 +327,27 @@ __device__ __forceinline__ void lds(const uint8_t *p, uint32_t (&w)[N]) {
   }
 }
 
-// In the mma tiles, thread (r = lane / 4, t = lane % 4) of a warp holds head r
-// and, of the 8 slots of an n-tile, columns 2t and 2t + 1, which stand for
-// slots t and t + 4: then the four t of a V load read four neighbouring rows.
-template <int W>
-__global__ void __launch_bounds__(kThreads, Cfg<W>::kCtas) kv4_attn_kernel(AttnArgs a) {
-  using C = Cfg<W>;
-  constexpr int TP = C::kTile, NT = TP / 8, KS = TP / 16, dP = 32 * W;
+// A warp's thread is (r = lane / 4, t = lane % 4).  It holds head t (and 4 + t)
+// at slots r, r + 8, ... of a tile's scores, and in the output head t at the four
+// elements that start at 32 c + 4 r of every piece c.
+template <int W, int G>
+__global__ void __launch_bounds__(kThreads, Cfg<W, G>::kCtas) kv4_attn_kernel(AttnArgs a) {
+  using C = Cfg<W, G>;
+  constexpr int TP = C::kTile, KS = TP / 16, dP = 32 * W;
   pdl_trigger();
   extern __shared__ __align__(16) uint8_t sm[];
   __shared__ int64_t sh[kThreads];
   const Cache &c = a.c;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, r = lane >> 2, t = lane & 3;
-  uint8_t *ring = sm + warp * kStages * C::kStage;
+  uint8_t *kbuf = sm + warp * (kKBufs + 1) * C::kPart, *vbuf = kbuf + kKBufs * C::kPart;
+  const uint32_t kbuf_s = (uint32_t)__cvta_generic_to_shared(kbuf), vbuf_s = kbuf_s + kKBufs * C::kPart;
+  uint32_t off[(W + 1) / 2];      // this lane's row and piece for ldmatrix
+#pragma unroll
+  for (int i = 0; i < (W + 1) / 2; i++) {
+    const int row = lane & 15;
+    off[i] = row * C::kRow + 16 * ((2 * i + (lane >> 4)) ^ swizzle<W>(row));
+    if (W % 2 && i == W / 2) off[i] = row * C::kRow + 16 * (W - 1);
+  }
   pdl_wait();
   for (int64_t b = blockIdx.x; b < a.B; b += gridDim.x)
     if (length(a, b) == 0)
@@ -285,268 +355,306 @@ __global__ void __launch_bounds__(kThreads, Cfg<W>::kCtas) kv4_attn_kernel(AttnA
   const Plan plan = make_plan<TP>(a, sh);
   int64_t u = blockIdx.x * plan.per;
   const int64_t end = min(u + plan.per, plan.total);
-  if (u >= end) return;
-  Place at = find<TP>(a, u, sh);
+  Cut cut{0, 0, 0};
+  Place at{-1, 0, 0, 0};
+  if (u < end) at = find<TP>(a, u, sh);
   while (at.b >= 0 && at.b < a.B) {
     // this run's part [t0, t1) of the segment
-    const int64_t t0 = at.tile, t1 = min(at.tiles, t0 + (end - u));
+    const int t0 = (int)at.tile, t1 = (int)min(at.tiles, at.tile + (end - u));
     const int h = at.seg / a.hg, h0 = h * a.g + (at.seg % a.hg) * a.gs;   // kv head, first q head
     const int heads = min(a.gs, (h + 1) * a.g - h0);
-    const int64_t n = length(a, at.b);
+    const int n = (int)length(a, at.b);
 
-    // q of head r: words t W .. t W + W of a row face this thread, eight
-    // elements each, in the order that the masks below take a code word apart
-    uint32_t qa[2 * W][4];
-    float qf, qb;
-    {
-      const float *q = a.q + at.b * a.ld_q + (int64_t)(h0 + r) * c.dH;
-      float big = 0.f, sum = 0.f;
+    // a tile's k and v are copy groups of their own: k one tile ahead, v as soon
+    // as the last tile's has been used
+    auto issue_k = [&](int tile, int buf) {
+      if (tile < t1) issue<C, W>(c, c.k, c.kg, at.b, h, tile * TP, min(TP, n - tile * TP), kbuf + buf * C::kPart);
+      asm volatile("cp.async.commit_group;");
+    };
+    auto issue_v = [&](int tile) {
+      if (tile < t1) issue<C, W>(c, c.v, c.vg, at.b, h, tile * TP, min(TP, n - tile * TP), vbuf);
+      asm volatile("cp.async.commit_group;");
+    };
+    int kb = 0;
+    issue_k(t0 + warp, 0);
+    issue_v(t0 + warp);
+
+    // scale * log2 e * q of head r / 2 (its hi part for even r, the remainder
+    // for odd r) against the eight elements of word t of every piece, in the
+    // order that the masks below take a code word apart
+    uint32_t qb[G][2 * W][2];
+    float qs[G], qf[G];      // for head t: sum of the scaled q in the units of the tile's sums; those units
 #pragma unroll
-      for (int i = 0; i < W; i++)
+    for (int g = 0; g < G; g++) {
+      const int head = 4 * g + (r >> 1);
+      const float *q = a.q + at.b * a.ld_q + (int64_t)(h0 + head) * c.dH;
+      const float sc = a.scale * kLog2e;
+      float x[8 * W], big = 0.f, sum = 0.f;
 #pragma unroll
-        for (int e = 0; e < 8; e++) {
-          const int d = (t * W + i) * 8 + e;
-          const float x = r < heads && d < c.dH ? q[d] : 0.f;
-          big = fmaxf(big, fabsf(x));
-          sum += x;
+      for (int i = 0; i < 8 * W; i += 4) {
+        const int d = 32 * (i / 8) + 8 * t + i % 8;
+        if (a.vec) {
+          const float4 f = head < heads && d < c.dH ? *reinterpret_cast<const float4 *>(q + d) : float4{0.f, 0.f, 0.f, 0.f};
+          x[i] = f.x, x[i + 1] = f.y, x[i + 2] = f.z, x[i + 3] = f.w;
+        } else {
+#pragma unroll
+          for (int e = 0; e < 4; e++) x[i + e] = head < heads && d + e < c.dH ? q[d + e] : 0.f;
         }
+      }
+#pragma unroll
+      for (int i = 0; i < 8 * W; i++) {
+        big = fmaxf(big, fabsf(x[i]));
+        sum += x[i];
+      }
       big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, 1));
-      big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, 2));
+      big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, 2)) * fabsf(sc);
       sum += __shfl_xor_sync(0xffffffffu, sum, 1);
       sum += __shfl_xor_sync(0xffffffffu, sum, 2);
-      // q * up below 2^14, up a power of two (from 2^-115 to 2^113)
-      const int ex = max(27, (int)(__float_as_uint(big) >> 23));
+      // x * sc * up below 2^14, up a power of two; the codes carry 2^-24
+      const int ex = min(240, max(27, (int)(__float_as_uint(big) >> 23)));
       const float up = __uint_as_float((uint32_t)(267 - ex) << 23);
-      // codes carry 2^-24
-      qf = a.scale * kLog2e * __uint_as_float((uint32_t)min(254, ex + 11) << 23);
-      qb = a.scale * kLog2e * sum;
+      const float f = __uint_as_float((uint32_t)(ex + 11) << 23);          // 2^24 / up
+      const float inv = __uint_as_float((uint32_t)(243 - ex) << 23);       // up / 2^24
+      const float up0 = sc * up, up1 = up0 * 0.0625f;       // odd nibbles are met at 16 times their value
+      const uint32_t sel = r & 1 ? 0x7632 : 0x5410;
 #pragma unroll
       for (int i = 0; i < W; i++) {
-        float x[8];
+        uint32_t y[8];
 #pragma unroll
-        for (int e = 0; e < 8; e++) {
-          const int d = (t * W + i) * 8 + e;
-          x[e] = (r < heads && d < c.dH ? q[d] : 0.f) * up;
-          if (e & 1) x[e] *= 0.0625f;      // odd nibbles are met at 16 times their value
-        }
-        split(x[0], x[4], &qa[2 * i][0], &qa[2 * i][1]);
-        split(x[2], x[6], &qa[2 * i][2], &qa[2 * i][3]);
-        split(x[1], x[5], &qa[2 * i + 1][0], &qa[2 * i + 1][1]);
-        split(x[3], x[7], &qa[2 * i + 1][2], &qa[2 * i + 1][3]);
+        for (int e = 0; e < 8; e++) y[e] = split(x[8 * i + e] * (e & 1 ? up1 : up0));
+        qb[g][2 * i][0] = __byte_perm(y[0], y[4], sel);
+        qb[g][2 * i][1] = __byte_perm(y[2], y[6], sel);
+        qb[g][2 * i + 1][0] = __byte_perm(y[1], y[5], sel);
+        qb[g][2 * i + 1][1] = __byte_perm(y[3], y[7], sel);
       }
+      qs[g] = __shfl_sync(0xffffffffu, sum * sc * inv, 8 * t);
+      qf[g] = __shfl_sync(0xffffffffu, f, 8 * t);
     }
 
-    float m = -INFINITY, l = 0.f, z = 0.f;
-    float o[4 * W][2];
+    // the running maximum, in the units of the tile's sums and, for head t
+    float m[G], l[G], z[G], o[G][4 * W];
 #pragma unroll
-    for (int i = 0; i < 4 * W; i++) o[i][0] = o[i][1] = 0.f;
-    float *sc = a.scores ? a.scores + (at.b * a.nH + h0 + r) * c.cap : nullptr;
-
-    int64_t next = t0 + warp;
-    int put = 0, get = 0;
+    for (int g = 0; g < G; g++) {
+      m[g] = -INFINITY;
+      l[g] = z[g] = 0.f;
 #pragma unroll
-    for (int s = 0; s < kStages - 1; s++) {
-      if (next < t1) issue<W>(c, at.b, h, next * TP, (int)min((int64_t)TP, n - next * TP), ring + put * C::kStage);
-      asm volatile("cp.async.commit_group;");
-      put = put + 1 == kStages ? 0 : put + 1;
-      next += kWarps;
+      for (int i = 0; i < 4 * W; i++) o[g][i] = 0.f;
     }
-    for (int64_t tile = t0 + warp; tile < t1; tile += kWarps) {
-      if (next < t1) issue<W>(c, at.b, h, next * TP, (int)min((int64_t)TP, n - next * TP), ring + put * C::kStage);
-      asm volatile("cp.async.commit_group;");
-      put = put + 1 == kStages ? 0 : put + 1;
-      next += kWarps;
-      asm volatile("cp.async.wait_group %0;" ::"n"(kStages - 1));
+
+    for (int tile = t0 + warp; tile < t1; tile += kWarps) {
+      const uint8_t *ks = kbuf + kb * C::kPart;
+      kb ^= 1;
+      issue_k(tile + kWarps, kb);
+      asm volatile("cp.async.wait_group 2;");
       __syncwarp();
-      const uint8_t *ks = ring + get * C::kStage, *vs = ks + C::kCodes, *kgs = vs + C::kCodes;
-      const uint8_t *vgs = kgs + 16 * C::kGridStride;
-      get = get + 1 == kStages ? 0 : get + 1;
-      const int64_t j0 = tile * TP;
-      const int cnt = (int)min((int64_t)TP, n - j0);
+      const int j0 = tile * TP, cnt = min(TP, n - j0);
 
-      // scores of head r against slots 8 nt + 4 e + t
-      float s[NT][2];
+      // s[g][2 k + e]: head 4 g + t, slot 16 k + 8 e + r
+      float s[G][2 * KS];
       {
-        const uint8_t *kp = ks + ((r & 1) * 4 + (r >> 1)) * C::kRow + 4 * W * t;
+        const uint32_t ks_s = kbuf_s + (uint32_t)(ks - kbuf);
+        uint32_t gr[2 * KS];
+        lds<2 * KS>(ks + C::kCodes + 4 * r * C::kGridStride, gr);
+        constexpr int KB = KS < 2 ? KS : 2;   // row tiles whose chains of sums run side by side
 #pragma unroll
-        for (int nt = 0; nt < NT; nt++) {
-          uint32_t w[W];
-          lds<W>(kp + nt * 8 * C::kRow, w);
-          float acc[4] = {0.f, 0.f, 0.f, 0.f};
+        for (int k0 = 0; k0 < KS; k0 += KB) {
+          uint32_t w[KB][2][W];
 #pragma unroll
-          for (int i = 0; i < W; i++) {
-            const uint32_t x = w[i], y = x >> 8;
-            mma(acc, qa[2 * i], x & 0x000f000fu, y & 0x000f000fu);
-            mma(acc, qa[2 * i + 1], x & 0x00f000f0u, y & 0x00f000f0u);
-          }
-          s[nt][0] = (acc[0] + acc[2]) * qf;
-          s[nt][1] = (acc[1] + acc[3]) * qf;
-        }
-      }
-      float top = -INFINITY;
+          for (int k = 0; k < KB; k++) rows16<W, false>(ks_s, off, k0 + k, w[k]);
+          float acc[KB][G][4];
 #pragma unroll
-      for (int i = 0; i < NT / 2; i++) {
-        uint32_t g[4];
-        lds<4>(kgs + 4 * (t * C::kGridStride + 4 * i), g);
+          for (int i = 0; i < W; i++)
 #pragma unroll
-        for (int e = 0; e < 4; e++) {
-          float &x = s[2 * i + e / 2][e & 1];
-          x = fmaf(x, grid_step(g[e]), qb * grid_base(g[e]));
+            for (int k = 0; k < KB; k++) {
+              const uint32_t x0 = w[k][0][i], x1 = w[k][1][i], y0 = x0 >> 8, y1 = x1 >> 8;
+              const uint32_t lo[4] = {x0 & 0x000f000fu, x1 & 0x000f000fu, y0 & 0x000f000fu, y1 & 0x000f000fu};
+              const uint32_t hi[4] = {x0 & 0x00f000f0u, x1 & 0x00f000f0u, y0 & 0x00f000f0u, y1 & 0x00f000f0u};
+#pragma unroll
+              for (int g = 0; g < G; g++) {
+                if (i == 0) mma0(acc[k][g], lo, qb[g][0][0], qb[g][0][1]);
+                else mma(acc[k][g], lo, qb[g][2 * i][0], qb[g][2 * i][1]);
+                mma(acc[k][g], hi, qb[g][2 * i + 1][0], qb[g][2 * i + 1][1]);
+              }
+            }
+#pragma unroll
+          for (int k = 0; k < KB; k++)
+#pragma unroll
+            for (int g = 0; g < G; g++)
+#pragma unroll
+              for (int e = 0; e < 2; e++) {
+                const uint32_t gd = gr[2 * (k0 + k) + e];
+                s[g][2 * (k0 + k) + e] = fmaf(acc[k][g][2 * e] + acc[k][g][2 * e + 1], grid_step(gd), qs[g] * grid_base(gd));
+              }
         }
       }
       if (cnt < TP) {
 #pragma unroll
-        for (int nt = 0; nt < NT; nt++)
+        for (int i = 0; i < 2 * KS; i++)
+          if (8 * i + r >= cnt)
 #pragma unroll
-          for (int e = 0; e < 2; e++)
-            if (8 * nt + 4 * e + t >= cnt) s[nt][e] = -INFINITY;
+            for (int g = 0; g < G; g++) s[g][i] = -INFINITY;
       }
-      if (sc && r < heads) {
+      if (a.scores) {
 #pragma unroll
-        for (int nt = 0; nt < NT; nt++)
+        for (int g = 0; g < G; g++)
+          if (4 * g + t < heads) {
+            float *sc = a.scores + (at.b * a.nH + h0 + 4 * g + t) * c.cap + j0 + r;
 #pragma unroll
-          for (int e = 0; e < 2; e++)
-            if (8 * nt + 4 * e + t < cnt) sc[j0 + 8 * nt + 4 * e + t] = s[nt][e];
-      }
-#pragma unroll
-      for (int nt = 0; nt < NT; nt++) top = fmaxf(top, fmaxf(s[nt][0], s[nt][1]));
-      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
-      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-      if (__any_sync(0xffffffffu, top > m)) {
-        const float m1 = fmaxf(m, top), f = m1 > m ? ex2(m - m1) : 1.f;
-        m = m1;
-        l *= f;
-        z *= f;
-#pragma unroll
-        for (int i = 0; i < 4 * W; i++) {
-          o[i][0] *= f;
-          o[i][1] *= f;
-        }
-      }
-      // p_j step_j as fp16 pairs: the tile's steps are scaled by a power of two
-      // that brings the largest into [2^13, 2^14)
-      uint32_t big = 0;
-#pragma unroll
-      for (int i = 0; i < TP / 32; i++)
-        big = max(big, *reinterpret_cast<const uint32_t *>(vgs + 4 * (t * C::kGridStride + r + 8 * i)) << 16 & 0x7fff0000u);
-      big = __reduce_max_sync(0xffffffffu, big);
-      const int ex = max(13, (int)(big >> 23));
-      const float up = __uint_as_float((uint32_t)(267 - ex) << 23);
-      const float down = __uint_as_float((uint32_t)min(254, ex + 11) << 23);   // 2^24 / up
-      uint32_t pa[KS][4];
-      float tl = 0.f, tz = 0.f;
-#pragma unroll
-      for (int i = 0; i < NT / 2; i++) {
-        uint32_t g[4];
-        float w[4];
-        lds<4>(vgs + 4 * (t * C::kGridStride + 4 * i), g);
-#pragma unroll
-        for (int e = 0; e < 4; e++) {
-          const float p = ex2(s[2 * i + e / 2][e & 1] - m);
-          tl += p;
-          tz = fmaf(p, grid_base(g[e]), tz);
-          w[e] = p * (grid_step(g[e]) * up);
-        }
-        split(w[0], w[1], &pa[i][0], &pa[i][1]);
-        split(w[2], w[3], &pa[i][2], &pa[i][3]);
-      }
-      l += tl;
-      z += tz;
-
-      // o: column n of an n-tile is element 4 W n + 4 u + v for 16-bit unit u of
-      // lane group n's part of the row and nibble v of the unit
-      constexpr int VW = W % 2 ? W : W / 2;    // registers a row's part takes (odd W: one unit each)
-      uint32_t vw[KS][4][VW];
-      {
-        const uint8_t *vp = vs + t * C::kRow + 2 * W * r;
-#pragma unroll
-        for (int k = 0; k < KS; k++)
-#pragma unroll
-          for (int x = 0; x < 4; x++) {          // slots 16 k + 4 x + t
-            const uint8_t *row = vp + (16 * k + 4 * x) * C::kRow;
-            if constexpr (W % 2) {
-#pragma unroll
-              for (int i = 0; i < W; i++) vw[k][x][i] = *reinterpret_cast<const uint16_t *>(row + 2 * i);
-            } else {
-              lds<VW>(row, vw[k][x]);
-            }
+            for (int i = 0; i < 2 * KS; i++)
+              if (8 * i + r < cnt) sc[8 * i] = s[g][i] * qf[g];
           }
       }
+      float top[G];
+      bool grows = false;
 #pragma unroll
-      for (int u = 0; u < W; u++) {
-        float acc[4][4];
+      for (int g = 0; g < G; g++) {
+        top[g] = s[g][0];
 #pragma unroll
-        for (int v = 0; v < 4; v++) acc[v][0] = acc[v][1] = acc[v][2] = acc[v][3] = 0.f;
-        constexpr uint32_t kLow = 0x5410, kHigh = 0x7632;
-        const int wi = W % 2 ? u : u / 2;
-        const uint32_t sel = W % 2 == 0 && (u & 1) ? kHigh : kLow;
+        for (int i = 1; i < 2 * KS; i++) top[g] = fmaxf(top[g], s[g][i]);
 #pragma unroll
-        for (int k = 0; k < KS; k++) {
-          const uint32_t x = __byte_perm(vw[k][0][wi], vw[k][1][wi], sel), x8 = x >> 8;
-          const uint32_t y = __byte_perm(vw[k][2][wi], vw[k][3][wi], sel), y8 = y >> 8;
-          mma(acc[0], pa[k], x & 0x000f000fu, y & 0x000f000fu);
-          mma(acc[1], pa[k], x & 0x00f000f0u, y & 0x00f000f0u);
-          mma(acc[2], pa[k], x8 & 0x000f000fu, y8 & 0x000f000fu);
-          mma(acc[3], pa[k], x8 & 0x00f000f0u, y8 & 0x00f000f0u);
-        }
+        for (int x = 4; x < 32; x <<= 1) top[g] = fmaxf(top[g], __shfl_xor_sync(0xffffffffu, top[g], x));
+        grows |= top[g] > m[g];
+      }
+      if (__any_sync(0xffffffffu, grows)) {
 #pragma unroll
-        for (int v = 0; v < 4; v++) {
-          const float f = v & 1 ? down * 0.0625f : down;
-          o[4 * u + v][0] = fmaf(acc[v][0] + acc[v][2], f, o[4 * u + v][0]);
-          o[4 * u + v][1] = fmaf(acc[v][1] + acc[v][3], f, o[4 * u + v][1]);
+        for (int g = 0; g < G; g++) {
+          const float m1 = fmaxf(m[g], top[g]), f = m1 > m[g] ? ex2((m[g] - m1) * qf[g]) : 1.f;
+          m[g] = m1;
+          l[g] *= f;
+          z[g] *= f;
+#pragma unroll
+          for (int i = 0; i < 4 * W; i++) o[g][i] *= f;
         }
       }
-      __syncwarp();   // the stage is written again by the next issue
+      // p_j step_j as (hi, lo) pairs, transposed into the operand's columns: the
+      // tile's steps are scaled by a power of two that brings the largest into
+      // [2^13, 2^14)
+      asm volatile("cp.async.wait_group 1;");
+      __syncwarp();
+      uint32_t pb[G][KS][2];
+      float down;
+      {
+        uint32_t gr[2 * KS];
+        float big = 0.f;
+        lds<2 * KS>(vbuf + C::kCodes + 4 * r * C::kGridStride, gr);
+#pragma unroll
+        for (int i = 0; i < 2 * KS; i++) big = fmaxf(big, fabsf(grid_step(gr[i])));
+        const int ex = max(13, (int)(__reduce_max_sync(0xffffffffu, __float_as_uint(big)) >> 23));
+        const float up = __uint_as_float((uint32_t)(267 - ex) << 23);
+        down = __uint_as_float((uint32_t)min(254, ex + 11) << 23);   // 2^24 / up
+        float tl[G], tz[G];
+#pragma unroll
+        for (int g = 0; g < G; g++) tl[g] = tz[g] = 0.f;
+#pragma unroll
+        for (int i = 0; i < 2 * KS; i++) {
+          const float step = grid_step(gr[i]) * up, base = grid_base(gr[i]);
+#pragma unroll
+          for (int g = 0; g < G; g++) {
+            const float p = ex2((s[g][i] - m[g]) * qf[g]);
+            tl[g] += p;
+            tz[g] = fmaf(p, base, tz[g]);
+            pb[g][i / 2][i & 1] = transpose8(split(p * step));
+          }
+        }
+#pragma unroll
+        for (int g = 0; g < G; g++) {
+          l[g] += tl[g];
+          z[g] += tz[g];
+        }
+      }
+
+      // o: rows i and i + 8 of an m-tile are elements v and v + 1 of unit i of
+      // piece c (16 bits, four elements), at 32 c + 4 i + v
+      uint32_t vw[KS][2][W];
+#pragma unroll
+      for (int k = 0; k < KS; k++) rows16<W, true>(vbuf_s, off, k, vw[k]);
+      const float down16 = down * 0.0625f;
+#pragma unroll
+      for (int u = 0; u < W; u++) {
+        float acc[G][2][4];
+#pragma unroll
+        for (int k = 0; k < KS; k++) {
+          const uint32_t x = vw[k][0][u], x8 = x >> 8, y = vw[k][1][u], y8 = y >> 8;
+          const uint32_t a0[4] = {x & 0x000f000fu, x & 0x00f000f0u, y & 0x000f000fu, y & 0x00f000f0u};
+          const uint32_t a1[4] = {x8 & 0x000f000fu, x8 & 0x00f000f0u, y8 & 0x000f000fu, y8 & 0x00f000f0u};
+#pragma unroll
+          for (int g = 0; g < G; g++) {
+            if (k == 0) {
+              mma0(acc[g][0], a0, pb[g][0][0], pb[g][0][1]);
+              mma0(acc[g][1], a1, pb[g][0][0], pb[g][0][1]);
+            } else {
+              mma(acc[g][0], a0, pb[g][k][0], pb[g][k][1]);
+              mma(acc[g][1], a1, pb[g][k][0], pb[g][k][1]);
+            }
+          }
+        }
+#pragma unroll
+        for (int g = 0; g < G; g++)
+#pragma unroll
+          for (int x = 0; x < 2; x++) {
+            o[g][4 * u + 2 * x] = fmaf(acc[g][x][0] + acc[g][x][1], down, o[g][4 * u + 2 * x]);
+            o[g][4 * u + 2 * x + 1] = fmaf(acc[g][x][2] + acc[g][x][3], down16, o[g][4 * u + 2 * x + 1]);
+          }
+      }
+      __syncwarp();
+      issue_v(tile + kWarps);
     }
     asm volatile("cp.async.wait_group 0;");
 
     // the four warps' parts of the segment
-    l += __shfl_xor_sync(0xffffffffu, l, 1);
-    l += __shfl_xor_sync(0xffffffffu, l, 2);
-    z += __shfl_xor_sync(0xffffffffu, z, 1);
-    z += __shfl_xor_sync(0xffffffffu, z, 2);
     __syncthreads();
-    float *part = reinterpret_cast<float *>(sm);            // [kWarps][kHeads][dP + 2]
-    {
-      float *mine = part + (warp * kHeads + r) * (dP + 2);
+    float *part = reinterpret_cast<float *>(sm);            // [kWarps][kHeads][dP + 4]: o, m, l
 #pragma unroll
-      for (int u = 0; u < W; u++)
+    for (int g = 0; g < G; g++) {
 #pragma unroll
-        for (int v = 0; v < 4; v++)
-#pragma unroll
-          for (int e = 0; e < 2; e++) mine[4 * W * (2 * t + e) + 4 * u + v] = o[4 * u + v][e] + z;
-      if (t == 0) {
-        mine[dP] = m;
-        mine[dP + 1] = l;
+      for (int x = 4; x < 32; x <<= 1) {
+        l[g] += __shfl_xor_sync(0xffffffffu, l[g], x);
+        z[g] += __shfl_xor_sync(0xffffffffu, z[g], x);
       }
+      float *mine = part + (warp * C::kHeads + 4 * g + t) * (dP + 4);
+#pragma unroll
+      for (int i = 0; i < W; i++)
+        *reinterpret_cast<float4 *>(mine + 32 * i + 4 * r) =
+            make_float4(o[g][4 * i] + z[g], o[g][4 * i + 1] + z[g], o[g][4 * i + 2] + z[g], o[g][4 * i + 3] + z[g]);
+      if (r == 0) *reinterpret_cast<float2 *>(mine + dP) = make_float2(m[g] * qf[g], l[g]);   // log2 units from here on
     }
     __syncthreads();
     const bool whole = t0 == 0 && t1 == at.tiles;
-    for (int i = threadIdx.x; i < heads * c.dH; i += kThreads) {
-      const int hd = i / c.dH, e = i - hd * c.dH;
-      const float *x = part + hd * (dP + 2);
-      float M = -INFINITY, L = 0.f, O = 0.f;
-#pragma unroll
-      for (int w = 0; w < kWarps; w++) M = fmaxf(M, x[w * kHeads * (dP + 2) + dP]);
+    const int64_t bh0 = at.b * a.nH + h0;
+    if (t0 == 0 && !whole)
+      cut = Cut{1 + (int)((at.tiles - t1 + plan.per - 1) / plan.per), heads, bh0};
+    if (a.ml && t0 == 0 && !whole && threadIdx.x < heads)
+      a.ml[bh0 + threadIdx.x] = make_float2(__int_as_float(blockIdx.x), -(float)cut.pieces);
+    for (int i = threadIdx.x; i < heads * (dP / 4); i += kThreads) {
+      const int hd = i / (dP / 4), e = 4 * (i - hd * (dP / 4));
+      const float *x = part + hd * (dP + 4);
+      float M = -INFINITY, L = 0.f;
+      float4 O = {0.f, 0.f, 0.f, 0.f};
+      float2 ml[kWarps];
 #pragma unroll
       for (int w = 0; w < kWarps; w++) {
-        const float *y = x + w * kHeads * (dP + 2);
-        const float f = y[dP + 1] == 0.f ? 0.f : ex2(y[dP] - M);     // a warp without tiles has l = 0
-        L += y[dP + 1] * f;
-        O = fmaf(y[e], f, O);
+        ml[w] = *reinterpret_cast<const float2 *>(x + w * C::kHeads * (dP + 4) + dP);
+        if (ml[w].y != 0.f) M = fmaxf(M, ml[w].x);       // a warp without tiles has l = 0
       }
-      const int64_t bh = at.b * a.nH + h0 + hd;
+#pragma unroll
+      for (int w = 0; w < kWarps; w++) {
+        const float4 y = *reinterpret_cast<const float4 *>(x + w * C::kHeads * (dP + 4) + e);
+        const float f = ml[w].y == 0.f ? 0.f : ex2(ml[w].x - M);
+        L += ml[w].y * f;
+        O.x = fmaf(y.x, f, O.x), O.y = fmaf(y.y, f, O.y), O.z = fmaf(y.z, f, O.z), O.w = fmaf(y.w, f, O.w);
+      }
+      float *dst;
       if (whole) {
-        a.out[bh * c.dH + e] = O / L;
-        if (a.ml && e == 0) a.ml[bh] = make_float2(M, L);
+        const float inv = 1.f / L;
+        O.x *= inv, O.y *= inv, O.z *= inv, O.w *= inv;
+        dst = a.out + (bh0 + hd) * c.dH;
+        if (a.ml && e == 0) a.ml[bh0 + hd] = make_float2(M, L);
       } else {
-        float *dst = a.part + ((int64_t)(2 * blockIdx.x + (t0 == 0)) * kHeads + hd) * (c.dH + 2);
-        dst[e] = O;
-        if (e == 0) {
-          dst[c.dH] = M;
-          dst[c.dH + 1] = L;
-        }
+        dst = a.part + ((int64_t)(2 * blockIdx.x + (t0 == 0)) * kMaxHeads + hd) * (c.dH + 2);
+        if (e == 0) dst[c.dH] = M, dst[c.dH + 1] = L;
       }
+      if (e < c.dH) *reinterpret_cast<float2 *>(dst + e) = make_float2(O.x, O.y);            // dH is even
+      if (e + 2 < c.dH) *reinterpret_cast<float2 *>(dst + e + 2) = make_float2(O.z, O.w);
     }
     __syncthreads();
     u += t1 - t0;
@@ -566,75 +674,134 @@ __global__ void __launch_bounds__(kThreads, Cfg<W>::kCtas) kv4_attn_kernel(AttnA
       __syncthreads();
     }
   }
+  if (threadIdx.x == 0) a.cuts[blockIdx.x] = cut;
 }
 
-// Merges the pieces of the segments that run borders cut: block i looks at the
-// border before run i and takes the segment if it is the first border inside it.
-template <int TILE>
-__global__ void __launch_bounds__(kThreads) kv4_attn_merge_kernel(AttnArgs a) {
-  pdl_trigger();
-  __shared__ int64_t sh[kThreads];
-  const Cache &c = a.c;
-  pdl_wait();
-  const Plan plan = make_plan<TILE>(a, sh);
-  const int64_t i = blockIdx.x + 1, u = i * plan.per;
-  if (u >= plan.total) return;
-  const Place at = find<TILE>(a, u, sh);
-  if (at.b < 0 || at.tile == 0 || at.tile > plan.per) return;
-  const int h = at.seg / a.hg, h0 = h * a.g + (at.seg % a.hg) * a.gs, hd = blockIdx.y;
-  if (hd >= min(a.gs, (h + 1) * a.g - h0)) return;
-  const int64_t stride = (int64_t)kHeads * (c.dH + 2);
-  const int64_t last = u - at.tile + at.tiles;                       // the segment's end
-  const int pieces = 1 + (int)((last - u + plan.per - 1) / plan.per);
-  // run i - 1 holds the beginning (slot 1), runs i, i + 1, ... the rest (slot 0)
-  const float *base = a.part + hd * (c.dH + 2) + 2 * i * stride;
-  auto piece = [&](int p) { return p == 0 ? base - stride : base + 2 * (p - 1) * stride; };
-  float M = -INFINITY, L = 0.f;
-  const int lane = threadIdx.x & 31;
-  for (int p = lane; p < pieces; p += 32) M = fmaxf(M, piece(p)[c.dH]);
-  M = warp_max(M);
-  for (int p = lane; p < pieces; p += 32) L += piece(p)[c.dH + 1] * ex2(piece(p)[c.dH] - M);
-  L = warp_sum(L);
-  const int64_t bh = at.b * a.nH + h0 + hd;
-  for (int e = threadIdx.x; e < c.dH; e += kThreads) {
-    float O = 0.f;
-#pragma unroll 4
-    for (int p = 0; p < pieces; p++) O = fmaf(piece(p)[e], ex2(piece(p)[c.dH] - M), O);
-    a.out[bh * c.dH + e] = O / L;
+// The (m, l) of a head whose segment begins in run `run` and has `pieces`
+// pieces: run `run` holds the first (slot 1), runs run + 1, ... the rest (slot
+// 0).  By a warp.
+struct Pieces {
+  const float *first;
+  int64_t stride;
+  __device__ Pieces(const AttnArgs &a, int run, int hd) {
+    stride = (int64_t)kMaxHeads * (a.c.dH + 2);
+    first = a.part + (2 * (int64_t)run + 1) * stride + hd * (a.c.dH + 2);
   }
-  if (a.ml && threadIdx.x == 0) a.ml[bh] = make_float2(M, L);
-}
+  __device__ const float *operator[](int p) const { return first + (p == 0 ? 0 : 2 * p - 1) * stride; }
+  __device__ float2 ml(int pieces, int dH) const {
+    const int lane = threadIdx.x & 31;
+    float M = -INFINITY, L = 0.f;
+    for (int p = lane; p < pieces; p += 32) {
+      const float m = (*this)[p][dH], l = (*this)[p][dH + 1];
+      const float m1 = fmaxf(M, m);
+      L = (L == 0.f ? 0.f : L * ex2(M - m1)) + l * ex2(m - m1);
+      M = m1;
+    }
+    const float top = warp_max(M);
+    return make_float2(top, warp_sum(L == 0.f ? 0.f : L * ex2(M - top)));
+  }
+};
 
-// weight_j += sum over the group's q heads of p_j.
-constexpr int kWtThreads = 256;
-__global__ void __launch_bounds__(kWtThreads) kv4_attn_weights_kernel(AttnArgs a) {
+// What is left when all runs are done.  The first (ctas - 1) gs blocks merge
+// the pieces of the segment that begins in run blockIdx.x / gs and goes past its
+// end, one head each; where weights are kept the others add them up,
+// weight_j += sum over the group's q heads of p_j, kWtSlots slots each.
+constexpr int kFinishThreads = 256;
+constexpr int kFinishWarps = kFinishThreads / 32;
+constexpr int kWtSlots = 1024;
+template <int W>
+__global__ void __launch_bounds__(kFinishThreads) kv4_attn_finish_kernel(AttnArgs a) {
   pdl_trigger();
-  const Cache &c = a.c;
-  const int h = blockIdx.y, b = blockIdx.z;
+  __shared__ float o_s[kFinishWarps][32 * W];
   __shared__ float m_s[kMaxGroup], il_s[kMaxGroup];
+  const Cache &c = a.c;
+  const int dH = c.dH, lane = threadIdx.x & 31, warp = threadIdx.x >> 5, merges = (a.ctas - 1) * a.gs;
   pdl_wait();
-  const int64_t n = length(a, b), j = (int64_t)blockIdx.x * kWtThreads + threadIdx.x;
-  if ((int64_t)blockIdx.x * kWtThreads >= n) return;
-  if (threadIdx.x < a.g) {
-    const float2 x = a.ml[(int64_t)b * a.nH + h * a.g + threadIdx.x];
-    m_s[threadIdx.x] = x.x;
-    il_s[threadIdx.x] = 1.f / x.y;
+  if (blockIdx.x < merges) {
+    const int run = blockIdx.x / a.gs, hd = blockIdx.x - run * a.gs;
+    const Cut cut = a.cuts[run];
+    if (cut.pieces == 0 || hd >= cut.heads) return;
+    const int pieces = min(cut.pieces, a.ctas - run);
+    const Pieces part(a, run, hd);
+    // each warp its share of the pieces; everything of a piece is asked for at once
+    float M = -INFINITY, L = 0.f, O[W];
+#pragma unroll
+    for (int i = 0; i < W; i++) O[i] = 0.f;
+#pragma unroll(W <= 2 ? 8 : W <= 4 ? 4 : 2)
+    for (int p = warp; p < pieces; p += kFinishWarps) {
+      const float *x = part[p];
+      const float m = x[dH], l = x[dH + 1];
+      float o[W];
+#pragma unroll
+      for (int i = 0; i < W; i++) o[i] = lane + 32 * i < dH ? x[lane + 32 * i] : 0.f;
+      const float m1 = fmaxf(M, m), f0 = L == 0.f ? 0.f : ex2(M - m1), f1 = ex2(m - m1);
+      L = L * f0 + l * f1;
+      M = m1;
+#pragma unroll
+      for (int i = 0; i < W; i++) O[i] = O[i] * f0 + o[i] * f1;
+    }
+    if (lane == 0) {
+      m_s[warp] = M;
+      il_s[warp] = L;
+    }
+#pragma unroll
+    for (int i = 0; i < W; i++)
+      if (lane + 32 * i < dH) o_s[warp][lane + 32 * i] = O[i];
+    __syncthreads();
+    const int warps = min(pieces, kFinishWarps);
+    M = m_s[0];
+    for (int w = 1; w < warps; w++) M = fmaxf(M, m_s[w]);
+    L = 0.f;
+    for (int w = 0; w < warps; w++) L += il_s[w] * ex2(m_s[w] - M);
+    for (int e = threadIdx.x; e < dH; e += kFinishThreads) {
+      float o = 0.f;
+      for (int w = 0; w < warps; w++) o = fmaf(o_s[w][e], ex2(m_s[w] - M), o);
+      a.out[(cut.bh + hd) * dH + e] = o / L;
+    }
+    return;
+  }
+  const int64_t i = blockIdx.x - merges, chunks = (c.cap + kWtSlots - 1) / kWtSlots;
+  const int64_t bk = i / chunks, j0 = (i - bk * chunks) * kWtSlots, b = bk / c.nKV;
+  const int h = (int)(bk - b * c.nKV);
+  const int64_t n = length(a, b);
+  if (j0 >= n) return;
+  for (int hd = warp; hd < a.g; hd += kFinishWarps) {
+    float2 x = a.ml[b * a.nH + h * a.g + hd];
+    // a cut segment's: the run it begins in, and minus its pieces
+    if (x.y < 0.f) {
+      const int run = __float_as_int(x.x), pieces = min((int)-x.y, a.ctas - run);
+      x = Pieces(a, run, hd % a.gs).ml(pieces, dH);
+    }
+    if (lane == 0) {
+      m_s[hd] = x.x;
+      il_s[hd] = 1.f / x.y;
+    }
   }
   __syncthreads();
-  if (j >= n) return;
-  const int64_t row = row_of(c, b, h, j);
-  if (row < 0) return;
-  const float *sc = a.scores + ((int64_t)b * a.nH + h * a.g) * c.cap + j;
-  float w = 0.f;
-  for (int i = 0; i < a.g; i++) w = fmaf(ex2(sc[i * c.cap] - m_s[i]), il_s[i], w);
-  c.weight[row] += w;
+  const float *sc = a.scores + (b * a.nH + h * a.g) * c.cap;
+  float w[kWtSlots / kFinishThreads], old[kWtSlots / kFinishThreads];
+  int64_t row[kWtSlots / kFinishThreads];
+#pragma unroll
+  for (int x = 0; x < kWtSlots / kFinishThreads; x++) {
+    const int64_t j = j0 + threadIdx.x + x * kFinishThreads;
+    row[x] = j < n ? row_of(c, b, h, j) : -1;
+    old[x] = row[x] >= 0 ? c.weight[row[x]] : 0.f;
+    w[x] = 0.f;
+  }
+  for (int hd = 0; hd < a.g; hd++)
+#pragma unroll
+    for (int x = 0; x < kWtSlots / kFinishThreads; x++)
+      if (row[x] >= 0) w[x] = fmaf(ex2(sc[hd * c.cap + j0 + threadIdx.x + x * kFinishThreads] - m_s[hd]), il_s[hd], w[x]);
+#pragma unroll
+  for (int x = 0; x < kWtSlots / kFinishThreads; x++)
+    if (row[x] >= 0) c.weight[row[x]] = old[x] + w[x];
 }
 
-// Floats of workspace: the pieces and, where weights are kept, (m, l) and the
-// scores.
-int64_t part_floats(const Cache &c, int ctas) { return (int64_t)ctas * 2 * kHeads * (c.dH + 2); }
+// Floats of workspace: the cuts, the pieces and, where weights are kept, (m, l)
+// and the scores.
+int64_t part_floats(const Cache &c, int ctas) { return (int64_t)ctas * 2 * kMaxHeads * (c.dH + 2); }
 int64_t work_floats(const Cache &c, int B, int nH, int ctas) {
-  return part_floats(c, ctas) + (c.weight ? (int64_t)B * nH * (c.cap + 2) : 0);
+  return (int64_t)ctas * (sizeof(Cut) / 4) + part_floats(c, ctas) + (c.weight ? (int64_t)B * nH * (c.cap + 2) : 0);
 }
 
 int checked(const char *who, const fcu_kv4 *cache, int B, int nH, bool arrays, Cache *c) {
@@ -647,39 +814,65 @@ int checked(const char *who, const fcu_kv4 *cache, int B, int nH, bool arrays, C
 
 // CTAs of the main kernel: all that are resident, or one per tile if the cache
 // cannot hold that many.
-template <int W>
+template <int W, int G>
 int plan_ctas(const fcu_ctx *ctx, const Cache &c, int B, int hg) {
-  const int64_t tiles = (int64_t)B * c.nKV * hg * ((c.cap + Cfg<W>::kTile - 1) / Cfg<W>::kTile);
-  const int64_t all = (int64_t)ctx->num_sms * Cfg<W>::kCtas;
+  using C = Cfg<W, G>;
+  const int64_t tiles = (int64_t)B * c.nKV * hg * ((c.cap + C::kTile - 1) / C::kTile);
+  const int64_t all = (int64_t)ctx->num_sms * C::kCtas;
   return (int)(tiles < all ? tiles : all);
 }
 
-int plan_ctas(const fcu_ctx *ctx, const Cache &c, int B, int hg) {
-  switch (c.rb / 16) {
-    case 1: return plan_ctas<1>(ctx, c, B, hg);
-    case 2: return plan_ctas<2>(ctx, c, B, hg);
-    case 3: return plan_ctas<3>(ctx, c, B, hg);
-    case 4: return plan_ctas<4>(ctx, c, B, hg);
-    case 6: return plan_ctas<6>(ctx, c, B, hg);
-    default: return plan_ctas<8>(ctx, c, B, hg);
-  }
-}
-
-template <int W>
+template <int W, int G>
 int launch(fcu_ctx *ctx, const AttnArgs &a) {
-  using C = Cfg<W>;
+  using C = Cfg<W, G>;
   static bool set[64] = {false};
   if (!set[ctx->device & 63]) {
-    FCU_CHECK_CUDA(cudaFuncSetAttribute(kv4_attn_kernel<W>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem));
+    FCU_CHECK_CUDA(cudaFuncSetAttribute(kv4_attn_kernel<W, G>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem));
     set[ctx->device & 63] = true;
   }
-  FCU_CHECK_CUDA(launch_pdl(kv4_attn_kernel<W>, dim3(a.ctas), dim3(kThreads), C::kSmem, ctx->stream, a));
+  FCU_CHECK_CUDA(launch_pdl(kv4_attn_kernel<W, G>, dim3(a.ctas), dim3(kThreads), C::kSmem, ctx->stream, a));
   note_launch();
-  if (a.ctas > 1) {
-    FCU_CHECK_CUDA(launch_pdl(kv4_attn_merge_kernel<C::kTile>, dim3(a.ctas - 1, a.gs), dim3(kThreads), 0, ctx->stream, a));
+  const int64_t blocks = (int64_t)(a.ctas - 1) * a.gs +
+                         (a.scores ? (int64_t)a.B * a.c.nKV * ((a.c.cap + kWtSlots - 1) / kWtSlots) : 0);
+  if (blocks > 0) {
+    FCU_CHECK_CUDA(launch_pdl(kv4_attn_finish_kernel<W>, dim3((unsigned)blocks), dim3(kFinishThreads), 0, ctx->stream, a));
     note_launch();
   }
   return FCU_OK;
+}
+
+// f(W, G) for a cache's row width and a segment's heads
+#define FCU_KV4_WIDTHS(f, rb, gs)                                      \
+  switch ((rb) / 16 * 2 + ((gs) > 4)) {                                \
+    case 2: f(1, 1); break;                                            \
+    case 3: f(1, 2); break;                                            \
+    case 4: f(2, 1); break;                                            \
+    case 5: f(2, 2); break;                                            \
+    case 6: f(3, 1); break;                                            \
+    case 7: f(3, 2); break;                                            \
+    case 8: f(4, 1); break;                                            \
+    case 9: f(4, 2); break;                                            \
+    case 12: f(6, 1); break;                                           \
+    case 13: f(6, 2); break;                                           \
+    case 16: f(8, 1); break;                                           \
+    default: f(8, 2); break;                                           \
+  }
+
+// How the heads are dealt: q heads per kv head, segments per kv head (a CTA
+// takes at most 8 heads), q heads of a segment, and the CTAs.
+struct Heads {
+  int g, hg, gs, ctas;
+};
+Heads plan_heads(const fcu_ctx *ctx, const Cache &c, int B, int nH) {
+  Heads p;
+  p.g = nH / c.nKV;
+  p.hg = p.g > kMaxHeads ? 2 : 1;
+  p.gs = (p.g + p.hg - 1) / p.hg;
+  p.ctas = 0;
+#define FCU_CASE(W, G) p.ctas = plan_ctas<W, G>(ctx, c, B, p.hg)
+  FCU_KV4_WIDTHS(FCU_CASE, c.rb, p.gs)
+#undef FCU_CASE
+  return p;
 }
 
 }  // namespace
@@ -694,8 +887,7 @@ extern "C" {
 int64_t fcu_kv4_attn_work(fcu_ctx *ctx, const fcu_kv4 *cache, int B, int nH) {
   Cache c;
   if (!ctx || checked("fcu_kv4_attn_work", cache, B, nH, false, &c)) return -1;
-  const int g = nH / c.nKV;
-  return 4 * work_floats(c, B, nH, plan_ctas(ctx, c, B, g > kHeads ? 2 : 1));
+  return 4 * work_floats(c, B, nH, plan_heads(ctx, c, B, nH).ctas);
 }
 
 int fcu_kv4_attn(fcu_ctx *ctx, const float *q, int64_t ld_q, const fcu_kv4 *cache, const int32_t *seq_lens, int B,
@@ -707,39 +899,34 @@ int fcu_kv4_attn(fcu_ctx *ctx, const float *q, int64_t ld_q, const fcu_kv4 *cach
   FCU_REQUIRE(ld_q >= (int64_t)nH * a.c.dH, "fcu_kv4_attn: q row stride %lld too small", (long long)ld_q);
   if (B == 0) return FCU_OK;
   FCU_REQUIRE(q && seq_lens && out, "fcu_kv4_attn: null pointer");
+  FCU_REQUIRE(((uintptr_t)out & 7) == 0, "fcu_kv4_attn: out is not 8-byte aligned");
   a.q = q;
   a.ld_q = ld_q;
   a.lens = seq_lens;
   a.B = B;
   a.nH = nH;
-  a.g = nH / a.c.nKV;
-  a.hg = a.g > kHeads ? 2 : 1;
-  a.gs = (a.g + a.hg - 1) / a.hg;
-  a.ctas = plan_ctas(ctx, a.c, B, a.hg);
+  const Heads p = plan_heads(ctx, a.c, B, nH);
+  a.g = p.g;
+  a.hg = p.hg;
+  a.gs = p.gs;
+  a.ctas = p.ctas;
+  a.vec = ld_q % 4 == 0 && a.c.dH % 4 == 0 && ((uintptr_t)q & 15) == 0;
   a.scale = (float)scale;
   a.out = out;
+  FCU_REQUIRE(!a.c.weight || (double)B * a.c.nKV * (a.c.cap / kWtSlots + 1) < 1e9, "fcu_kv4_attn: the cache is too large");
   const int64_t need = 4 * work_floats(a.c, B, nH, a.ctas);
   FCU_REQUIRE(work && work_bytes >= need && ((uintptr_t)work & 15) == 0,
               "fcu_kv4_attn: workspace of %lld bytes, %lld needed", (long long)work_bytes, (long long)need);
-  a.part = (float *)work;
+  a.cuts = (Cut *)work;
+  a.part = (float *)(a.cuts + a.ctas);
   if (a.c.weight) {
     a.ml = (float2 *)(a.part + part_floats(a.c, a.ctas));
     a.scores = (float *)(a.ml + (int64_t)B * nH);
   }
-  switch (a.c.rb / 16) {
-    case 1: rc = launch<1>(ctx, a); break;
-    case 2: rc = launch<2>(ctx, a); break;
-    case 3: rc = launch<3>(ctx, a); break;
-    case 4: rc = launch<4>(ctx, a); break;
-    case 6: rc = launch<6>(ctx, a); break;
-    default: rc = launch<8>(ctx, a); break;
-  }
+#define FCU_CASE(W, G) rc = launch<W, G>(ctx, a)
+  FCU_KV4_WIDTHS(FCU_CASE, a.c.rb, a.gs)
+#undef FCU_CASE
   if (rc) return rc;
-  if (a.scores) {
-    FCU_CHECK_CUDA(launch_pdl(kv4_attn_weights_kernel, dim3(div_up(a.c.cap, kWtThreads), a.c.nKV, B), dim3(kWtThreads),
-                              0, ctx->stream, a));
-    note_launch();
-  }
   return FCU_OK;
 }
 
