@@ -8,28 +8,36 @@ namespace fcu {
 namespace {
 
 // ------------------------------------------------------------------ selection
-// Two kernels.  beam_rows reads every logit once: a CTA takes one slice of one
-// row, keeps the slice's running maximum and sum of exponentials and its W
-// best (logit, token) pairs.  beam_merge, one CTA per sequence, turns the
-// slices' sums into each row's log-sum-exp and picks the W best of the
-// W x slices x W survivors.  Within a row the order of the candidates is the
-// order of the logits, so W per slice are enough.  The bound is reading the
-// logits (HBM).
+// Two kernels.  beam_rows reads every logit once: a warp walks 512 logits at a
+// time of one slice of one row, with a running maximum and sum of exponentials
+// per lane, and keeps the W best (logit, token) pairs it has met, one per lane,
+// sorted.  After its first tile a logit is only looked at again if it beats the
+// W-th best, about W ln(n / 512) times for n logits in no particular order.
+// beam_merge, one CTA per sequence, turns the slices' sums into each row's
+// log-sum-exp and picks the W best of the W rows' W best.  Within a row the
+// candidates order as the logits do, so W per slice are enough.  The bound is
+// reading the logits (HBM).
 constexpr int kBeamThreads = 256;
+constexpr int kBeamWarps = kBeamThreads / 32;
 constexpr int kMaxW = 32;
-constexpr int kPer = 16;                            // logits a thread holds at a time
-constexpr int kTile = kBeamThreads * kPer;
+constexpr int kTile = 512;                          // logits a warp takes at a time
 constexpr int kMaxSlices = 64;
+constexpr float kLog2e = 1.4426950408889634f;
 
 using Key = unsigned long long;
 
-// Larger logit, larger key; equal logits (0 and -0 too), lower token first.
-// NaN is below -inf; 0 is below every key.
+// Larger logit, larger key; equal logits (0 and -0 too), lower token first.  0
+// is below every key.
+__device__ __forceinline__ uint32_t order_bits(float x) {
+  const uint32_t u = __float_as_uint(x + 0.0f);
+  return u & 0x80000000u ? ~u : u | 0x80000000u;
+}
 __device__ __forceinline__ Key beam_key(float x, uint32_t token) {
-  uint32_t u = __float_as_uint(x + 0.0f);
-  u = u & 0x80000000u ? ~u : u | 0x80000000u;
-  if (x != x) u = 1;
-  return (Key)u << 32 | (0xffffffffu - token);
+  return (Key)order_bits(x) << 32 | (0xffffffffu - token);
+}
+__device__ __forceinline__ float key_logit(Key k) {
+  const uint32_t u = (uint32_t)(k >> 32);
+  return __uint_as_float(u & 0x80000000u ? u & 0x7fffffffu : ~u);
 }
 
 struct BeamArgs {
@@ -37,215 +45,231 @@ struct BeamArgs {
   int64_t ld;
   const float *scores;
   const uint8_t *done;
-  int64_t V;
-  int B, W, eos, slices;
-  int64_t slice;         // logits per slice
-  float2 *sums;          // [rows][slices] maximum, sum of exp(x - maximum)
+  int V, B, W, eos, slices;
+  int slice;             // logits per slice
+  float2 *sums;          // [rows][slices]: M, the maximum times kLog2e, and sum of 2^(x kLog2e - M)
   Key *best;             // [rows][slices][W]
   float *out_scores;
   int32_t *tokens, *parents;
   uint8_t *out_done;
 };
 
+__device__ __forceinline__ float beam_ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+// Four logits from p on, those of tokens in [v0, v1) (v: the first one's); the others -inf.
+__device__ __forceinline__ float4 load4(const float *p, int v, int v0, int v1) {
+  if (v >= v0 && v + 4 <= v1) return __ldcs(reinterpret_cast<const float4 *>(p));
+  float4 f = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+  if (v >= v0 && v < v1) f.x = p[0];
+  if (v + 1 >= v0 && v + 1 < v1) f.y = p[1];
+  if (v + 2 >= v0 && v + 2 < v1) f.z = p[2];
+  if (v + 3 >= v0 && v + 3 < v1) f.w = p[3];
+  return f;
+}
+
 __global__ void __launch_bounds__(kBeamThreads) beam_rows_kernel(BeamArgs a) {
   pdl_trigger();
-  __shared__ Key tops[kBeamThreads];
-  __shared__ Key pool[kMaxW * (kPer + 1)];   // the W best so far, then a tile's newcomers
-  __shared__ Key sorted[kMaxW];
-  __shared__ int count;
-  __shared__ float red_m[kBeamThreads / 32], red_s[kBeamThreads / 32];
-  const int tid = threadIdx.x, W = a.W;
+  __shared__ Key lists[kBeamWarps * kMaxW];
+  __shared__ float red_m[kBeamWarps], red_s[kBeamWarps];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, W = a.W;
   const int64_t row = blockIdx.y;
-  const int64_t v0 = (int64_t)blockIdx.x * a.slice, v1 = min(a.V, v0 + a.slice);
-  if (tid < W) sorted[tid] = 0;
+  const int v0 = blockIdx.x * a.slice, v1 = (int)min((int64_t)a.V, (int64_t)v0 + a.slice);
   pdl_wait();
   const float *x = a.logits + row * a.ld;
-  float m = -INFINITY, s = 0.f;
-  bool nan = false;
-  Key bar = 0;                               // the W-th best so far
-  __syncthreads();
-  for (int64_t t0 = v0; t0 < v1; t0 += kTile) {
-    float f[kPer];
-    Key top = 0;
+  // tiles start where a 16-byte line does: at most three tokens before v0
+  const int skew = (int)(((uintptr_t)(x + v0) >> 2) & 3);
+  float M = -INFINITY, s = 0.f;              // this lane's
+  Key key = 0;                               // this lane's place in the warp's list
+  float bar = -INFINITY;                     // its last entry's logit
+  bool full = false;
+  int64_t t0 = (int64_t)v0 - skew + warp * kTile;
+  float4 next[4];
 #pragma unroll
-    for (int i = 0; i < kPer; i++) {
-      const int64_t v = t0 + i * kBeamThreads + tid;
-      f[i] = v < v1 ? x[v] : -INFINITY;
-    }
-    float tm = m;
+  for (int i = 0; i < 4; i++) {
+    const int64_t v = t0 + 128 * i + 4 * lane;
+    next[i] = v < v1 ? load4(x + v, (int)v, v0, v1) : float4{-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+  }
+  for (; t0 < v1; t0 += kTile * kBeamWarps) {
+    float f[16];
 #pragma unroll
-    for (int i = 0; i < kPer; i++) {
-      const int64_t v = t0 + i * kBeamThreads + tid;
-      nan |= f[i] != f[i];
-      tm = fmaxf(tm, f[i]);
-      if (v < v1) {
-        const Key k = beam_key(f[i], (uint32_t)v);
-        top = k > top ? k : top;
-      }
+    for (int i = 0; i < 4; i++) {
+      f[4 * i] = next[i].x, f[4 * i + 1] = next[i].y, f[4 * i + 2] = next[i].z, f[4 * i + 3] = next[i].w;
+      const int64_t v = t0 + kTile * kBeamWarps + 128 * i + 4 * lane;
+      next[i] = v < v1 ? load4(x + v, (int)v, v0, v1) : float4{-INFINITY, -INFINITY, -INFINITY, -INFINITY};
     }
-    if (tm > -INFINITY) {
-      s *= expf(m - tm);
+    float top = f[0];
+#pragma unroll
+    for (int i = 1; i < 16; i++) top = fmaxf(top, f[i]);
+    const float M1 = fmaxf(M, top * kLog2e);
+    if (M1 > -INFINITY) {
       float ts = 0.f;
 #pragma unroll
-      for (int i = 0; i < kPer; i++) ts += expf(f[i] - tm);
-      s += ts;
-      m = tm;
+      for (int i = 0; i < 16; i++) ts += beam_ex2(fmaf(f[i], kLog2e, -M1));
+      s = s * beam_ex2(M - M1) + ts;
+      M = M1;
     }
-    if (!__syncthreads_or(top > bar)) continue;
-    // Of the threads' best keys the W largest bound the tile's W best from
-    // below, and only their threads can hold one of those.
-    tops[tid] = top;
-    if (tid == 0) count = W;
-    if (tid < W) pool[tid] = sorted[tid];
-    __syncthreads();
-    if (top > bar) {
-      int above = 0;
-      for (int i = 0; i < kBeamThreads; i++) above += tops[i] > top;
-      if (above < W)
+    // Earlier tiles hold lower tokens, so only a larger logit displaces one of theirs.
+    uint32_t hit = __ballot_sync(0xffffffffu, top > bar || !full);
+    if (hit == 0) continue;
+    float least = bar;
+    if (__popc(hit) > W) {
+      // no logit below the W-th largest of the lanes' maxima is among the W best
+      uint32_t mine = order_bits(top), w_th = 0;
+      for (int i = 0; i < W && (i == 0 || w_th); i++) {
+        w_th = __reduce_max_sync(0xffffffffu, mine);
+        if (mine == w_th) mine = 0;
+      }
+      if (w_th) least = fmaxf(least, __uint_as_float(w_th & 0x80000000u ? w_th & 0x7fffffffu : ~w_th));
+    }
 #pragma unroll
-        for (int i = 0; i < kPer; i++) {
-          const int64_t v = t0 + i * kBeamThreads + tid;
-          if (v < v1) {
-            const Key k = beam_key(f[i], (uint32_t)v);
-            if (k > bar) pool[atomicAdd(&count, 1)] = k;
-          }
-        }
+    for (int i = 0; i < 16; i++) {
+      uint32_t who = __ballot_sync(0xffffffffu, f[i] >= least);
+      while (who) {
+        const int from = __ffs(who) - 1;
+        who &= who - 1;
+        const int64_t v = t0 + 128 * (i / 4) + 4 * from + i % 4;
+        if (v < v0 || v >= v1) continue;
+        const Key k = beam_key(__shfl_sync(0xffffffffu, f[i], from), (uint32_t)v);
+        const int at = __popc(__ballot_sync(0xffffffffu, key > k));
+        if (at >= W) continue;
+        const Key up = __shfl_up_sync(0xffffffffu, key, 1);
+        if (lane == at) key = k;
+        else if (lane > at) key = lane < W ? up : 0;
+      }
     }
-    __syncthreads();
-    const int n = count;
-    for (int i = tid; i < n; i += kBeamThreads) {
-      const Key k = pool[i];
-      int above = 0;
-      for (int j = 0; j < n; j++) above += pool[j] > k;
-      if (above < W && k) sorted[above] = k;
-    }
-    __syncthreads();
-    bar = sorted[W - 1];
+    const Key last = __shfl_sync(0xffffffffu, key, W - 1);
+    full = last != 0;
+    if (full) bar = key_logit(last);
   }
   // the slice's maximum and sum: lanes, then warps, in a fixed order
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) {
-    const float om = __shfl_xor_sync(0xffffffffu, m, o), os = __shfl_xor_sync(0xffffffffu, s, o);
-    const float M = fmaxf(m, om);
-    s = M > -INFINITY ? s * expf(m - M) + os * expf(om - M) : 0.f;
-    m = M;
+    const float oM = __shfl_xor_sync(0xffffffffu, M, o), os = __shfl_xor_sync(0xffffffffu, s, o);
+    const float M1 = fmaxf(M, oM);
+    if (M1 > -INFINITY) s = s * beam_ex2(M - M1) + os * beam_ex2(oM - M1);
+    M = M1;
   }
-  nan = __syncthreads_or(nan);
-  if ((tid & 31) == 0) red_m[tid >> 5] = m, red_s[tid >> 5] = s;
+  if (lane == 0) red_m[warp] = M, red_s[warp] = s;
+  if (lane < W) lists[warp * W + lane] = key;
   __syncthreads();
   const int64_t at = row * a.slices + blockIdx.x;
-  if (tid == 0) {
-    float M = -INFINITY, S = 0.f;
-    for (int w = 0; w < kBeamThreads / 32; w++) M = fmaxf(M, red_m[w]);
-    for (int w = 0; w < kBeamThreads / 32; w++) S += M > -INFINITY ? red_s[w] * expf(red_m[w] - M) : 0.f;
-    a.sums[at] = make_float2(M, nan ? NAN : S);
+  if (threadIdx.x == 0) {
+    float M1 = -INFINITY, S = 0.f;
+    for (int w = 0; w < kBeamWarps; w++) M1 = fmaxf(M1, red_m[w]);
+    if (M1 > -INFINITY)
+      for (int w = 0; w < kBeamWarps; w++) S += red_s[w] * beam_ex2(red_m[w] - M1);
+    a.sums[at] = make_float2(M1, S);
   }
-  if (tid < W) a.best[at * W + tid] = sorted[tid];
+  // the warps' lists are sorted and share no key: one's rank is its own place
+  // plus what every other list has above it
+  if (threadIdx.x < W) a.best[at * W + threadIdx.x] = 0;
+  __syncthreads();
+  for (int i = threadIdx.x; i < kBeamWarps * W; i += kBeamThreads) {
+    const Key k = lists[i];
+    int rank = i % W;
+    for (int w = 0; w < kBeamWarps && rank < W; w++)
+      if (w != i / W)
+        for (int j = 0; j < W && lists[w * W + j] > k; j++) rank++;
+    if (k && rank < W) a.best[at * W + rank] = k;
+  }
 }
 
-// A candidate of the merge: score, then lowest w * V + token.
-struct Cand {
-  double score;
-  int64_t flat;
-};
-__device__ __forceinline__ bool beats(const Cand &x, const Cand &y) {
-  return x.score > y.score || (x.score == y.score && x.flat < y.flat);
-}
-
+// rank of (score, flat) among the W rows' sorted lists: those with a larger
+// score, or the same score and a lower flat index
 __global__ void __launch_bounds__(kBeamThreads) beam_merge_kernel(BeamArgs a) {
   pdl_trigger();
-  extern __shared__ __align__(16) uint8_t dyn[];
-  Cand *cand = reinterpret_cast<Cand *>(dyn);          // [W * slices * W]
-  __shared__ Cand tops[kBeamThreads];
+  extern __shared__ __align__(16) Key raw[];           // [W][slices][W]
+  __shared__ Key best[kMaxW][kMaxW];
+  __shared__ double score[kMaxW][kMaxW];
+  __shared__ int token[kMaxW][kMaxW];                  // -1: no candidate
   __shared__ double lse[kMaxW];
-  __shared__ int picked[kBeamThreads], npicked;
-  const int tid = threadIdx.x, W = a.W;
+  const int tid = threadIdx.x, lane = tid & 31, W = a.W, per = a.slices * W, N = W * per;
   const int64_t b = blockIdx.x;
+  for (int i = tid; i < W * W; i += kBeamThreads) best[i / W][i % W] = 0;
   pdl_wait();
-  if (tid == 0) npicked = 0;
-  for (int w = tid; w < W; w += kBeamThreads) {
-    const float2 *sm = a.sums + (b * W + w) * a.slices;
-    float M = -INFINITY;
-    for (int i = 0; i < a.slices; i++) M = fmaxf(M, sm[i].x);
-    double S = 0;
-    for (int i = 0; i < a.slices; i++) S += sm[i].x > -INFINITY || sm[i].y != sm[i].y ? sm[i].y * exp((double)sm[i].x - M) : 0.0;
-    lse[w] = (double)M + log(S);
+  for (int i = tid; i < N; i += kBeamThreads) raw[i] = a.best[b * N + i];
+  for (int w = tid >> 5; w < W; w += kBeamWarps) {
+    float M = -INFINITY, S = 0.f;
+    for (int i = lane; i < a.slices; i += 32) {
+      const float2 x = a.sums[(b * W + w) * a.slices + i];
+      const float M1 = fmaxf(M, x.x);
+      if (M1 > -INFINITY) S = S * beam_ex2(M - M1) + x.y * beam_ex2(x.x - M1);
+      M = M1;
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+      const float oM = __shfl_xor_sync(0xffffffffu, M, o), oS = __shfl_xor_sync(0xffffffffu, S, o);
+      const float M1 = fmaxf(M, oM);
+      if (M1 > -INFINITY) S = S * beam_ex2(M - M1) + oS * beam_ex2(oM - M1);
+      M = M1;
+    }
+    // 2^M S in units of kLog2e's fp32 value: what the terms were raised with
+    if (lane == 0) lse[w] = ((double)M + log2((double)S)) / (double)kLog2e;
   }
   __syncthreads();
-  const int per = a.slices * W, N = W * per;
   for (int i = tid; i < N; i += kBeamThreads) {
-    const int w = i / per, r = i - w * per;
-    const int64_t row = b * W + w;
-    const double cum = a.scores[row];
-    const bool done = a.done[row] != 0;
-    // beams with nothing finite to offer stand for their lowest tokens
+    const int w = i / per, mine = (i - w * per) / W;
+    const Key k = raw[i];
+    int rank = i % W;
+    for (int x = 0; x < a.slices && rank < W; x++)
+      if (x != mine)
+        for (int j = 0; j < W && raw[w * per + x * W + j] > k; j++) rank++;
+    if (k && rank < W) best[w][rank] = k;
+  }
+  __syncthreads();
+  for (int i = tid; i < W * W; i += kBeamThreads) {
+    const int w = i / W, r = i - w * W;
+    const double cum = a.scores[b * W + w];
+    const bool done = a.done[b * W + w] != 0;
+    // a beam with nothing finite to offer stands for its lowest tokens
     const bool dead = !isfinite(cum) || (!done && !isfinite(lse[w]));
-    Cand c{-INFINITY, INT64_MAX};
-    if (done || dead) {
-      // eos first, then the other tokens in order; only W of them can count
-      int64_t token = r;
-      if (done && !dead) token = r == 0 ? a.eos : r - (r <= a.eos);
-      if (r < W && token < a.V) {
-        c.score = done && !dead && r == 0 ? cum : -INFINITY;
-        c.flat = (int64_t)w * a.V + token;
-      }
-    } else {
-      const Key k = a.best[row * per + r];
-      if (k) {
-        const uint32_t token = 0xffffffffu - (uint32_t)k, u = (uint32_t)(k >> 32);
-        const float x = __uint_as_float(u & 0x80000000u ? u & 0x7fffffffu : ~u);   // beam_key's logit back
-        const double v = cum + ((double)x - lse[w]);
-        c.score = isfinite(v) ? v : -INFINITY;
-        c.flat = (int64_t)w * a.V + token;
-      }
+    double v = -INFINITY;
+    int tok = r < a.V ? r : -1;
+    if (done && !dead) {
+      // eos, then the other tokens in order
+      tok = r >= a.V ? -1 : r == 0 ? a.eos : r - (r <= a.eos);
+      if (r == 0) v = cum;
+    } else if (!dead) {
+      const Key k = best[w][r];
+      tok = k ? (int)(0xffffffffu - (uint32_t)k) : -1;
+      v = cum + ((double)key_logit(k) - lse[w]);
+      if (!isfinite(v)) v = -INFINITY;
     }
-    cand[i] = c;
+    score[w][r] = v;
+    token[w][r] = tok;
   }
   __syncthreads();
-  // the threads whose best is among the W best of those
-  Cand top{-INFINITY, INT64_MAX};
-  for (int i = tid; i < N; i += kBeamThreads)
-    if (beats(cand[i], top)) top = cand[i];
-  tops[tid] = top;
-  __syncthreads();
-  int above = 0;
-  for (int i = 0; i < kBeamThreads; i++) above += beats(tops[i], top);
-  if (above < W && top.flat != INT64_MAX) picked[atomicAdd(&npicked, 1)] = tid;
-  __syncthreads();
-  // every candidate of those threads against every other
-  const int rounds = (N + kBeamThreads - 1) / kBeamThreads, np = npicked;
-  for (int i = tid; i < np * rounds; i += kBeamThreads) {
-    const int me = picked[i % np] + i / np * kBeamThreads;
-    if (me >= N || cand[me].flat == INT64_MAX) continue;
-    const Cand c = cand[me];
+  for (int i = tid; i < W * W; i += kBeamThreads) {
+    const int w = i / W, r = i - w * W, tok = token[w][r];
+    if (tok < 0) continue;
+    const double v = score[w][r];
     int rank = 0;
-    for (int p = 0; p < np && rank < W; p++)
-      for (int q = picked[p]; q < N; q += kBeamThreads) rank += beats(cand[q], c);
+    for (int x = 0; x < W && rank < W; x++)
+      for (int j = 0; j < W && token[x][j] >= 0 && score[x][j] >= v; j++)
+        rank += score[x][j] > v || x < w || (x == w && token[x][j] < tok);
     if (rank < W) {
-      const int w = (int)(c.flat / a.V);
       const int64_t o = b * W + rank;
-      const int32_t token = (int32_t)(c.flat - (int64_t)w * a.V);
-      a.out_scores[o] = (float)c.score;
-      a.tokens[o] = token;
+      a.out_scores[o] = (float)v;
+      a.tokens[o] = tok;
       a.parents[o] = w;
-      a.out_done[o] = a.done[b * W + w] != 0 || token == a.eos;
+      a.out_done[o] = a.done[b * W + w] != 0 || tok == a.eos;
     }
   }
 }
 
-// Slices per row: enough CTAs for four per SM, of at least half a tile each.
-int beam_slices(int num_sms, int64_t rows, int64_t V) {
-  int64_t s = (4 * (int64_t)num_sms + rows - 1) / (rows > 0 ? rows : 1);
-  const int64_t most = (V + kTile / 2 - 1) / (kTile / 2);
+// Slices per row: enough warps for about 24 on each SM, none of them with less
+// than a tile, and few enough that the merge ranks at most 256 survivors a row.
+int beam_slices(int num_sms, int B, int W, int64_t V) {
+  const int64_t rows = (int64_t)B * W > 0 ? (int64_t)B * W : 1;
+  int64_t s = ((int64_t)num_sms * 24 / kBeamWarps + rows - 1) / rows;
+  const int64_t most = (V + kTile * kBeamWarps / 2 - 1) / (kTile * kBeamWarps / 2);
   s = s < most ? s : most;
+  s = s < 256 / W ? s : 256 / W;
   return (int)(s < 1 ? 1 : s > kMaxSlices ? kMaxSlices : s);
-}
-
-// The merge holds W * slices * W candidates in shared memory.
-int beam_plan(int num_sms, int B, int W, int64_t V) {
-  int s = beam_slices(num_sms, (int64_t)B * W, V);
-  while (s > 1 && (size_t)W * W * s * sizeof(Cand) > 160 * 1024) s--;
-  return s;
 }
 
 // ------------------------------------------------------------------ reordering
@@ -355,7 +379,7 @@ extern "C" {
 
 int64_t fcu_beam_work(fcu_ctx *ctx, int B, int W, int64_t V) {
   if (!ctx || B < 0 || W < 1 || W > kMaxW || V < 1) return -1;
-  const int64_t parts = (int64_t)B * W * beam_plan(ctx->num_sms, B, W, V);
+  const int64_t parts = (int64_t)B * W * beam_slices(ctx->num_sms, B, W, V);
   return parts * (sizeof(float2) + W * sizeof(Key));
 }
 
@@ -364,7 +388,7 @@ int fcu_beam_step(fcu_ctx *ctx, const float *logits, int64_t ld, const float *sc
                   uint8_t *out_done, void *work, int64_t work_bytes) {
   FCU_CTX(ctx);
   FCU_REQUIRE(B >= 0 && W >= 1 && W <= kMaxW, "fcu_beam_step: %d sequences of %d beams (1..%d)", B, W, kMaxW);
-  FCU_REQUIRE(V >= 1 && V <= INT_MAX, "fcu_beam_step: a vocabulary of %lld", (long long)V);
+  FCU_REQUIRE(V >= 1 && V <= 1 << 30, "fcu_beam_step: a vocabulary of %lld", (long long)V);
   FCU_REQUIRE(eos >= 0 && eos < V, "fcu_beam_step: eos %d outside the vocabulary", eos);
   FCU_REQUIRE(ld >= V, "fcu_beam_step: row stride %lld too small", (long long)ld);
   FCU_REQUIRE((int64_t)B * W <= 65535, "fcu_beam_step: %d x %d rows in one call", B, W);
@@ -379,22 +403,22 @@ int fcu_beam_step(fcu_ctx *ctx, const float *logits, int64_t ld, const float *sc
   a.ld = ld;
   a.scores = scores;
   a.done = done;
-  a.V = V;
+  a.V = (int)V;
   a.B = B;
   a.W = W;
   a.eos = eos;
-  a.slices = beam_plan(ctx->num_sms, B, W, V);
-  a.slice = (V + a.slices - 1) / a.slices;
+  a.slices = beam_slices(ctx->num_sms, B, W, V);
+  a.slice = (int)((V + a.slices - 1) / a.slices);
   a.best = (Key *)work;
   a.sums = (float2 *)(a.best + (int64_t)B * W * a.slices * W);
   a.out_scores = out_scores;
   a.tokens = tokens;
   a.parents = parents;
   a.out_done = out_done;
-  const size_t smem = (size_t)W * W * a.slices * sizeof(Cand);
+  const size_t smem = (size_t)W * W * a.slices * sizeof(Key);
   static bool set[64] = {false};
   if (!set[ctx->device & 63]) {
-    FCU_CHECK_CUDA(cudaFuncSetAttribute(beam_merge_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 160 * 1024));
+    FCU_CHECK_CUDA(cudaFuncSetAttribute(beam_merge_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 64 * 1024));
     set[ctx->device & 63] = true;
   }
   FCU_CHECK_CUDA(launch_pdl(beam_rows_kernel, dim3(a.slices, B * W), dim3(kBeamThreads), 0, ctx->stream, a));

@@ -23,11 +23,16 @@ import math
 import numpy as np
 import torch
 
-from ._lib import CacheArray, Kv4, call, lib
-from .autograd import ctx, device
+from ._lib import CacheArray, Context, Kv4, check, lib
+from .autograd import device
 from .infer import KVCache, _dev_f32
 
-_U8, _BF, _F32, _I32 = torch.uint8, torch.bfloat16, torch.float32, torch.int32
+_U8, _BF, _F32, _I32, _BOOL = torch.uint8, torch.bfloat16, torch.float32, torch.int32, torch.bool
+_ROW_BYTES: dict = {}
+
+# A decode step makes these calls once per layer, and the kernels take a few
+# microseconds, so the common path of every function is one test per tensor; what
+# fails it is looked at again for the message.
 
 
 def _need(ok, what: str) -> None:
@@ -35,12 +40,36 @@ def _need(ok, what: str) -> None:
         raise ValueError(what)
 
 
-def _check(name: str, t, dtype, shape=None) -> None:
-    """t is a contiguous tensor of `dtype` (and `shape`) on the current device."""
+def _on(dev: int):
+    """The fcu_ctx of the current device `dev`, bound to its current stream."""
+    c = Context._per_device.get(dev) or Context.get(dev)
+    c.bind_stream(torch._C._cuda_getCurrentRawStream(dev))
+    return c.handle
+
+
+def _device() -> int:
+    if not torch.cuda.is_initialized():
+        device()                        # no CUDA device: the package's error
+        torch.cuda.init()
+    return torch.cuda.current_device()
+
+
+def _call(name: str, *args) -> None:
+    rc = getattr(lib(), name)(*args)
+    if rc:
+        check(rc, name)
+
+
+def _ok(t, dtype, dev: int) -> bool:
+    return t.dtype is dtype and t.get_device() == dev and t.is_contiguous()
+
+
+def _check(name: str, t, dtype, dev: int, shape=None) -> None:
+    """t is a contiguous tensor of `dtype` (and `shape`) on device `dev`."""
     if not isinstance(t, torch.Tensor) or t.dtype != dtype:
         raise ValueError(f"{name}: a {dtype} tensor is needed, got "
                          f"{t.dtype if isinstance(t, torch.Tensor) else type(t).__name__}")
-    if not t.is_cuda or t.device.index != torch.cuda.current_device():
+    if t.get_device() != dev:
         raise ValueError(f"{name} is on {t.device}, not on the current CUDA device")
     if shape is not None and tuple(t.shape) != shape:
         raise ValueError(f"{name}: shape {tuple(t.shape)}, {shape} is needed")
@@ -48,49 +77,63 @@ def _check(name: str, t, dtype, shape=None) -> None:
         raise ValueError(f"{name} is not contiguous")
 
 
-def _cache(k, kg, v, vg, dHead, B, table, weight=None, pos=None, layers=False) -> Kv4:
+def _row_bytes(dHead: int) -> int:
+    rb = _ROW_BYTES.get(dHead)
+    if rb is None:
+        rb = lib().fcu_kv4_row_bytes(int(dHead))
+        _need(rb > 0, f"head dim {dHead}: even, 2 to 256")
+        _ROW_BYTES[dHead] = rb
+    return rb
+
+
+def _cache(dev, k, kg, v, vg, dHead, B, table, weight=None, pos=None, layers=False) -> Kv4:
     """The C-ABI's view of one layer's arrays (five dimensions: of all layers)."""
-    _check("k", k, _U8)
-    _need(k.ndim == (5 if layers else 4), f"k: {k.ndim} dimensions")
-    rb = lib().fcu_kv4_row_bytes(int(dHead))
-    _need(rb > 0, f"head dim {dHead}: even, 2 to 256")
-    _need(k.shape[-1] == rb, f"k: rows of {k.shape[-1]} bytes, head dim {dHead} has {rb}")
-    lead = tuple(k.shape[:-1])
-    _check("v", v, _U8, tuple(k.shape))
-    _check("kg", kg, _BF, (*lead, 2))
-    _check("vg", vg, _BF, (*lead, 2))
+    rb = _row_bytes(dHead)
+    ndim = 5 if layers else 4
+    if not (isinstance(k, torch.Tensor) and isinstance(v, torch.Tensor) and isinstance(kg, torch.Tensor)
+            and isinstance(vg, torch.Tensor) and len(k.shape) == ndim and k.shape[-1] == rb and k.shape == v.shape and kg.shape == vg.shape
+            and kg.shape[:-1] == k.shape[:-1] and kg.shape[-1] == 2 and _ok(k, _U8, dev) and _ok(v, _U8, dev)
+            and _ok(kg, _BF, dev) and _ok(vg, _BF, dev)):
+        _check("k", k, _U8, dev)
+        _need(k.ndim == ndim, f"k: {k.ndim} dimensions")
+        _need(k.shape[-1] == rb, f"k: rows of {k.shape[-1]} bytes, head dim {dHead} has {rb}")
+        _check("v", v, _U8, dev, tuple(k.shape))
+        _check("kg", kg, _BF, dev, (*k.shape[:-1], 2))
+        _check("vg", vg, _BF, dev, (*k.shape[:-1], 2))
+    lead = k.shape[:-1]
     if weight is not None:
-        _check("weight", weight, _F32, lead)
+        _check("weight", weight, _F32, dev, tuple(lead))
     if pos is not None:
-        _check("pos", pos, _I32, lead)
-    L, (blocks, nKV, bs) = (lead[0] if layers else 1), lead[-3:]
+        _check("pos", pos, _I32, dev, tuple(lead))
+    blocks, nKV, bs = lead[-3:]
     if table is not None:
+        _check("table", table, _I32, dev)
         _need(table.ndim == 2 and table.shape[0] == B, f"table: shape {tuple(table.shape)} for {B} sequences")
-        _check("table", table, _I32)
         mb = table.shape[1]
     else:
         _need(blocks % max(B, 1) == 0, f"{blocks} blocks do not divide among {B} sequences")
         mb = blocks // max(B, 1)
     return Kv4(k.data_ptr(), v.data_ptr(), kg.data_ptr(), vg.data_ptr(),
                weight.data_ptr() if weight is not None else None, pos.data_ptr() if pos is not None else None,
-               table.data_ptr() if table is not None else None, L, blocks, nKV, int(dHead), bs, mb)
+               table.data_ptr() if table is not None else None, lead[0] if layers else 1, blocks, nKV, dHead, bs, mb)
 
 
-def _work(nbytes: int) -> torch.Tensor | None:
-    """A call's workspace.  The allocator hands it out again only to work queued
-    behind the call on the same stream (in a capture: from the graph's pool)."""
-    return torch.empty(nbytes, dtype=_U8, device=device()) if nbytes > 0 else None
-
-
-def _rows(name: str, t, cols_min: int) -> int:
+def _rows(name: str, t, dev: int) -> int:
     """Row stride of a two-dimensional fp32 tensor with unit column stride."""
-    if not isinstance(t, torch.Tensor) or t.dtype != _F32 or t.ndim != 2:
+    if not isinstance(t, torch.Tensor) or t.dtype is not _F32 or t.ndim != 2:
         raise ValueError(f"{name}: a two-dimensional float32 tensor is needed")
-    if not t.is_cuda or t.device.index != torch.cuda.current_device():
+    if t.get_device() != dev:
         raise ValueError(f"{name} is on {t.device}, not on the current CUDA device")
-    if t.shape[1] < cols_min or (t.shape[1] > 1 and t.stride(1) != 1):
+    rows, cols = t.shape
+    ld = t.stride(0)
+    if cols < 1 or (cols > 1 and t.stride(1) != 1) or (rows > 1 and ld < cols):
         raise ValueError(f"{name}: shape {tuple(t.shape)} with strides {t.stride()}")
-    return t.stride(0) if t.shape[0] > 1 else t.shape[1]
+    return ld if rows > 1 else cols
+
+
+# A call's workspace comes from torch's allocator, which hands it out again only
+# to work queued behind the call on the same stream (in a capture: from the
+# graph's own pool), so calls on two streams and captured graphs share none.
 
 
 def kv4Put(qkv, nHeads: int, positions, slots, k, kg, v, vg, T: int = 1, theta: float = 10000.0, table=None,
@@ -101,32 +144,32 @@ def kv4Put(qkv, nHeads: int, positions, slots, k, kg, v, vg, T: int = 1, theta: 
     go to the cache in 4 bits; their columns of qkv stay as they are.  theta 0:
     the rows carry their rotation already.  A token whose slot is outside the
     cache, or whose position is negative, changes nothing."""
-    _check("positions", positions, _I32)
+    dev = _device()
+    _check("positions", positions, _I32, dev)
     B = positions.numel()
-    _check("slots", slots, _I32)
+    _check("slots", slots, _I32, dev)
     _need(slots.numel() == B, f"{slots.numel()} slots for {B} sequences")
     _need(T >= 1 and nHeads >= 0 and theta >= 0, f"T={T}, nHeads={nHeads}, theta={theta}")
     _need(k.ndim == 4, f"k: {k.ndim} dimensions")
     heads = nHeads + 2 * k.shape[1]
-    ld = _rows("qkv", qkv, 1)
+    ld = _rows("qkv", qkv, dev)
     _need(qkv.shape[0] == B * T and qkv.shape[1] % heads == 0,
           f"qkv: shape {tuple(qkv.shape)} for {B} x {T} tokens of {heads} heads")
-    _need(qkv.shape[0] < 2 or ld >= qkv.shape[1], "qkv: its rows overlap")
-    c = _cache(k, kg, v, vg, qkv.shape[1] // heads, B, table, weight, pos)
-    call("fcu_kv4_put", ctx().handle, qkv.data_ptr(), ld, B, T, nHeads, float(theta), positions.data_ptr(),
+    c = _cache(dev, k, kg, v, vg, qkv.shape[1] // heads, B, table, weight, pos)
+    _call("fcu_kv4_put", _on(dev), qkv.data_ptr(), ld, B, T, nHeads, float(theta), positions.data_ptr(),
          slots.data_ptr(), c)
 
 
 def kv4Values(k, kg, v, vg, dHead: int, start, T: int, table=None):
     """(K, V) fp32 [B, T, nKV, dHead]: the values of slots start[b] .. start[b] + T
     (start int32 [B]).  A slot outside the cache gives NaN."""
-    _check("start", start, _I32)
+    dev = _device()
+    _check("start", start, _I32, dev)
     B = start.numel()
     _need(T >= 0, f"T={T}")
-    c = _cache(k, kg, v, vg, dHead, B, table)
-    out = torch.empty(2, B, T, c.n_kv, dHead, dtype=_F32, device=k.device)
-    K, V = out[0], out[1]
-    call("fcu_kv4_values", ctx().handle, c, start.data_ptr(), B, T, K.data_ptr(), V.data_ptr())
+    c = _cache(dev, k, kg, v, vg, dHead, B, table)
+    K, V = k.new_empty((2, B, T, c.n_kv, dHead), dtype=_F32).unbind(0)
+    _call("fcu_kv4_values", _on(dev), c, start.data_ptr(), B, T, K.data_ptr(), V.data_ptr())
     return K, V
 
 
@@ -136,24 +179,27 @@ def kv4Attention(q, k, kg, v, vg, lens, scale: float | None = None, table=None, 
     0 gives zeros), grouped heads as in attentionDecode.  scale: 1 / sqrt(dHead)
     unless given.  With `weight`, every slot's attention weight, summed over its
     kv head's q heads, is added to it."""
-    _need(isinstance(q, torch.Tensor) and q.dtype == _F32 and q.ndim == 3, "q: a float32 [B, nHeads, dHead] is needed")
+    dev = _device()
+    _need(isinstance(q, torch.Tensor) and q.dtype is _F32 and q.ndim == 3, "q: a float32 [B, nHeads, dHead] is needed")
     B, nH, dH = q.shape
-    _need(q.is_cuda and q.device.index == torch.cuda.current_device(), f"q is on {q.device}, not on the current CUDA device")
-    _need((dH == 1 or q.stride(2) == 1) and (nH == 1 or q.stride(1) == dH) and (B == 1 or q.stride(0) >= nH * dH),
-          f"q: strides {q.stride()}")
-    _check("lens", lens, _I32, (B,))
-    c = _cache(k, kg, v, vg, dH, B, table, weight)
+    _need(q.get_device() == dev, "q is not on the current CUDA device")
+    ld = nH * dH
+    if not q.is_contiguous():
+        s = q.stride()
+        _need((dH == 1 or s[2] == 1) and (nH == 1 or s[1] == dH) and (B == 1 or s[0] >= ld), f"q: strides {s}")
+        ld = s[0] if B > 1 else ld
+    _check("lens", lens, _I32, dev, (B,))
+    c = _cache(dev, k, kg, v, vg, dH, B, table, weight)
     if out is None:
-        out = torch.empty((B, nH, dH), dtype=_F32, device=q.device)
+        out = q.new_empty((B, nH, dH))
     else:
-        _check("out", out, _F32)
-        _need(out.numel() == q.numel(), f"out: shape {tuple(out.shape)}")
-    h = ctx().handle
+        _check("out", out, _F32, dev)
+        _need(out.numel() == B * nH * dH, f"out: shape {tuple(out.shape)}")
+    h = _on(dev)
     nbytes = lib().fcu_kv4_attn_work(h, c, B, nH)
-    work = _work(nbytes)
-    call("fcu_kv4_attn", h, q.data_ptr(), q.stride(0) if B > 1 else nH * dH, c, lens.data_ptr(), B, nH,
-         1 / math.sqrt(dH) if scale is None else float(scale), out.data_ptr(),
-         work.data_ptr() if work is not None else None, max(nbytes, 0))
+    work = k.new_empty((nbytes,)).data_ptr() if nbytes > 0 else None
+    _call("fcu_kv4_attn", h, q.data_ptr(), ld, c, lens.data_ptr(), B, nH,
+          dH ** -0.5 if scale is None else float(scale), out.data_ptr(), work, nbytes)
     return out
 
 
@@ -162,22 +208,20 @@ def kv4Evict(k, kg, v, vg, weight, pos, lens, budget: int, recent: int, table=No
     of sequences longer than `budget` down to it: the slots of the `recent`
     newest positions and those of largest weight stay (ties: the lowest slot),
     moved into the freed slots.  Returns the new lengths, min(lens, budget)."""
-    _check("lens", lens, _I32)
+    dev = _device()
+    _check("lens", lens, _I32, dev)
     B = lens.numel()
     _need(weight is not None and pos is not None, "eviction goes by `weight` and `pos`")
     _need(budget >= 1 and 0 <= recent <= budget, f"budget {budget}, recent {recent}")
-    _need(k.ndim == 5, f"k: {k.ndim} dimensions")
-    rb = k.shape[-1]
-    c = _cache(k, kg, v, vg, 2 * rb, B, table, weight, pos, layers=True)
+    c = _cache(dev, k, kg, v, vg, 2 * k.shape[-1], B, table, weight, pos, layers=True)
     if newLens is None:
         newLens = torch.empty_like(lens)
     else:
-        _check("newLens", newLens, _I32, tuple(lens.shape))
-    h = ctx().handle
+        _check("newLens", newLens, _I32, dev, tuple(lens.shape))
+    h = _on(dev)
     nbytes = lib().fcu_kv4_evict_work(h, c, B)
-    work = _work(nbytes)
-    call("fcu_kv4_evict", h, c, lens.data_ptr(), B, budget, recent, newLens.data_ptr(),
-         work.data_ptr() if work is not None else None, max(nbytes, 0))
+    work = k.new_empty((nbytes,)).data_ptr() if nbytes > 0 else None
+    _call("fcu_kv4_evict", h, c, lens.data_ptr(), B, budget, recent, newLens.data_ptr(), work, nbytes)
     return newLens
 
 
@@ -187,25 +231,23 @@ def beamStep(logits, scores, done, beams: int, eos: int):
     parents, done), [B, beams] each, best first: score + log softmax(logits) over
     all beams and tokens of a sequence, ties to the lowest (beam, token); a beam
     that is done goes on as (eos, its score)."""
-    ld = _rows("logits", logits, 1)
+    dev = _device()
+    ld = _rows("logits", logits, dev)
     R, V = logits.shape
-    _need(R < 2 or ld >= V, "logits: its rows overlap")
     _need(1 <= beams <= 32 and R % beams == 0, f"{R} rows for searches of {beams} beams (1 to 32)")
     _need(0 <= eos < V, f"eos {eos} outside the vocabulary of {V}")
-    _check("scores", scores, _F32)
-    _check("done", done, torch.bool)
+    _check("scores", scores, _F32, dev)
+    _check("done", done, _BOOL, dev)
     _need(scores.numel() == R and done.numel() == R, f"{scores.numel()} scores, {done.numel()} done for {R} rows")
     B = R // beams
-    dev = logits.device
-    outScores = torch.empty((B, beams), dtype=_F32, device=dev)
-    tokens, parents = torch.empty((2, B, beams), dtype=_I32, device=dev).unbind(0)
-    outDone = torch.empty((B, beams), dtype=torch.bool, device=dev)
-    h = ctx().handle
+    outScores = scores.new_empty((B, beams))
+    tokens, parents = scores.new_empty((2, B, beams), dtype=_I32).unbind(0)
+    outDone = done.new_empty((B, beams))
+    h = _on(dev)
     nbytes = lib().fcu_beam_work(h, B, beams, V)
-    work = _work(nbytes)
-    call("fcu_beam_step", h, logits.data_ptr(), ld, scores.data_ptr(), done.data_ptr(), B, beams, V, eos,
-         outScores.data_ptr(), tokens.data_ptr(), parents.data_ptr(), outDone.data_ptr(),
-         work.data_ptr() if work is not None else None, max(nbytes, 0))
+    work = scores.new_empty((nbytes // 4 + 1,)).data_ptr()
+    _call("fcu_beam_step", h, logits.data_ptr(), ld, scores.data_ptr(), done.data_ptr(), B, beams, V, eos,
+          outScores.data_ptr(), tokens.data_ptr(), parents.data_ptr(), outDone.data_ptr(), work, nbytes)
     return outScores, tokens, parents, outDone
 
 
@@ -215,28 +257,33 @@ def cacheReorder(arrays, parents, lens, table=None) -> None:
     of its source b * W + parents[b, w].  arrays: up to 8 tensors [layers, blocks,
     heads, blockSize, ...] whose slots hold a multiple of 4 bytes (an fp32 cache
     has one head: its rows); parents int32 [B, W]; lens int32 [B * W]."""
-    _check("parents", parents, _I32)
-    _need(parents.ndim == 2 and parents.shape[1] <= 32, f"parents: shape {tuple(parents.shape)} (at most 32 beams)")
+    dev = _device()
+    _check("parents", parents, _I32, dev)
+    _need(parents.ndim == 2 and 1 <= parents.shape[1] <= 32, f"parents: shape {tuple(parents.shape)} (1 to 32 beams)")
     B, W = parents.shape
-    _check("lens", lens, _I32)
+    _check("lens", lens, _I32, dev)
     _need(lens.numel() == B * W, f"{lens.numel()} lengths for {B} x {W} beams")
-    _need(1 <= len(arrays) <= 8, f"{len(arrays)} arrays (1 to 8)")
-    L, blocks, bs = arrays[0].shape[0], arrays[0].shape[1], arrays[0].shape[3]
-    spec = (CacheArray * len(arrays))()
+    n = len(arrays)
+    _need(1 <= n <= 8, f"{n} arrays (1 to 8)")
+    L, blocks, _, bs = arrays[0].shape[:4]
+    spec = (CacheArray * n)()
     for i, t in enumerate(arrays):
-        _check(f"arrays[{i}]", t, t.dtype)
-        _need(t.ndim >= 4 and (t.shape[0], t.shape[1], t.shape[3]) == (L, blocks, bs),
-              f"arrays[{i}]: shape {tuple(t.shape)} beside {tuple(arrays[0].shape)}")
-        spec[i] = CacheArray(t.data_ptr(), t.shape[2], math.prod(t.shape[4:]) * t.element_size())
+        shape = t.shape
+        if not (t.get_device() == dev and t.is_contiguous() and len(shape) >= 4 and shape[0] == L and shape[1] == blocks
+                and shape[3] == bs):
+            _check(f"arrays[{i}]", t, t.dtype, dev)
+            raise ValueError(f"arrays[{i}]: shape {tuple(shape)} beside {tuple(arrays[0].shape)}")
+        s = spec[i]
+        s.base, s.heads, s.unit = t.data_ptr(), shape[2], math.prod(shape[4:]) * t.element_size()
     if table is not None:
+        _check("table", table, _I32, dev)
         _need(table.ndim == 2 and table.shape[0] == B * W, f"table: shape {tuple(table.shape)} for {B * W} beams")
-        _check("table", table, _I32)
         mb = table.shape[1]
     else:
-        _need(W > 0 and blocks % max(B * W, 1) == 0, f"{blocks} blocks do not divide among {B * W} beams")
+        _need(blocks % max(B * W, 1) == 0, f"{blocks} blocks do not divide among {B * W} beams")
         mb = blocks // max(B * W, 1)
-    call("fcu_cache_reorder", ctx().handle, spec, len(arrays), L, blocks,
-         table.data_ptr() if table is not None else None, bs, mb, parents.data_ptr(), lens.data_ptr(), B, W)
+    _call("fcu_cache_reorder", _on(dev), spec, n, L, blocks, table.data_ptr() if table is not None else None, bs, mb,
+          parents.data_ptr(), lens.data_ptr(), B, W)
 
 
 class QuantKVCache(KVCache):
@@ -248,8 +295,7 @@ class QuantKVCache(KVCache):
 
     def __init__(self, nLayers: int, maxSeq: int, nKvHeads: int, dHead: int, batch: int = 1,
                  blockSize: int | None = None, table=None, physBlocks: int | None = None, track: bool = False):
-        rb = lib().fcu_kv4_row_bytes(int(dHead))
-        _need(rb > 0, f"head dim {dHead}: even, 2 to 256")
+        rb = _row_bytes(dHead)
         self.nLayers, self.maxSeq, self.batch = nLayers, maxSeq, batch
         self.nKvHeads, self.dHead, self.kvDim = nKvHeads, dHead, nKvHeads * dHead
         self.block_size = maxSeq if blockSize is None else blockSize

@@ -130,7 +130,7 @@ def test_python_refuses_tensors_off_the_device():
               lambda: F.kv4Values(k, kg, k, kg, 64, i, 1), lambda: F.beamStep(z(4, 9), z(4), z(4, t=torch.bool), 2, 1),
               lambda: F.kv4Evict(k[None], kg[None], k[None], kg[None], z(1, 4, 2, 16), z(1, 4, 2, 16), i, 4, 2),
               lambda: F.cacheReorder([k[None]], z(2, 2, t=torch.int32), i)):
-        with pytest.raises(ValueError):
+        with pytest.raises((ValueError, F.ForgeCUError)):      # the latter where there is no device at all
             f()
 
 
