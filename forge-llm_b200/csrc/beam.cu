@@ -273,11 +273,16 @@ int beam_slices(int num_sms, int B, int W, int64_t V) {
 }
 
 // ------------------------------------------------------------------ reordering
-// A thread owns 16 bytes at one place of every beam of a sequence: it reads
-// them from the beams that another beam continues, then writes the beams that
-// continue another.  No other thread touches that place, so the permutation
-// (with repetitions) is done in place without a wait.
+// A warp takes up to kReBytes of one head of one block at a time, at the same
+// place of all beams of a sequence: it reads them from the beams that another
+// beam continues into its part of shared memory, all copies in flight at once,
+// then writes the beams that continue another.  A lane writes only places it has
+// read itself and no other warp touches them, so the permutation (with
+// repetitions) is done in place without a barrier.  The bound is HBM: every
+// beam that is continued is read once, every beam that changes written once.
 constexpr int kReThreads = 128;
+constexpr int kReWarps = kReThreads / 32;
+constexpr int kReSlots = 16;           // 16-byte pieces of a lane, over all beams
 
 struct ReArgs {
   uint8_t *base[8];
@@ -285,23 +290,16 @@ struct ReArgs {
   int n_arrays;
   int64_t layers, blocks;
   const int32_t *table, *parents, *lens;
-  int bs, mb, B, W;
+  int bs, mb, B, W, depth;     // depth: pieces of a lane from one beam, depth * W <= kReSlots (W <= 16)
   int64_t cap;
 };
 
-__device__ __forceinline__ int64_t re_block(const ReArgs &a, int64_t r, int64_t i) {
-  if (!a.table) return r * a.mb + i;
-  const int64_t p = a.table[r * a.mb + i];
-  return p >= 0 && p < a.blocks ? p : -1;
-}
-
-// copies [off, off + n) bytes of a block's head segment, n <= 16, off and n multiples of 4
-__device__ __forceinline__ void re_load(uint4 *dst, const uint8_t *src, int n, bool wide) {
+// n <= 16 bytes, a multiple of 4; `wide`: 16-byte aligned
+__device__ __forceinline__ void re_load(uint32_t dst, const uint8_t *src, int n, bool wide) {
   if (wide && n == 16) {
-    *dst = *reinterpret_cast<const uint4 *>(src);
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src));
   } else {
-    uint32_t *d = reinterpret_cast<uint32_t *>(dst);
-    for (int i = 0; 4 * i < n; i++) d[i] = reinterpret_cast<const uint32_t *>(src)[i];
+    for (int i = 0; i < n; i += 4) asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(dst + i), "l"(src + i));
   }
 }
 __device__ __forceinline__ void re_store(uint8_t *dst, const uint4 *src, int n, bool wide) {
@@ -315,56 +313,66 @@ __device__ __forceinline__ void re_store(uint8_t *dst, const uint4 *src, int n, 
 
 __global__ void __launch_bounds__(kReThreads) cache_reorder_kernel(ReArgs a) {
   pdl_trigger();
-  extern __shared__ __align__(16) uint4 hold[];     // [W][kReThreads]
-  __shared__ int src_s[kMaxW];                      // the beam each one becomes; itself if it stays
-  __shared__ int64_t len_s[kMaxW];
-  __shared__ uint32_t needed_s;
-  const int tid = threadIdx.x, W = a.W;
+  extern __shared__ __align__(16) uint4 hold[];     // [warp][W][depth][32]
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, W = a.W;
   const int b = blockIdx.y;
   const int64_t layer = blockIdx.z;
+  uint4 *mine = hold + warp * W * a.depth * 32 + lane;
+  const uint32_t mine_s = (uint32_t)__cvta_generic_to_shared(mine);
   pdl_wait();
-  if (tid < W) {
-    const int p = a.parents[(int64_t)b * W + tid];
-    src_s[tid] = p >= 0 && p < W ? p : tid;
-    const int64_t n = a.lens[(int64_t)b * W + tid];
-    len_s[tid] = n < 0 ? 0 : n > a.cap ? a.cap : n;
+  // lane w: the beam that beam w becomes (itself if it stays) and beam w's length
+  int src = lane, len = 0;
+  if (lane < W) {
+    const int p = a.parents[(int64_t)b * W + lane];
+    src = p >= 0 && p < W ? p : lane;
+    const int64_t n = a.lens[(int64_t)b * W + lane];
+    len = (int)(n < 0 ? 0 : n > a.cap ? a.cap : n);
   }
-  __syncthreads();
-  if (tid == 0) {
-    uint32_t needed = 0;
-    for (int w = 0; w < W; w++)
-      if (src_s[w] != w) needed |= 1u << src_s[w];
-    needed_s = needed;
-  }
-  __syncthreads();
-  const uint32_t needed = needed_s;
+  const uint32_t moves = __ballot_sync(0xffffffffu, lane < W && src != lane);
+  uint32_t needed = 0;
+  for (uint32_t m = moves; m; m &= m - 1) needed |= 1u << __shfl_sync(0xffffffffu, src, __ffs(m) - 1);
   if (!needed) return;
-  int64_t longest = 0;
-  for (int w = 0; w < W; w++)
-    if (needed >> w & 1) longest = max(longest, len_s[w]);
+  const int longest = __reduce_max_sync(0xffffffffu, needed >> lane & 1 ? len : 0);
+  const int chunk = 512 * a.depth;                          // bytes of one step
   for (int x = 0; x < a.n_arrays; x++) {
     const int64_t unit = a.unit[x], seg = a.bs * unit;      // bytes of one head of one block
     const bool wide = seg % 16 == 0;
-    const int per_seg = (int)((seg + 15) / 16);             // pieces of one segment
-    const int64_t segs = (longest + a.bs - 1) / a.bs;
-    const int64_t pieces = a.heads[x] * segs * per_seg;
-    for (int64_t i = (int64_t)blockIdx.x * kReThreads + tid; i < pieces; i += (int64_t)gridDim.x * kReThreads) {
-      const int64_t hs = i / per_seg, off = (i - hs * per_seg) * 16;
-      const int64_t h = hs / segs, blk = hs - h * segs;
+    const int64_t used = min(seg, longest * unit);          // no block holds more
+    const int steps = (int)((used + chunk - 1) / chunk), blks = (longest + a.bs - 1) / a.bs;
+    const int64_t items = (int64_t)a.heads[x] * blks * steps;
+    for (int64_t i = (int64_t)blockIdx.x * kReWarps + warp; i < items; i += (int64_t)gridDim.x * kReWarps) {
+      const int64_t hb = i / steps;
+      const int h = (int)(hb / blks), blk = (int)(hb - (int64_t)h * blks);
+      const int64_t off = (i - hb * steps) * chunk;
+      // lane w: beam w's place of this step and the bytes of it that its length covers
+      int64_t at = -1, valid = 0;
+      if (lane < W) {
+        const int64_t r = (int64_t)b * W + lane;
+        int64_t p = r * a.mb + blk;
+        if (a.table) {
+          p = a.table[p];
+          if (p >= a.blocks) p = -1;
+        }
+        if (p >= 0) at = ((layer * a.blocks + p) * a.heads[x] + h) * seg + off;
+        valid = min(seg, ((int64_t)len - (int64_t)blk * a.bs) * unit) - off;
+      }
+      const int bytes = (int)max((int64_t)0, min((int64_t)chunk, valid));
       for (uint32_t m = needed; m; m &= m - 1) {
         const int w = __ffs(m) - 1;
-        const int64_t p = re_block(a, (int64_t)b * W + w, blk);
-        const int n = (int)min(min((int64_t)16, seg - off), (len_s[w] - blk * a.bs) * unit - off);
-        if (p >= 0 && n > 0)
-          re_load(hold + w * kReThreads + tid, a.base[x] + ((layer * a.blocks + p) * a.heads[x] + h) * seg + off, n, wide);
+        const int64_t from = __shfl_sync(0xffffffffu, at, w);
+        const int n = __shfl_sync(0xffffffffu, bytes, w);
+        if (from < 0) continue;
+        for (int d = 0; d < a.depth && 512 * d + 16 * lane < n; d++)
+          re_load(mine_s + (w * a.depth + d) * 512, a.base[x] + from + 512 * d + 16 * lane, min(16, n - 512 * d - 16 * lane), wide);
       }
-      for (int w = 0; w < W; w++) {
-        const int src = src_s[w];
-        if (src == w) continue;
-        const int64_t p = re_block(a, (int64_t)b * W + w, blk), ps = re_block(a, (int64_t)b * W + src, blk);
-        const int n = (int)min(min((int64_t)16, seg - off), (len_s[src] - blk * a.bs) * unit - off);
-        if (p >= 0 && ps >= 0 && n > 0)
-          re_store(a.base[x] + ((layer * a.blocks + p) * a.heads[x] + h) * seg + off, hold + src * kReThreads + tid, n, wide);
+      asm volatile("cp.async.commit_group;\n\tcp.async.wait_group 0;" ::: "memory");
+      for (uint32_t m = moves; m; m &= m - 1) {
+        const int w = __ffs(m) - 1, s = __shfl_sync(0xffffffffu, src, w);
+        const int64_t to = __shfl_sync(0xffffffffu, at, w), from = __shfl_sync(0xffffffffu, at, s);
+        const int n = __shfl_sync(0xffffffffu, bytes, s);
+        if (to < 0 || from < 0) continue;
+        for (int d = 0; d < a.depth && 512 * d + 16 * lane < n; d++)
+          re_store(a.base[x] + to + 512 * d + 16 * lane, mine + (s * a.depth + d) * 32, min(16, n - 512 * d - 16 * lane), wide);
       }
     }
   }
@@ -443,6 +451,8 @@ int fcu_cache_reorder(fcu_ctx *ctx, const fcu_cache_array *arrays, int n_arrays,
   ReArgs a{};
   a.cap = (int64_t)block_size * max_blocks;
   FCU_REQUIRE(a.cap <= 1 << 30, "fcu_cache_reorder: %lld slots per sequence (at most 2^30)", (long long)a.cap);
+  a.depth = W >= kReSlots ? 1 : kReSlots / W;
+  a.depth = a.depth > 4 ? 4 : a.depth;
   int64_t most = 0;
   for (int i = 0; i < n_arrays; i++) {
     FCU_REQUIRE(arrays[i].base && ((uintptr_t)arrays[i].base & 15) == 0, "fcu_cache_reorder: array %d is null or not 16-byte aligned", i);
@@ -453,8 +463,9 @@ int fcu_cache_reorder(fcu_ctx *ctx, const fcu_cache_array *arrays, int n_arrays,
     a.base[i] = (uint8_t *)arrays[i].base;
     a.heads[i] = arrays[i].heads;
     a.unit[i] = arrays[i].unit;
-    const int64_t pieces = arrays[i].heads * max_blocks * (((int64_t)block_size * arrays[i].unit + 15) / 16);
-    most = pieces > most ? pieces : most;
+    const int64_t chunk = 512 * a.depth, steps = ((int64_t)block_size * arrays[i].unit + chunk - 1) / chunk;
+    const int64_t items = arrays[i].heads * max_blocks * steps;
+    most = items > most ? items : most;
   }
   if (B == 0 || layers == 0 || n_arrays == 0 || W == 1) return FCU_OK;
   FCU_REQUIRE(parents && lens, "fcu_cache_reorder: null pointer");
@@ -468,11 +479,11 @@ int fcu_cache_reorder(fcu_ctx *ctx, const fcu_cache_array *arrays, int n_arrays,
   a.mb = max_blocks;
   a.B = B;
   a.W = W;
-  // CTAs over a (sequence, layer): up to eight waves of them in all, a thread then walks the rest
-  const int64_t pairs = (int64_t)B * layers, fill = (8 * 16 * (int64_t)ctx->num_sms + pairs - 1) / pairs;
-  int64_t gx = (most + kReThreads - 1) / kReThreads;
+  // CTAs over a (sequence, layer): about eight waves of them in all, a warp then walks the rest
+  const int64_t pairs = (int64_t)B * layers, fill = (8 * 6 * (int64_t)ctx->num_sms + pairs - 1) / pairs;
+  int64_t gx = (most + kReWarps - 1) / kReWarps;
   gx = gx < fill ? gx : fill;
-  const size_t smem = (size_t)W * kReThreads * 16;
+  const size_t smem = (size_t)W * a.depth * kReThreads * 16;
   static bool set[64] = {false};
   if (!set[ctx->device & 63]) {
     FCU_CHECK_CUDA(cudaFuncSetAttribute(cache_reorder_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,

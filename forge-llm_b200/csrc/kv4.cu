@@ -1,6 +1,8 @@
 // The 4-bit KV cache (layout and grid: kv4.cuh, include/forgecu.h): RoPE and
 // quantized writes, values read back, and eviction by accumulated attention
 // weight.  Its attention is in kv4_attn.cu.
+#include <string.h>
+
 #include "kv4.cuh"
 
 namespace fcu {
@@ -247,19 +249,33 @@ __global__ void __launch_bounds__(kValThreads) kv4_values_kernel(ValArgs a) {
 }
 
 // ------------------------------------------------------------------ evict
-constexpr int kEvThreads = 1024;
+constexpr int kEvThreads = 512;
+constexpr int kEvWarps = kEvThreads / 32;
 constexpr int kEvBins = 2048;
-constexpr int64_t kEvSmemSlots = 40 * 1024;   // keys of one head kept in shared memory
+constexpr int kEvBatch = 2;                   // loads of a thread in flight, of four slots each where they line up
+constexpr int kEvPieces = 4;
+constexpr int kEvInline = 512;                // moves of one head that the selecting CTA makes itself
+constexpr int kEvFew = kEvThreads;            // keys that are ranked directly
+constexpr int kEvSmemSlots = 40 * 1024;   // keys of one head kept in shared memory
 
 struct EvArgs {
   Cache c;
   const int32_t *lens;
   int B, budget, recent;
   int32_t *new_lens;
-  uint32_t *work;   // keys [layers * B * nKV][cap] where they do not fit in shared memory
+  uint32_t *keys;   // [heads][padded cap] where they do not fit in shared memory (heads: layers * B * nKV)
+  // for kv4_move_kernel, where a head may have more moves than kEvInline: their
+  // number, and slots to and from [heads][most]
+  uint32_t *count;
+  int32_t *to, *from;
+  int most;
 };
 
-// Exclusive block scan of v over kEvThreads threads; total in *sum.
+// Keys are kept with a word of padding after every 32, so that threads that walk
+// neighbouring runs of slots meet different banks.
+__host__ __device__ inline int ev_at(int j) { return j + (j >> 5); }   // (j at most 2^26)
+
+// Exclusive block scan of v; total in *sum.
 __device__ __forceinline__ uint32_t scan_excl(uint32_t v, uint32_t *warp_sums, uint32_t *sum) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   uint32_t x = v;
@@ -271,7 +287,7 @@ __device__ __forceinline__ uint32_t scan_excl(uint32_t v, uint32_t *warp_sums, u
   __syncthreads();   // warp_sums may still be read from the previous scan
   if (lane == 31) warp_sums[warp] = x;
   __syncthreads();
-  uint32_t w = warp_sums[lane];
+  const uint32_t w = lane < kEvWarps ? warp_sums[lane] : 0;
   uint32_t incl = w;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
@@ -279,8 +295,7 @@ __device__ __forceinline__ uint32_t scan_excl(uint32_t v, uint32_t *warp_sums, u
     if (lane >= o) incl += y;
   }
   *sum = __shfl_sync(0xffffffffu, incl, 31);
-  const uint32_t before = __shfl_sync(0xffffffffu, incl - w, warp);
-  return before + x - v;
+  return __shfl_sync(0xffffffffu, incl - w, warp) + x - v;
 }
 
 // Keys order as the weights: larger weight, larger key; NaN 0 (below -inf's
@@ -291,109 +306,340 @@ __device__ __forceinline__ uint32_t weight_key(float w) {
   return u & 0x80000000u ? ~u : u | 0x80000000u;
 }
 
-// One CTA per (head, sequence, layer): the budget-th largest key by three
-// histogram passes (11 + 11 + 10 bits) over keys in shared memory, then the
-// freed slots and the slots that move, both in slot order, and the moves.
-__global__ void __launch_bounds__(kEvThreads) kv4_evict_kernel(EvArgs a) {
+// G neighbouring values, or `other`.
+template <int G, typename T>
+__device__ __forceinline__ void load_slots(T (&x)[G], const T *p, bool on, T other) {
+  if constexpr (G == 4) {
+    static_assert(sizeof(T) == 4, "");
+    const int4 v = on ? *reinterpret_cast<const int4 *>(p) : int4{0, 0, 0, 0};
+    const int y[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+    for (int e = 0; e < 4; e++) {
+      T f;
+      memcpy(&f, &y[e], 4);
+      x[e] = on ? f : other;
+    }
+  } else {
+    x[0] = on ? *p : other;
+  }
+}
+
+// One CTA per (head, sequence, layer).  The budget-th largest key is found by
+// histograms over the range that the keys span: 2048 bins of equal width, then
+// the bin that holds it again, until its keys are few enough to be ranked one
+// against the other (weights spread over many magnitudes; bins of the range
+// itself meet fewer collisions than bins of leading bits).  Then the freed slots
+// and the slots that move are listed, both in slot order, and moved.
+// VEC: four slots of a head are 16 aligned bytes of weight and pos.  CTAS:
+// resident per SM, by registers: 3 while a head's keys are short, since then a
+// few hundred heads run at once (12 x 8 x 4 heads of 1025 slots: 14.3 us, 18.4
+// with 2); with long ones shared memory leaves no more anyway and the registers
+// are worth more (4 x 16 x 8 heads of 16001 slots: 155 us, 177 with 3).
+template <bool SMEM, bool VEC, int CTAS>
+__global__ void __launch_bounds__(kEvThreads, CTAS) kv4_evict_kernel(EvArgs a) {
   pdl_trigger();
   extern __shared__ __align__(16) uint32_t keys_sm[];
   __shared__ uint32_t hist[kEvBins];
   __shared__ uint32_t wsum[32];
-  __shared__ int s_max;
-  __shared__ uint32_t s_bin, s_need;
+  __shared__ int s_max, s_n;
+  __shared__ uint32_t s_lo, s_hi, s_bin, s_need, s_few;
   const Cache &c = a.c;
   const int h = blockIdx.x % c.nKV;
   const int64_t r = blockIdx.x / c.nKV;
   const int b = (int)(r % a.B);
   const int64_t l = r / a.B;
-  const int tid = threadIdx.x;
-  if (tid == 0) s_max = INT_MIN;
+  const int tid = threadIdx.x, lane = tid & 31;
+  constexpr int G = VEC ? 4 : 1;
   pdl_wait();
-  const int64_t len = a.lens[b];
-  const int n = (int)(len < 0 ? 0 : len > c.cap ? c.cap : len);
-  // a block that the cache does not have: the sequence stays as it is
-  int bad = 0;
-  if (c.table)
-    for (int64_t i = tid; i * c.bs < n; i += kEvThreads) bad |= block_of(c, b, i) < 0;
-  bad = __syncthreads_or(bad);
-  if (l == 0 && h == 0 && tid == 0) a.new_lens[b] = bad ? a.lens[b] : min(n, a.budget);
-  if (bad || n <= a.budget) return;
-  const int64_t lrow = l * c.blocks * c.nKV * c.bs;
-  uint32_t *keys = a.work ? a.work + (int64_t)blockIdx.x * c.cap : keys_sm;
-  int mx = INT_MIN;
-  for (int j = tid; j < n; j += kEvThreads) mx = max(mx, c.pos[lrow + row_of(c, b, h, j)]);
-  mx = __reduce_max_sync(0xffffffffu, mx);
-  if ((tid & 31) == 0) atomicMax(&s_max, mx);
-  __syncthreads();
-  const int64_t newest = (int64_t)s_max - a.recent;
-  for (int j = tid; j < n; j += kEvThreads) {
-    const int64_t row = lrow + row_of(c, b, h, j);
-    keys[j] = c.pos[row] > newest ? 0xffffffffu : weight_key(c.weight[row]);
+  if (tid == 0) {
+    s_max = INT_MIN, s_lo = 0xffffffffu, s_hi = 0, s_few = 0;
+    const int64_t len = a.lens[b];
+    s_n = (int)(len < 0 ? 0 : len > c.cap ? c.cap : len);      // one reader, so that the threads agree
   }
-  uint32_t prefix = 0, mask = 0, need = a.budget, equal = 0;
-  for (int pass = 0; pass < 3; pass++) {
-    const int bits = pass < 2 ? 11 : 10, shift = pass == 0 ? 21 : pass == 1 ? 10 : 0;
-    for (int i = tid; i < kEvBins; i += kEvThreads) hist[i] = 0;
-    __syncthreads();
-    for (int j = tid; j < n; j += kEvThreads) {
-      const uint32_t k = keys[j];
-      if ((k & mask) == prefix) atomicAdd(&hist[(k >> shift) & ((1u << bits) - 1)], 1u);
+  __syncthreads();
+  const int n = s_n;
+  const int64_t lrow = l * c.blocks * c.nKV * c.bs;
+  const bool cut = n > a.budget;
+  uint32_t *keys = SMEM ? keys_sm : a.keys + (int64_t)blockIdx.x * ev_at((int)c.cap);
+  // keys and the newest position; a block that the cache does not have leaves
+  // the sequence as it is
+  int bad = 0, mx = INT_MIN;
+  if (cut || (l == 0 && h == 0 && c.table)) {
+    for (int j0 = G * tid; j0 < n; j0 += kEvBatch * G * kEvThreads) {
+      float w[kEvBatch][G];
+      int p[kEvBatch][G];
+#pragma unroll
+      for (int i = 0; i < kEvBatch; i++) {
+        const int j = j0 + i * G * kEvThreads;
+        const int64_t at = j < n ? row_of(c, b, h, j) : -2;
+        bad |= at == -1;
+        load_slots<G>(w[i], c.weight + lrow + at, cut && at >= 0, 0.f);
+        load_slots<G>(p[i], c.pos + lrow + at, cut && at >= 0, INT_MIN);
+      }
+#pragma unroll
+      for (int i = 0; i < kEvBatch; i++)
+#pragma unroll
+        for (int e = 0; e < G; e++) {
+          const int j = j0 + i * G * kEvThreads + e;
+          if (cut && j < n) {
+            mx = max(mx, p[i][e]);
+            keys[ev_at(j)] = weight_key(w[i][e]);
+          }
+        }
     }
-    __syncthreads();
-    // bins from the largest down, two to a thread
-    const int hi = (1 << bits) - 1 - 2 * tid;
-    const uint32_t c0 = hi >= 0 ? hist[hi] : 0, c1 = hi >= 1 ? hist[hi - 1] : 0;
-    uint32_t total;
-    const uint32_t before = scan_excl(c0 + c1, wsum, &total);
-    if (before < need && need <= before + c0) s_bin = hi, s_need = need - before;
-    else if (before + c0 < need && need <= before + c0 + c1) s_bin = hi - 1, s_need = need - before - c0;
-    __syncthreads();
-    need = s_need;
-    equal = hist[s_bin];
-    prefix |= s_bin << shift;
-    mask |= ((1u << bits) - 1) << shift;
-    __syncthreads();
+    mx = __reduce_max_sync(0xffffffffu, mx);
+    if (lane == 0) atomicMax(&s_max, mx);
+    bad = __syncthreads_or(bad);
+  }
+  if (a.most && tid == 0 && (bad || !cut)) a.count[blockIdx.x] = 0;
+  if (l == 0 && h == 0 && tid == 0) a.new_lens[b] = bad ? n : min(n, a.budget);
+  if (bad || !cut) return;
+  // positions from `fresh` on are protected (none if there are no recent ones)
+  const int64_t first = (int64_t)s_max - a.recent + 1;
+  const int fresh = a.recent == 0 ? INT_MAX : first < INT_MIN ? INT_MIN : (int)first;
+  const bool some = a.recent > 0;
+  uint32_t lo = 0xffffffffu, hi = 0, safe = 0;      // the other slots' range; the protected ones
+  for (int j0 = G * tid; j0 < n; j0 += 2 * kEvBatch * G * kEvThreads) {
+    int p[2 * kEvBatch][G];
+#pragma unroll
+    for (int i = 0; i < 2 * kEvBatch; i++) {
+      const int j = j0 + i * G * kEvThreads;
+      load_slots<G>(p[i], c.pos + lrow + (j < n ? row_of(c, b, h, j) : 0), j < n, 0);
+    }
+#pragma unroll
+    for (int i = 0; i < 2 * kEvBatch; i++)
+#pragma unroll
+      for (int e = 0; e < G; e++) {
+        const int j = j0 + i * G * kEvThreads + e;
+        if (j >= n) continue;
+        if (some && p[i][e] >= fresh) {
+          keys[ev_at(j)] = 0xffffffffu;
+          safe++;
+        } else {
+          const uint32_t k = keys[ev_at(j)];
+          lo = min(lo, k);
+          hi = max(hi, k);
+        }
+      }
+  }
+  lo = __reduce_min_sync(0xffffffffu, lo);
+  hi = __reduce_max_sync(0xffffffffu, hi);
+  if (lane == 0) {
+    atomicMin(&s_lo, lo);
+    atomicMax(&s_hi, hi);
+  }
+  uint32_t protect;
+  scan_excl(safe, wsum, &protect);                  // (its barriers cover s_lo and s_hi)
+  lo = s_lo;
+  hi = s_hi;
+  // the threshold: keys above it stay, and `need` of the `equal` keys that are it
+  uint32_t prefix = 0xffffffffu, need = a.budget, equal = protect;
+  if (protect < (uint32_t)a.budget) {
+    need -= protect;                                // of the keys in [lo, hi]
+    while (true) {
+      const uint32_t span = hi - lo;
+      const int shift = span < kEvBins ? 0 : 21 - __clz(span);   // span >> shift < kEvBins
+      for (int i = tid; i < kEvBins; i += kEvThreads) hist[i] = 0;
+      __syncthreads();
+#pragma unroll 4
+      for (int j = tid; j < n; j += kEvThreads) {
+        const uint32_t k = keys[ev_at(j)] - lo;
+        if (k <= span) atomicAdd(&hist[k >> shift], 1u);
+      }
+      __syncthreads();
+      // bins from the largest down, four to a thread
+      uint32_t cnt[kEvBins / kEvThreads], sum = 0, total;
+#pragma unroll
+      for (int i = 0; i < kEvBins / kEvThreads; i++) {
+        cnt[i] = hist[kEvBins - 1 - (kEvBins / kEvThreads * tid + i)];
+        sum += cnt[i];
+      }
+      uint32_t before = scan_excl(sum, wsum, &total);
+#pragma unroll
+      for (int i = 0; i < kEvBins / kEvThreads; i++) {
+        if (before < need && need <= before + cnt[i]) {
+          s_bin = kEvBins - 1 - (kEvBins / kEvThreads * tid + i);
+          s_need = need - before;
+        }
+        before += cnt[i];
+      }
+      __syncthreads();
+      need = s_need;
+      equal = hist[s_bin];
+      lo += s_bin << shift;
+      hi = min(hi, lo + ((1u << shift) - 1));
+      prefix = lo;
+      __syncthreads();
+      if (shift == 0) break;
+      if (equal <= kEvFew) {
+        // the bin's keys, each ranked against the others; equal ones share a rank
+        for (int j = tid; j < n; j += kEvThreads) {
+          const uint32_t k = keys[ev_at(j)];
+          if (k - lo <= hi - lo) hist[atomicAdd(&s_few, 1u)] = k;
+        }
+        __syncthreads();
+        if (tid < (int)equal) {
+          const uint32_t k = hist[tid];
+          uint32_t above = 0, same = 0;
+          for (uint32_t i = 0; i < equal; i++) {
+            above += hist[i] > k;
+            same += hist[i] == k;
+          }
+          if (above < need && need <= above + same) {   // (by every thread that holds this key)
+            s_lo = k;
+            s_need = need - above;
+            s_bin = same;
+          }
+        }
+        __syncthreads();
+        prefix = s_lo;
+        need = s_need;
+        equal = s_bin;
+        break;
+      }
+    }
   }
   // kept: keys above the threshold, and of those equal to it the first `need`
-  // slots.  Freed slots below the budget and kept ones past it are listed in
-  // the key array itself: an entry's place is never past the slot it is for,
-  // and a tile's keys are read before its entries are written.
+  // slots.  A thread takes a run of up to 32 slots; the freed slots below the
+  // budget and the kept ones past it are listed in the key array itself: an
+  // entry's place is never past the slot it is for, and the runs' keys are read
+  // before their entries are written.
   uint32_t holes = 0, movers = 0, eq_before = 0;
-  for (int j0 = 0; j0 < n; j0 += kEvThreads) {
-    const int j = j0 + tid;
-    const uint32_t k = j < n ? keys[j] : 0;
-    const bool eq = j < n && k == prefix;
-    bool keep = j < n && (k > prefix || eq);
-    uint32_t total;
-    if (equal != need) {
-      const uint32_t er = eq_before + scan_excl(eq, wsum, &total);
-      if (eq) keep = er < need;
-      eq_before += total;
+  const int run = min(32, (n + kEvThreads - 1) / kEvThreads);
+  for (int j0 = 0; j0 < n; j0 += run * kEvThreads) {
+    const int j1 = j0 + tid * run;
+    uint32_t gt = 0, eq = 0;
+    if (run == 32) {
+      const uint32_t *p = keys + ev_at(j1);        // (a run does not cross a word of padding)
+#pragma unroll
+      for (int i = 0; i < 32; i++) {
+        const uint32_t k = j1 + i < n ? p[i] : 0;
+        gt |= k > prefix ? 1u << i : 0;
+        eq |= k == prefix ? 1u << i : 0;
+      }
+    } else {
+      for (int i = 0; i < run && j1 + i < n; i++) {
+        const uint32_t k = keys[ev_at(j1 + i)];
+        gt |= (uint32_t)(k > prefix) << i;
+        eq |= (uint32_t)(k == prefix) << i;
+      }
     }
-    const bool hole = j < a.budget && !keep, mover = j >= a.budget && keep;
-    const uint32_t at = scan_excl((uint32_t)hole | (uint32_t)mover << 16, wsum, &total);
-    if (hole) keys[holes + (at & 0xffffu)] = j;
-    if (mover) keys[a.budget + movers + (at >> 16)] = j;
+    const int below = min(max(a.budget - j1, 0), 32), inside = min(max(n - j1, 0), run);   // slots of the run
+    const uint32_t low = below == 32 ? 0xffffffffu : (1u << below) - 1;
+    const uint32_t real = inside == 32 ? 0xffffffffu : (1u << inside) - 1;
+    gt &= real;
+    eq &= real;
+    uint32_t total, keep = gt | eq;
+    if (equal != need) {
+      uint32_t er = eq_before + scan_excl(__popc(eq), wsum, &total);
+      eq_before += total;
+      keep = gt;
+      for (uint32_t m = eq; m && er < need; m &= m - 1, er++) keep |= m & -m;
+    }
+    uint32_t hole = ~keep & low & real, mover = keep & ~low & real;
+    uint32_t at = scan_excl((uint32_t)__popc(hole) | (uint32_t)__popc(mover) << 16, wsum, &total);
+    uint32_t ha = holes + (at & 0xffffu), ma = a.budget + movers + (at >> 16);
+    if (a.most) {
+      int32_t *to = a.to + (int64_t)blockIdx.x * a.most, *from = a.from + (int64_t)blockIdx.x * a.most - a.budget;
+      for (; hole; hole &= hole - 1) to[ha++] = j1 + __ffs(hole) - 1;
+      for (; mover; mover &= mover - 1) from[ma++] = j1 + __ffs(mover) - 1;
+    } else {
+      for (; hole; hole &= hole - 1) keys[ev_at(ha++)] = j1 + __ffs(hole) - 1;
+      for (; mover; mover &= mover - 1) keys[ev_at(ma++)] = j1 + __ffs(mover) - 1;
+    }
     holes += total & 0xffffu;
     movers += total >> 16;
   }
   __syncthreads();
+  if (a.most) {
+    if (tid == 0) a.count[blockIdx.x] = holes;
+    return;
+  }
+  // a thread takes one 16-byte piece of k or v, or the four words
   const int per = c.rb / 16, units = 2 * per + 1;
-  const uint32_t work = holes * units;
-  for (uint32_t i = tid; i < work; i += kEvThreads) {
+  for (uint32_t i = tid; i < holes * units; i += kEvThreads) {
     const uint32_t m = i / units, u = i - m * units;
-    const int64_t dst = lrow + row_of(c, b, h, keys[m]), src = lrow + row_of(c, b, h, keys[a.budget + m]);
+    const int64_t dst = lrow + row_of(c, b, h, keys[ev_at(m)]), src = lrow + row_of(c, b, h, keys[ev_at(a.budget + m)]);
     if (u < (uint32_t)(2 * per)) {
       uint8_t *x = u < (uint32_t)per ? c.k : c.v;
       const int q = u < (uint32_t)per ? u : u - per;
       reinterpret_cast<uint4 *>(x + dst * c.rb)[q] = reinterpret_cast<const uint4 *>(x + src * c.rb)[q];
     } else {
-      c.kg[dst] = c.kg[src];
-      c.vg[dst] = c.vg[src];
-      c.weight[dst] = c.weight[src];
-      c.pos[dst] = c.pos[src];
+      const uint32_t kg = c.kg[src], vg = c.vg[src];
+      const float w = c.weight[src];
+      const int p = c.pos[src];
+      c.kg[dst] = kg;
+      c.vg[dst] = vg;
+      c.weight[dst] = w;
+      c.pos[dst] = p;
     }
   }
+}
+
+// The moves, evenly over the GPU (a head's selection leaves it waiting for the
+// slowest): a warp takes 32 of a head's, a lane finds one's rows, and the lanes
+// then copy the rows' 16-byte pieces side by side.  Sources lie past the budget
+// and destinations below it, so loads may pass stores.
+constexpr int kMvThreads = 256;
+__global__ void __launch_bounds__(kMvThreads) kv4_move_kernel(EvArgs a) {
+  pdl_trigger();
+  const Cache &c = a.c;
+  const int chunks = (a.most + kMvThreads - 1) / kMvThreads, lane = threadIdx.x & 31;
+  const int64_t head = blockIdx.x / chunks;
+  const int m0 = (blockIdx.x - (int)(head * chunks)) * kMvThreads + (threadIdx.x & ~31);
+  const int h = (int)(head % c.nKV);
+  const int64_t r = head / c.nKV, b = r % a.B, lrow = r / a.B * c.blocks * c.nKV * c.bs;
+  pdl_wait();
+  const int count = (int)a.count[head];
+  if (m0 >= count) return;
+  const bool on = m0 + lane < count;
+  int64_t src = 0, dst = 0;
+  uint4 w;
+  if (on) {
+    src = lrow + row_of(c, b, h, a.from[head * a.most + m0 + lane]);
+    dst = lrow + row_of(c, b, h, a.to[head * a.most + m0 + lane]);
+    w = make_uint4(c.kg[src], c.vg[src], __float_as_uint(c.weight[src]), (uint32_t)c.pos[src]);
+  }
+  const int per = c.rb / 16, pieces = min(32, count - m0) * per;
+#pragma unroll
+  for (int v = 0; v < 2; v++) {
+    uint8_t *codes = v ? c.v : c.k;
+    for (int p0 = 0; p0 < pieces; p0 += 32 * kEvPieces) {
+      uint4 x[kEvPieces];
+      int64_t to[kEvPieces];
+#pragma unroll
+      for (int i = 0; i < kEvPieces; i++) {
+        const int p = p0 + 32 * i + lane, m = p / per, u = p - m * per;
+        const int64_t from = __shfl_sync(0xffffffffu, src, m & 31) * c.rb + 16 * u;
+        to[i] = __shfl_sync(0xffffffffu, dst, m & 31) * c.rb + 16 * u;
+        if (p < pieces) x[i] = *reinterpret_cast<const uint4 *>(codes + from);
+      }
+#pragma unroll
+      for (int i = 0; i < kEvPieces; i++)
+        if (p0 + 32 * i + lane < pieces) *reinterpret_cast<uint4 *>(codes + to[i]) = x[i];
+    }
+  }
+  if (on) {
+    c.kg[dst] = w.x;
+    c.vg[dst] = w.y;
+    c.weight[dst] = __uint_as_float(w.z);
+    c.pos[dst] = (int)w.w;
+  }
+}
+
+// Words of workspace: keys that do not fit in shared memory; the lists of moves
+// where a head can have more than kEvInline.
+struct EvWork {
+  int64_t keys, lists;
+  int most;
+};
+EvWork ev_work(const Cache &c, int B, int budget) {
+  const int64_t heads = c.layers * B * c.nKV, most = c.cap - budget < budget ? c.cap - budget : budget;
+  EvWork w;
+  w.keys = c.cap <= kEvSmemSlots ? 0 : heads * ev_at((int)c.cap);
+  w.most = most > kEvInline ? (int)most : 0;
+  w.lists = w.most ? heads * (2 * w.most + 1) : 0;
+  return w;
 }
 
 }  // namespace
@@ -466,10 +712,11 @@ int fcu_kv4_values(fcu_ctx *ctx, const fcu_kv4 *cache, const int32_t *start, int
   return FCU_OK;
 }
 
-int64_t fcu_kv4_evict_work(fcu_ctx *ctx, const fcu_kv4 *cache, int B) {
+int64_t fcu_kv4_evict_work(fcu_ctx *ctx, const fcu_kv4 *cache, int B, int budget) {
   Cache c;
-  if (!ctx || B < 0 || view("fcu_kv4_evict_work", cache, B, false, &c)) return -1;
-  return c.cap <= kEvSmemSlots ? 0 : c.layers * B * c.nKV * c.cap * 4;
+  if (!ctx || B < 0 || budget < 1 || view("fcu_kv4_evict_work", cache, B, false, &c)) return -1;
+  const EvWork w = ev_work(c, B, budget);
+  return 4 * (w.keys + w.lists);
 }
 
 int fcu_kv4_evict(fcu_ctx *ctx, const fcu_kv4 *cache, const int32_t *seq_lens, int B, int budget, int recent,
@@ -485,25 +732,42 @@ int fcu_kv4_evict(fcu_ctx *ctx, const fcu_kv4 *cache, const int32_t *seq_lens, i
   if (B == 0) return FCU_OK;
   FCU_REQUIRE(seq_lens && new_lens, "fcu_kv4_evict: null pointer");
   FCU_REQUIRE(new_lens + B <= seq_lens || seq_lens + B <= new_lens, "fcu_kv4_evict: new_lens overlaps seq_lens");
-  const int64_t need = fcu_kv4_evict_work(ctx, cache, B);
+  const EvWork w = ev_work(a.c, B, budget);
+  const int64_t need = 4 * (w.keys + w.lists), heads = a.c.layers * B * a.c.nKV;
   FCU_REQUIRE(need == 0 || (work && work_bytes >= need && ((uintptr_t)work & 3) == 0),
               "fcu_kv4_evict: workspace of %lld bytes, %lld needed", (long long)work_bytes, (long long)need);
-  const int64_t grid = a.c.layers * B * a.c.nKV;
-  FCU_REQUIRE(grid <= INT_MAX, "fcu_kv4_evict: %lld heads in one call", (long long)grid);
+  const int64_t moves = heads * ((w.most + kMvThreads - 1) / kMvThreads);
+  FCU_REQUIRE(heads <= INT_MAX && moves <= INT_MAX, "fcu_kv4_evict: %lld heads in one call", (long long)heads);
   a.lens = seq_lens;
   a.B = B;
   a.budget = budget;
   a.recent = recent;
   a.new_lens = new_lens;
-  a.work = need ? (uint32_t *)work : nullptr;
+  a.keys = (uint32_t *)work;
+  a.most = w.most;
+  if (w.most) {
+    a.count = a.keys + w.keys;
+    a.to = (int32_t *)(a.count + heads);
+    a.from = a.to + heads * w.most;
+  }
+  const bool vec = a.c.bs % 4 == 0 && (((uintptr_t)a.c.weight | (uintptr_t)a.c.pos) & 15) == 0;
+  void (*kernel)(EvArgs) = w.keys ? (vec ? kv4_evict_kernel<false, true, 2> : kv4_evict_kernel<false, false, 2>)
+                           : a.c.cap <= 8192 ? (vec ? kv4_evict_kernel<true, true, 3> : kv4_evict_kernel<true, false, 3>)
+                                             : (vec ? kv4_evict_kernel<true, true, 2> : kv4_evict_kernel<true, false, 2>);
   static bool set[64] = {false};
   if (!set[ctx->device & 63]) {
-    FCU_CHECK_CUDA(cudaFuncSetAttribute(kv4_evict_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                        (int)(kEvSmemSlots * 4)));
+    const int most = ev_at(kEvSmemSlots) * 4;
+    FCU_CHECK_CUDA(cudaFuncSetAttribute(kv4_evict_kernel<true, true, 2>, cudaFuncAttributeMaxDynamicSharedMemorySize, most));
+    FCU_CHECK_CUDA(cudaFuncSetAttribute(kv4_evict_kernel<true, false, 2>, cudaFuncAttributeMaxDynamicSharedMemorySize, most));
     set[ctx->device & 63] = true;
   }
-  FCU_CHECK_CUDA(launch_pdl(kv4_evict_kernel, dim3(grid), dim3(kEvThreads), need ? 0 : (size_t)a.c.cap * 4,
-                            ctx->stream, a));
+  const cudaError_t e = launch_pdl(kernel, dim3((unsigned)heads), dim3(kEvThreads),
+                                   w.keys ? 0 : (size_t)ev_at((int)a.c.cap) * 4, ctx->stream, a);
+  FCU_CHECK_CUDA(e);
+  if (moves) {
+    note_launch();
+    FCU_CHECK_CUDA(launch_pdl(kv4_move_kernel, dim3((unsigned)moves), dim3(kMvThreads), 0, ctx->stream, a));
+  }
   note_launch();
   return FCU_OK;
 }

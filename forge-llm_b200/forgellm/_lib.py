@@ -151,7 +151,7 @@ _SIGS = {
     "fcu_kv4_values": (_INT, [_P, C.POINTER(Kv4), _P, _INT, _INT, _P, _P]),
     "fcu_kv4_attn_work": (_I64, [_P, C.POINTER(Kv4), _INT, _INT]),
     "fcu_kv4_attn": (_INT, [_P, _P, _I64, C.POINTER(Kv4), _P, _INT, _INT, _D, _P, _P, _I64]),
-    "fcu_kv4_evict_work": (_I64, [_P, C.POINTER(Kv4), _INT]),
+    "fcu_kv4_evict_work": (_I64, [_P, C.POINTER(Kv4), _INT, _INT]),
     "fcu_kv4_evict": (_INT, [_P, C.POINTER(Kv4), _P, _INT, _INT, _INT, _P, _P, _I64]),
     "fcu_beam_work": (_I64, [_P, _INT, _INT, _I64]),
     "fcu_beam_step": (_INT, [_P, _P, _I64, _P, _P, _INT, _INT, _I64, _INT, _P, _P, _P, _P, _P, _I64]),

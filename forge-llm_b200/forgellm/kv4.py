@@ -219,7 +219,7 @@ def kv4Evict(k, kg, v, vg, weight, pos, lens, budget: int, recent: int, table=No
     else:
         _check("newLens", newLens, _I32, dev, tuple(lens.shape))
     h = _on(dev)
-    nbytes = lib().fcu_kv4_evict_work(h, c, B)
+    nbytes = lib().fcu_kv4_evict_work(h, c, B, budget)
     work = k.new_empty((nbytes,)).data_ptr() if nbytes > 0 else None
     _call("fcu_kv4_evict", h, c, lens.data_ptr(), B, budget, recent, newLens.data_ptr(), work, nbytes)
     return newLens

@@ -530,8 +530,8 @@ int64_t fcu_kv4_attn_work(fcu_ctx *ctx, const fcu_kv4 *cache, int B, int nH);
  * aligned) and may be reused once the call's work on the stream is done. */
 int fcu_kv4_attn(fcu_ctx *ctx, const float *q, int64_t ld_q, const fcu_kv4 *cache, const int32_t *seq_lens, int B,
                  int nH, double scale, float *out, void *work, int64_t work_bytes);
-/* Bytes of workspace fcu_kv4_evict needs; 0 if none. */
-int64_t fcu_kv4_evict_work(fcu_ctx *ctx, const fcu_kv4 *cache, int B);
+/* Bytes of workspace fcu_kv4_evict needs; 0 if none, -1 for bad arguments. */
+int64_t fcu_kv4_evict_work(fcu_ctx *ctx, const fcu_kv4 *cache, int B, int budget);
 /* Every (layer, sequence, kv head) of more than `budget` slots is cut down to
  * `budget`.  Slots whose pos is among the newest `recent` positions (pos >
  * max pos - recent) stay, then those of largest weight, ties to the lowest

@@ -74,7 +74,8 @@ def test_bad_arguments_are_refused(L, ctx):
                 dict(recent=9), dict(new=None), dict(new=4096), dict(new=4104)):
         assert ev(**bad) == ARG, bad
     long = cache(weight=4096, pos=4096, block_size=1 << 17, max_blocks=1, blocks=4)
-    assert L.fcu_kv4_evict_work(ctx, long, 4) == 4 * 2 * (1 << 17) * 4
+    assert L.fcu_kv4_evict_work(ctx, long, 4, 8) == 4 * 2 * ((1 << 17) + (1 << 12)) * 4
+    assert L.fcu_kv4_evict_work(ctx, long, 4, 1000) == 4 * 2 * ((1 << 17) + (1 << 12) + 2 * 1000 + 1) * 4
     assert ev(c=long) == ARG and ev(c=long, work=4096, n=100) == ARG
     beam = lambda **k: L.fcu_beam_step(*{**dict(ctx=ctx, x=4096, ld=100, s=4096, d=4096, B=2, W=4, V=100, eos=2,  # noqa: E731
                                                 os=8192, t=4096, p=4096, od=8192, work=4096, n=1 << 40), **k}.values())
@@ -115,7 +116,8 @@ def test_work_sizes_are_refused_for_bad_arguments(L, ctx):
     assert L.fcu_kv4_attn_work(None, cache(), 4, 4) == -1
     assert L.fcu_kv4_attn_work(ctx, cache(dH=3), 4, 4) == -1
     assert L.fcu_kv4_attn_work(ctx, cache(), 4, 3) == -1
-    assert L.fcu_kv4_evict_work(ctx, cache(), -1) == -1
+    assert L.fcu_kv4_evict_work(ctx, cache(), -1, 8) == -1
+    assert L.fcu_kv4_evict_work(ctx, cache(), 4, 0) == -1
     assert L.fcu_beam_work(ctx, 1, 33, 100) == -1
     assert L.fcu_beam_work(ctx, 1, 4, 0) == -1
 
