@@ -54,8 +54,11 @@ int view(const char *who, const fcu_kv4 *in, int64_t B, bool need_values, Cache 
 namespace {
 
 // ------------------------------------------------------------------ put
+// A CTA takes up to kPutTokens tokens of one sequence.  Bound by HBM for a
+// prompt's tokens (q both ways, k and v in), by latency for one token.
 constexpr int kPutThreads = 256;
-constexpr int kPutTokens = 8;    // tokens of one CTA, which share the frequencies' pow
+constexpr int kPutTokens = 8;    // share the frequencies' pow
+constexpr int kPutBatch = 4;     // 16-byte loads of q that a thread has in flight
 
 struct PutArgs {
   float *qkv;
@@ -67,183 +70,289 @@ struct PutArgs {
   int vec;             // rows and heads start on 16 bytes
 };
 
-// G lanes hold one head, 8 consecutive elements (one word of codes) each.
-template <int G>
-__global__ void __launch_bounds__(kPutThreads) kv4_put_kernel(PutArgs a) {
+// The rotation of neighbouring pairs by angles whose (cos, sin) are given, as a
+// rotation in double rounds to fp32.  The products' and the sum's errors are
+// carried along in fp32, about 2^-46 of the result in all, so that the roundings
+// agree but for results that near a tie (conversions to and from fp64 run at a
+// sixteenth of the rate and took a third of a prompt chunk's time); values that
+// leave fp32's normal range on the way take doubles.
+__device__ __forceinline__ float diff_of_products(float a, float b, float c, float d) {
+  const float p = a * b, pe = fmaf(a, b, -p), q = c * d, qe = fmaf(c, d, -q);
+  const float s = p - q, z = s - p, e = (p - (s - z)) - (q + z);
+  return s + (e + (pe - qe));
+}
+template <int N>
+__device__ __forceinline__ void rotate(float (&x)[N], const float2 (&w)[N / 2]) {
+  float lo = INFINITY, hi = 0.f;
+#pragma unroll
+  for (int u = 0; u < N; u += 2) {
+    const float m = fmaxf(fabsf(x[u]), fabsf(x[u + 1]));
+    lo = fminf(lo, m);
+    hi = fmaxf(hi, m);
+  }
+  float y[N], sum = 0.f;
+#pragma unroll
+  for (int u = 0; u < N; u += 2) {
+    y[u] = diff_of_products(x[u], w[u / 2].x, x[u + 1], w[u / 2].y);
+    y[u + 1] = diff_of_products(x[u], w[u / 2].y, -x[u + 1], w[u / 2].x);
+    sum += y[u] + y[u + 1];
+  }
+  if (!(lo > 0x1p-60f && hi < 0x1p120f && sum == sum)) {
+#pragma unroll
+    for (int u = 0; u < N; u += 2) {
+      const double p = x[u], q = x[u + 1], co = w[u / 2].x, s = w[u / 2].y;
+      y[u] = (float)(p * co - q * s);
+      y[u + 1] = (float)(p * s + q * co);
+    }
+  }
+#pragma unroll
+  for (int u = 0; u < N; u++) x[u] = y[u];
+}
+
+// FULL: a head has no padding (dH == 32 W).
+template <int W, bool FULL>
+__global__ void __launch_bounds__(kPutThreads, 4) kv4_put_kernel(PutArgs a) {
   pdl_trigger();
-  __shared__ double freq[kMaxDh / 2];
-  __shared__ float2 cs[kPutTokens][kMaxDh / 2];
+  __shared__ double freq[16 * W];
+  __shared__ float2 cs[kPutTokens][16 * W];
+  __shared__ int64_t row_s[kPutTokens];      // head 0's row of each token's slot; -1: the token changes nothing
   const Cache &c = a.c;
-  const int half = c.dH / 2, chunks = (a.T + a.tokens - 1) / a.tokens;
+  const int dH = FULL ? 32 * W : c.dH, half = dH / 2, chunks = (a.T + a.tokens - 1) / a.tokens, tid = threadIdx.x;
   const int64_t b = blockIdx.x / chunks;
   const int t0 = (blockIdx.x % chunks) * a.tokens;
   const int nt = min(a.tokens, a.T - t0);
   if (a.theta > 0)
-    for (int i = threadIdx.x; i < half; i += kPutThreads) freq[i] = 1.0 / pow(a.theta, (double)(2 * i) / c.dH);
+    for (int i = tid; i < half; i += kPutThreads) freq[i] = 1.0 / pow(a.theta, (double)(2 * i) / dH);
   pdl_wait();
   const int64_t pos0 = (int64_t)a.positions[b] + t0, slot0 = (int64_t)a.slots[b] + t0;
+  if (tid < nt) {
+    const int64_t j = slot0 + tid;
+    row_s[tid] = j >= 0 && j < c.cap && pos0 + tid >= 0 ? row_of(c, b, 0, j) : -1;
+  }
+  __syncthreads();
+  float *x0 = a.qkv + (b * a.T + t0) * a.ld;
   if (a.theta > 0) {
-    __syncthreads();
-    for (int i = threadIdx.x; i < nt * half; i += kPutThreads) {
+    for (int i = tid; i < nt * half; i += kPutThreads) {
       const int t = i / half, e = i - t * half;
       double s, co;
       sincos((double)(pos0 + t) * freq[e], &s, &co);
       cs[t][e] = make_float2((float)co, (float)s);
     }
     __syncthreads();
-  }
-  const int heads = a.nH + 2 * c.nKV, items = nt * heads;
-  const int li = threadIdx.x % G, e0 = li * 8;
-  // every lane of a warp stays in the loop for the shuffles
-  for (int i0 = threadIdx.x / G; i0 - (int)(threadIdx.x / G) < items; i0 += kPutThreads / G) {
-    const bool on = i0 < items;
-    const int t = on ? i0 / heads : 0, head = on ? i0 - t * heads : 0;
-    const int64_t j = slot0 + t;
-    int64_t row = -1;
-    if (on && j >= 0 && j < c.cap && pos0 + t >= 0) row = row_of(c, b, head < a.nH ? 0 : (head - a.nH) % c.nKV, j);
-    float *src = a.qkv + (b * a.T + t0 + t) * a.ld + (int64_t)head * c.dH + e0;
-    float x[8];
+    // q, four elements to a thread, the same ones of every token
+    if (a.vec) {
+      for (int i = tid; i < a.nH * (8 * W); i += kPutThreads) {
+        const int h = i / (8 * W), e = 4 * (i - h * 8 * W);
+        if (e >= dH) continue;
+        float *p = x0 + h * dH + e;
+        for (int t1 = 0; t1 < nt; t1 += kPutBatch) {
+          float4 x[kPutBatch];
 #pragma unroll
-    for (int u = 0; u < 8; u++) x[u] = 0.f;
-    if (row >= 0) {
-      if (a.vec) {
+          for (int k = 0; k < kPutBatch; k++)
+            if (t1 + k < nt && row_s[t1 + k] >= 0) x[k] = *reinterpret_cast<const float4 *>(p + (t1 + k) * a.ld);
 #pragma unroll
-        for (int u = 0; u < 8; u += 4)
-          if (e0 + u < c.dH) {
-            const float4 f = *reinterpret_cast<const float4 *>(src + u);
-            x[u] = f.x, x[u + 1] = f.y, x[u + 2] = f.z, x[u + 3] = f.w;
-          }
-      } else {
-#pragma unroll
-        for (int u = 0; u < 8; u++)
-          if (e0 + u < c.dH) x[u] = src[u];
+          for (int k = 0; k < kPutBatch; k++)
+            if (t1 + k < nt && row_s[t1 + k] >= 0) {
+              const float2 w[2] = {cs[t1 + k][e / 2], cs[t1 + k][e / 2 + 1]};
+              float y[4] = {x[k].x, x[k].y, x[k].z, x[k].w};
+              rotate(y, w);
+              *reinterpret_cast<float4 *>(p + (t1 + k) * a.ld) = make_float4(y[0], y[1], y[2], y[3]);
+            }
+        }
       }
-      if (a.theta > 0 && head < a.nH + c.nKV) {
-#pragma unroll
-        for (int u = 0; u < 8; u += 2)
-          if (e0 + u < c.dH) {
-            const float2 w = cs[t][(e0 + u) / 2];
-            const double p = x[u], q = x[u + 1], co = w.x, s = w.y;
-            x[u] = (float)(p * co - q * s);
-            x[u + 1] = (float)(p * s + q * co);
-          }
+    } else {
+      for (int i = tid; i < nt * a.nH * half; i += kPutThreads) {
+        const int th = i / half, e = i - th * half, t = th / a.nH, h = th - t * a.nH;
+        if (row_s[t] < 0) continue;
+        float *p = x0 + t * a.ld + (int64_t)h * dH + 2 * e, y[2] = {p[0], p[1]};
+        const float2 w[1] = {cs[t][e]};
+        rotate(y, w);
+        p[0] = y[0];
+        p[1] = y[1];
       }
     }
-    if (row >= 0 && head < a.nH) {
-      if (a.theta > 0) {
+  }
+  // k and v: G lanes hold one head of a token, eight consecutive elements (one
+  // word of codes) each; every lane of a warp stays in the loops for the shuffles
+  constexpr int G = W == 1 ? 4 : W == 2 ? 8 : W <= 4 ? 16 : 32;
+  const int heads = 2 * c.nKV, li = tid % G, e0 = li * 8;
+  for (int h0 = tid / G; h0 - tid / G < heads; h0 += kPutThreads / G) {
+    const bool on = h0 < heads, is_v = h0 >= c.nKV;
+    const float *src = x0 + (int64_t)(a.nH + h0) * dH + e0;
+    uint8_t *codes = is_v ? c.v : c.k;
+    uint32_t *grids = is_v ? c.vg : c.kg;
+    const int64_t head = (int64_t)(is_v ? h0 - c.nKV : h0) * c.bs;
+    for (int t = 0; t < nt; t++, src += a.ld) {
+      const int64_t row = on && row_s[t] >= 0 ? row_s[t] + head : -1;
+      float x[8];
+#pragma unroll
+      for (int u = 0; u < 8; u++) x[u] = 0.f;
+      if (row >= 0) {
         if (a.vec) {
 #pragma unroll
           for (int u = 0; u < 8; u += 4)
-            if (e0 + u < c.dH) *reinterpret_cast<float4 *>(src + u) = make_float4(x[u], x[u + 1], x[u + 2], x[u + 3]);
+            if (e0 + u < dH) {
+              const float4 f = *reinterpret_cast<const float4 *>(src + u);
+              x[u] = f.x, x[u + 1] = f.y, x[u + 2] = f.z, x[u + 3] = f.w;
+            }
         } else {
 #pragma unroll
           for (int u = 0; u < 8; u++)
-            if (e0 + u < c.dH) src[u] = x[u];
+            if (e0 + u < dH) x[u] = src[u];
+        }
+        if (a.theta > 0 && !is_v) {
+          if (e0 + 8 <= dH) {
+            const float2 w[4] = {cs[t][e0 / 2], cs[t][e0 / 2 + 1], cs[t][e0 / 2 + 2], cs[t][e0 / 2 + 3]};
+            rotate(x, w);
+          } else {
+#pragma unroll
+            for (int u = 0; u < 8; u += 2)
+              if (e0 + u < dH) {
+                float y[2] = {x[u], x[u + 1]};
+                const float2 w[1] = {cs[t][(e0 + u) / 2]};
+                rotate(y, w);
+                x[u] = y[0];
+                x[u + 1] = y[1];
+              }
+          }
         }
       }
-    }
-    float lo = INFINITY, hi = -INFINITY;
-    int bad = 0;
-#pragma unroll
-    for (int u = 0; u < 8; u++)
-      if (e0 + u < c.dH) {
-        lo = fminf(lo, x[u]);
-        hi = fmaxf(hi, x[u]);
-        bad |= !(fabsf(x[u]) < 0x1p127f);
-      }
-#pragma unroll
-    for (int o = G / 2; o > 0; o >>= 1) {
-      lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, o));
-      hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, o));
-      bad |= __shfl_xor_sync(0xffffffffu, bad, o);
-    }
-    if (row < 0 || head < a.nH) continue;
-    const __nv_bfloat16 base_b = __float2bfloat16_rn(lo);
-    const float base = __bfloat162float(base_b);
-    double range = (double)hi - (double)base;
-    range = range > 0 ? range : 0;
-    const __nv_bfloat16 step_b = __float2bfloat16_rn((float)(range / 15.0));
-    const float step = __bfloat162float(step_b);
-    uint32_t word = 0;
-    if (!bad && step > 0) {
-      const float inv = 1.0f / step;
+      float lo = INFINITY, hi = -INFINITY;
+      bool bad = false;
 #pragma unroll
       for (int u = 0; u < 8; u++)
-        if (e0 + u < c.dH) {
-          // The quotient in fp32 is within 4e-6 of the true one (at most 15.1
-          // here), so its rounding is the true one's unless it is that near
-          // a half; then, and where 1 / step left the normal range, divide in
-          // double.
-          const float d = x[u] - base, qf = d * inv, r = rintf(qf);
-          int code = (int)fminf(fmaxf(r, 0.f), 15.f);
-          if (!(fabsf(fabsf(qf - r) - 0.5f) > 1e-4f) || !(step > 1e-30f && step < 1e30f))
-            code = (int)fmin(fmax(rint(((double)x[u] - (double)base) / (double)step), 0.0), 15.0);
-          word |= (uint32_t)code << (4 * u);
+        if (e0 + u < dH) {
+          lo = fminf(lo, x[u]);
+          hi = fmaxf(hi, x[u]);
+          bad |= x[u] != x[u];
         }
-    }
-    const uint32_t grid = bad ? kNanGrid
-                              : (uint32_t)__bfloat16_as_ushort(step_b) | (uint32_t)__bfloat16_as_ushort(base_b) << 16;
-    const bool is_v = head >= a.nH + c.nKV;
-    if (4 * li < c.rb) reinterpret_cast<uint32_t *>((is_v ? c.v : c.k) + row * c.rb)[li] = word;
-    if (li == 0) {
-      (is_v ? c.vg : c.kg)[row] = grid;
-      if (!is_v) {
-        if (c.weight) c.weight[row] = 0.f;
-        if (c.pos) c.pos[row] = (int32_t)(pos0 + t);
+      if (bad) lo = -INFINITY;                      // (fminf passes a NaN over)
+#pragma unroll
+      for (int o = G / 2; o > 0; o >>= 1) {
+        lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, o));
+        hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, o));
+      }
+      if (row < 0) continue;
+      bad = !(lo > -0x1p127f && hi < 0x1p127f);
+      const __nv_bfloat16 base_b = __float2bfloat16_rn(lo);
+      const float base = __bfloat162float(base_b);
+      // step = bf16(fp32((hi - base) / 15)): the product below is within 4 units
+      // of its last place of that fp32 value, so it rounds to the same bf16 unless
+      // it is that near the middle of two
+      float q15 = fmaxf(hi - base, 0.f) * (1.0f / 15.0f);
+      if (abs((int)(__float_as_uint(q15) & 0xffffu) - 0x8000) <= 16 || q15 < 1e-30f) {
+        const double range = (double)hi - (double)base;
+        q15 = (float)((range > 0 ? range : 0.0) / 15.0);
+      }
+      const __nv_bfloat16 step_b = __float2bfloat16_rn(q15);
+      const float step = __bfloat162float(step_b);
+      uint32_t word = 0;
+      if (!bad && step > 0) {
+        // The quotient in fp32 is within 4e-6 of the true one (at most 15.1 here),
+        // so its rounding is the true one's unless it is that near a half; then,
+        // and where 1 / step left the normal range, divide in double.
+        const float inv = 1.0f / step;
+        float near = 1.f;
+#pragma unroll
+        for (int u = 0; u < 8; u++) {
+          const float q = fminf(fmaxf((x[u] - base) * inv, 0.f), 15.f), m = q + 0x1.8p23f;   // m: q rounded, ties to even
+          near = fminf(near, fabsf(fabsf(q - (m - 0x1.8p23f)) - 0.5f));
+          if (e0 + u < dH) word |= (__float_as_uint(m) & 15u) << (4 * u);
+        }
+        if (!(near > 1e-4f) || !(step > 1e-30f && step < 1e30f)) {
+          word = 0;
+#pragma unroll
+          for (int u = 0; u < 8; u++)
+            if (e0 + u < dH)
+              word |= (uint32_t)fmin(fmax(rint(((double)x[u] - (double)base) / (double)step), 0.0), 15.0) << (4 * u);
+        }
+      }
+      const uint32_t grid = bad ? kNanGrid
+                                : (uint32_t)__bfloat16_as_ushort(step_b) | (uint32_t)__bfloat16_as_ushort(base_b) << 16;
+      if (4 * li < c.rb) reinterpret_cast<uint32_t *>(codes + row * c.rb)[li] = word;
+      if (li == 0) {
+        grids[row] = grid;
+        if (!is_v) {
+          if (c.weight) c.weight[row] = 0.f;
+          if (c.pos) c.pos[row] = (int32_t)(pos0 + t);
+        }
       }
     }
   }
 }
 
 // ------------------------------------------------------------------ values
+// Four elements to a thread, one 16-byte store each of K and V.  Bound by HBM
+// (the values written).
 constexpr int kValThreads = 256;
+constexpr int kValBatch = 4;
+constexpr int kValTokens = 8;    // slots of a CTA
 
 struct ValArgs {
   Cache c;
   const int32_t *start;
-  int T, tokens, lanes_log;   // tokens per CTA; lanes of one row
+  int T;
   float *K, *V;
   int vec;
 };
 
+template <int W>
 __global__ void __launch_bounds__(kValThreads) kv4_values_kernel(ValArgs a) {
   pdl_trigger();
+  __shared__ int64_t row_s[kValTokens];      // head 0's row of each slot; -1: there is none
   const Cache &c = a.c;
-  const int chunks = (a.T + a.tokens - 1) / a.tokens;
+  const int chunks = (a.T + kValTokens - 1) / kValTokens;
   const int64_t b = blockIdx.x / chunks;
-  const int t0 = (blockIdx.x % chunks) * a.tokens;
-  const int nt = min(a.tokens, a.T - t0);
+  const int t0 = (blockIdx.x % chunks) * kValTokens;
+  const int nt = min(kValTokens, a.T - t0);
   pdl_wait();
-  const int64_t s0 = (int64_t)a.start[b] + t0;
-  const int items = (nt * c.nKV) << a.lanes_log, li = threadIdx.x & ((1 << a.lanes_log) - 1), e0 = 8 * li;
-  for (int i = threadIdx.x; i < items; i += kValThreads) {
-    const int r = i >> a.lanes_log, t = r / c.nKV, h = r - t * c.nKV;
-    if (e0 >= c.dH) continue;
-    const int64_t j = s0 + t;
-    const int64_t row = j >= 0 && j < c.cap ? row_of(c, b, h, j) : -1;
-    const int64_t o = (((int64_t)b * a.T + t0 + t) * c.nKV + h) * c.dH + e0;
+  if (threadIdx.x < nt) {
+    const int64_t j = (int64_t)a.start[b] + t0 + threadIdx.x;
+    row_s[threadIdx.x] = j >= 0 && j < c.cap ? row_of(c, b, 0, j) : -1;
+  }
+  __syncthreads();
+  const int kvd = c.nKV * c.dH;
+  // four elements to a thread, the same ones of every slot
+  for (int i = threadIdx.x; i < c.nKV * (8 * W); i += kValThreads) {
+    const int h = i / (8 * W), e = 4 * (i - h * 8 * W);
+    if (e >= c.dH) continue;
+    const int64_t o = (b * a.T + t0) * kvd + h * c.dH + e;
+    for (int t1 = 0; t1 < nt; t1 += kValBatch) {
+      uint32_t code[kValBatch][2], grid[kValBatch][2];
 #pragma unroll
-    for (int w = 0; w < 2; w++) {
-      float *out = w ? a.V : a.K;
-      if (!out) continue;
-      uint32_t word = 0, grid = kNanGrid;
-      if (row >= 0) {
-        word = reinterpret_cast<const uint32_t *>((w ? c.v : c.k) + row * c.rb)[li];
-        grid = (w ? c.vg : c.kg)[row];
+      for (int k = 0; k < kValBatch; k++) {
+        const int64_t row = t1 + k < nt && row_s[t1 + k] >= 0 ? row_s[t1 + k] + (int64_t)h * c.bs : -1;
+        code[k][0] = code[k][1] = 0;
+        grid[k][0] = grid[k][1] = kNanGrid;
+        if (row >= 0) {
+          code[k][0] = reinterpret_cast<const uint16_t *>(c.k + row * c.rb)[e / 4];
+          code[k][1] = reinterpret_cast<const uint16_t *>(c.v + row * c.rb)[e / 4];
+          grid[k][0] = c.kg[row];
+          grid[k][1] = c.vg[row];
+        }
       }
-      const float step = grid_step(grid), base = grid_base(grid);
-      float x[8];
 #pragma unroll
-      for (int u = 0; u < 8; u++) x[u] = base + step * (float)((word >> (4 * u)) & 15u);   // the product is exact
-      if (a.vec) {
+      for (int k = 0; k < kValBatch; k++)
 #pragma unroll
-        for (int u = 0; u < 8; u += 4)
-          if (e0 + u < c.dH) *reinterpret_cast<float4 *>(out + o + u) = make_float4(x[u], x[u + 1], x[u + 2], x[u + 3]);
-      } else {
+        for (int w = 0; w < 2; w++) {
+          float *out = w ? a.V : a.K;
+          if (t1 + k >= nt || !out) continue;
+          out += o + (int64_t)(t1 + k) * kvd;
+          const float step = grid_step(grid[k][w]), base = grid_base(grid[k][w]);
+          float x[4];
 #pragma unroll
-        for (int u = 0; u < 8; u++)
-          if (e0 + u < c.dH) out[o + u] = x[u];
-      }
+          for (int u = 0; u < 4; u++) {
+            const float code_f = __uint_as_float(((code[k][w] >> (4 * u)) & 15u) | 0x4b000000u) - 0x1p23f;
+            x[u] = base + step * code_f;                  // the product is exact
+          }
+          if (a.vec) {
+            *reinterpret_cast<float4 *>(out) = make_float4(x[0], x[1], x[2], x[3]);
+          } else {
+#pragma unroll
+            for (int u = 0; u < 4; u++)
+              if (e + u < c.dH) out[u] = x[u];
+          }
+        }
     }
   }
 }
@@ -649,6 +758,17 @@ EvWork ev_work(const Cache &c, int B, int budget) {
 using namespace fcu;
 using namespace fcu::kv4;
 
+// f(W) for rows of W 16-byte pieces
+#define FCU_KV4_ROWS(f, rb)   \
+  switch ((rb) / 16) {        \
+    case 1: f(1); break;      \
+    case 2: f(2); break;      \
+    case 3: f(3); break;      \
+    case 4: f(4); break;      \
+    case 6: f(6); break;      \
+    default: f(8); break;     \
+  }
+
 extern "C" {
 
 int fcu_kv4_row_bytes(int dH) { return dH < 2 || dH > kMaxDh || dH % 2 ? -1 : pad(dH) / 2; }
@@ -677,12 +797,12 @@ int fcu_kv4_put(fcu_ctx *ctx, float *qkv, int64_t ld_qkv, int B, int T, int nH, 
   a.vec = ld_qkv % 4 == 0 && a.c.dH % 4 == 0 && ((uintptr_t)qkv & 15) == 0;
   const int64_t grid = (int64_t)B * ((T + a.tokens - 1) / a.tokens);
   FCU_REQUIRE(grid <= INT_MAX, "fcu_kv4_put: %d x %d tokens in one call", B, T);
-  const int words = a.c.rb / 4;
-  cudaError_t e;
-  if (words <= 4) e = launch_pdl(kv4_put_kernel<4>, dim3(grid), dim3(kPutThreads), 0, ctx->stream, a);
-  else if (words <= 8) e = launch_pdl(kv4_put_kernel<8>, dim3(grid), dim3(kPutThreads), 0, ctx->stream, a);
-  else if (words <= 16) e = launch_pdl(kv4_put_kernel<16>, dim3(grid), dim3(kPutThreads), 0, ctx->stream, a);
-  else e = launch_pdl(kv4_put_kernel<32>, dim3(grid), dim3(kPutThreads), 0, ctx->stream, a);
+  cudaError_t e = cudaSuccess;
+#define FCU_CASE(W)                                                                                             \
+  e = launch_pdl(a.c.dH == 32 * W ? kv4_put_kernel<W, true> : kv4_put_kernel<W, false>, dim3((unsigned)grid), \
+                 dim3(kPutThreads), 0, ctx->stream, a)
+  FCU_KV4_ROWS(FCU_CASE, a.c.rb)
+#undef FCU_CASE
   FCU_CHECK_CUDA(e);
   note_launch();
   return FCU_OK;
@@ -701,13 +821,13 @@ int fcu_kv4_values(fcu_ctx *ctx, const fcu_kv4 *cache, const int32_t *start, int
   a.K = K;
   a.V = V;
   a.vec = a.c.dH % 4 == 0 && (((uintptr_t)K | (uintptr_t)V) & 15) == 0;
-  while ((1 << a.lanes_log) < a.c.rb / 4) a.lanes_log++;
-  // about four rounds of a CTA's threads
-  a.tokens = (4 * kValThreads >> a.lanes_log) / a.c.nKV;
-  a.tokens = a.tokens < 1 ? 1 : a.tokens > T ? T : a.tokens;
-  const int64_t grid = (int64_t)B * ((T + a.tokens - 1) / a.tokens);
+  const int64_t grid = (int64_t)B * ((T + kValTokens - 1) / kValTokens);
   FCU_REQUIRE(grid <= INT_MAX, "fcu_kv4_values: %d x %d tokens in one call", B, T);
-  FCU_CHECK_CUDA(launch_pdl(kv4_values_kernel, dim3(grid), dim3(kValThreads), 0, ctx->stream, a));
+  cudaError_t e = cudaSuccess;
+#define FCU_CASE(W) e = launch_pdl(kv4_values_kernel<W>, dim3((unsigned)grid), dim3(kValThreads), 0, ctx->stream, a)
+  FCU_KV4_ROWS(FCU_CASE, a.c.rb)
+#undef FCU_CASE
+  FCU_CHECK_CUDA(e);
   note_launch();
   return FCU_OK;
 }

@@ -229,6 +229,26 @@ __device__ __forceinline__ uint32_t grid_at(int x) {
   return 4 * ((x & 7) * C::kGridStride + (x >> 3));
 }
 
+// issue() for blocks that sixteen slots may straddle.
+template <class C, int W>
+__device__ __noinline__ void issue_scattered(const Cache &c, const uint8_t *codes, const uint32_t *grids, int64_t b, int h,
+                                             int j0, int cnt, uint8_t *part) {
+  const int lane = threadIdx.x & 31;
+  const uint32_t code_s = (uint32_t)__cvta_generic_to_shared(part), grid_s = code_s + C::kCodes;
+  for (int x = lane; x < C::kTile; x += 32) {
+    const uint32_t at = grid_at<C>(x);
+    const int64_t row = x < cnt ? row_of(c, b, h, j0 + x) : -1;
+    if (row >= 0 || x >= cnt) cp_async4(grid_s + at, row >= 0 ? grids + row : grids, row >= 0);
+    else *reinterpret_cast<uint32_t *>(part + C::kCodes + at) = kNanGrid;
+  }
+  for (int x = lane; x < C::kTile * W; x += 32) {
+    const int j = x / W;
+    const int64_t row = j < cnt ? row_of(c, b, h, j0 + j) : -1;
+    cp_async16(code_s + 16 * (W % 2 == 0 ? x - x % W + (x % W ^ swizzle<W>(j)) : x),
+               row >= 0 ? codes + row * C::kRow + 16 * (x - j * W) : codes, row >= 0);
+  }
+}
+
 // Starts the copies of one tile's k or v (slots j0 .. j0 + cnt of head h of
 // sequence b) into shared memory.  Slots past cnt are zero; those of a bad block
 // have NaN grids.
@@ -251,30 +271,30 @@ __device__ __forceinline__ void issue(const Cache &c, const uint8_t *codes, cons
     const uint32_t *g = grids + row + lane;
 #pragma unroll
     for (int i = 0; i < C::kTile / 32; i++) cp_async4(grid_s + grid_at<C>(lane) + 16 * i, g + 32 * i, true);
-  } else {
-    int64_t rows[C::kTile / 32];        // of slots lane and lane + 32
+  } else if (c.bs % 16 == 0) {
+    // sixteen slots at a time lie in one block: lane i finds the i-th sixteen's
+    // first row
+    int64_t first = -1;
+    if (16 * lane < cnt) first = row_of(c, b, h, j0 + 16 * lane);
 #pragma unroll
     for (int i = 0; i < C::kTile / 32; i++) {
       const int x = i * 32 + lane;
-      rows[i] = x < cnt ? row_of(c, b, h, j0 + x) : -1;
+      const int64_t row = __shfl_sync(0xffffffffu, first, x >> 4);
       const uint32_t at = grid_at<C>(x);
-      if (rows[i] >= 0 || x >= cnt) cp_async4(grid_s + at, rows[i] >= 0 ? grids + rows[i] : grids, rows[i] >= 0);
+      const bool on = row >= 0 && x < cnt;
+      if (on || x >= cnt) cp_async4(grid_s + at, on ? grids + row + (x & 15) : grids, on);
       else *reinterpret_cast<uint32_t *>(part + C::kCodes + at) = kNanGrid;
     }
 #pragma unroll
     for (int i = 0; i < C::kTile * W / 32; i++) {
       const int x = i * 32 + lane, j = x / W;
-      // the warp's pieces x are of slots that at most two of the rows[] hold
-      constexpr int kLast = C::kTile / 32 - 1;
-      const int lo = i * 32 / W / 32, hi = (i * 32 + 31) / W / 32;
-      int64_t row = __shfl_sync(0xffffffffu, rows[lo < kLast ? lo : kLast], j & 31);
-      if (hi != lo) {
-        const int64_t up = __shfl_sync(0xffffffffu, rows[hi < kLast ? hi : kLast], j & 31);
-        if (j >= 32 * hi) row = up;
-      }
+      const int64_t row = __shfl_sync(0xffffffffu, first, j >> 4);
+      const bool on = row >= 0 && j < cnt;
       cp_async16(code_s + 16 * (W % 2 == 0 ? x - x % W + (x % W ^ swizzle<W>(j)) : x),
-                 row >= 0 ? codes + row * C::kRow + 16 * (x - j * W) : codes, row >= 0);
+                 on ? codes + row * C::kRow + 16 * (x - (j & ~15) * W) : codes, on);
     }
+  } else {
+    issue_scattered<C, W>(c, codes, grids, b, h, j0, cnt, part);
   }
 }
 
@@ -702,10 +722,13 @@ struct Pieces {
   }
 };
 
-// What is left when all runs are done.  The first (ctas - 1) gs blocks merge
-// the pieces of the segment that begins in run blockIdx.x / gs and goes past its
-// end, one head each; where weights are kept the others add them up,
+// What is left when all runs are done.  The first ctas - 1 blocks merge the
+// pieces of the segments that begin in a run and go past its end: block i those
+// of run i, a warp to a head, if they are at most kFewPieces; a segment of more
+// pieces has as many runs to itself, and block i + d takes its d-th head, all
+// warps together.  Where weights are kept the other blocks add them up,
 // weight_j += sum over the group's q heads of p_j, kWtSlots slots each.
+constexpr int kFewPieces = 12;
 constexpr int kFinishThreads = 256;
 constexpr int kFinishWarps = kFinishThreads / 32;
 constexpr int kWtSlots = 1024;
@@ -715,20 +738,31 @@ __global__ void __launch_bounds__(kFinishThreads) kv4_attn_finish_kernel(AttnArg
   __shared__ float o_s[kFinishWarps][32 * W];
   __shared__ float m_s[kMaxGroup], il_s[kMaxGroup];
   const Cache &c = a.c;
-  const int dH = c.dH, lane = threadIdx.x & 31, warp = threadIdx.x >> 5, merges = (a.ctas - 1) * a.gs;
+  const int dH = c.dH, lane = threadIdx.x & 31, warp = threadIdx.x >> 5, merges = a.ctas - 1;
   pdl_wait();
   if (blockIdx.x < merges) {
-    const int run = blockIdx.x / a.gs, hd = blockIdx.x - run * a.gs;
-    const Cut cut = a.cuts[run];
-    if (cut.pieces == 0 || hd >= cut.heads) return;
+    Cut cut{0, 0, 0};
+    const int run0 = (int)blockIdx.x - lane;
+    if (lane < kMaxHeads && run0 >= 0) cut = a.cuts[run0];
+    const bool mine = lane == 0 ? cut.pieces > 0 : cut.pieces > kFewPieces && lane < cut.heads;
+    const uint32_t who = __ballot_sync(0xffffffffu, mine);
+    if (!who) return;
+    const int d = __ffs(who) - 1, run = (int)blockIdx.x - d;
+    cut.pieces = __shfl_sync(0xffffffffu, cut.pieces, d);
+    cut.heads = __shfl_sync(0xffffffffu, cut.heads, d);
+    cut.bh = __shfl_sync(0xffffffffu, cut.bh, d);
     const int pieces = min(cut.pieces, a.ctas - run);
+    const bool few = cut.pieces <= kFewPieces;
+    // few: a warp takes a head; else each warp its share of the pieces of head d.
+    // Everything of a piece is asked for at once.
+    const int hd = few ? warp : d;
+    if (few && hd >= cut.heads) return;
     const Pieces part(a, run, hd);
-    // each warp its share of the pieces; everything of a piece is asked for at once
     float M = -INFINITY, L = 0.f, O[W];
 #pragma unroll
     for (int i = 0; i < W; i++) O[i] = 0.f;
 #pragma unroll(W <= 2 ? 8 : W <= 4 ? 4 : 2)
-    for (int p = warp; p < pieces; p += kFinishWarps) {
+    for (int p = few ? 0 : warp; p < pieces; p += few ? 1 : kFinishWarps) {
       const float *x = part[p];
       const float m = x[dH], l = x[dH + 1];
       float o[W];
@@ -740,23 +774,29 @@ __global__ void __launch_bounds__(kFinishThreads) kv4_attn_finish_kernel(AttnArg
 #pragma unroll
       for (int i = 0; i < W; i++) O[i] = O[i] * f0 + o[i] * f1;
     }
+    float *out = a.out + (cut.bh + hd) * dH;
+    if (few) {
+#pragma unroll
+      for (int i = 0; i < W; i++)
+        if (lane + 32 * i < dH) out[lane + 32 * i] = O[i] / L;
+      return;
+    }
     if (lane == 0) {
       m_s[warp] = M;
       il_s[warp] = L;
     }
 #pragma unroll
-    for (int i = 0; i < W; i++)
-      if (lane + 32 * i < dH) o_s[warp][lane + 32 * i] = O[i];
+    for (int i = 0; i < W; i++) o_s[warp][lane + 32 * i] = O[i];
     __syncthreads();
-    const int warps = min(pieces, kFinishWarps);
     M = m_s[0];
-    for (int w = 1; w < warps; w++) M = fmaxf(M, m_s[w]);
+    for (int w = 1; w < kFinishWarps; w++) M = fmaxf(M, m_s[w]);
     L = 0.f;
-    for (int w = 0; w < warps; w++) L += il_s[w] * ex2(m_s[w] - M);
+    for (int w = 0; w < kFinishWarps; w++) L += il_s[w] * ex2(m_s[w] - M);
     for (int e = threadIdx.x; e < dH; e += kFinishThreads) {
       float o = 0.f;
-      for (int w = 0; w < warps; w++) o = fmaf(o_s[w][e], ex2(m_s[w] - M), o);
-      a.out[(cut.bh + hd) * dH + e] = o / L;
+#pragma unroll
+      for (int w = 0; w < kFinishWarps; w++) o = fmaf(o_s[w][e], ex2(m_s[w] - M), o);
+      out[e] = o / L;
     }
     return;
   }
@@ -832,8 +872,7 @@ int launch(fcu_ctx *ctx, const AttnArgs &a) {
   }
   FCU_CHECK_CUDA(launch_pdl(kv4_attn_kernel<W, G>, dim3(a.ctas), dim3(kThreads), C::kSmem, ctx->stream, a));
   note_launch();
-  const int64_t blocks = (int64_t)(a.ctas - 1) * a.gs +
-                         (a.scores ? (int64_t)a.B * a.c.nKV * ((a.c.cap + kWtSlots - 1) / kWtSlots) : 0);
+  const int64_t blocks = a.ctas - 1 + (a.scores ? (int64_t)a.B * a.c.nKV * ((a.c.cap + kWtSlots - 1) / kWtSlots) : 0);
   if (blocks > 0) {
     FCU_CHECK_CUDA(launch_pdl(kv4_attn_finish_kernel<W>, dim3((unsigned)blocks), dim3(kFinishThreads), 0, ctx->stream, a));
     note_launch();
