@@ -761,18 +761,34 @@ __global__ void __launch_bounds__(kFinishThreads) kv4_attn_finish_kernel(AttnArg
     float M = -INFINITY, L = 0.f, O[W];
 #pragma unroll
     for (int i = 0; i < W; i++) O[i] = 0.f;
-#pragma unroll(W <= 2 ? 8 : W <= 4 ? 4 : 2)
-    for (int p = few ? 0 : warp; p < pieces; p += few ? 1 : kFinishWarps) {
-      const float *x = part[p];
-      const float m = x[dH], l = x[dH + 1];
-      float o[W];
+    constexpr int kBatch = W <= 2 ? 8 : W <= 4 ? 4 : 2;
+    const int stride = few ? 1 : kFinishWarps;
+    for (int p0 = few ? 0 : warp; p0 < pieces; p0 += kBatch * stride) {
+      float m[kBatch], l[kBatch], o[kBatch][W];
 #pragma unroll
-      for (int i = 0; i < W; i++) o[i] = lane + 32 * i < dH ? x[lane + 32 * i] : 0.f;
-      const float m1 = fmaxf(M, m), f0 = L == 0.f ? 0.f : ex2(M - m1), f1 = ex2(m - m1);
-      L = L * f0 + l * f1;
+      for (int k = 0; k < kBatch; k++) {
+        const int p = p0 + k * stride;
+        const float *x = part[min(p, pieces - 1)];
+        m[k] = p < pieces ? x[dH] : -INFINITY;
+        l[k] = p < pieces ? x[dH + 1] : 0.f;
+#pragma unroll
+        for (int i = 0; i < W; i++) o[k][i] = p < pieces && lane + 32 * i < dH ? x[lane + 32 * i] : 0.f;
+      }
+      float m1 = M;
+#pragma unroll
+      for (int k = 0; k < kBatch; k++) m1 = fmaxf(m1, m[k]);
+      const float f0 = L == 0.f ? 0.f : ex2(M - m1);
       M = m1;
+      L *= f0;
 #pragma unroll
-      for (int i = 0; i < W; i++) O[i] = O[i] * f0 + o[i] * f1;
+      for (int i = 0; i < W; i++) O[i] *= f0;
+#pragma unroll
+      for (int k = 0; k < kBatch; k++) {
+        const float f = p0 + k * stride < pieces ? ex2(m[k] - m1) : 0.f;
+        L = fmaf(l[k], f, L);
+#pragma unroll
+        for (int i = 0; i < W; i++) O[i] = fmaf(o[k][i], f, O[i]);
+      }
     }
     float *out = a.out + (cut.bh + hd) * dH;
     if (few) {
@@ -805,6 +821,20 @@ __global__ void __launch_bounds__(kFinishThreads) kv4_attn_finish_kernel(AttnArg
   const int h = (int)(bk - b * c.nKV);
   const int64_t n = length(a, b);
   if (j0 >= n) return;
+  // what does not wait for (m, l) is asked for first
+  constexpr int kPer = kWtSlots / kFinishThreads, kAhead = 4;
+  const float *sc = a.scores + (b * a.nH + h * a.g) * c.cap + j0 + threadIdx.x;
+  float w[kPer], old[kPer], s[kAhead][kPer];
+  int64_t row[kPer];
+#pragma unroll
+  for (int x = 0; x < kPer; x++) {
+    const int64_t j = j0 + threadIdx.x + x * kFinishThreads;
+    row[x] = j < n ? row_of(c, b, h, j) : -1;
+    old[x] = row[x] >= 0 ? c.weight[row[x]] : 0.f;
+    w[x] = 0.f;
+#pragma unroll
+    for (int i = 0; i < kAhead; i++) s[i][x] = i < a.g && row[x] >= 0 ? sc[i * c.cap + x * kFinishThreads] : 0.f;
+  }
   for (int hd = warp; hd < a.g; hd += kFinishWarps) {
     float2 x = a.ml[b * a.nH + h * a.g + hd];
     // a cut segment's: the run it begins in, and minus its pieces
@@ -818,22 +848,19 @@ __global__ void __launch_bounds__(kFinishThreads) kv4_attn_finish_kernel(AttnArg
     }
   }
   __syncthreads();
-  const float *sc = a.scores + (b * a.nH + h * a.g) * c.cap;
-  float w[kWtSlots / kFinishThreads], old[kWtSlots / kFinishThreads];
-  int64_t row[kWtSlots / kFinishThreads];
+  for (int hd = 0; hd < a.g; hd += kAhead) {
 #pragma unroll
-  for (int x = 0; x < kWtSlots / kFinishThreads; x++) {
-    const int64_t j = j0 + threadIdx.x + x * kFinishThreads;
-    row[x] = j < n ? row_of(c, b, h, j) : -1;
-    old[x] = row[x] >= 0 ? c.weight[row[x]] : 0.f;
-    w[x] = 0.f;
+    for (int i = 0; i < kAhead; i++)
+      if (hd + i < a.g) {
+#pragma unroll
+        for (int x = 0; x < kPer; x++) {
+          w[x] = fmaf(ex2(s[i][x] - m_s[hd + i]), il_s[hd + i], w[x]);
+          s[i][x] = hd + i + kAhead < a.g && row[x] >= 0 ? sc[(hd + i + kAhead) * c.cap + x * kFinishThreads] : 0.f;
+        }
+      }
   }
-  for (int hd = 0; hd < a.g; hd++)
 #pragma unroll
-    for (int x = 0; x < kWtSlots / kFinishThreads; x++)
-      if (row[x] >= 0) w[x] = fmaf(ex2(sc[hd * c.cap + j0 + threadIdx.x + x * kFinishThreads] - m_s[hd]), il_s[hd], w[x]);
-#pragma unroll
-  for (int x = 0; x < kWtSlots / kFinishThreads; x++)
+  for (int x = 0; x < kPer; x++)
     if (row[x] >= 0) c.weight[row[x]] = old[x] + w[x];
 }
 
