@@ -48,16 +48,28 @@ def _on(dev: int):
 
 
 def _device() -> int:
-    if not torch.cuda.is_initialized():
+    try:
+        return torch.cuda.current_device()
+    except Exception:
         device()                        # no CUDA device: the package's error
-        torch.cuda.init()
-    return torch.cuda.current_device()
+        raise
 
 
 def _call(name: str, *args) -> None:
-    rc = getattr(lib(), name)(*args)
+    rc = _FN[name](*args)
     if rc:
         check(rc, name)
+
+
+class _Functions(dict):
+    """The library's functions by name, each looked up once."""
+
+    def __missing__(self, name):
+        fn = self[name] = getattr(lib(), name)
+        return fn
+
+
+_FN = _Functions()
 
 
 def _ok(t, dtype, dev: int) -> bool:
@@ -66,22 +78,25 @@ def _ok(t, dtype, dev: int) -> bool:
 
 def _check(name: str, t, dtype, dev: int, shape=None) -> None:
     """t is a contiguous tensor of `dtype` (and `shape`) on device `dev`."""
-    if not isinstance(t, torch.Tensor) or t.dtype != dtype:
+    if isinstance(t, torch.Tensor) and t.dtype is dtype and t.get_device() == dev and t.is_contiguous() and (
+            shape is None or t.shape == shape):
+        return
+    if not isinstance(t, torch.Tensor) or t.dtype is not dtype:
         raise ValueError(f"{name}: a {dtype} tensor is needed, got "
                          f"{t.dtype if isinstance(t, torch.Tensor) else type(t).__name__}")
     if t.get_device() != dev:
         raise ValueError(f"{name} is on {t.device}, not on the current CUDA device")
-    if shape is not None and tuple(t.shape) != shape:
-        raise ValueError(f"{name}: shape {tuple(t.shape)}, {shape} is needed")
-    if not t.is_contiguous():
-        raise ValueError(f"{name} is not contiguous")
+    if shape is not None and t.shape != shape:
+        raise ValueError(f"{name}: shape {tuple(t.shape)}, {tuple(shape)} is needed")
+    raise ValueError(f"{name} is not contiguous")
 
 
 def _row_bytes(dHead: int) -> int:
     rb = _ROW_BYTES.get(dHead)
     if rb is None:
-        rb = lib().fcu_kv4_row_bytes(int(dHead))
-        _need(rb > 0, f"head dim {dHead}: even, 2 to 256")
+        rb = _FN["fcu_kv4_row_bytes"](int(dHead))
+        if rb <= 0:
+            raise ValueError(f"head dim {dHead}: even, 2 to 256")
         _ROW_BYTES[dHead] = rb
     return rb
 
@@ -89,29 +104,32 @@ def _row_bytes(dHead: int) -> int:
 def _cache(dev, k, kg, v, vg, dHead, B, table, weight=None, pos=None, layers=False) -> Kv4:
     """The C-ABI's view of one layer's arrays (five dimensions: of all layers)."""
     rb = _row_bytes(dHead)
-    ndim = 5 if layers else 4
-    if not (isinstance(k, torch.Tensor) and isinstance(v, torch.Tensor) and isinstance(kg, torch.Tensor)
-            and isinstance(vg, torch.Tensor) and len(k.shape) == ndim and k.shape[-1] == rb and k.shape == v.shape and kg.shape == vg.shape
-            and kg.shape[:-1] == k.shape[:-1] and kg.shape[-1] == 2 and _ok(k, _U8, dev) and _ok(v, _U8, dev)
-            and _ok(kg, _BF, dev) and _ok(vg, _BF, dev)):
+    shape = k.shape
+    lead = shape[:-1]
+    if not (v.shape == shape and len(shape) == (5 if layers else 4) and shape[-1] == rb and kg.shape == vg.shape
+            and kg.shape == (*lead, 2) and _ok(k, _U8, dev) and _ok(v, _U8, dev) and _ok(kg, _BF, dev)
+            and _ok(vg, _BF, dev)):
         _check("k", k, _U8, dev)
-        _need(k.ndim == ndim, f"k: {k.ndim} dimensions")
-        _need(k.shape[-1] == rb, f"k: rows of {k.shape[-1]} bytes, head dim {dHead} has {rb}")
-        _check("v", v, _U8, dev, tuple(k.shape))
-        _check("kg", kg, _BF, dev, (*k.shape[:-1], 2))
-        _check("vg", vg, _BF, dev, (*k.shape[:-1], 2))
-    lead = k.shape[:-1]
+        if k.ndim != (5 if layers else 4):
+            raise ValueError(f"k: {k.ndim} dimensions")
+        if shape[-1] != rb:
+            raise ValueError(f"k: rows of {shape[-1]} bytes, head dim {dHead} has {rb}")
+        _check("v", v, _U8, dev, shape)
+        _check("kg", kg, _BF, dev, (*lead, 2))
+        _check("vg", vg, _BF, dev, (*lead, 2))
     if weight is not None:
-        _check("weight", weight, _F32, dev, tuple(lead))
+        _check("weight", weight, _F32, dev, lead)
     if pos is not None:
-        _check("pos", pos, _I32, dev, tuple(lead))
+        _check("pos", pos, _I32, dev, lead)
     blocks, nKV, bs = lead[-3:]
     if table is not None:
         _check("table", table, _I32, dev)
-        _need(table.ndim == 2 and table.shape[0] == B, f"table: shape {tuple(table.shape)} for {B} sequences")
+        if table.ndim != 2 or table.shape[0] != B:
+            raise ValueError(f"table: shape {tuple(table.shape)} for {B} sequences")
         mb = table.shape[1]
     else:
-        _need(blocks % max(B, 1) == 0, f"{blocks} blocks do not divide among {B} sequences")
+        if blocks % max(B, 1):
+            raise ValueError(f"{blocks} blocks do not divide among {B} sequences")
         mb = blocks // max(B, 1)
     return Kv4(k.data_ptr(), v.data_ptr(), kg.data_ptr(), vg.data_ptr(),
                weight.data_ptr() if weight is not None else None, pos.data_ptr() if pos is not None else None,
@@ -148,13 +166,16 @@ def kv4Put(qkv, nHeads: int, positions, slots, k, kg, v, vg, T: int = 1, theta: 
     _check("positions", positions, _I32, dev)
     B = positions.numel()
     _check("slots", slots, _I32, dev)
-    _need(slots.numel() == B, f"{slots.numel()} slots for {B} sequences")
-    _need(T >= 1 and nHeads >= 0 and theta >= 0, f"T={T}, nHeads={nHeads}, theta={theta}")
-    _need(k.ndim == 4, f"k: {k.ndim} dimensions")
+    if slots.numel() != B:
+        raise ValueError(f"{slots.numel()} slots for {B} sequences")
+    if T < 1 or nHeads < 0 or not theta >= 0:
+        raise ValueError(f"T={T}, nHeads={nHeads}, theta={theta}")
+    if k.ndim != 4:
+        raise ValueError(f"k: {k.ndim} dimensions")
     heads = nHeads + 2 * k.shape[1]
     ld = _rows("qkv", qkv, dev)
-    _need(qkv.shape[0] == B * T and qkv.shape[1] % heads == 0,
-          f"qkv: shape {tuple(qkv.shape)} for {B} x {T} tokens of {heads} heads")
+    if qkv.shape[0] != B * T or qkv.shape[1] % heads:
+        raise ValueError(f"qkv: shape {tuple(qkv.shape)} for {B} x {T} tokens of {heads} heads")
     c = _cache(dev, k, kg, v, vg, qkv.shape[1] // heads, B, table, weight, pos)
     _call("fcu_kv4_put", _on(dev), qkv.data_ptr(), ld, B, T, nHeads, float(theta), positions.data_ptr(),
          slots.data_ptr(), c)
@@ -166,7 +187,8 @@ def kv4Values(k, kg, v, vg, dHead: int, start, T: int, table=None):
     dev = _device()
     _check("start", start, _I32, dev)
     B = start.numel()
-    _need(T >= 0, f"T={T}")
+    if T < 0:
+        raise ValueError(f"T={T}")
     c = _cache(dev, k, kg, v, vg, dHead, B, table)
     K, V = k.new_empty((2, B, T, c.n_kv, dHead), dtype=_F32).unbind(0)
     _call("fcu_kv4_values", _on(dev), c, start.data_ptr(), B, T, K.data_ptr(), V.data_ptr())
@@ -180,13 +202,16 @@ def kv4Attention(q, k, kg, v, vg, lens, scale: float | None = None, table=None, 
     unless given.  With `weight`, every slot's attention weight, summed over its
     kv head's q heads, is added to it."""
     dev = _device()
-    _need(isinstance(q, torch.Tensor) and q.dtype is _F32 and q.ndim == 3, "q: a float32 [B, nHeads, dHead] is needed")
+    if not (isinstance(q, torch.Tensor) and q.dtype is _F32 and q.ndim == 3):
+        raise ValueError("q: a float32 [B, nHeads, dHead] is needed")
     B, nH, dH = q.shape
-    _need(q.get_device() == dev, "q is not on the current CUDA device")
+    if q.get_device() != dev:
+        raise ValueError("q is not on the current CUDA device")
     ld = nH * dH
     if not q.is_contiguous():
         s = q.stride()
-        _need((dH == 1 or s[2] == 1) and (nH == 1 or s[1] == dH) and (B == 1 or s[0] >= ld), f"q: strides {s}")
+        if not ((dH == 1 or s[2] == 1) and (nH == 1 or s[1] == dH) and (B == 1 or s[0] >= ld)):
+            raise ValueError(f"q: strides {s}")
         ld = s[0] if B > 1 else ld
     _check("lens", lens, _I32, dev, (B,))
     c = _cache(dev, k, kg, v, vg, dH, B, table, weight)
@@ -194,12 +219,14 @@ def kv4Attention(q, k, kg, v, vg, lens, scale: float | None = None, table=None, 
         out = q.new_empty((B, nH, dH))
     else:
         _check("out", out, _F32, dev)
-        _need(out.numel() == B * nH * dH, f"out: shape {tuple(out.shape)}")
+        if out.numel() != B * nH * dH:
+            raise ValueError(f"out: shape {tuple(out.shape)}")
     h = _on(dev)
-    nbytes = lib().fcu_kv4_attn_work(h, c, B, nH)
-    work = k.new_empty((nbytes,)).data_ptr() if nbytes > 0 else None
+    nbytes = _FN["fcu_kv4_attn_work"](h, c, B, nH)
+    work = k.new_empty((nbytes,)) if nbytes > 0 else None
     _call("fcu_kv4_attn", h, q.data_ptr(), ld, c, lens.data_ptr(), B, nH,
-          dH ** -0.5 if scale is None else float(scale), out.data_ptr(), work, nbytes)
+          dH ** -0.5 if scale is None else float(scale), out.data_ptr(),
+          work.data_ptr() if work is not None else None, nbytes)
     return out
 
 
@@ -211,17 +238,20 @@ def kv4Evict(k, kg, v, vg, weight, pos, lens, budget: int, recent: int, table=No
     dev = _device()
     _check("lens", lens, _I32, dev)
     B = lens.numel()
-    _need(weight is not None and pos is not None, "eviction goes by `weight` and `pos`")
-    _need(budget >= 1 and 0 <= recent <= budget, f"budget {budget}, recent {recent}")
+    if weight is None or pos is None:
+        raise ValueError("eviction goes by `weight` and `pos`")
+    if budget < 1 or not 0 <= recent <= budget:
+        raise ValueError(f"budget {budget}, recent {recent}")
     c = _cache(dev, k, kg, v, vg, 2 * k.shape[-1], B, table, weight, pos, layers=True)
     if newLens is None:
         newLens = torch.empty_like(lens)
     else:
         _check("newLens", newLens, _I32, dev, tuple(lens.shape))
     h = _on(dev)
-    nbytes = lib().fcu_kv4_evict_work(h, c, B, budget)
-    work = k.new_empty((nbytes,)).data_ptr() if nbytes > 0 else None
-    _call("fcu_kv4_evict", h, c, lens.data_ptr(), B, budget, recent, newLens.data_ptr(), work, nbytes)
+    nbytes = _FN["fcu_kv4_evict_work"](h, c, B, budget)
+    work = k.new_empty((nbytes,)) if nbytes > 0 else None
+    _call("fcu_kv4_evict", h, c, lens.data_ptr(), B, budget, recent, newLens.data_ptr(),
+          work.data_ptr() if work is not None else None, nbytes)
     return newLens
 
 
@@ -234,20 +264,23 @@ def beamStep(logits, scores, done, beams: int, eos: int):
     dev = _device()
     ld = _rows("logits", logits, dev)
     R, V = logits.shape
-    _need(1 <= beams <= 32 and R % beams == 0, f"{R} rows for searches of {beams} beams (1 to 32)")
-    _need(0 <= eos < V, f"eos {eos} outside the vocabulary of {V}")
+    if not 1 <= beams <= 32 or R % beams:
+        raise ValueError(f"{R} rows for searches of {beams} beams (1 to 32)")
+    if not 0 <= eos < V:
+        raise ValueError(f"eos {eos} outside the vocabulary of {V}")
     _check("scores", scores, _F32, dev)
     _check("done", done, _BOOL, dev)
-    _need(scores.numel() == R and done.numel() == R, f"{scores.numel()} scores, {done.numel()} done for {R} rows")
+    if scores.numel() != R or done.numel() != R:
+        raise ValueError(f"{scores.numel()} scores, {done.numel()} done for {R} rows")
     B = R // beams
     outScores = scores.new_empty((B, beams))
     tokens, parents = scores.new_empty((2, B, beams), dtype=_I32).unbind(0)
     outDone = done.new_empty((B, beams))
     h = _on(dev)
-    nbytes = lib().fcu_beam_work(h, B, beams, V)
-    work = scores.new_empty((nbytes // 4 + 1,)).data_ptr()
+    nbytes = _FN["fcu_beam_work"](h, B, beams, V)
+    work = scores.new_empty((nbytes // 4 + 1,))
     _call("fcu_beam_step", h, logits.data_ptr(), ld, scores.data_ptr(), done.data_ptr(), B, beams, V, eos,
-          outScores.data_ptr(), tokens.data_ptr(), parents.data_ptr(), outDone.data_ptr(), work, nbytes)
+          outScores.data_ptr(), tokens.data_ptr(), parents.data_ptr(), outDone.data_ptr(), work.data_ptr(), nbytes)
     return outScores, tokens, parents, outDone
 
 
@@ -259,12 +292,15 @@ def cacheReorder(arrays, parents, lens, table=None) -> None:
     has one head: its rows); parents int32 [B, W]; lens int32 [B * W]."""
     dev = _device()
     _check("parents", parents, _I32, dev)
-    _need(parents.ndim == 2 and 1 <= parents.shape[1] <= 32, f"parents: shape {tuple(parents.shape)} (1 to 32 beams)")
+    if parents.ndim != 2 or not 1 <= parents.shape[1] <= 32:
+        raise ValueError(f"parents: shape {tuple(parents.shape)} (1 to 32 beams)")
     B, W = parents.shape
     _check("lens", lens, _I32, dev)
-    _need(lens.numel() == B * W, f"{lens.numel()} lengths for {B} x {W} beams")
+    if lens.numel() != B * W:
+        raise ValueError(f"{lens.numel()} lengths for {B} x {W} beams")
     n = len(arrays)
-    _need(1 <= n <= 8, f"{n} arrays (1 to 8)")
+    if not 1 <= n <= 8:
+        raise ValueError(f"{n} arrays (1 to 8)")
     L, blocks, _, bs = arrays[0].shape[:4]
     spec = (CacheArray * n)()
     for i, t in enumerate(arrays):
@@ -277,10 +313,12 @@ def cacheReorder(arrays, parents, lens, table=None) -> None:
         s.base, s.heads, s.unit = t.data_ptr(), shape[2], math.prod(shape[4:]) * t.element_size()
     if table is not None:
         _check("table", table, _I32, dev)
-        _need(table.ndim == 2 and table.shape[0] == B * W, f"table: shape {tuple(table.shape)} for {B * W} beams")
+        if table.ndim != 2 or table.shape[0] != B * W:
+            raise ValueError(f"table: shape {tuple(table.shape)} for {B * W} beams")
         mb = table.shape[1]
     else:
-        _need(blocks % max(B * W, 1) == 0, f"{blocks} blocks do not divide among {B * W} beams")
+        if blocks % max(B * W, 1):
+            raise ValueError(f"{blocks} blocks do not divide among {B * W} beams")
         mb = blocks // max(B * W, 1)
     _call("fcu_cache_reorder", _on(dev), spec, n, L, blocks, table.data_ptr() if table is not None else None, bs, mb,
           parents.data_ptr(), lens.data_ptr(), B, W)
