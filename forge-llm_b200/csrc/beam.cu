@@ -32,6 +32,10 @@ __device__ __forceinline__ uint32_t order_bits(float x) {
   const uint32_t u = __float_as_uint(x + 0.0f);
   return u & 0x80000000u ? ~u : u | 0x80000000u;
 }
+// (0 gives -inf)
+__device__ __forceinline__ float bits_float(uint32_t u) {
+  return u == 0 ? -INFINITY : __uint_as_float(u & 0x80000000u ? u & 0x7fffffffu : ~u);
+}
 __device__ __forceinline__ Key beam_key(float x, uint32_t token) {
   return (Key)order_bits(x) << 32 | (0xffffffffu - token);
 }
@@ -75,8 +79,11 @@ __global__ void __launch_bounds__(kBeamThreads) beam_rows_kernel(BeamArgs a) {
   pdl_trigger();
   __shared__ Key lists[kBeamWarps * kMaxW];
   __shared__ float red_m[kBeamWarps], red_s[kBeamWarps];
+  __shared__ uint32_t shared_bar;            // order_bits of a logit that W others of the slice reach
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, W = a.W;
   const int64_t row = blockIdx.y;
+  if (threadIdx.x == 0) shared_bar = 0;
+  __syncthreads();
   const int v0 = blockIdx.x * a.slice, v1 = (int)min((int64_t)a.V, (int64_t)v0 + a.slice);
   pdl_wait();
   const float *x = a.logits + row * a.ld;
@@ -88,19 +95,26 @@ __global__ void __launch_bounds__(kBeamThreads) beam_rows_kernel(BeamArgs a) {
   bool full = false;
   int64_t t0 = (int64_t)v0 - skew + warp * kTile;
   float4 next[4];
+  auto fetch = [&](int64_t t) {
+    if (t >= v0 && t + kTile <= v1) {
+      const float4 *p = reinterpret_cast<const float4 *>(x + t) + lane;
 #pragma unroll
-  for (int i = 0; i < 4; i++) {
-    const int64_t v = t0 + 128 * i + 4 * lane;
-    next[i] = v < v1 ? load4(x + v, (int)v, v0, v1) : float4{-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-  }
+      for (int i = 0; i < 4; i++) next[i] = __ldcs(p + 32 * i);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 4; i++) {
+        const int64_t v = t + 128 * i + 4 * lane;
+        next[i] = v < v1 ? load4(x + v, (int)v, v0, v1) : float4{-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+      }
+    }
+  };
+  fetch(t0);
   for (; t0 < v1; t0 += kTile * kBeamWarps) {
     float f[16];
 #pragma unroll
-    for (int i = 0; i < 4; i++) {
+    for (int i = 0; i < 4; i++)
       f[4 * i] = next[i].x, f[4 * i + 1] = next[i].y, f[4 * i + 2] = next[i].z, f[4 * i + 3] = next[i].w;
-      const int64_t v = t0 + kTile * kBeamWarps + 128 * i + 4 * lane;
-      next[i] = v < v1 ? load4(x + v, (int)v, v0, v1) : float4{-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-    }
+    fetch(t0 + kTile * kBeamWarps);
     float top = f[0];
 #pragma unroll
     for (int i = 1; i < 16; i++) top = fmaxf(top, f[i]);
@@ -112,10 +126,12 @@ __global__ void __launch_bounds__(kBeamThreads) beam_rows_kernel(BeamArgs a) {
       s = s * beam_ex2(M - M1) + ts;
       M = M1;
     }
-    // Earlier tiles hold lower tokens, so only a larger logit displaces one of theirs.
-    uint32_t hit = __ballot_sync(0xffffffffu, top > bar || !full);
+    // Earlier tiles hold lower tokens, so only a larger logit displaces one of
+    // theirs; another warp's W-th best is no bound on equal ones.
+    const float others = bits_float(*(volatile uint32_t *)&shared_bar);
+    uint32_t hit = __ballot_sync(0xffffffffu, (top > bar || !full) && top >= others);
     if (hit == 0) continue;
-    float least = bar;
+    float least = fmaxf(bar, others);
     if (__popc(hit) > W) {
       // no logit below the W-th largest of the lanes' maxima is among the W best
       uint32_t mine = order_bits(top), w_th = 0;
@@ -123,7 +139,7 @@ __global__ void __launch_bounds__(kBeamThreads) beam_rows_kernel(BeamArgs a) {
         w_th = __reduce_max_sync(0xffffffffu, mine);
         if (mine == w_th) mine = 0;
       }
-      if (w_th) least = fmaxf(least, __uint_as_float(w_th & 0x80000000u ? w_th & 0x7fffffffu : ~w_th));
+      if (w_th) least = fmaxf(least, bits_float(w_th));
     }
 #pragma unroll
     for (int i = 0; i < 16; i++) {
@@ -143,7 +159,10 @@ __global__ void __launch_bounds__(kBeamThreads) beam_rows_kernel(BeamArgs a) {
     }
     const Key last = __shfl_sync(0xffffffffu, key, W - 1);
     full = last != 0;
-    if (full) bar = key_logit(last);
+    if (full) {
+      bar = key_logit(last);
+      if (lane == 0 && bar > others) atomicMax(&shared_bar, order_bits(bar));
+    }
   }
   // the slice's maximum and sum: lanes, then warps, in a fixed order
 #pragma unroll

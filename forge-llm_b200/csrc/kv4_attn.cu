@@ -72,6 +72,7 @@ struct AttnArgs {
   int B, nH, g;          // g: q heads per kv head
   int gs, hg;            // q heads of one segment, segments per kv head
   int ctas;              // runs (CTAs of the main kernel)
+  int whole;             // every segment is one CTA's: nothing is cut
   int vec;               // q rows and heads start on 16 bytes
   float scale;
   float *out;
@@ -86,11 +87,25 @@ __device__ __forceinline__ int64_t length(const AttnArgs &a, int64_t b) {
   return n < 0 ? 0 : n > a.c.cap ? a.c.cap : n;
 }
 
-// The cut into runs, the same in every kernel of a call: `total` tiles, `per`
-// of them to a run.  A run is at least a tile for every warp of the CTA, unless
-// no segment is that long.
+// What a sequence's segments count for in the cut into runs: their tiles, or one
+// where segments stay whole.
+template <int TILE>
+__device__ __forceinline__ int64_t units(const AttnArgs &a, int64_t b) {
+  const int64_t t = (length(a, b) + TILE - 1) / TILE;
+  return a.whole && t > 1 ? 1 : t;
+}
+
+// The cut into runs: `total` units, `per` of them to a run.  A run is at least a
+// tile for every warp of the CTA, unless no segment is that long.
 struct Plan {
   int64_t total, per;
+};
+
+// A unit's place: sequence, segment of the sequence, unit of the segment.
+struct Place {
+  int64_t b;
+  int seg;
+  int64_t tile, tiles;
 };
 
 // Block-wide; sh: 2 * kWarps int64.
@@ -99,7 +114,7 @@ __device__ Plan make_plan(const AttnArgs &a, int64_t *sh) {
   const int segs = a.c.nKV * a.hg;
   int64_t total = 0, longest = 0;
   for (int64_t b = threadIdx.x; b < a.B; b += kThreads) {
-    const int64_t t = (length(a, b) + TILE - 1) / TILE;
+    const int64_t t = units<TILE>(a, b);
     total += t;
     longest = max(longest, t);
   }
@@ -126,21 +141,14 @@ __device__ Plan make_plan(const AttnArgs &a, int64_t *sh) {
   return p;
 }
 
-// A tile's place: sequence, segment of the sequence, tile of the segment.
-struct Place {
-  int64_t b;
-  int seg;
-  int64_t tile, tiles;
-};
-
-// The place of tile u < total (b = -1 if the lengths have changed since the
+// The place of unit u < total (b = -1 if the lengths have changed since the
 // total was taken).  Block-wide, the same for all threads; sh: kThreads int64.
 template <int TILE>
 __device__ Place find(const AttnArgs &a, int64_t u, int64_t *sh) {
   const int segs = a.c.nKV * a.hg, tid = threadIdx.x;
   int64_t before = 0;
   for (int64_t b0 = 0; b0 < a.B; b0 += kThreads) {
-    const int64_t t = b0 + tid < a.B ? (length(a, b0 + tid) + TILE - 1) / TILE : 0;
+    const int64_t t = b0 + tid < a.B ? units<TILE>(a, b0 + tid) : 0;
     int64_t x = t * segs;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
@@ -167,6 +175,53 @@ __device__ Place find(const AttnArgs &a, int64_t u, int64_t *sh) {
     __syncthreads();
   }
   return Place{-1, 0, 0, 0};
+}
+
+// make_plan, and find() for the first unit of run `run`, at once for at most
+// kThreads sequences (their lengths are read once).  b = -1: the run is empty.
+template <int TILE>
+__device__ Plan plan_small(const AttnArgs &a, int64_t run, int64_t *sh, Place *at) {
+  const int segs = a.c.nKV * a.hg, tid = threadIdx.x;
+  const int t = tid < a.B ? (int)units<TILE>(a, tid) : 0;      // at most 2^25 tiles of 2^30 slots
+  int64_t x = t;
+  int longest = t;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int64_t y = __shfl_up_sync(0xffffffffu, x, o);
+    if ((tid & 31) >= o) x += y;
+  }
+  longest = __reduce_max_sync(0xffffffffu, longest);
+  if ((tid & 31) == 31) {
+    sh[tid >> 5] = x;
+    sh[kWarps + (tid >> 5)] = longest;
+  }
+  __syncthreads();
+  Plan p;
+  p.total = 0;
+#pragma unroll
+  for (int w = 0; w < kWarps; w++) {
+    if (w < (tid >> 5)) x += sh[w];
+    p.total += sh[w];
+    longest = max(longest, (int)sh[kWarps + w]);
+  }
+  p.total *= segs;
+  p.per = max((p.total + a.ctas - 1) / a.ctas, min((int64_t)kWarps, (int64_t)longest));
+  const int64_t u = run * p.per;
+  __syncthreads();
+  if (tid == 0) sh[0] = -1;
+  __syncthreads();
+  if (u < p.total && (x - t) * segs <= u && u < x * segs) {     // one thread's sequence
+    sh[0] = tid;
+    sh[1] = u - (x - t) * segs;
+    sh[2] = t;
+  }
+  __syncthreads();
+  at->b = sh[0];
+  at->tiles = sh[2];
+  at->seg = sh[0] < 0 ? 0 : (int)(sh[1] / sh[2]);
+  at->tile = sh[0] < 0 ? 0 : sh[1] - at->seg * sh[2];
+  __syncthreads();
+  return p;
 }
 
 __device__ __forceinline__ float ex2(float x) {
@@ -229,10 +284,14 @@ __device__ __forceinline__ uint32_t grid_at(int x) {
   return 4 * ((x & 7) * C::kGridStride + (x >> 3));
 }
 
-// issue() for blocks that sixteen slots may straddle.
+// issue() for blocks that sixteen slots may straddle.  (Not inlined, and so the
+// cache's geometry goes by value: a reference would put all of it on the stack.)
 template <class C, int W>
-__device__ __noinline__ void issue_scattered(const Cache &c, const uint8_t *codes, const uint32_t *grids, int64_t b, int h,
+__device__ __noinline__ void issue_scattered(const int32_t *table, int64_t blocks, int mb, int nKV, int bs, uint32_t div_mul,
+                                             int div_shift, const uint8_t *codes, const uint32_t *grids, int64_t b, int h,
                                              int j0, int cnt, uint8_t *part) {
+  Cache c;
+  c.table = table, c.blocks = blocks, c.mb = mb, c.nKV = nKV, c.bs = bs, c.div_mul = div_mul, c.div_shift = div_shift;
   const int lane = threadIdx.x & 31;
   const uint32_t code_s = (uint32_t)__cvta_generic_to_shared(part), grid_s = code_s + C::kCodes;
   for (int x = lane; x < C::kTile; x += 32) {
@@ -251,17 +310,20 @@ __device__ __noinline__ void issue_scattered(const Cache &c, const uint8_t *code
 
 // Starts the copies of one tile's k or v (slots j0 .. j0 + cnt of head h of
 // sequence b) into shared memory.  Slots past cnt are zero; those of a bad block
-// have NaN grids.
+// have NaN grids.  flat: the row of slot 0 where all slots lie in one block, else
+// -1.
 template <class C, int W>
-__device__ __forceinline__ void issue(const Cache &c, const uint8_t *codes, const uint32_t *grids, int64_t b, int h,
-                                      int j0, int cnt, uint8_t *part) {
+__device__ __forceinline__ void issue(const Cache &c, const uint8_t *codes, const uint32_t *grids, int64_t flat, int64_t b,
+                                      int h, int j0, int cnt, uint8_t *part) {
   const int lane = threadIdx.x & 31;
   const uint32_t code_s = (uint32_t)__cvta_generic_to_shared(part), grid_s = code_s + C::kCodes;
-  const int blk = (int)block_index(c, j0), off = j0 - blk * c.bs;
-  const int64_t p = block_of(c, b, blk);
-  if (cnt == C::kTile && off + C::kTile <= c.bs && p >= 0) {
-    // a full tile inside one block: its rows are contiguous
-    const int64_t row = (p * c.nKV + h) * c.bs + off;
+  int64_t row = flat + j0;             // where a full tile's rows are contiguous; -1: they are not
+  if (flat < 0) {
+    const int blk = (int)block_index(c, j0), off = j0 - blk * c.bs;
+    const int64_t p = block_of(c, b, blk);
+    row = off + C::kTile <= c.bs && p >= 0 ? (p * c.nKV + h) * c.bs + off : -1;
+  }
+  if (cnt == C::kTile && row >= 0) {
     const uint8_t *src = codes + row * C::kRow + 16 * lane;
 #pragma unroll
     for (int i = 0; i < C::kTile * W / 32; i++) {
@@ -294,7 +356,7 @@ __device__ __forceinline__ void issue(const Cache &c, const uint8_t *codes, cons
                  on ? codes + row * C::kRow + 16 * (x - (j & ~15) * W) : codes, on);
     }
   } else {
-    issue_scattered<C, W>(c, codes, grids, b, h, j0, cnt, part);
+    issue_scattered<C, W>(c.table, c.blocks, c.mb, c.nKV, c.bs, c.div_mul, c.div_shift, codes, grids, b, h, j0, cnt, part);
   }
 }
 
@@ -372,27 +434,34 @@ __global__ void __launch_bounds__(kThreads, Cfg<W, G>::kCtas) kv4_attn_kernel(At
   for (int64_t b = blockIdx.x; b < a.B; b += gridDim.x)
     if (length(a, b) == 0)
       for (int i = threadIdx.x; i < a.nH * c.dH; i += kThreads) a.out[b * a.nH * c.dH + i] = 0.f;
-  const Plan plan = make_plan<TP>(a, sh);
+  Place at{-1, 0, 0, 0};
+  const Plan plan = a.B <= kThreads ? plan_small<TP>(a, blockIdx.x, sh, &at) : make_plan<TP>(a, sh);
   int64_t u = blockIdx.x * plan.per;
   const int64_t end = min(u + plan.per, plan.total);
   Cut cut{0, 0, 0};
-  Place at{-1, 0, 0, 0};
-  if (u < end) at = find<TP>(a, u, sh);
+  if (a.B > kThreads && u < end) at = find<TP>(a, u, sh);
   while (at.b >= 0 && at.b < a.B) {
     // this run's part [t0, t1) of the segment
-    const int t0 = (int)at.tile, t1 = (int)min(at.tiles, at.tile + (end - u));
+    const int t0 = (int)at.tile;
     const int h = at.seg / a.hg, h0 = h * a.g + (at.seg % a.hg) * a.gs;   // kv head, first q head
     const int heads = min(a.gs, (h + 1) * a.g - h0);
     const int n = (int)length(a, at.b);
+    const int t1 = a.whole ? (n + TP - 1) / TP : (int)min(at.tiles, at.tile + (end - u));
+
+    int64_t flat = -1;
+    if (c.mb == 1) {
+      flat = block_of(c, at.b, 0);
+      if (flat >= 0) flat = (flat * c.nKV + h) * c.bs;
+    }
 
     // a tile's k and v are copy groups of their own: k one tile ahead, v as soon
     // as the last tile's has been used
     auto issue_k = [&](int tile, int buf) {
-      if (tile < t1) issue<C, W>(c, c.k, c.kg, at.b, h, tile * TP, min(TP, n - tile * TP), kbuf + buf * C::kPart);
+      if (tile < t1) issue<C, W>(c, c.k, c.kg, flat, at.b, h, tile * TP, min(TP, n - tile * TP), kbuf + buf * C::kPart);
       asm volatile("cp.async.commit_group;");
     };
     auto issue_v = [&](int tile) {
-      if (tile < t1) issue<C, W>(c, c.v, c.vg, at.b, h, tile * TP, min(TP, n - tile * TP), vbuf);
+      if (tile < t1) issue<C, W>(c, c.v, c.vg, flat, at.b, h, tile * TP, min(TP, n - tile * TP), vbuf);
       asm volatile("cp.async.commit_group;");
     };
     int kb = 0;
@@ -639,7 +708,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<W, G>::kCtas) kv4_attn_kernel(At
       if (r == 0) *reinterpret_cast<float2 *>(mine + dP) = make_float2(m[g] * qf[g], l[g]);   // log2 units from here on
     }
     __syncthreads();
-    const bool whole = t0 == 0 && t1 == at.tiles;
+    const bool whole = a.whole || (t0 == 0 && t1 == at.tiles);
     const int64_t bh0 = at.b * a.nH + h0;
     if (t0 == 0 && !whole)
       cut = Cut{1 + (int)((at.tiles - t1 + plan.per - 1) / plan.per), heads, bh0};
@@ -677,13 +746,13 @@ __global__ void __launch_bounds__(kThreads, Cfg<W, G>::kCtas) kv4_attn_kernel(At
       if (e + 2 < c.dH) *reinterpret_cast<float2 *>(dst + e + 2) = make_float2(O.z, O.w);
     }
     __syncthreads();
-    u += t1 - t0;
+    u += a.whole ? 1 : t1 - t0;
     if (u >= end) break;
     at.tile = 0;
     if (++at.seg == c.nKV * a.hg) {
       at.seg = 0;
       if (threadIdx.x == 0) {      // one reader, so that the threads agree
-        do at.tiles = ++at.b < a.B ? (length(a, at.b) + TP - 1) / TP : 1;
+        do at.tiles = ++at.b < a.B ? units<TP>(a, at.b) : 1;
         while (at.tiles == 0);
         sh[0] = at.b;
         sh[1] = at.tiles;
@@ -694,7 +763,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<W, G>::kCtas) kv4_attn_kernel(At
       __syncthreads();
     }
   }
-  if (threadIdx.x == 0) a.cuts[blockIdx.x] = cut;
+  if (threadIdx.x == 0 && !a.whole) a.cuts[blockIdx.x] = cut;
 }
 
 // The (m, l) of a head whose segment begins in run `run` and has `pieces`
@@ -738,7 +807,7 @@ __global__ void __launch_bounds__(kFinishThreads) kv4_attn_finish_kernel(AttnArg
   __shared__ float o_s[kFinishWarps][32 * W];
   __shared__ float m_s[kMaxGroup], il_s[kMaxGroup];
   const Cache &c = a.c;
-  const int dH = c.dH, lane = threadIdx.x & 31, warp = threadIdx.x >> 5, merges = a.ctas - 1;
+  const int dH = c.dH, lane = threadIdx.x & 31, warp = threadIdx.x >> 5, merges = a.whole ? 0 : a.ctas - 1;
   pdl_wait();
   if (blockIdx.x < merges) {
     Cut cut{0, 0, 0};
@@ -864,11 +933,19 @@ __global__ void __launch_bounds__(kFinishThreads) kv4_attn_finish_kernel(AttnArg
     if (row[x] >= 0) c.weight[row[x]] = old[x] + w[x];
 }
 
+// How the heads are dealt: q heads per kv head, segments per kv head (a CTA
+// takes at most 8 heads), q heads of a segment, and the CTAs.
+struct Heads {
+  int g, hg, gs, ctas, whole;
+};
+
 // Floats of workspace: the cuts, the pieces and, where weights are kept, (m, l)
 // and the scores.
-int64_t part_floats(const Cache &c, int ctas) { return (int64_t)ctas * 2 * kMaxHeads * (c.dH + 2); }
-int64_t work_floats(const Cache &c, int B, int nH, int ctas) {
-  return (int64_t)ctas * (sizeof(Cut) / 4) + part_floats(c, ctas) + (c.weight ? (int64_t)B * nH * (c.cap + 2) : 0);
+int64_t part_floats(const Cache &c, const Heads &p) {
+  return p.whole ? 0 : (int64_t)p.ctas * (2 * kMaxHeads * (c.dH + 2) + sizeof(Cut) / 4);
+}
+int64_t work_floats(const Cache &c, int B, int nH, const Heads &p) {
+  return part_floats(c, p) + (c.weight ? (int64_t)B * nH * (c.cap + 2) : 0);
 }
 
 int checked(const char *who, const fcu_kv4 *cache, int B, int nH, bool arrays, Cache *c) {
@@ -880,13 +957,18 @@ int checked(const char *who, const fcu_kv4 *cache, int B, int nH, bool arrays, C
 }
 
 // CTAs of the main kernel: all that are resident, or one per tile if the cache
-// cannot hold that many.
+// cannot hold that many.  A cache of at most kWholeTiles tiles per sequence
+// whose segments are all resident at once gives each a CTA of its own: its two
+// steps per warp cost less than the second kernel that would merge pieces (one
+// sequence of 37 slots in a cache of 1024: 12 us a call, 18 with the merge).
+constexpr int kWholeTiles = 8;
 template <int W, int G>
-int plan_ctas(const fcu_ctx *ctx, const Cache &c, int B, int hg) {
+void plan_ctas(const fcu_ctx *ctx, const Cache &c, int B, Heads *p) {
   using C = Cfg<W, G>;
-  const int64_t tiles = (int64_t)B * c.nKV * hg * ((c.cap + C::kTile - 1) / C::kTile);
+  const int64_t tiles = (c.cap + C::kTile - 1) / C::kTile, segs = (int64_t)B * c.nKV * p->hg;
   const int64_t all = (int64_t)ctx->num_sms * C::kCtas;
-  return (int)(tiles < all ? tiles : all);
+  p->whole = tiles <= kWholeTiles && segs <= all;
+  p->ctas = (int)(p->whole ? segs : segs * tiles < all ? segs * tiles : all);
 }
 
 template <int W, int G>
@@ -899,7 +981,7 @@ int launch(fcu_ctx *ctx, const AttnArgs &a) {
   }
   FCU_CHECK_CUDA(launch_pdl(kv4_attn_kernel<W, G>, dim3(a.ctas), dim3(kThreads), C::kSmem, ctx->stream, a));
   note_launch();
-  const int64_t blocks = a.ctas - 1 + (a.scores ? (int64_t)a.B * a.c.nKV * ((a.c.cap + kWtSlots - 1) / kWtSlots) : 0);
+  const int64_t blocks = (a.whole ? 0 : a.ctas - 1) + (a.scores ? (int64_t)a.B * a.c.nKV * ((a.c.cap + kWtSlots - 1) / kWtSlots) : 0);
   if (blocks > 0) {
     FCU_CHECK_CUDA(launch_pdl(kv4_attn_finish_kernel<W>, dim3((unsigned)blocks), dim3(kFinishThreads), 0, ctx->stream, a));
     note_launch();
@@ -924,18 +1006,12 @@ int launch(fcu_ctx *ctx, const AttnArgs &a) {
     default: f(8, 2); break;                                           \
   }
 
-// How the heads are dealt: q heads per kv head, segments per kv head (a CTA
-// takes at most 8 heads), q heads of a segment, and the CTAs.
-struct Heads {
-  int g, hg, gs, ctas;
-};
 Heads plan_heads(const fcu_ctx *ctx, const Cache &c, int B, int nH) {
   Heads p;
   p.g = nH / c.nKV;
   p.hg = p.g > kMaxHeads ? 2 : 1;
   p.gs = (p.g + p.hg - 1) / p.hg;
-  p.ctas = 0;
-#define FCU_CASE(W, G) p.ctas = plan_ctas<W, G>(ctx, c, B, p.hg)
+#define FCU_CASE(W, G) plan_ctas<W, G>(ctx, c, B, &p)
   FCU_KV4_WIDTHS(FCU_CASE, c.rb, p.gs)
 #undef FCU_CASE
   return p;
@@ -953,7 +1029,7 @@ extern "C" {
 int64_t fcu_kv4_attn_work(fcu_ctx *ctx, const fcu_kv4 *cache, int B, int nH) {
   Cache c;
   if (!ctx || checked("fcu_kv4_attn_work", cache, B, nH, false, &c)) return -1;
-  return 4 * work_floats(c, B, nH, plan_heads(ctx, c, B, nH).ctas);
+  return 4 * work_floats(c, B, nH, plan_heads(ctx, c, B, nH));
 }
 
 int fcu_kv4_attn(fcu_ctx *ctx, const float *q, int64_t ld_q, const fcu_kv4 *cache, const int32_t *seq_lens, int B,
@@ -976,17 +1052,18 @@ int fcu_kv4_attn(fcu_ctx *ctx, const float *q, int64_t ld_q, const fcu_kv4 *cach
   a.hg = p.hg;
   a.gs = p.gs;
   a.ctas = p.ctas;
+  a.whole = p.whole;
   a.vec = ld_q % 4 == 0 && a.c.dH % 4 == 0 && ((uintptr_t)q & 15) == 0;
   a.scale = (float)scale;
   a.out = out;
   FCU_REQUIRE(!a.c.weight || (double)B * a.c.nKV * (a.c.cap / kWtSlots + 1) < 1e9, "fcu_kv4_attn: the cache is too large");
-  const int64_t need = 4 * work_floats(a.c, B, nH, a.ctas);
-  FCU_REQUIRE(work && work_bytes >= need && ((uintptr_t)work & 15) == 0,
+  const int64_t need = 4 * work_floats(a.c, B, nH, p);
+  FCU_REQUIRE(need == 0 || (work && work_bytes >= need && ((uintptr_t)work & 15) == 0),
               "fcu_kv4_attn: workspace of %lld bytes, %lld needed", (long long)work_bytes, (long long)need);
   a.cuts = (Cut *)work;
   a.part = (float *)(a.cuts + a.ctas);
   if (a.c.weight) {
-    a.ml = (float2 *)(a.part + part_floats(a.c, a.ctas));
+    a.ml = (float2 *)((float *)work + part_floats(a.c, p));
     a.scores = (float *)(a.ml + (int64_t)B * nH);
   }
 #define FCU_CASE(W, G) rc = launch<W, G>(ctx, a)

@@ -526,3 +526,15 @@ def test_python_refusals():
             pytest.fail(f"case {i} was accepted")
     with pytest.raises(fw.ForgeCUError):
         fw.kv4Attention(torch.zeros(2, 3, 64, device="cuda"), k, kg, v, vg, lens, **ok)
+
+
+def test_attention_of_more_sequences_than_a_block_has_threads():
+    """300 sequences, most of them short or empty, and one long."""
+    rng = np.random.default_rng(20)
+    lens = rng.choice([0, 1, 2, 30, 70], 300)
+    lens[170] = 700
+    lens[299] = 65
+    c = Cache(300, 704, 1, 16, 64, seed=12)
+    q = rng.standard_normal((300, 3, 16)).astype(np.float32)
+    check_attention(c, q, lens.tolist(), weight=np.zeros((c.phys, 1, 64), np.float32))
+    check_attention(c, q, [0] * 300)
