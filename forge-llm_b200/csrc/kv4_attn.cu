@@ -10,9 +10,8 @@
 //
 // Both products run on mma.sync m16n8k16 with the codes as the 16-row operand,
 // fp16 operands and fp32 sums.  The codes are exact in fp16 without a
-// conversion: a nibble in the low byte of a 16-bit half IS the subnormal
-// c 2^-24 (or 16 c 2^-24), so two ANDs on a word give four operands.  The other
-// operand carries 22 bits, x = hi + lo, in columns 2i and 2i + 1 (four heads to
+// conversion: a nibble in the mantissa of a 16-bit half is a subnormal, so a
+// shift and an AND give two operands.  The other operand carries 22 bits, x = hi + lo, in columns 2i and 2i + 1 (four heads to
 // an 8-column tile), whose sums one thread holds side by side and adds in fp32;
 // a power of two keeps x in fp16's range.  (A tcgen05 tile would want the codes
 // expanded to 16 bits in shared memory first, four times the traffic of the
@@ -242,6 +241,20 @@ __device__ __forceinline__ void mma0(float (&c)[4], const uint32_t (&a)[4], uint
       "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
       : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.f));
+}
+
+// Codes N (of 0..3) of the two 16-bit halves of x as fp16 operands: moved to bits
+// 6..9, where a subnormal's value is c 2^-18.  Where in the mantissa they sit
+// matters: the tensor core lines its products up by their exponent fields and
+// drops what falls below, so the zeros above a code are bits lost.  Errors against
+// 64 bits over sixteen sizes: 2e-7 to 6e-7 here, the same as for codes made
+// normal by an extra fp16 subtraction (20 % slower); 3e-7 to 7e-7 at bits 4..7
+// (one shift fewer, 2 % faster); 1e-6 to 1e-5 where they lie, at bits 0..3 and
+// 4..7 (10 % faster).
+constexpr int kCodeExp = 18;
+template <int N>
+__device__ __forceinline__ uint32_t codes(uint32_t x) {
+  return (N == 0 ? x << 6 : N == 1 ? x << 2 : N == 2 ? x >> 2 : x >> 6) & 0x03c003c0u;
 }
 
 // x as (hi, lo) fp16: its first 11 bits, which fp16 holds, and the rest rounded
@@ -499,18 +512,18 @@ __global__ void __launch_bounds__(kThreads, Cfg<W, G>::kCtas) kv4_attn_kernel(At
       big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, 2)) * fabsf(sc);
       sum += __shfl_xor_sync(0xffffffffu, sum, 1);
       sum += __shfl_xor_sync(0xffffffffu, sum, 2);
-      // x * sc * up below 2^14, up a power of two; the codes carry 2^-24
+      // x * sc * up below 2^14, up a power of two; the codes carry 2^-kCodeExp
       const int ex = min(240, max(27, (int)(__float_as_uint(big) >> 23)));
       const float up = __uint_as_float((uint32_t)(267 - ex) << 23);
-      const float f = __uint_as_float((uint32_t)(ex + 11) << 23);          // 2^24 / up
-      const float inv = __uint_as_float((uint32_t)(243 - ex) << 23);       // up / 2^24
-      const float up0 = sc * up, up1 = up0 * 0.0625f;       // odd nibbles are met at 16 times their value
+      const float f = __uint_as_float((uint32_t)(ex + kCodeExp - 13) << 23);      // 2^kCodeExp / up
+      const float inv = __uint_as_float((uint32_t)(267 - kCodeExp - ex) << 23);   // its inverse
+      const float sc_up = sc * up;
       const uint32_t sel = r & 1 ? 0x7632 : 0x5410;
 #pragma unroll
       for (int i = 0; i < W; i++) {
         uint32_t y[8];
 #pragma unroll
-        for (int e = 0; e < 8; e++) y[e] = split(x[8 * i + e] * (e & 1 ? up1 : up0));
+        for (int e = 0; e < 8; e++) y[e] = split(x[8 * i + e] * sc_up);
         qb[g][2 * i][0] = __byte_perm(y[0], y[4], sel);
         qb[g][2 * i][1] = __byte_perm(y[2], y[6], sel);
         qb[g][2 * i + 1][0] = __byte_perm(y[1], y[5], sel);
@@ -555,9 +568,9 @@ __global__ void __launch_bounds__(kThreads, Cfg<W, G>::kCtas) kv4_attn_kernel(At
           for (int i = 0; i < W; i++)
 #pragma unroll
             for (int k = 0; k < KB; k++) {
-              const uint32_t x0 = w[k][0][i], x1 = w[k][1][i], y0 = x0 >> 8, y1 = x1 >> 8;
-              const uint32_t lo[4] = {x0 & 0x000f000fu, x1 & 0x000f000fu, y0 & 0x000f000fu, y1 & 0x000f000fu};
-              const uint32_t hi[4] = {x0 & 0x00f000f0u, x1 & 0x00f000f0u, y0 & 0x00f000f0u, y1 & 0x00f000f0u};
+              const uint32_t x0 = w[k][0][i], x1 = w[k][1][i];
+              const uint32_t lo[4] = {codes<0>(x0), codes<0>(x1), codes<2>(x0), codes<2>(x1)};
+              const uint32_t hi[4] = {codes<1>(x0), codes<1>(x1), codes<3>(x0), codes<3>(x1)};
 #pragma unroll
               for (int g = 0; g < G; g++) {
                 if (i == 0) mma0(acc[k][g], lo, qb[g][0][0], qb[g][0][1]);
@@ -630,7 +643,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<W, G>::kCtas) kv4_attn_kernel(At
         for (int i = 0; i < 2 * KS; i++) big = fmaxf(big, fabsf(grid_step(gr[i])));
         const int ex = max(13, (int)(__reduce_max_sync(0xffffffffu, __float_as_uint(big)) >> 23));
         const float up = __uint_as_float((uint32_t)(267 - ex) << 23);
-        down = __uint_as_float((uint32_t)min(254, ex + 11) << 23);   // 2^24 / up
+        down = __uint_as_float((uint32_t)min(254, ex + kCodeExp - 13) << 23);   // 2^kCodeExp / up
         float tl[G], tz[G];
 #pragma unroll
         for (int g = 0; g < G; g++) tl[g] = tz[g] = 0.f;
@@ -657,15 +670,14 @@ __global__ void __launch_bounds__(kThreads, Cfg<W, G>::kCtas) kv4_attn_kernel(At
       uint32_t vw[KS][2][W];
 #pragma unroll
       for (int k = 0; k < KS; k++) rows16<W, true>(vbuf_s, off, k, vw[k]);
-      const float down16 = down * 0.0625f;
 #pragma unroll
       for (int u = 0; u < W; u++) {
         float acc[G][2][4];
 #pragma unroll
         for (int k = 0; k < KS; k++) {
-          const uint32_t x = vw[k][0][u], x8 = x >> 8, y = vw[k][1][u], y8 = y >> 8;
-          const uint32_t a0[4] = {x & 0x000f000fu, x & 0x00f000f0u, y & 0x000f000fu, y & 0x00f000f0u};
-          const uint32_t a1[4] = {x8 & 0x000f000fu, x8 & 0x00f000f0u, y8 & 0x000f000fu, y8 & 0x00f000f0u};
+          const uint32_t x = vw[k][0][u], y = vw[k][1][u];
+          const uint32_t a0[4] = {codes<0>(x), codes<1>(x), codes<0>(y), codes<1>(y)};
+          const uint32_t a1[4] = {codes<2>(x), codes<3>(x), codes<2>(y), codes<3>(y)};
 #pragma unroll
           for (int g = 0; g < G; g++) {
             if (k == 0) {
@@ -682,7 +694,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<W, G>::kCtas) kv4_attn_kernel(At
 #pragma unroll
           for (int x = 0; x < 2; x++) {
             o[g][4 * u + 2 * x] = fmaf(acc[g][x][0] + acc[g][x][1], down, o[g][4 * u + 2 * x]);
-            o[g][4 * u + 2 * x + 1] = fmaf(acc[g][x][2] + acc[g][x][3], down16, o[g][4 * u + 2 * x + 1]);
+            o[g][4 * u + 2 * x + 1] = fmaf(acc[g][x][2] + acc[g][x][3], down, o[g][4 * u + 2 * x + 1]);
           }
       }
       __syncwarp();

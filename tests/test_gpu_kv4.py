@@ -12,7 +12,9 @@ Tolerances, from the arithmetic:
   the whole (|s| itself is below A, so its own rounding is in there).  A weight p
   then has the relative error 2 d plus 2^-20 (the exponential, its argument, the
   sums), and an output is a mean of values below C = max_j b_j:
-  |error| <= C * (4 d + 2^-19).  An accumulated weight adds g such p.
+  |error| <= C * (4 d + 2^-19).  Over a whole sequence the errors of the weights
+  are as many as the outputs: the relative error of its output in the 2-norm is
+  held to 2 d + 2^-20.  An accumulated weight adds g such p.
 - eviction moves bytes: everything equal.
 """
 import math
@@ -97,6 +99,7 @@ def check_attention(c, q, lens, scale=None, weight=None, got=None):
     for b, n in enumerate(lens):
         n = max(0, min(n, c.mb * c.bs))
         blk, off = c.places(b, n)
+        off2 = norm2 = 0.0
         for h in range(c.nKV):
             K, V = c.rows(0, b, h, n), c.rows(1, b, h, n)
             for hg in range(g):
@@ -104,8 +107,10 @@ def check_attention(c, q, lens, scale=None, weight=None, got=None):
                 err = np.abs(want - got[b, h * g + hg])
                 assert not np.isnan(got[b, h * g + hg]).any(), (b, n, h, hg)
                 assert err.max(initial=0) <= tol, (b, n, h, hg, err.max(), tol)
+                off2, norm2 = off2 + float((err ** 2).sum()), norm2 + float((want ** 2).sum())
                 if want_w is not None:
                     want_w[blk, h, off] += p
+        assert math.sqrt(off2) <= math.sqrt(norm2) * (2 * score_error(c, q, sc) + 2.0 ** -20), (b, n, math.sqrt(off2 / norm2))
     if want_w is not None:
         # every p within its relative error; adding it to the slot rounds once (2^-24 of the sum)
         err = np.abs(w.cpu().numpy() - want_w)
