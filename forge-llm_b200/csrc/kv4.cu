@@ -470,31 +470,30 @@ __global__ void __launch_bounds__(kEvThreads, CTAS) kv4_evict_kernel(EvArgs a) {
   const int64_t lrow = l * c.blocks * c.nKV * c.bs;
   const bool cut = n > a.budget;
   uint32_t *keys = SMEM ? keys_sm : a.keys + (int64_t)blockIdx.x * ev_at((int)c.cap);
-  // keys and the newest position; a block that the cache does not have leaves
-  // the sequence as it is
-  int bad = 0, mx = INT_MIN;
+  // the row of slot 0 where all slots lie in one block
+  int64_t flat = -1;
+  if (c.mb == 1) {
+    flat = block_of(c, b, 0);
+    if (flat >= 0) flat = (flat * c.nKV + h) * c.bs;
+  }
+  // the newest position; a block that the cache does not have leaves the sequence
+  // as it is
+  int bad = c.mb == 1 && flat < 0 && n > 0, mx = INT_MIN;
   if (cut || (l == 0 && h == 0 && c.table)) {
-    for (int j0 = G * tid; j0 < n; j0 += kEvBatch * G * kEvThreads) {
-      float w[kEvBatch][G];
-      int p[kEvBatch][G];
+    for (int j0 = G * tid; j0 < n; j0 += 2 * kEvBatch * G * kEvThreads) {
+      int p[2 * kEvBatch][G];
 #pragma unroll
-      for (int i = 0; i < kEvBatch; i++) {
+      for (int i = 0; i < 2 * kEvBatch; i++) {
         const int j = j0 + i * G * kEvThreads;
-        const int64_t at = j < n ? row_of(c, b, h, j) : -2;
+        const int64_t at = j >= n ? -2 : flat >= 0 ? flat + j : row_of(c, b, h, j);
         bad |= at == -1;
-        load_slots<G>(w[i], c.weight + lrow + at, cut && at >= 0, 0.f);
         load_slots<G>(p[i], c.pos + lrow + at, cut && at >= 0, INT_MIN);
       }
 #pragma unroll
-      for (int i = 0; i < kEvBatch; i++)
+      for (int i = 0; i < 2 * kEvBatch; i++)
 #pragma unroll
-        for (int e = 0; e < G; e++) {
-          const int j = j0 + i * G * kEvThreads + e;
-          if (cut && j < n) {
-            mx = max(mx, p[i][e]);
-            keys[ev_at(j)] = weight_key(w[i][e]);
-          }
-        }
+        for (int e = 0; e < G; e++)
+          if (j0 + i * G * kEvThreads + e < n) mx = max(mx, p[i][e]);
     }
     mx = __reduce_max_sync(0xffffffffu, mx);
     if (lane == 0) atomicMax(&s_max, mx);
@@ -505,31 +504,37 @@ __global__ void __launch_bounds__(kEvThreads, CTAS) kv4_evict_kernel(EvArgs a) {
   if (bad || !cut) return;
   // positions from `fresh` on are protected (none if there are no recent ones)
   const int64_t first = (int64_t)s_max - a.recent + 1;
-  const int fresh = a.recent == 0 ? INT_MAX : first < INT_MIN ? INT_MIN : (int)first;
+  const int fresh = first < INT_MIN ? INT_MIN : first > INT_MAX ? INT_MAX : (int)first;
   const bool some = a.recent > 0;
   uint32_t lo = 0xffffffffu, hi = 0, safe = 0;      // the other slots' range; the protected ones
-  for (int j0 = G * tid; j0 < n; j0 += 2 * kEvBatch * G * kEvThreads) {
-    int p[2 * kEvBatch][G];
+  for (int j0 = G * tid; j0 < n; j0 += kEvBatch * G * kEvThreads) {
+    float w[kEvBatch][G];
+    int p[kEvBatch][G];
 #pragma unroll
-    for (int i = 0; i < 2 * kEvBatch; i++) {
+    for (int i = 0; i < kEvBatch; i++) {
       const int j = j0 + i * G * kEvThreads;
-      load_slots<G>(p[i], c.pos + lrow + (j < n ? row_of(c, b, h, j) : 0), j < n, 0);
+      const int64_t at = j >= n ? 0 : flat >= 0 ? flat + j : row_of(c, b, h, j);
+      load_slots<G>(w[i], c.weight + lrow + at, j < n, 0.f);
+      load_slots<G>(p[i], c.pos + lrow + at, j < n, 0);
     }
 #pragma unroll
-    for (int i = 0; i < 2 * kEvBatch; i++)
+    for (int i = 0; i < kEvBatch; i++) {
+      const int j = j0 + i * G * kEvThreads;
+      uint32_t *dst = keys + ev_at(j);              // (four slots do not cross a word of padding)
 #pragma unroll
-      for (int e = 0; e < G; e++) {
-        const int j = j0 + i * G * kEvThreads + e;
-        if (j >= n) continue;
-        if (some && p[i][e] >= fresh) {
-          keys[ev_at(j)] = 0xffffffffu;
-          safe++;
-        } else {
-          const uint32_t k = keys[ev_at(j)];
-          lo = min(lo, k);
-          hi = max(hi, k);
+      for (int e = 0; e < G; e++)
+        if (j + e < n) {
+          uint32_t k = weight_key(w[i][e]);
+          if (some && p[i][e] >= fresh) {
+            k = 0xffffffffu;
+            safe++;
+          } else {
+            lo = min(lo, k);
+            hi = max(hi, k);
+          }
+          dst[e] = k;
         }
-      }
+    }
   }
   lo = __reduce_min_sync(0xffffffffu, lo);
   hi = __reduce_max_sync(0xffffffffu, hi);

@@ -813,7 +813,7 @@ constexpr int kFewPieces = 12;
 constexpr int kFinishThreads = 256;
 constexpr int kFinishWarps = kFinishThreads / 32;
 constexpr int kWtSlots = 1024;
-template <int W>
+template <int W, bool VEC>
 __global__ void __launch_bounds__(kFinishThreads) kv4_attn_finish_kernel(AttnArgs a) {
   pdl_trigger();
   __shared__ float o_s[kFinishWarps][32 * W];
@@ -904,18 +904,36 @@ __global__ void __launch_bounds__(kFinishThreads) kv4_attn_finish_kernel(AttnArg
   if (j0 >= n) return;
   // what does not wait for (m, l) is asked for first
   constexpr int kPer = kWtSlots / kFinishThreads, kAhead = 4;
-  const float *sc = a.scores + (b * a.nH + h * a.g) * c.cap + j0 + threadIdx.x;
-  float w[kPer], old[kPer], s[kAhead][kPer];
+  static_assert(kPer == 4, "");
+  const float *sc = a.scores + (b * a.nH + h * a.g) * c.cap + j0;
+  // VEC: a thread's four slots are neighbours, 16 aligned bytes of scores and weight
+  constexpr int kStep = VEC ? 1 : kFinishThreads;
+  const int mine = VEC ? 4 * threadIdx.x : threadIdx.x;
+  float w[kPer] = {0.f, 0.f, 0.f, 0.f}, old[kPer], s[kAhead][kPer];
   int64_t row[kPer];
+  auto load = [&](float (&x)[kPer], const float *p) {
+    if constexpr (VEC) {
+      const float4 f = row[0] >= 0 ? *reinterpret_cast<const float4 *>(p) : float4{0.f, 0.f, 0.f, 0.f};
+      x[0] = f.x, x[1] = f.y, x[2] = f.z, x[3] = f.w;
+    } else {
 #pragma unroll
-  for (int x = 0; x < kPer; x++) {
-    const int64_t j = j0 + threadIdx.x + x * kFinishThreads;
-    row[x] = j < n ? row_of(c, b, h, j) : -1;
-    old[x] = row[x] >= 0 ? c.weight[row[x]] : 0.f;
-    w[x] = 0.f;
+      for (int k = 0; k < kPer; k++) x[k] = row[k] >= 0 ? p[k * kStep] : 0.f;
+    }
+  };
 #pragma unroll
-    for (int i = 0; i < kAhead; i++) s[i][x] = i < a.g && row[x] >= 0 ? sc[i * c.cap + x * kFinishThreads] : 0.f;
+  for (int k = 0; k < kPer; k++) {
+    const int64_t j = j0 + mine + k * kStep;
+    row[k] = VEC && k > 0 ? (j < n && row[0] >= 0 ? row[0] + k : -1) : j < n ? row_of(c, b, h, j) : -1;
   }
+  if constexpr (VEC) {
+    load(old, c.weight + row[0]);
+  } else {
+#pragma unroll
+    for (int k = 0; k < kPer; k++) old[k] = row[k] >= 0 ? c.weight[row[k]] : 0.f;
+  }
+#pragma unroll
+  for (int i = 0; i < kAhead; i++)
+    if (i < a.g) load(s[i], sc + i * c.cap + mine);
   for (int hd = warp; hd < a.g; hd += kFinishWarps) {
     float2 x = a.ml[b * a.nH + h * a.g + hd];
     // a cut segment's: the run it begins in, and minus its pieces
@@ -933,16 +951,19 @@ __global__ void __launch_bounds__(kFinishThreads) kv4_attn_finish_kernel(AttnArg
 #pragma unroll
     for (int i = 0; i < kAhead; i++)
       if (hd + i < a.g) {
+        const float m = m_s[hd + i], il = il_s[hd + i];
 #pragma unroll
-        for (int x = 0; x < kPer; x++) {
-          w[x] = fmaf(ex2(s[i][x] - m_s[hd + i]), il_s[hd + i], w[x]);
-          s[i][x] = hd + i + kAhead < a.g && row[x] >= 0 ? sc[(hd + i + kAhead) * c.cap + x * kFinishThreads] : 0.f;
-        }
+        for (int k = 0; k < kPer; k++) w[k] = fmaf(ex2(s[i][k] - m), il, w[k]);
+        if (hd + i + kAhead < a.g) load(s[i], sc + (hd + i + kAhead) * c.cap + mine);
       }
   }
+  if (VEC && row[3] >= 0) {
+    *reinterpret_cast<float4 *>(c.weight + row[0]) = make_float4(old[0] + w[0], old[1] + w[1], old[2] + w[2], old[3] + w[3]);
+  } else {
 #pragma unroll
-  for (int x = 0; x < kPer; x++)
-    if (row[x] >= 0) c.weight[row[x]] = old[x] + w[x];
+    for (int k = 0; k < kPer; k++)
+      if (row[k] >= 0) c.weight[row[k]] = old[k] + w[k];
+  }
 }
 
 // How the heads are dealt: q heads per kv head, segments per kv head (a CTA
@@ -956,8 +977,9 @@ struct Heads {
 int64_t part_floats(const Cache &c, const Heads &p) {
   return p.whole ? 0 : (int64_t)p.ctas * (2 * kMaxHeads * (c.dH + 2) + sizeof(Cut) / 4);
 }
+int64_t ml_floats(int B, int nH) { return (2 * (int64_t)B * nH + 3) & ~(int64_t)3; }
 int64_t work_floats(const Cache &c, int B, int nH, const Heads &p) {
-  return part_floats(c, p) + (c.weight ? (int64_t)B * nH * (c.cap + 2) : 0);
+  return part_floats(c, p) + (c.weight ? ml_floats(B, nH) + (int64_t)B * nH * c.cap : 0);
 }
 
 int checked(const char *who, const fcu_kv4 *cache, int B, int nH, bool arrays, Cache *c) {
@@ -995,7 +1017,8 @@ int launch(fcu_ctx *ctx, const AttnArgs &a) {
   note_launch();
   const int64_t blocks = (a.whole ? 0 : a.ctas - 1) + (a.scores ? (int64_t)a.B * a.c.nKV * ((a.c.cap + kWtSlots - 1) / kWtSlots) : 0);
   if (blocks > 0) {
-    FCU_CHECK_CUDA(launch_pdl(kv4_attn_finish_kernel<W>, dim3((unsigned)blocks), dim3(kFinishThreads), 0, ctx->stream, a));
+    const bool vec = a.scores && a.c.cap % 4 == 0 && a.c.bs % 4 == 0 && ((uintptr_t)a.c.weight & 15) == 0;
+    FCU_CHECK_CUDA(launch_pdl(vec ? kv4_attn_finish_kernel<W, true> : kv4_attn_finish_kernel<W, false>, dim3((unsigned)blocks), dim3(kFinishThreads), 0, ctx->stream, a));
     note_launch();
   }
   return FCU_OK;
@@ -1076,7 +1099,7 @@ int fcu_kv4_attn(fcu_ctx *ctx, const float *q, int64_t ld_q, const fcu_kv4 *cach
   a.part = (float *)(a.cuts + a.ctas);
   if (a.c.weight) {
     a.ml = (float2 *)((float *)work + part_floats(a.c, p));
-    a.scores = (float *)(a.ml + (int64_t)B * nH);
+    a.scores = (float *)a.ml + ml_floats(B, nH);
   }
 #define FCU_CASE(W, G) rc = launch<W, G>(ctx, a)
   FCU_KV4_WIDTHS(FCU_CASE, a.c.rb, a.gs)
