@@ -316,7 +316,6 @@ int beam_slices(int num_sms, int B, int W, int64_t V) {
 // beam that is continued is read once, every beam that changes written once.
 constexpr int kReThreads = 128;
 constexpr int kReWarps = kReThreads / 32;
-constexpr int kReSlots = 16;           // 16-byte pieces of a lane, over all beams
 
 struct ReArgs {
   uint8_t *base[8];
@@ -324,7 +323,7 @@ struct ReArgs {
   int n_arrays;
   int64_t layers, blocks;
   const int32_t *table, *parents, *lens;
-  int bs, mb, B, W, depth;     // depth: pieces of a lane from one beam, depth * W <= kReSlots (W <= 16)
+  int bs, mb, B, W;
   int64_t cap;
 };
 
@@ -345,13 +344,15 @@ __device__ __forceinline__ void re_store(uint8_t *dst, const uint4 *src, int n, 
   }
 }
 
+// D: 16-byte pieces of a lane from one beam in one step.
+template <int D>
 __global__ void __launch_bounds__(kReThreads) cache_reorder_kernel(ReArgs a) {
   pdl_trigger();
-  extern __shared__ __align__(16) uint4 hold[];     // [warp][W][depth][32]
+  extern __shared__ __align__(16) uint4 hold[];     // [warp][W][D][32]
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, W = a.W;
   const int b = blockIdx.y;
   const int64_t layer = blockIdx.z;
-  uint4 *mine = hold + warp * W * a.depth * 32 + lane;
+  uint4 *mine = hold + warp * W * D * 32 + lane;
   const uint32_t mine_s = (uint32_t)__cvta_generic_to_shared(mine);
   pdl_wait();
   // lane w: the beam that beam w becomes (itself if it stays) and beam w's length
@@ -367,7 +368,7 @@ __global__ void __launch_bounds__(kReThreads) cache_reorder_kernel(ReArgs a) {
   for (uint32_t m = moves; m; m &= m - 1) needed |= 1u << __shfl_sync(0xffffffffu, src, __ffs(m) - 1);
   if (!needed) return;
   const int longest = __reduce_max_sync(0xffffffffu, needed >> lane & 1 ? len : 0);
-  const int chunk = 512 * a.depth;                          // bytes of one step
+  constexpr int chunk = 512 * D;                            // bytes of one step
   for (int x = 0; x < a.n_arrays; x++) {
     const int64_t unit = a.unit[x], seg = a.bs * unit;      // bytes of one head of one block
     const bool wide = seg % 16 == 0;
@@ -396,8 +397,15 @@ __global__ void __launch_bounds__(kReThreads) cache_reorder_kernel(ReArgs a) {
         const int64_t from = __shfl_sync(0xffffffffu, at, w);
         const int n = __shfl_sync(0xffffffffu, bytes, w);
         if (from < 0) continue;
-        for (int d = 0; d < a.depth && 512 * d + 16 * lane < n; d++)
-          re_load(mine_s + (w * a.depth + d) * 512, a.base[x] + from + 512 * d + 16 * lane, min(16, n - 512 * d - 16 * lane), wide);
+        const uint8_t *p = a.base[x] + from + 16 * lane;
+        const uint32_t to = mine_s + w * D * 512;
+        if (wide && n == chunk) {
+#pragma unroll
+          for (int d = 0; d < D; d++) re_load(to + 512 * d, p + 512 * d, 16, true);
+        } else {
+          for (int d = 0; d < D && 512 * d + 16 * lane < n; d++)
+            re_load(to + 512 * d, p + 512 * d, min(16, n - 512 * d - 16 * lane), wide);
+        }
       }
       asm volatile("cp.async.commit_group;\n\tcp.async.wait_group 0;" ::: "memory");
       for (uint32_t m = moves; m; m &= m - 1) {
@@ -405,8 +413,15 @@ __global__ void __launch_bounds__(kReThreads) cache_reorder_kernel(ReArgs a) {
         const int64_t to = __shfl_sync(0xffffffffu, at, w), from = __shfl_sync(0xffffffffu, at, s);
         const int n = __shfl_sync(0xffffffffu, bytes, s);
         if (to < 0 || from < 0) continue;
-        for (int d = 0; d < a.depth && 512 * d + 16 * lane < n; d++)
-          re_store(a.base[x] + to + 512 * d + 16 * lane, mine + (s * a.depth + d) * 32, min(16, n - 512 * d - 16 * lane), wide);
+        uint8_t *p = a.base[x] + to + 16 * lane;
+        const uint4 *y = mine + s * D * 32;
+        if (wide && n == chunk) {
+#pragma unroll
+          for (int d = 0; d < D; d++) re_store(p + 512 * d, y + 32 * d, 16, true);
+        } else {
+          for (int d = 0; d < D && 512 * d + 16 * lane < n; d++)
+            re_store(p + 512 * d, y + 32 * d, min(16, n - 512 * d - 16 * lane), wide);
+        }
       }
     }
   }
@@ -485,8 +500,8 @@ int fcu_cache_reorder(fcu_ctx *ctx, const fcu_cache_array *arrays, int n_arrays,
   ReArgs a{};
   a.cap = (int64_t)block_size * max_blocks;
   FCU_REQUIRE(a.cap <= 1 << 30, "fcu_cache_reorder: %lld slots per sequence (at most 2^30)", (long long)a.cap);
-  a.depth = W >= kReSlots ? 1 : kReSlots / W;
-  a.depth = a.depth > 4 ? 4 : a.depth;
+  // 8 KB of shared memory a warp up to 16 beams, 16 KB for 32
+  const int depth = W <= 4 ? 4 : W <= 8 ? 2 : 1;
   int64_t most = 0;
   for (int i = 0; i < n_arrays; i++) {
     FCU_REQUIRE(arrays[i].base && ((uintptr_t)arrays[i].base & 15) == 0, "fcu_cache_reorder: array %d is null or not 16-byte aligned", i);
@@ -497,7 +512,7 @@ int fcu_cache_reorder(fcu_ctx *ctx, const fcu_cache_array *arrays, int n_arrays,
     a.base[i] = (uint8_t *)arrays[i].base;
     a.heads[i] = arrays[i].heads;
     a.unit[i] = arrays[i].unit;
-    const int64_t chunk = 512 * a.depth, steps = ((int64_t)block_size * arrays[i].unit + chunk - 1) / chunk;
+    const int64_t chunk = 512 * depth, steps = ((int64_t)block_size * arrays[i].unit + chunk - 1) / chunk;
     const int64_t items = arrays[i].heads * max_blocks * steps;
     most = items > most ? items : most;
   }
@@ -517,14 +532,15 @@ int fcu_cache_reorder(fcu_ctx *ctx, const fcu_cache_array *arrays, int n_arrays,
   const int64_t pairs = (int64_t)B * layers, fill = (8 * 6 * (int64_t)ctx->num_sms + pairs - 1) / pairs;
   int64_t gx = (most + kReWarps - 1) / kReWarps;
   gx = gx < fill ? gx : fill;
-  const size_t smem = (size_t)W * a.depth * kReThreads * 16;
+  const size_t smem = (size_t)W * depth * kReThreads * 16;
   static bool set[64] = {false};
   if (!set[ctx->device & 63]) {
-    FCU_CHECK_CUDA(cudaFuncSetAttribute(cache_reorder_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+    FCU_CHECK_CUDA(cudaFuncSetAttribute(cache_reorder_kernel<1>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                         kMaxW * kReThreads * 16));
     set[ctx->device & 63] = true;
   }
-  FCU_CHECK_CUDA(launch_pdl(cache_reorder_kernel, dim3((unsigned)gx, B, (unsigned)layers), dim3(kReThreads), smem,
+  void (*kernel)(ReArgs) = depth == 4 ? cache_reorder_kernel<4> : depth == 2 ? cache_reorder_kernel<2> : cache_reorder_kernel<1>;
+  FCU_CHECK_CUDA(launch_pdl(kernel, dim3((unsigned)gx, B, (unsigned)layers), dim3(kReThreads), smem,
                             ctx->stream, a));
   note_launch();
   return FCU_OK;
