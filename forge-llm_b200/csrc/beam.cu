@@ -426,6 +426,7 @@ __global__ void __launch_bounds__(kReThreads) cache_reorder_kernel(ReArgs a) {
             re_store(p + 512 * d, y + 32 * d, min(16, n - 512 * d - 16 * lane), wide);
         }
       }
+      asm volatile("" ::: "memory");      // `mine` is read before the next step's copies into it
     }
   }
 }
@@ -454,7 +455,18 @@ int fcu_beam_step(fcu_ctx *ctx, const float *logits, int64_t ld, const float *sc
   FCU_REQUIRE((int64_t)B * W <= 65535, "fcu_beam_step: %d x %d rows in one call", B, W);
   if (B == 0) return FCU_OK;
   FCU_REQUIRE(logits && scores && done && out_scores && tokens && parents && out_done, "fcu_beam_step: null pointer");
-  FCU_REQUIRE((const void *)out_scores != scores && out_done != done, "fcu_beam_step: an output is an input");
+  const int64_t R = (int64_t)B * W;
+  auto apart = [&](const void *p, int64_t n, const void *q, int64_t m) {
+    return (uintptr_t)p + n <= (uintptr_t)q || (uintptr_t)q + m <= (uintptr_t)p;
+  };
+  const void *outs[4] = {out_scores, tokens, parents, out_done};
+  for (int i = 0; i < 4; i++) {
+    const int64_t n = i < 3 ? 4 * R : R;
+    bool ok = apart(outs[i], n, scores, 4 * R) && apart(outs[i], n, done, R) &&
+              apart(outs[i], n, logits, 4 * ((R - 1) * ld + V));
+    for (int j = 0; j < i; j++) ok &= apart(outs[i], n, outs[j], 4 * R);
+    FCU_REQUIRE(ok, "fcu_beam_step: an output overlaps another or an input");
+  }
   const int64_t need = fcu_beam_work(ctx, B, W, V);
   FCU_REQUIRE(work && work_bytes >= need && ((uintptr_t)work & 15) == 0,
               "fcu_beam_step: workspace of %lld bytes, %lld needed", (long long)work_bytes, (long long)need);
@@ -515,6 +527,13 @@ int fcu_cache_reorder(fcu_ctx *ctx, const fcu_cache_array *arrays, int n_arrays,
     a.base[i] = (uint8_t *)arrays[i].base;
     a.heads[i] = arrays[i].heads;
     a.unit[i] = arrays[i].unit;
+    // (sizes in double: their products may pass 64 bits)
+    const double bytes = (double)layers * blocks * block_size;
+    for (int j = 0; j < i; j++) {
+      const uintptr_t p = (uintptr_t)a.base[i], q = (uintptr_t)a.base[j];
+      FCU_REQUIRE(p < q ? (double)(q - p) >= bytes * a.heads[i] * a.unit[i] : (double)(p - q) >= bytes * a.heads[j] * a.unit[j],
+                  "fcu_cache_reorder: arrays %d and %d overlap", j, i);
+    }
     const int64_t chunk = 512 * depth, steps = ((int64_t)block_size * arrays[i].unit + chunk - 1) / chunk;
     const int64_t items = arrays[i].heads * max_blocks * steps;
     most = items > most ? items : most;

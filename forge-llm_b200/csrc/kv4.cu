@@ -131,7 +131,7 @@ __global__ void __launch_bounds__(kPutThreads, 4) kv4_put_kernel(PutArgs a) {
   const int64_t pos0 = (int64_t)a.positions[b] + t0, slot0 = (int64_t)a.slots[b] + t0;
   if (tid < nt) {
     const int64_t j = slot0 + tid;
-    row_s[tid] = j >= 0 && j < c.cap && pos0 + tid >= 0 ? row_of(c, b, 0, j) : -1;
+    row_s[tid] = j >= 0 && j < c.cap && pos0 + tid >= 0 && pos0 + tid <= INT_MAX ? row_of(c, b, 0, j) : -1;
   }
   __syncthreads();
   float *x0 = a.qkv + (b * a.T + t0) * a.ld;

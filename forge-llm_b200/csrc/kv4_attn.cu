@@ -1110,6 +1110,8 @@ int fcu_kv4_attn(fcu_ctx *ctx, const float *q, int64_t ld_q, const fcu_kv4 *cach
               "fcu_kv4_attn: workspace of %lld bytes, %lld needed", (long long)work_bytes, (long long)need);
   a.cuts = (Cut *)work;
   a.part = (float *)(a.cuts + a.ctas);
+  FCU_REQUIRE(out + (int64_t)B * nH * a.c.dH <= q || q + (B - 1) * ld_q + (int64_t)nH * a.c.dH <= out,
+              "fcu_kv4_attn: out overlaps q");
   if (a.c.weight) {
     a.ml = (float2 *)((float *)work + part_floats(a.c, p));
     a.scores = (float *)a.ml + ml_floats(B, nH);

@@ -287,6 +287,8 @@ class Transformer:
         bf = self._buffers(B)
         # the cache row of each token: its position, but for a cache that evicts
         q4 = hasattr(cache, "slotOf")
+        if q4 and (cache.nLayers, cache.nKvHeads, cache.dHead) != (c.nLayers, c.nKvHeads, c.dHead):
+            raise ValueError(f"a cache of {cache.nLayers} layers of {cache.nKvHeads} heads of {cache.dHead}")
         slots = [cache.slotOf(p, b) for b, p in enumerate(positions)] if q4 else list(positions)
         host = np.array([list(tokens), list(positions), [s + 1 for s in slots], slots], np.int32)
         dev_host = torch.from_numpy(host)
@@ -340,6 +342,14 @@ class Transformer:
         if not ids or maxNew < 1 or cache.batch != beams or cache.len:
             raise ValueError(f"beamSearch: {len(ids)} prompt tokens, maxNew {maxNew}, {beams} beams on "
                              f"{'a used' if cache.len else 'a'} cache of {cache.batch}")
+        rows, last = cache.max_blocks * cache.block_size, len(ids) + maxNew - 1
+        if last > rows and (budget is None or budget >= rows):
+            raise ValueError(f"beamSearch: {last} positions in a cache of {rows}")
+        if not 1 <= beams <= 32 or not 0 <= eos < c.vocabSize:
+            raise ValueError(f"beamSearch: {beams} beams (1 to 32), eosId {eos} of {c.vocabSize} tokens")
+        if budget is not None and (getattr(cache, "weight", None) is None or not 0 <= recent <= budget or budget < 1):
+            raise ValueError(f"beamSearch: budget {budget}, recent {recent}, on a cache "
+                             f"{'without' if getattr(cache, 'weight', None) is None else 'with'} weights")
         for p, t in enumerate(ids):
             logits = self.forward(t, p, cache, graph=graph)
             if budget is not None:

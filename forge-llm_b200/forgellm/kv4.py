@@ -13,7 +13,9 @@ reference has no counterpart: its caches are fp32 and it samples one sequence.
 
 All tensors are on the current CUDA device and every call runs on its current
 stream.  A call that finds them anywhere else, or of another type, shape or
-stride than it takes, raises ValueError before anything is launched.
+stride than it takes, raises ValueError before anything is launched.  As for the
+rest of the package, one host thread at a time makes calls on a device: its
+context is bound to one stream at a time.
 """
 from __future__ import annotations
 
@@ -91,6 +93,12 @@ def _check(name: str, t, dtype, dev: int, shape=None) -> None:
     raise ValueError(f"{name} is not contiguous")
 
 
+def _tensors(**ts) -> None:
+    for name, t in ts.items():
+        if not isinstance(t, torch.Tensor):
+            raise ValueError(f"{name}: a tensor is needed, got {type(t).__name__}")
+
+
 def _row_bytes(dHead: int) -> int:
     rb = _ROW_BYTES.get(dHead)
     if rb is None:
@@ -161,7 +169,8 @@ def kv4Put(qkv, nHeads: int, positions, slots, k, kg, v, vg, T: int = 1, theta: 
     and slot slots[b] + t (int32 [B]).  The q heads are rotated in place, k and v
     go to the cache in 4 bits; their columns of qkv stay as they are.  theta 0:
     the rows carry their rotation already.  A token whose slot is outside the
-    cache, or whose position is negative, changes nothing."""
+    cache, or whose position is negative or past int32, changes nothing.  No two
+    tokens of a call may go to the same place."""
     dev = _device()
     _check("positions", positions, _I32, dev)
     B = positions.numel()
@@ -170,6 +179,7 @@ def kv4Put(qkv, nHeads: int, positions, slots, k, kg, v, vg, T: int = 1, theta: 
         raise ValueError(f"{slots.numel()} slots for {B} sequences")
     if T < 1 or nHeads < 0 or not theta >= 0:
         raise ValueError(f"T={T}, nHeads={nHeads}, theta={theta}")
+    _tensors(k=k, kg=kg, v=v, vg=vg)
     if k.ndim != 4:
         raise ValueError(f"k: {k.ndim} dimensions")
     heads = nHeads + 2 * k.shape[1]
@@ -189,6 +199,7 @@ def kv4Values(k, kg, v, vg, dHead: int, start, T: int, table=None):
     B = start.numel()
     if T < 0:
         raise ValueError(f"T={T}")
+    _tensors(k=k, kg=kg, v=v, vg=vg)
     c = _cache(dev, k, kg, v, vg, dHead, B, table)
     K, V = k.new_empty((2, B, T, c.n_kv, dHead), dtype=_F32).unbind(0)
     _call("fcu_kv4_values", _on(dev), c, start.data_ptr(), B, T, K.data_ptr(), V.data_ptr())
@@ -200,7 +211,8 @@ def kv4Attention(q, k, kg, v, vg, lens, scale: float | None = None, table=None, 
     may be strided) over the first lens[b] slots of each sequence (int32 [B];
     0 gives zeros), grouped heads as in attentionDecode.  scale: 1 / sqrt(dHead)
     unless given.  With `weight`, every slot's attention weight, summed over its
-    kv head's q heads, is added to it."""
+    kv head's q heads, is added to it; the sequences may then share no block among
+    those slots.  `out` may not overlap q."""
     dev = _device()
     if not (isinstance(q, torch.Tensor) and q.dtype is _F32 and q.ndim == 3):
         raise ValueError("q: a float32 [B, nHeads, dHead] is needed")
@@ -214,6 +226,7 @@ def kv4Attention(q, k, kg, v, vg, lens, scale: float | None = None, table=None, 
             raise ValueError(f"q: strides {s}")
         ld = s[0] if B > 1 else ld
     _check("lens", lens, _I32, dev, (B,))
+    _tensors(k=k, kg=kg, v=v, vg=vg)
     c = _cache(dev, k, kg, v, vg, dH, B, table, weight)
     if out is None:
         out = q.new_empty((B, nH, dH))
@@ -234,14 +247,17 @@ def kv4Evict(k, kg, v, vg, weight, pos, lens, budget: int, recent: int, table=No
     """Cuts every head of every layer (arrays with a leading layer dimension)
     of sequences longer than `budget` down to it: the slots of the `recent`
     newest positions and those of largest weight stay (ties: the lowest slot),
-    moved into the freed slots.  Returns the new lengths, min(lens, budget)."""
+    moved into the freed slots.  No two sequences may share a block.  Returns the new lengths, min(lens, budget)."""
     dev = _device()
     _check("lens", lens, _I32, dev)
     B = lens.numel()
     if weight is None or pos is None:
         raise ValueError("eviction goes by `weight` and `pos`")
-    if budget < 1 or not 0 <= recent <= budget:
+    if not 1 <= budget < 2 ** 31 or not 0 <= recent <= budget:
         raise ValueError(f"budget {budget}, recent {recent}")
+    _tensors(k=k, kg=kg, v=v, vg=vg)
+    if k.ndim != 5:
+        raise ValueError(f"k: {k.ndim} dimensions")
     c = _cache(dev, k, kg, v, vg, 2 * k.shape[-1], B, table, weight, pos, layers=True)
     if newLens is None:
         newLens = torch.empty_like(lens)
@@ -289,7 +305,8 @@ def cacheReorder(arrays, parents, lens, table=None) -> None:
     of sequence b (cache sequence b * W + w) takes over slots [0, lens[source])
     of its source b * W + parents[b, w].  arrays: up to 8 tensors [layers, blocks,
     heads, blockSize, ...] whose slots hold a multiple of 4 bytes (an fp32 cache
-    has one head: its rows); parents int32 [B, W]; lens int32 [B * W]."""
+    has one head: its rows); parents int32 [B, W]; lens int32 [B * W].  No two
+    beams may share a block, and no two arrays memory."""
     dev = _device()
     _check("parents", parents, _I32, dev)
     if parents.ndim != 2 or not 1 <= parents.shape[1] <= 32:
@@ -301,6 +318,9 @@ def cacheReorder(arrays, parents, lens, table=None) -> None:
     n = len(arrays)
     if not 1 <= n <= 8:
         raise ValueError(f"{n} arrays (1 to 8)")
+    _tensors(**{f"arrays[{i}]": t for i, t in enumerate(arrays)})
+    if arrays[0].ndim < 4:
+        raise ValueError(f"arrays[0]: {arrays[0].ndim} dimensions")
     L, blocks, _, bs = arrays[0].shape[:4]
     spec = (CacheArray * n)()
     for i, t in enumerate(arrays):
@@ -352,6 +372,8 @@ class QuantKVCache(KVCache):
             t = np.ascontiguousarray(table, np.int32).reshape(batch, self.max_blocks)
             if t.min() < 0 or t.max() >= phys:
                 raise ValueError("QuantKVCache: block table entry outside the physical blocks")
+            if track and np.unique(t).size < t.size:
+                raise ValueError("QuantKVCache: sequences that share blocks cannot keep their weights apart")
             self._table_host, self.table = t, torch.from_numpy(t).to(dev)
         elif phys != batch * self.max_blocks:
             raise ValueError(f"QuantKVCache: {phys} physical blocks need a block table")
@@ -441,9 +463,8 @@ class QuantKVCache(KVCache):
         """cacheReorder for searches of parents.shape[1] beams over all `batch`
         sequences (parents: a host or device int array [B, W])."""
         self._own_blocks()
-        _reorder(self, [t for t in (self.k, self.kg, self.v, self.vg, self.weight, self.pos) if t is not None],
-                 parents, self.lens)
         p = np.asarray(parents.cpu() if isinstance(parents, torch.Tensor) else parents)
+        _reorder(self, [t for t in (self.k, self.kg, self.v, self.vg, self.weight, self.pos) if t is not None], p, self.lens)
         src = (np.arange(p.shape[0])[:, None] * p.shape[1] + p).reshape(-1)
         self.lens, self.dropped = self.lens[src].copy(), self.dropped[src].copy()
         self.len = int(self.lens.max(initial=0))
@@ -455,8 +476,12 @@ class QuantKVCache(KVCache):
 
 def _reorder(cache, arrays, parents, lens) -> None:
     p = parents if isinstance(parents, torch.Tensor) else torch.as_tensor(np.asarray(parents))
-    _need(p.ndim == 2 and p.numel() == cache.batch, f"parents: shape {tuple(p.shape)} for a cache of {cache.batch}")
+    _need(p.ndim == 2 and p.numel() == cache.batch and not p.is_floating_point(),
+          f"parents: {p.dtype} of shape {tuple(p.shape)} for a cache of {cache.batch}")
     if not p.is_cuda and p.numel():
         _need(int(p.min()) >= 0 and int(p.max()) < p.shape[1], "parents outside their search's beams")
     lens = torch.from_numpy(np.ascontiguousarray(lens, np.int32)).to(cache.k.device)
-    cacheReorder(arrays, p.to(device=cache.k.device, dtype=_I32).contiguous(), lens, table=cache.table)
+    table = cache.table
+    if table is None and arrays[0].shape[1] != cache.batch * cache.max_blocks:      # more blocks than it uses
+        table = torch.arange(cache.batch * cache.max_blocks, dtype=_I32, device=cache.k.device).view(cache.batch, -1)
+    cacheReorder(arrays, p.to(device=cache.k.device, dtype=_I32).contiguous(), lens, table=table)

@@ -509,8 +509,9 @@ int fcu_kv4_row_bytes(int dH);
  * rotates them (theta 0: not at all), then k and v are quantized into the
  * slot; its weight becomes 0 and its pos the position where those are kept.
  * The k and v columns of qkv stay as they are.  A token whose slot is outside
- * [0, max_blocks * block_size), in a bad block, or whose position is negative,
- * leaves everything untouched. */
+ * [0, max_blocks * block_size), in a bad block, or whose position is negative or
+ * past int32, leaves everything untouched.  No two tokens of a call may go to
+ * the same place (sequences may share the blocks they only read). */
 int fcu_kv4_put(fcu_ctx *ctx, float *qkv, int64_t ld_qkv, int B, int T, int nH, double theta,
                 const int32_t *positions, const int32_t *slots, const fcu_kv4 *cache);
 /* K[b, t, h, :], V[b, t, h, :] (fp32 [B, T, nKV, dH]; either may be NULL) =
@@ -525,8 +526,9 @@ int64_t fcu_kv4_attn_work(fcu_ctx *ctx, const fcu_kv4 *cache, int B, int nH);
  * the capacity), p = softmax_j(scale * q_bh . k^_j), kv head h / (nH / nKV):
  * fcu_attn_decode over the 4-bit cache.  A length of 0 gives zeros.  q rows are
  * ld_q floats apart, out is [B, nH * dH].  Where the cache keeps weights, the
- * slot's weight grows by its p summed over the q heads of its kv head.
- * nH / nKV <= 16.  `work` is the caller's (fcu_kv4_attn_work bytes, 16-byte
+ * slot's weight grows by its p summed over the q heads of its kv head; sequences
+ * may then share no block among their first seq_lens slots.  nH / nKV <= 16, B at
+ * most 65535, out overlaps no part of q.  `work` is the caller's (fcu_kv4_attn_work bytes, 16-byte
  * aligned) and may be reused once the call's work on the stream is done. */
 int fcu_kv4_attn(fcu_ctx *ctx, const float *q, int64_t ld_q, const fcu_kv4 *cache, const int32_t *seq_lens, int B,
                  int nH, double scale, float *out, void *work, int64_t work_bytes);
@@ -556,8 +558,8 @@ int64_t fcu_beam_work(fcu_ctx *ctx, int B, int W, int64_t V);
  * in double; a beam that has ended offers (w, eos) at scores[w] alone; whatever
  * is not finite counts as -inf.  The W best, by score and then by lowest
  * w * V + token, give out_scores, tokens, parents (= w) and out_done (ended
- * before, or token is eos), [B, W] each, best first; none of them may be an
- * input's buffer.  1 <= W <= 32.  logits may hold -inf (a banned token); a NaN
+ * before, or token is eos), [B, W] each, best first; none of them may overlap
+ * another or an input.  1 <= W <= 32.  logits may hold -inf (a banned token); a NaN
  * or +inf makes all of its row's candidates -inf. */
 int fcu_beam_step(fcu_ctx *ctx, const float *logits, int64_t ld, const float *scores, const uint8_t *done, int B,
                   int W, int64_t V, int eos, float *out_scores, int32_t *tokens, int32_t *parents,
@@ -574,8 +576,8 @@ typedef struct {
  * [0, lens[src]) of beam w become those of src = b * W + parents[b * W + w] as
  * they were before the call; slots past that stay.  A parent outside [0, W)
  * leaves its beam as it is, and so does a block outside [0, blocks).  Slots map
- * to blocks as in fcu_kv4; no two beams may share a block.  1 <= W <= 32, at
- * most 8 arrays. */
+ * to blocks as in fcu_kv4; no two beams may share a block, and no two arrays
+ * memory.  1 <= W <= 32, at most 8 arrays. */
 int fcu_cache_reorder(fcu_ctx *ctx, const fcu_cache_array *arrays, int n_arrays, int64_t layers, int64_t blocks,
                       const int32_t *table, int block_size, int max_blocks, const int32_t *parents,
                       const int32_t *lens, int B, int W);

@@ -297,3 +297,40 @@ def test_search_with_eviction(model):
         c.slotOf(0)
     w = c.weight.sum().item()
     assert np.isfinite(w) and w > 0
+
+
+def test_reorder_of_a_paged_cache_with_spare_blocks():
+    """Without a table the beams' blocks are the first of a larger pool."""
+    fw = F()
+    c = fw.PagedKVCache(2, 24, 8, blockSize=8, batch=3, physBlocks=18)
+    c.k.copy_(torch.arange(c.k.numel(), device="cuda").view_as(c.k))
+    c.v.copy_(-c.k)
+    c.len = 20
+    want = c.k.clone()
+    for w, p in enumerate([2, 2, 0]):
+        want[:, 24 * w:24 * w + 20] = c.k[:, 24 * p:24 * p + 20]
+    c.reorder([[2, 2, 0]])
+    assert torch.equal(c.k, want) and torch.equal(c.v, -want)
+
+
+def test_search_refusals(model):
+    """Refused before the first step, so that the cache stays unused."""
+    cfg, tr = model
+    fw = F()
+    fp = fw.KVCache(cfg.nLayers, 16, cfg.kvDim, batch=2)
+    q4 = fw.QuantKVCache(cfg.nLayers, 16, cfg.nKvHeads, cfg.dHead, batch=2, track=True)
+    other = fw.QuantKVCache(cfg.nLayers, 16, cfg.nKvHeads, cfg.dHead - 4, batch=2)
+    ids = list(range(3, 13))
+    for f in (lambda: tr.beamSearch(ids, 2, 8, fp), lambda: tr.beamSearch(ids, 2, 8, q4),
+              lambda: tr.beamSearch(ids, 2, 8, q4, budget=16), lambda: tr.beamSearch(ids, 2, 4, fp, budget=8),
+              lambda: tr.beamSearch(ids, 2, 4, q4, budget=8, recent=9), lambda: tr.beamSearch(ids, 2, 4, q4, budget=0),
+              lambda: tr.beamSearch(ids, 2, 4, q4, eosId=cfg.vocabSize), lambda: tr.beamSearch(ids, 3, 4, q4),
+              lambda: tr.beamSearch(ids, 33, 4, fw.QuantKVCache(1, 16, 1, 8, batch=33)),
+              lambda: tr.beamSearch([], 2, 4, q4), lambda: tr.beamSearch(ids, 2, 0, q4),
+              lambda: tr.beamSearch(ids, 2, 4, other), lambda: tr.forward(3, 16, q4), lambda: tr.forward(3, -1, q4)):
+        with pytest.raises(ValueError):
+            f()
+    assert fp.len == q4.len == other.len == 0
+    for n, c in ((7, fp), (7, q4)):            # the last new token is never written
+        assert len(tr.beamSearch(ids, 2, n, c)) == 2 and c.len == 16
+    assert len(tr.beamSearch(ids, 1, 1, fw.QuantKVCache(cfg.nLayers, 16, cfg.nKvHeads, cfg.dHead))[0][0]) == 1

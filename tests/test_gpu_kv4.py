@@ -396,6 +396,16 @@ def test_put_outside_the_cache_changes_nothing():
     same = [torch.equal(d[i], q0[i]) for i in range(10)]
     # (the fourth's second token stands at position 0, whose rotation is the identity)
     assert same == [False, True, True, True, True, True, True, True, True, True]
+    # the last position of int32 is one, the next is none
+    before, q0 = [a.clone() for a in c.args()], d.clone()
+    pos = np.full(5, 2 ** 31 - 1, np.int32)
+    fw.kv4Put(d, 2, dev(pos), dev(np.full(5, 8, np.int32)), *c.args(), T=2, table=t)
+    hit = {(c.table[b, 0], 8) for b in range(5)}
+    for a, b in zip(c.args(), before):
+        for blk in range(c.phys):
+            for off in range(16):
+                assert torch.equal(a[blk, :, off].view(torch.int8), b[blk, :, off].view(torch.int8)) != ((blk, off) in hit)
+    assert [torch.equal(d[i], q0[i]) for i in range(10)] == [False, True] * 5
     t.fill_(c.phys + 3)
     before, q0 = [a.clone() for a in c.args()], d.clone()
     fw.kv4Put(d, 2, dev(np.full(5, 3, np.int32)), dev(np.zeros(5, np.int32)), *c.args(), T=2, table=t)
@@ -520,6 +530,17 @@ def test_python_refusals():
         lambda: fw.kv4Put(torch.zeros(2, 512, device="cuda"), 4, lens, lens, k, kg, v, vg, theta=-1.0, **ok),
         lambda: fw.kv4Values(k, kg, v, vg, 63, lens, 1, **ok),
         lambda: fw.kv4Evict(k[None], kg[None], v[None], vg[None], None, None, lens, 4, 2, **ok),
+        lambda: fw.kv4Attention(q, None, kg, v, vg, lens, **ok),
+        lambda: fw.kv4Values(k, kg, v, None, 64, lens, 1, **ok),
+        lambda: fw.kv4Put(torch.zeros(2, 512, device="cuda"), 4, lens, lens, k.cpu().numpy(), kg, v, vg, **ok),
+        lambda: fw.kv4Evict(k, kg, v, vg, torch.zeros(1, device="cuda"), lens, lens, 4, 2, **ok),
+        lambda: fw.kv4Evict(None, kg, v, vg, torch.zeros(1, device="cuda"), lens, lens, 4, 2, **ok),
+        lambda: fw.kv4Evict(k[None], kg[None], v[None], vg[None], k, k, lens, 2 ** 32 + 4, 2, **ok),
+        lambda: fw.cacheReorder([None], lens.view(1, 2), lens),
+        lambda: fw.cacheReorder([lens], lens.view(1, 2), lens),
+        lambda: fw.QuantKVCache(1, 16, 1, 8, batch=2, blockSize=16, table=[[0], [0]], physBlocks=1, track=True),
+        lambda: fw.QuantKVCache(1, 16, 1, 8, batch=2).reorder([[0.0, 1.0]]),
+        lambda: fw.QuantKVCache(1, 16, 1, 8, batch=2).reorder(torch.tensor([[0, 2]], device="cuda")),
         lambda: fw.QuantKVCache(1, 16, 1, 7),
         lambda: fw.QuantKVCache(1, 16, 1, 8, blockSize=4, table=[[0, 1, 2, 9]], physBlocks=4),
         lambda: fw.QuantKVCache(1, 16, 1, 8).evict(4, 2),
@@ -531,6 +552,11 @@ def test_python_refusals():
             pytest.fail(f"case {i} was accepted")
     with pytest.raises(fw.ForgeCUError):
         fw.kv4Attention(torch.zeros(2, 3, 64, device="cuda"), k, kg, v, vg, lens, **ok)
+    with pytest.raises(fw.ForgeCUError):
+        fw.kv4Attention(q, k, kg, v, vg, lens, out=q, **ok)
+    with pytest.raises(fw.ForgeCUError):
+        x = torch.zeros(1, 2, 4, 8, device="cuda")
+        fw.cacheReorder([x, x], lens.view(1, 2), lens)
 
 
 def test_attention_of_more_sequences_than_a_block_has_threads():

@@ -61,9 +61,10 @@ def test_bad_arguments_are_refused(L, ctx):
     for bad in (dict(ctx=None), dict(c=None), dict(start=None), dict(B=5), dict(B=-1), dict(T=-1)):
         assert val(**bad) == ARG, bad
     att = lambda **k: L.fcu_kv4_attn(*{**dict(ctx=ctx, q=4096, ld=256, c=ok, lens=4096, B=4, nH=4, scale=1.0,  # noqa: E731
-                                              out=4096, work=4096, n=1 << 40), **k}.values())
+                                              out=1 << 20, work=4096, n=1 << 40), **k}.values())
     for bad in (dict(ctx=None), dict(q=None), dict(ld=255), dict(c=None), dict(lens=None), dict(B=-1), dict(B=70000),
-                dict(nH=3), dict(nH=0), dict(nH=34), dict(out=None)):
+                dict(nH=3), dict(nH=0), dict(nH=34), dict(out=None), dict(out=4096), dict(out=4096 + 4 * 1016),
+                dict(ld=1000, out=4096 + 4 * 3000), dict(q=1 << 20), dict(q=(1 << 20) + 4 * 1020)):
         assert att(**bad) == ARG, bad
     tracked = cache(weight=4096, pos=4096)
     for bad in (dict(work=None), dict(n=16), dict(work=4100)):
@@ -77,11 +78,14 @@ def test_bad_arguments_are_refused(L, ctx):
     assert L.fcu_kv4_evict_work(ctx, long, 4, 8) == 4 * 2 * ((1 << 17) + (1 << 12)) * 4
     assert L.fcu_kv4_evict_work(ctx, long, 4, 1000) == 4 * 2 * ((1 << 17) + (1 << 12) + 2 * 1000 + 1) * 4
     assert ev(c=long) == ARG and ev(c=long, work=4096, n=100) == ARG
-    beam = lambda **k: L.fcu_beam_step(*{**dict(ctx=ctx, x=4096, ld=100, s=4096, d=4096, B=2, W=4, V=100, eos=2,  # noqa: E731
-                                                os=8192, t=4096, p=4096, od=8192, work=4096, n=1 << 40), **k}.values())
+    beam = lambda **k: L.fcu_beam_step(*{**dict(ctx=ctx, x=4096, ld=100, s=8192, d=8256, B=2, W=4, V=100, eos=2,  # noqa: E731
+                                                os=8320, t=8352, p=8384, od=8416, work=16384, n=1 << 40), **k}.values())
     for bad in (dict(ctx=None), dict(x=None), dict(ld=99), dict(s=None), dict(d=None), dict(B=-1), dict(B=20000),
                 dict(W=0), dict(W=33), dict(V=0), dict(V=1 << 31, ld=1 << 32), dict(eos=-1), dict(eos=100),
-                dict(os=None), dict(os=4096), dict(od=4096), dict(t=None), dict(work=None), dict(n=8), dict(work=4100)):
+                dict(os=None), dict(t=None), dict(work=None), dict(n=8), dict(work=16388),
+                # outputs that overlap an input or one another
+                dict(os=8192), dict(od=8256), dict(os=8196), dict(od=8249), dict(t=8220), dict(p=8352), dict(od=8340),
+                dict(t=4096), dict(p=4096 + 3196)):
         assert beam(**bad) == ARG, bad
 
     def reorder(arrays=((4096, 2, 32),), **k):
@@ -93,7 +97,10 @@ def test_bad_arguments_are_refused(L, ctx):
     for bad in (dict(ctx=None), dict(n=9), dict(n=-1), dict(spec=None), dict(layers=-1), dict(blocks=15), dict(bs=0),
                 dict(mb=0), dict(parents=None), dict(lens=None), dict(B=-1), dict(W=0), dict(W=33),
                 dict(arrays=((None, 2, 32),)), dict(arrays=((4100, 2, 32),)), dict(arrays=((4096, 0, 32),)),
-                dict(arrays=((4096, 2, 30),)), dict(arrays=((4096, 2, 0),))):
+                dict(arrays=((4096, 2, 30),)), dict(arrays=((4096, 2, 0),)),
+                # 32 blocks of 16 slots: 32768 and 2048 bytes
+                dict(arrays=((4096, 2, 32), (4096, 2, 32))), dict(arrays=((4096, 2, 32), (4096 + 32752, 1, 4))),
+                dict(arrays=((4096 + 2032, 2, 32), (4096, 1, 4)))):
         assert reorder(**bad) == ARG, bad
 
 
