@@ -10,20 +10,25 @@ namespace {
 // ------------------------------------------------------------------ selection
 // Two kernels.  beam_rows reads every logit once: a warp walks 512 logits at a
 // time of one slice of one row, with a running maximum and sum of exponentials
-// per lane, and keeps the W best (logit, token) pairs it has met, one per lane,
-// sorted.  After its first tile a logit is only looked at again if it beats the
-// W-th best, about W ln(n / 512) times for n logits in no particular order.
+// per lane, and lists the tokens whose logits could be among the slice's W best.
+// What they have to reach: every lane keeps its largest logit so far, every warp
+// the (W / warps)-th largest of those, and W of the slice's logits reach the
+// least of the warps' values, about the W-th largest so far; of n logits in no
+// particular order some 2 W ln(n / 4096) get past it after the first 4096.  A
+// warp's list is cut down to its W best when it is full and at the end.
 // beam_merge, one CTA per sequence, turns the slices' sums into each row's
 // log-sum-exp and picks the W best of the W rows' W best.  Within a row the
 // candidates order as the logits do, so W per slice are enough.  The bound is
-// reading the logits (HBM): 32 x 8 rows of 100003, 102 MB, take about 42 us, 36
-// of them beam_rows (2.8 TB/s, issue slots 60 % busy); 4 rows of 32000 take 10
-// us, all latency.
+// reading the logits (HBM): 32 x 8 rows of 100003, 102 MB, take 34 us, 27 of
+// them beam_rows (3.8 TB/s, issue slots 55 % busy; 43 us with sorted lists kept
+// in registers, a bound per warp; 38 with three tiles of a warp in shared memory
+// in place of one ahead in registers); 4 rows of 32000 take 10 us, all latency.
 constexpr int kBeamThreads = 256;
 constexpr int kBeamWarps = kBeamThreads / 32;
 constexpr int kMaxW = 32;
 constexpr int kTile = 512;                          // logits a warp takes at a time
 constexpr int kMaxSlices = 64;
+constexpr int kFound = 64;                          // tokens a warp lists: kMaxW and 32 more at least
 constexpr float kLog2e = 1.4426950408889634f;
 
 using Key = unsigned long long;
@@ -77,24 +82,55 @@ __device__ __forceinline__ float4 load4(const float *p, int v, int v0, int v1) {
   return f;
 }
 
-__global__ void __launch_bounds__(kBeamThreads) beam_rows_kernel(BeamArgs a) {
+// Leaves a warp's n <= kFound tokens of a row the W best in order, their logits
+// read again; returns how many.  (Not inlined: a run of tiles rarely needs it.)
+__device__ __noinline__ int prune(const float *x, uint32_t *found, Key *keys, int n, int W) {
+  const int lane = threadIdx.x & 31;
+  __syncwarp();
+  Key k0 = 0, k1 = 0;
+  if (lane < n) k0 = beam_key(x[found[lane]], found[lane]);
+  if (lane + 32 < n) k1 = beam_key(x[found[lane + 32]], found[lane + 32]);
+  keys[lane] = k0;
+  keys[lane + 32] = k1;
+  __syncwarp();
+  int r0 = 0, r1 = 0;
+#pragma unroll 4
+  for (int j = 0; j < n; j++) {
+    const Key k = keys[j];
+    r0 += k > k0;
+    r1 += k > k1;
+  }
+  __syncwarp();
+  if (k0 && r0 < W) {
+    keys[r0] = k0;
+    found[r0] = 0xffffffffu - (uint32_t)k0;
+  }
+  if (k1 && r1 < W) {
+    keys[r1] = k1;
+    found[r1] = 0xffffffffu - (uint32_t)k1;
+  }
+  __syncwarp();
+  return n < W ? n : W;
+}
+
+__global__ void __launch_bounds__(kBeamThreads, 4) beam_rows_kernel(BeamArgs a) {
   pdl_trigger();
-  __shared__ Key lists[kBeamWarps * kMaxW];
+  __shared__ uint32_t found[kBeamWarps][kFound];
+  __shared__ Key keys[kBeamWarps][kFound];
   __shared__ float red_m[kBeamWarps], red_s[kBeamWarps];
-  __shared__ uint32_t shared_bar;            // order_bits of a logit that W others of the slice reach
+  // order_bits of what W / (the warps with tiles) of a warp's lanes have met at least
+  __shared__ uint32_t reached[kBeamWarps];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, W = a.W;
   const int64_t row = blockIdx.y;
-  if (threadIdx.x == 0) shared_bar = 0;
-  __syncthreads();
   const int v0 = blockIdx.x * a.slice, v1 = (int)min((int64_t)a.V, (int64_t)v0 + a.slice);
   pdl_wait();
   const float *x = a.logits + row * a.ld;
   // tiles start where a 16-byte line does: at most three tokens before v0
   const int skew = (int)(((uintptr_t)(x + v0) >> 2) & 3);
   float M = -INFINITY, s = 0.f;              // this lane's
-  Key key = 0;                               // this lane's place in the warp's list
-  float bar = -INFINITY;                     // its last entry's logit
-  bool full = false;
+  uint32_t *mine = found[warp];              // tokens
+  int n = 0;                                 // in it
+  float least = -INFINITY;                   // no smaller logit is among the slice's W best
   int64_t t0 = (int64_t)v0 - skew + warp * kTile;
   float4 next[4];
   auto fetch = [&](int64_t t) {
@@ -110,7 +146,29 @@ __global__ void __launch_bounds__(kBeamThreads) beam_rows_kernel(BeamArgs a) {
       }
     }
   };
+  // the nth largest (of different ones) of the lanes' order bits, or 0
+  auto nth = [&](uint32_t bits, int n) {
+    uint32_t w_th = 0;
+    for (int i = 0; i < n && (i == 0 || w_th); i++) {
+      w_th = __reduce_max_sync(0xffffffffu, bits);
+      if (bits == w_th) bits = 0;
+    }
+    return w_th;
+  };
   fetch(t0);
+  if (threadIdx.x < kBeamWarps) reached[threadIdx.x] = 0xffffffffu;
+  __syncthreads();
+  // W of the slice's logits reach the least of the warps' `reached`.  A warp raises
+  // its own with each tile and reads the others' as they stand.
+  const int warps = max(1, min(kBeamWarps, (v1 - v0 + skew + kTile - 1) / kTile)), share = (W + warps - 1) / warps;
+  float most = -INFINITY;                    // the lane's largest logit
+#pragma unroll
+  for (int i = 0; i < 4; i++) most = fmaxf(fmaxf(fmaxf(most, next[i].x), fmaxf(next[i].y, next[i].z)), next[i].w);
+  if (warp < warps) {
+    const uint32_t bits = nth(order_bits(most), share);
+    if (lane == 0) reached[warp] = bits;
+  }
+  __syncthreads();
   for (; t0 < v1; t0 += kTile * kBeamWarps) {
     float f[16];
 #pragma unroll
@@ -128,44 +186,50 @@ __global__ void __launch_bounds__(kBeamThreads) beam_rows_kernel(BeamArgs a) {
       s = s * beam_ex2(M - M1) + ts;
       M = M1;
     }
-    // Earlier tiles hold lower tokens, so only a larger logit displaces one of
-    // theirs; another warp's W-th best is no bound on equal ones.
-    const float others = bits_float(*(volatile uint32_t *)&shared_bar);
-    uint32_t hit = __ballot_sync(0xffffffffu, (top > bar || !full) && top >= others);
+    most = fmaxf(most, top);
+    const uint32_t bits = nth(order_bits(most), share);
+    if (lane == 0) *(volatile uint32_t *)&reached[warp] = bits;
+    const uint32_t all = *(volatile uint32_t *)&reached[lane % kBeamWarps];
+    least = fmaxf(least, bits_float(__reduce_min_sync(0xffffffffu, all)));
+    const uint32_t hit = __ballot_sync(0xffffffffu, top >= least);
     if (hit == 0) continue;
-    float least = fmaxf(bar, others);
+    // no logit below the W-th largest of the lanes' maxima is among the W best
     if (__popc(hit) > W) {
-      // no logit below the W-th largest of the lanes' maxima is among the W best
-      uint32_t mine = order_bits(top), w_th = 0;
-      for (int i = 0; i < W && (i == 0 || w_th); i++) {
-        w_th = __reduce_max_sync(0xffffffffu, mine);
-        if (mine == w_th) mine = 0;
-      }
+      const uint32_t w_th = nth(order_bits(top), W);
       if (w_th) least = fmaxf(least, bits_float(w_th));
     }
+    uint32_t is = 0;                         // the lane's logits that reach it
 #pragma unroll
-    for (int i = 0; i < 16; i++) {
-      uint32_t who = __ballot_sync(0xffffffffu, f[i] >= least);
-      while (who) {
-        const int from = __ffs(who) - 1;
-        who &= who - 1;
-        const int64_t v = t0 + 128 * (i / 4) + 4 * from + i % 4;
-        if (v < v0 || v >= v1) continue;
-        const Key k = beam_key(__shfl_sync(0xffffffffu, f[i], from), (uint32_t)v);
-        const int at = __popc(__ballot_sync(0xffffffffu, key > k));
-        if (at >= W) continue;
-        const Key up = __shfl_up_sync(0xffffffffu, key, 1);
-        if (lane == at) key = k;
-        else if (lane > at) key = lane < W ? up : 0;
+    for (int i = 0; i < 16; i++) is |= f[i] >= least ? 1u << i : 0;
+    if (t0 < v0 || t0 + kTile > v1)
+#pragma unroll
+      for (int i = 0; i < 16; i++) {
+        const int64_t v = t0 + 128 * (i / 4) + 4 * lane + i % 4;
+        if (v < v0 || v >= v1) is &= ~(1u << i);
       }
+    float own = -INFINITY;                   // the W-th best of a warp that has W
+    bool full = false;
+    while (true) {
+      const uint32_t who = __ballot_sync(0xffffffffu, is);
+      if (who == 0) break;
+      if (n + __popc(who) > kFound) {
+        n = prune(x, mine, keys[warp], n, W);
+        full = true;
+        own = key_logit(keys[warp][W - 1]);
+        least = fmaxf(least, own);
+      }
+      if (is) {
+        const int i = __ffs(is) - 1;
+        mine[n + __popc(who & ((1u << lane) - 1))] = (uint32_t)t0 + 128 * (i / 4) + 4 * lane + i % 4;
+        is &= is - 1;
+      }
+      n += __popc(who);
     }
-    const Key last = __shfl_sync(0xffffffffu, key, W - 1);
-    full = last != 0;
-    if (full) {
-      bar = key_logit(last);
-      if (lane == 0 && bar > others) atomicMax(&shared_bar, order_bits(bar));
-    }
+    // later tiles hold higher tokens: of theirs, only logits above this warp's own
+    // W-th are wanted (another's may be of later tokens)
+    if (full && own >= least) least = bits_float(order_bits(own) + 1);
   }
+  n = prune(x, mine, keys[warp], n, W);
   // the slice's maximum and sum: lanes, then warps, in a fixed order
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) {
@@ -175,7 +239,6 @@ __global__ void __launch_bounds__(kBeamThreads) beam_rows_kernel(BeamArgs a) {
     M = M1;
   }
   if (lane == 0) red_m[warp] = M, red_s[warp] = s;
-  if (lane < W) lists[warp * W + lane] = key;
   __syncthreads();
   const int64_t at = row * a.slices + blockIdx.x;
   if (threadIdx.x == 0) {
@@ -190,11 +253,11 @@ __global__ void __launch_bounds__(kBeamThreads) beam_rows_kernel(BeamArgs a) {
   if (threadIdx.x < W) a.best[at * W + threadIdx.x] = 0;
   __syncthreads();
   for (int i = threadIdx.x; i < kBeamWarps * W; i += kBeamThreads) {
-    const Key k = lists[i];
+    const Key k = keys[i / W][i % W];
     int rank = i % W;
     for (int w = 0; w < kBeamWarps && rank < W; w++)
       if (w != i / W)
-        for (int j = 0; j < W && lists[w * W + j] > k; j++) rank++;
+        for (int j = 0; j < W && keys[w][j] > k; j++) rank++;
     if (k && rank < W) a.best[at * W + rank] = k;
   }
 }
@@ -205,6 +268,7 @@ __global__ void __launch_bounds__(kBeamThreads) beam_merge_kernel(BeamArgs a) {
   __shared__ Key best[kMaxW][kMaxW];
   __shared__ double score[kMaxW][kMaxW];
   __shared__ int token[kMaxW][kMaxW];                  // -1: no candidate
+  __shared__ uint8_t order[kMaxW][kMaxW];              // a row's candidates, best first
   __shared__ double lse[kMaxW];
   const int tid = threadIdx.x, lane = tid & 31, W = a.W, per = a.slices * W, N = W * per;
   const int64_t b = blockIdx.x;
@@ -227,9 +291,10 @@ __global__ void __launch_bounds__(kBeamThreads) beam_merge_kernel(BeamArgs a) {
   __syncthreads();
   // A row's W best of its slices' sorted lists.  Few lists: a key's rank is its
   // own place plus what every other list has above it.  Many: W times the largest
-  // of their heads, of which a lane has up to two.  (2 lists of 8: 43.0 us for the
-  // whole step by rank, 45.3 by heads; 16 of 4: 12.3 and 10.3.)
-  if (a.slices <= 4) {
+  // of their heads, of which a lane has up to two.  (Whole steps: 2
+  // lists of 8 34.2 us by rank, 36.9 by heads; 2 of 32 79.5 and 98.5; 16 of 4 12.3
+  // and 10.3.)
+  if (a.slices <= 2) {
     for (int i = tid; i < N; i += kBeamThreads) {
       const int w = i / per, mine = (i - w * per) / W;
       const Key k = raw[i];
@@ -275,24 +340,46 @@ __global__ void __launch_bounds__(kBeamThreads) beam_merge_kernel(BeamArgs a) {
       v = cum + ((double)key_logit(k) - lse[w]);
       if (!isfinite(v)) v = -INFINITY;
     }
-    score[w][r] = v;
+    score[w][r] = v + 0.0;
     token[w][r] = tok;
   }
   __syncthreads();
+  // A row's scores fall as its logits do, but where the beam's score swallows the
+  // difference of two logits they tie, and the lower token is first.
   for (int i = tid; i < W * W; i += kBeamThreads) {
-    const int w = i / W, r = i - w * W, tok = token[w][r];
-    if (tok < 0) continue;
+    const int w = i / W, r = i - w * W;
     const double v = score[w][r];
-    int rank = 0;
-    for (int x = 0; x < W && rank < W; x++)
-      for (int j = 0; j < W && token[x][j] >= 0 && score[x][j] >= v; j++)
-        rank += score[x][j] > v || x < w || (x == w && token[x][j] < tok);
-    if (rank < W) {
-      const int64_t o = b * W + rank;
-      a.out_scores[o] = (float)v;
-      a.tokens[o] = tok;
-      a.parents[o] = w;
-      a.out_done[o] = a.done[b * W + w] != 0 || tok == a.eos;
+    int rank = r;
+    if (token[w][r] >= 0 && ((r > 0 && score[w][r - 1] == v) || (r + 1 < W && score[w][r + 1] == v))) {
+      rank = 0;
+      for (int j = 0; j < W && token[w][j] >= 0; j++)
+        rank += score[w][j] > v || (score[w][j] == v && token[w][j] < token[w][r]);
+    }
+    order[w][rank] = (uint8_t)r;
+  }
+  __syncthreads();
+  // W times the best of the rows' heads, a lane's row each; ties to the lowest row
+  if (tid >= 32) return;
+  auto bits = [&](int at) -> Key {             // orders as the score; 0: the row has no more
+    const int r = at < W ? order[lane][at] : 0;
+    if (at >= W || token[lane][r] < 0) return 0;
+    const Key u = __double_as_longlong(score[lane][r]);
+    return u >> 63 ? ~u : u | (Key)1 << 63;
+  };
+  int at = 0;
+  Key head = lane < W ? bits(0) : 0;
+  for (int i = 0; i < W; i++) {
+    const uint32_t hi = __reduce_max_sync(0xffffffffu, (uint32_t)(head >> 32));
+    const uint32_t lo = __reduce_max_sync(0xffffffffu, (uint32_t)(head >> 32) == hi ? (uint32_t)head : 0);
+    const uint32_t who = __ballot_sync(0xffffffffu, head == ((Key)hi << 32 | lo));
+    if (lane == __ffs(who) - 1 && head != 0) {
+      const int r = order[lane][at];
+      const int64_t o = b * W + i;
+      a.out_scores[o] = (float)score[lane][r];
+      a.tokens[o] = token[lane][r];
+      a.parents[o] = lane;
+      a.out_done[o] = a.done[b * W + lane] != 0 || token[lane][r] == a.eos;
+      head = bits(++at);
     }
   }
 }
@@ -309,7 +396,7 @@ int beam_slices(int num_sms, int B, int W, int64_t V) {
 }
 
 // ------------------------------------------------------------------ reordering
-// A warp takes up to kReBytes of one head of one block at a time, at the same
+// A warp takes up to 512 D bytes of one head of one block at a time, at the same
 // place of all beams of a sequence: it reads them from the beams that another
 // beam continues into its part of shared memory, all copies in flight at once,
 // then writes the beams that continue another.  A lane writes only places it has

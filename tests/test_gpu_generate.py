@@ -67,6 +67,22 @@ def test_beam_step_ties_go_to_the_lowest_beam_and_token():
         check_beam(x, np.array([[0.0, -1.0, -2.0, -3.0]] * 2), np.zeros((2, 4), bool), 1)
 
 
+def test_beam_step_ties_among_many_tiles():
+    """Warps that run ahead of one another meet equal logits again and again."""
+    rng = np.random.default_rng(8)
+    x = rng.integers(0, 6, (6, 16, 70001)).astype(np.float32)
+    x[1] = np.where(x[1] == 5, 0, 1)           # two values
+    x[2, :, 40000:] = 6                        # the largest all come late
+    x[3, :, :69990] = -np.inf                  # few are allowed at all
+    x[4] = 0
+    scores = -np.arange(16.0) * np.ones((6, 1))
+    done = np.zeros((6, 16), bool)
+    for _ in range(3):
+        check_beam(x, scores, done, 2)
+    done[:, ::3] = True
+    check_beam(x, scores, done, 2)
+
+
 def test_beam_step_ascending_logits():
     """The worst order for a running selection: every tile beats the last."""
     x = np.tile(np.arange(20000, dtype=np.float32) / 1000, (1, 32, 1)) + np.arange(32, dtype=np.float32)[None, :, None] * 0
