@@ -345,12 +345,13 @@ __global__ void __launch_bounds__(kBeamThreads) beam_merge_kernel(BeamArgs a) {
   }
   __syncthreads();
   // A row's scores fall as its logits do, but where the beam's score swallows the
-  // difference of two logits they tie, and the lower token is first.
+  // difference of two logits they tie, and the lower token is first.  (Those of
+  // -inf are in order: equal logits or none.)
   for (int i = tid; i < W * W; i += kBeamThreads) {
     const int w = i / W, r = i - w * W;
     const double v = score[w][r];
     int rank = r;
-    if (token[w][r] >= 0 && ((r > 0 && score[w][r - 1] == v) || (r + 1 < W && score[w][r + 1] == v))) {
+    if (v > -INFINITY && ((r > 0 && score[w][r - 1] == v) || (r + 1 < W && score[w][r + 1] == v))) {
       rank = 0;
       for (int j = 0; j < W && token[w][j] >= 0; j++)
         rank += score[w][j] > v || (score[w][j] == v && token[w][j] < token[w][r]);
