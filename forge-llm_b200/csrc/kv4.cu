@@ -713,14 +713,16 @@ __global__ void __launch_bounds__(kMvThreads) kv4_move_kernel(EvArgs a) {
   const int h = (int)(head % c.nKV);
   const int64_t r = head / c.nKV, b = r % a.B, lrow = r / a.B * c.blocks * c.nKV * c.bs;
   pdl_wait();
-  const int count = (int)a.count[head];
+  const int count = (int)min(a.count[head], (uint32_t)a.most);
   if (m0 >= count) return;
   const bool on = m0 + lane < count;
   int64_t src = 0, dst = 0;
   uint4 w;
   if (on) {
-    src = lrow + row_of(c, b, h, a.from[head * a.most + m0 + lane]);
-    dst = lrow + row_of(c, b, h, a.to[head * a.most + m0 + lane]);
+    // (inside the cache whatever another call made of the workspace)
+    const uint32_t last = (uint32_t)c.cap - 1;
+    src = lrow + max(row_of(c, b, h, min((uint32_t)a.from[head * a.most + m0 + lane], last)), (int64_t)0);
+    dst = lrow + max(row_of(c, b, h, min((uint32_t)a.to[head * a.most + m0 + lane], last)), (int64_t)0);
     w = make_uint4(c.kg[src], c.vg[src], __float_as_uint(c.weight[src]), (uint32_t)c.pos[src]);
   }
   const int per = c.rb / 16, pieces = min(32, count - m0) * per;

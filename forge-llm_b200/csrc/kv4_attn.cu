@@ -838,6 +838,8 @@ __global__ void __launch_bounds__(kFinishThreads) kv4_attn_finish_kernel(AttnArg
     Cut cut{0, 0, 0};
     const int run0 = (int)blockIdx.x - lane;
     if (lane < kMaxHeads && run0 >= 0) cut = a.cuts[run0];
+    // (nothing is written elsewhere whatever another call made of the workspace)
+    if (cut.heads < 0 || cut.heads > kMaxHeads || cut.bh < 0 || cut.bh + cut.heads > a.B * a.nH) cut.pieces = 0;
     const bool mine = lane == 0 ? cut.pieces > 0 : cut.pieces > kFewPieces && lane < cut.heads;
     const uint32_t who = __ballot_sync(0xffffffffu, mine);
     if (!who) return;
@@ -951,7 +953,7 @@ __global__ void __launch_bounds__(kFinishThreads) kv4_attn_finish_kernel(AttnArg
     float2 x = a.ml[b * a.nH + h * a.g + hd];
     // a cut segment's: the run it begins in, and minus its pieces
     if (x.y < 0.f) {
-      const int run = __float_as_int(x.x), pieces = min((int)-x.y, a.ctas - run);
+      const int run = min(max(__float_as_int(x.x), 0), a.ctas - 1), pieces = min((int)-x.y, a.ctas - run);
       x = Pieces(a, run, hd % a.gs).ml(pieces, dH);
     }
     if (lane == 0) {

@@ -13,14 +13,15 @@ reference has no counterpart: its caches are fp32 and it samples one sequence.
 
 All tensors are on the current CUDA device and every call runs on its current
 stream.  A call that finds them anywhere else, or of another type, shape or
-stride than it takes, raises ValueError before anything is launched.  As for the
-rest of the package, one host thread at a time makes calls on a device: its
-context is bound to one stream at a time.
+stride than it takes, raises ValueError before anything is launched.  Host
+threads may call at the same time, each on streams of its own.
 """
 from __future__ import annotations
 
 import ctypes as C
 import math
+import struct
+import threading
 
 import numpy as np
 import torch
@@ -33,8 +34,11 @@ _U8, _BF, _F32, _I32, _BOOL = torch.uint8, torch.bfloat16, torch.float32, torch.
 _ROW_BYTES: dict = {}
 
 # A decode step makes these calls once per layer, and the kernels take a few
-# microseconds, so the common path of every function is one test per tensor; what
-# fails it is looked at again for the message.
+# microseconds, so the common path of every function is one test per tensor (what
+# fails it is looked at again for the message), structures are packed bytes (a
+# ctypes structure takes three times as long to fill and pass), and results of
+# one shape are made like one another (torch.empty_like takes half of what
+# new_empty takes).
 
 
 def _need(ok, what: str) -> None:
@@ -42,9 +46,23 @@ def _need(ok, what: str) -> None:
         raise ValueError(what)
 
 
+class _Contexts(threading.local):
+    """This thread's contexts by device.  (The package's own is one per device: a
+    thread that binds it to its stream would take along a call that another has
+    begun, and the kernels of one call would run on two streams.)"""
+
+    def __init__(self):
+        self.of = {}
+
+
+_CONTEXTS = _Contexts()
+
+
 def _on(dev: int):
-    """The fcu_ctx of the current device `dev`, bound to its current stream."""
-    c = Context._per_device.get(dev) or Context.get(dev)
+    """This thread's fcu_ctx of the current device `dev`, bound to its current stream."""
+    c = _CONTEXTS.of.get(dev)
+    if c is None:
+        c = _CONTEXTS.of[dev] = Context(dev)
     c.bind_stream(torch._C._cuda_getCurrentRawStream(dev))
     return c.handle
 
@@ -57,25 +75,21 @@ def _device() -> int:
         raise
 
 
-def _call(name: str, *args) -> None:
-    rc = _FN[name](*args)
-    if rc:
-        check(rc, name)
-
-
 class _Functions(dict):
-    """The library's functions by name, each looked up once."""
+    """The library's functions by name, taking structures as their bytes."""
 
     def __missing__(self, name):
-        fn = self[name] = getattr(lib(), name)
+        declared, fn = getattr(lib(), name), lib()[name]
+        fn.restype = declared.restype
+        fn.argtypes = [C.c_void_p if t in (C.POINTER(Kv4), C.POINTER(CacheArray)) else t for t in declared.argtypes]
+        self[name] = fn
         return fn
 
 
 _FN = _Functions()
-
-
-def _ok(t, dtype, dev: int) -> bool:
-    return t.dtype is dtype and t.get_device() == dev and t.is_contiguous()
+_KV4 = struct.Struct("@7P2q4i")
+_ARRAYS = [struct.Struct("@" + "P2q" * n) for n in range(9)]
+assert _KV4.size == C.sizeof(Kv4) and _ARRAYS[8].size == C.sizeof(CacheArray * 8)
 
 
 def _check(name: str, t, dtype, dev: int, shape=None) -> None:
@@ -93,12 +107,6 @@ def _check(name: str, t, dtype, dev: int, shape=None) -> None:
     raise ValueError(f"{name} is not contiguous")
 
 
-def _tensors(**ts) -> None:
-    for name, t in ts.items():
-        if not isinstance(t, torch.Tensor):
-            raise ValueError(f"{name}: a tensor is needed, got {type(t).__name__}")
-
-
 def _row_bytes(dHead: int) -> int:
     rb = _ROW_BYTES.get(dHead)
     if rb is None:
@@ -109,39 +117,51 @@ def _row_bytes(dHead: int) -> int:
     return rb
 
 
-def _cache(dev, k, kg, v, vg, dHead, B, table, weight=None, pos=None, layers=False) -> Kv4:
-    """The C-ABI's view of one layer's arrays (five dimensions: of all layers)."""
-    rb = _row_bytes(dHead)
-    shape = k.shape
-    lead = shape[:-1]
-    if not (v.shape == shape and len(shape) == (5 if layers else 4) and shape[-1] == rb and kg.shape == vg.shape
-            and kg.shape == (*lead, 2) and _ok(k, _U8, dev) and _ok(v, _U8, dev) and _ok(kg, _BF, dev)
-            and _ok(vg, _BF, dev)):
+def _cache(dev, k, kg, v, vg, dHead, B, table, weight=None, pos=None, layers=False) -> bytes:
+    """The C-ABI's view (fcu_kv4) of one layer's arrays (five dimensions: of all layers)."""
+    rb = _ROW_BYTES.get(dHead) or _row_bytes(dHead)
+    try:
+        shape = k.shape
+        if layers:
+            L, blocks, nKV, bs, row = shape
+            grid = (L, blocks, nKV, bs, 2)
+        else:
+            blocks, nKV, bs, row = shape
+            grid, L = (blocks, nKV, bs, 2), 1
+        ok = (row == rb and v.shape == shape and kg.shape == grid and vg.shape == grid
+              and k.dtype is _U8 and v.dtype is _U8 and kg.dtype is _BF and vg.dtype is _BF
+              and k.get_device() == dev and v.get_device() == dev and kg.get_device() == dev and vg.get_device() == dev
+              and k.is_contiguous() and v.is_contiguous() and kg.is_contiguous() and vg.is_contiguous())
+    except (AttributeError, TypeError, ValueError):
+        ok = False
+    if not ok:
         _check("k", k, _U8, dev)
         if k.ndim != (5 if layers else 4):
             raise ValueError(f"k: {k.ndim} dimensions")
-        if shape[-1] != rb:
-            raise ValueError(f"k: rows of {shape[-1]} bytes, head dim {dHead} has {rb}")
-        _check("v", v, _U8, dev, shape)
-        _check("kg", kg, _BF, dev, (*lead, 2))
-        _check("vg", vg, _BF, dev, (*lead, 2))
+        if k.shape[-1] != rb:
+            raise ValueError(f"k: rows of {k.shape[-1]} bytes, head dim {dHead} has {rb}")
+        _check("v", v, _U8, dev, k.shape)
+        _check("kg", kg, _BF, dev, (*k.shape[:-1], 2))
+        _check("vg", vg, _BF, dev, (*k.shape[:-1], 2))
+        raise ValueError("k, kg, v, vg: not the arrays of a cache")
     if weight is not None:
-        _check("weight", weight, _F32, dev, lead)
+        _check("weight", weight, _F32, dev, grid[:-1])
     if pos is not None:
-        _check("pos", pos, _I32, dev, lead)
-    blocks, nKV, bs = lead[-3:]
+        _check("pos", pos, _I32, dev, grid[:-1])
     if table is not None:
         _check("table", table, _I32, dev)
         if table.ndim != 2 or table.shape[0] != B:
             raise ValueError(f"table: shape {tuple(table.shape)} for {B} sequences")
         mb = table.shape[1]
     else:
-        if blocks % max(B, 1):
+        mb, rest = divmod(blocks, B or 1)
+        if rest:
             raise ValueError(f"{blocks} blocks do not divide among {B} sequences")
-        mb = blocks // max(B, 1)
-    return Kv4(k.data_ptr(), v.data_ptr(), kg.data_ptr(), vg.data_ptr(),
-               weight.data_ptr() if weight is not None else None, pos.data_ptr() if pos is not None else None,
-               table.data_ptr() if table is not None else None, lead[0] if layers else 1, blocks, nKV, dHead, bs, mb)
+    if max(nKV, bs, mb) >= 2 ** 31:
+        raise ValueError(f"k: shape {tuple(shape)}")
+    return _KV4.pack(k.data_ptr(), v.data_ptr(), kg.data_ptr(), vg.data_ptr(),
+                     weight.data_ptr() if weight is not None else 0, pos.data_ptr() if pos is not None else 0,
+                     table.data_ptr() if table is not None else 0, L, blocks, nKV, dHead, bs, mb)
 
 
 def _rows(name: str, t, dev: int) -> int:
@@ -179,16 +199,17 @@ def kv4Put(qkv, nHeads: int, positions, slots, k, kg, v, vg, T: int = 1, theta: 
         raise ValueError(f"{slots.numel()} slots for {B} sequences")
     if T < 1 or nHeads < 0 or not theta >= 0:
         raise ValueError(f"T={T}, nHeads={nHeads}, theta={theta}")
-    _tensors(k=k, kg=kg, v=v, vg=vg)
-    if k.ndim != 4:
-        raise ValueError(f"k: {k.ndim} dimensions")
+    if not isinstance(k, torch.Tensor) or k.ndim != 4:
+        raise ValueError("k: an array of four dimensions is needed")
     heads = nHeads + 2 * k.shape[1]
     ld = _rows("qkv", qkv, dev)
     if qkv.shape[0] != B * T or qkv.shape[1] % heads:
         raise ValueError(f"qkv: shape {tuple(qkv.shape)} for {B} x {T} tokens of {heads} heads")
     c = _cache(dev, k, kg, v, vg, qkv.shape[1] // heads, B, table, weight, pos)
-    _call("fcu_kv4_put", _on(dev), qkv.data_ptr(), ld, B, T, nHeads, float(theta), positions.data_ptr(),
-         slots.data_ptr(), c)
+    rc = _FN["fcu_kv4_put"](_on(dev), qkv.data_ptr(), ld, B, T, nHeads, float(theta), positions.data_ptr(),
+                            slots.data_ptr(), c)
+    if rc:
+        check(rc, "fcu_kv4_put")
 
 
 def kv4Values(k, kg, v, vg, dHead: int, start, T: int, table=None):
@@ -199,10 +220,12 @@ def kv4Values(k, kg, v, vg, dHead: int, start, T: int, table=None):
     B = start.numel()
     if T < 0:
         raise ValueError(f"T={T}")
-    _tensors(k=k, kg=kg, v=v, vg=vg)
     c = _cache(dev, k, kg, v, vg, dHead, B, table)
-    K, V = k.new_empty((2, B, T, c.n_kv, dHead), dtype=_F32).unbind(0)
-    _call("fcu_kv4_values", _on(dev), c, start.data_ptr(), B, T, K.data_ptr(), V.data_ptr())
+    K = k.new_empty((B, T, k.shape[1], dHead), dtype=_F32)
+    V = torch.empty_like(K)
+    rc = _FN["fcu_kv4_values"](_on(dev), c, start.data_ptr(), B, T, K.data_ptr(), V.data_ptr())
+    if rc:
+        check(rc, "fcu_kv4_values")
     return K, V
 
 
@@ -219,17 +242,16 @@ def kv4Attention(q, k, kg, v, vg, lens, scale: float | None = None, table=None, 
     B, nH, dH = q.shape
     if q.get_device() != dev:
         raise ValueError("q is not on the current CUDA device")
-    ld = nH * dH
-    if not q.is_contiguous():
+    ld, plain = nH * dH, q.is_contiguous()
+    if not plain:
         s = q.stride()
         if not ((dH == 1 or s[2] == 1) and (nH == 1 or s[1] == dH) and (B == 1 or s[0] >= ld)):
             raise ValueError(f"q: strides {s}")
         ld = s[0] if B > 1 else ld
     _check("lens", lens, _I32, dev, (B,))
-    _tensors(k=k, kg=kg, v=v, vg=vg)
     c = _cache(dev, k, kg, v, vg, dH, B, table, weight)
     if out is None:
-        out = q.new_empty((B, nH, dH))
+        out = torch.empty_like(q) if plain else q.new_empty((B, nH, dH))
     else:
         _check("out", out, _F32, dev)
         if out.numel() != B * nH * dH:
@@ -237,9 +259,11 @@ def kv4Attention(q, k, kg, v, vg, lens, scale: float | None = None, table=None, 
     h = _on(dev)
     nbytes = _FN["fcu_kv4_attn_work"](h, c, B, nH)
     work = k.new_empty((nbytes,)) if nbytes > 0 else None
-    _call("fcu_kv4_attn", h, q.data_ptr(), ld, c, lens.data_ptr(), B, nH,
-          dH ** -0.5 if scale is None else float(scale), out.data_ptr(),
-          work.data_ptr() if work is not None else None, nbytes)
+    rc = _FN["fcu_kv4_attn"](h, q.data_ptr(), ld, c, lens.data_ptr(), B, nH,
+                             dH ** -0.5 if scale is None else float(scale), out.data_ptr(),
+                             work.data_ptr() if work is not None else None, nbytes)
+    if rc:
+        check(rc, "fcu_kv4_attn")
     return out
 
 
@@ -255,9 +279,8 @@ def kv4Evict(k, kg, v, vg, weight, pos, lens, budget: int, recent: int, table=No
         raise ValueError("eviction goes by `weight` and `pos`")
     if not 1 <= budget < 2 ** 31 or not 0 <= recent <= budget:
         raise ValueError(f"budget {budget}, recent {recent}")
-    _tensors(k=k, kg=kg, v=v, vg=vg)
-    if k.ndim != 5:
-        raise ValueError(f"k: {k.ndim} dimensions")
+    if not isinstance(k, torch.Tensor) or k.ndim != 5:
+        raise ValueError("k: an array of five dimensions is needed")
     c = _cache(dev, k, kg, v, vg, 2 * k.shape[-1], B, table, weight, pos, layers=True)
     if newLens is None:
         newLens = torch.empty_like(lens)
@@ -266,8 +289,10 @@ def kv4Evict(k, kg, v, vg, weight, pos, lens, budget: int, recent: int, table=No
     h = _on(dev)
     nbytes = _FN["fcu_kv4_evict_work"](h, c, B, budget)
     work = k.new_empty((nbytes,)) if nbytes > 0 else None
-    _call("fcu_kv4_evict", h, c, lens.data_ptr(), B, budget, recent, newLens.data_ptr(),
-          work.data_ptr() if work is not None else None, nbytes)
+    rc = _FN["fcu_kv4_evict"](h, c, lens.data_ptr(), B, budget, recent, newLens.data_ptr(),
+                              work.data_ptr() if work is not None else None, nbytes)
+    if rc:
+        check(rc, "fcu_kv4_evict")
     return newLens
 
 
@@ -290,13 +315,17 @@ def beamStep(logits, scores, done, beams: int, eos: int):
         raise ValueError(f"{scores.numel()} scores, {done.numel()} done for {R} rows")
     B = R // beams
     outScores = scores.new_empty((B, beams))
-    tokens, parents = scores.new_empty((2, B, beams), dtype=_I32).unbind(0)
-    outDone = done.new_empty((B, beams))
+    tokens = torch.empty_like(outScores, dtype=_I32)
+    parents = torch.empty_like(tokens)
+    outDone = torch.empty_like(outScores, dtype=_BOOL)
     h = _on(dev)
     nbytes = _FN["fcu_beam_work"](h, B, beams, V)
     work = scores.new_empty((nbytes // 4 + 1,))
-    _call("fcu_beam_step", h, logits.data_ptr(), ld, scores.data_ptr(), done.data_ptr(), B, beams, V, eos,
-          outScores.data_ptr(), tokens.data_ptr(), parents.data_ptr(), outDone.data_ptr(), work.data_ptr(), nbytes)
+    rc = _FN["fcu_beam_step"](h, logits.data_ptr(), ld, scores.data_ptr(), done.data_ptr(), B, beams, V, eos,
+                              outScores.data_ptr(), tokens.data_ptr(), parents.data_ptr(), outDone.data_ptr(),
+                              work.data_ptr(), nbytes)
+    if rc:
+        check(rc, "fcu_beam_step")
     return outScores, tokens, parents, outDone
 
 
@@ -318,19 +347,17 @@ def cacheReorder(arrays, parents, lens, table=None) -> None:
     n = len(arrays)
     if not 1 <= n <= 8:
         raise ValueError(f"{n} arrays (1 to 8)")
-    _tensors(**{f"arrays[{i}]": t for i, t in enumerate(arrays)})
-    if arrays[0].ndim < 4:
-        raise ValueError(f"arrays[0]: {arrays[0].ndim} dimensions")
-    L, blocks, _, bs = arrays[0].shape[:4]
-    spec = (CacheArray * n)()
+    spec = []
     for i, t in enumerate(arrays):
-        shape = t.shape
-        if not (t.get_device() == dev and t.is_contiguous() and len(shape) >= 4 and shape[0] == L and shape[1] == blocks
-                and shape[3] == bs):
+        if not isinstance(t, torch.Tensor) or t.ndim < 4:
+            raise ValueError(f"arrays[{i}]: a tensor of at least four dimensions is needed")
+        l, m, heads, slots, *rest = t.shape
+        if i == 0:
+            L, blocks, bs = l, m, slots
+        if not (t.get_device() == dev and t.is_contiguous() and l == L and m == blocks and slots == bs):
             _check(f"arrays[{i}]", t, t.dtype, dev)
-            raise ValueError(f"arrays[{i}]: shape {tuple(shape)} beside {tuple(arrays[0].shape)}")
-        s = spec[i]
-        s.base, s.heads, s.unit = t.data_ptr(), shape[2], math.prod(shape[4:]) * t.element_size()
+            raise ValueError(f"arrays[{i}]: shape {tuple(t.shape)} beside {tuple(arrays[0].shape)}")
+        spec += t.data_ptr(), heads, math.prod(rest) * t.element_size()
     if table is not None:
         _check("table", table, _I32, dev)
         if table.ndim != 2 or table.shape[0] != B * W:
@@ -340,8 +367,11 @@ def cacheReorder(arrays, parents, lens, table=None) -> None:
         if blocks % max(B * W, 1):
             raise ValueError(f"{blocks} blocks do not divide among {B * W} beams")
         mb = blocks // max(B * W, 1)
-    _call("fcu_cache_reorder", _on(dev), spec, n, L, blocks, table.data_ptr() if table is not None else None, bs, mb,
-          parents.data_ptr(), lens.data_ptr(), B, W)
+    rc = _FN["fcu_cache_reorder"](_on(dev), _ARRAYS[n].pack(*spec), n, L, blocks,
+                                  table.data_ptr() if table is not None else None, bs, mb, parents.data_ptr(),
+                                  lens.data_ptr(), B, W)
+    if rc:
+        check(rc, "fcu_cache_reorder")
 
 
 class QuantKVCache(KVCache):
@@ -464,7 +494,8 @@ class QuantKVCache(KVCache):
         sequences (parents: a host or device int array [B, W])."""
         self._own_blocks()
         p = np.asarray(parents.cpu() if isinstance(parents, torch.Tensor) else parents)
-        _reorder(self, [t for t in (self.k, self.kg, self.v, self.vg, self.weight, self.pos) if t is not None], p, self.lens)
+        _reorder(self, [t for t in (self.k, self.kg, self.v, self.vg, self.weight, self.pos) if t is not None], p,
+                 self.lens)
         src = (np.arange(p.shape[0])[:, None] * p.shape[1] + p).reshape(-1)
         self.lens, self.dropped = self.lens[src].copy(), self.dropped[src].copy()
         self.len = int(self.lens.max(initial=0))

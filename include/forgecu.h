@@ -529,7 +529,8 @@ int64_t fcu_kv4_attn_work(fcu_ctx *ctx, const fcu_kv4 *cache, int B, int nH);
  * slot's weight grows by its p summed over the q heads of its kv head; sequences
  * may then share no block among their first seq_lens slots.  nH / nKV <= 16, B at
  * most 65535, out overlaps no part of q.  `work` is the caller's (fcu_kv4_attn_work bytes, 16-byte
- * aligned) and may be reused once the call's work on the stream is done. */
+ * aligned) and may be reused once the call's work on the stream is done: two
+ * calls that may run at the same time, or graphs of them, have one each. */
 int fcu_kv4_attn(fcu_ctx *ctx, const float *q, int64_t ld_q, const fcu_kv4 *cache, const int32_t *seq_lens, int B,
                  int nH, double scale, float *out, void *work, int64_t work_bytes);
 /* Bytes of workspace fcu_kv4_evict needs; 0 if none, -1 for bad arguments. */

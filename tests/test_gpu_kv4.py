@@ -559,6 +559,34 @@ def test_python_refusals():
         fw.cacheReorder([x, x], lens.view(1, 2), lens)
 
 
+def test_two_host_threads():
+    """Calls of two kernels each from two threads, each on a stream of its own."""
+    import threading
+    fw = F()
+    rng = np.random.default_rng(31)
+    lens = dev(np.array([900, 0, 130, 1024], np.int32))
+    cs = [Cache(4, 1024, 2, 64, 64, seed=i) for i in range(2)]
+    qs = [dev(rng.standard_normal((4, 6, 64)).astype(np.float32)) for _ in cs]
+    want = [fw.kv4Attention(q, *c.args(), lens, table=c.dtable) for q, c in zip(qs, cs)]
+    torch.cuda.synchronize()
+    got = [[], []]
+
+    def work(i):
+        with torch.cuda.stream(torch.cuda.Stream()):
+            for _ in range(100):
+                out = fw.kv4Attention(qs[i], *cs[i].args(), lens, table=cs[i].dtable)
+                got[i].append(out.clone())
+            torch.cuda.current_stream().synchronize()
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    for g, w in zip(got, want):
+        assert len(g) == 100 and all(torch.equal(x, w) for x in g)
+
+
 def test_attention_of_more_sequences_than_a_block_has_threads():
     """300 sequences, most of them short or empty, and one long."""
     rng = np.random.default_rng(20)

@@ -143,6 +143,44 @@ def test_python_refuses_tensors_off_the_device():
             f()
 
 
+def test_every_thread_has_a_context_of_its_own(monkeypatch):
+    """A thread that binds its stream leaves the calls of others where they are."""
+    torch = pytest.importorskip("torch")
+    import threading
+    from forgellm import kv4
+
+    class Fake:
+        def __init__(self, device):
+            self.handle, self.stream = object(), None
+
+        def bind_stream(self, s):
+            self.stream = s
+
+    streams = threading.local()
+    monkeypatch.setattr(kv4, "Context", Fake)
+    monkeypatch.setattr(kv4, "_CONTEXTS", kv4._Contexts())
+    monkeypatch.setattr(torch._C, "_cuda_getCurrentRawStream", lambda d: streams.now, raising=False)
+    seen, gate = {}, threading.Barrier(3)
+
+    def work(i):
+        streams.now = i
+        first = kv4._on(0)
+        gate.wait(10)
+        c = kv4._CONTEXTS.of[0]
+        seen[i] = (first, kv4._on(0), kv4._on(1), c.stream)
+        gate.wait(10)
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in (1, 2)]
+    for t in threads:
+        t.start()
+    work(0)
+    for t in threads:
+        t.join()
+    for i in range(3):
+        assert seen[i][0] is seen[i][1] and seen[i][3] == i
+    assert len({id(h) for s in seen.values() for h in s[:3]}) == 6
+
+
 # ------------------------------------------------------------------ the restatements themselves
 def test_reference_quantizer_bound():
     """|x - x^| <= step / 2 inside the grid; the ends add the roundings of base and
