@@ -364,6 +364,26 @@ __device__ __forceinline__ void issue(const Cache &c, const uint8_t *codes, cons
     // first row
     int64_t first = -1;
     if (16 * lane < cnt) first = row_of(c, b, h, j0 + 16 * lane);
+    if (cnt == C::kTile && __all_sync(0xffffffffu, first >= 0 || lane >= C::kTile / 16)) {
+      // all there: sixteen slots are 16 W pieces in a row
+      const uint8_t *p = codes + first * C::kRow;
+#pragma unroll
+      for (int k = 0; k < C::kTile / 16; k++) {
+        const uint8_t *src = reinterpret_cast<const uint8_t *>(__shfl_sync(0xffffffffu, reinterpret_cast<uint64_t>(p), k)) + 16 * lane;
+#pragma unroll
+        for (int i = 0; i < (W + 1) / 2; i++) {
+          const int x = i * 32 + lane;
+          if (32 * i + 32 <= 16 * W || lane < 16)
+            cp_async16(code_s + 16 * (16 * W * k + (W % 2 == 0 ? x - x % W + (x % W ^ swizzle<W>(x / W)) : x)), src + 512 * i, true);
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < C::kTile / 32; i++) {
+        const int64_t row = __shfl_sync(0xffffffffu, first, 2 * i + (lane >> 4));
+        cp_async4(grid_s + grid_at<C>(lane) + 16 * i, grids + row + (lane & 15), true);
+      }
+      return;
+    }
 #pragma unroll
     for (int i = 0; i < C::kTile / 32; i++) {
       const int x = i * 32 + lane;
