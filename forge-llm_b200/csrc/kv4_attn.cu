@@ -29,12 +29,13 @@
 // is always on its way and three fit on chip.
 //
 // Measured, whole calls on one B200 (copy rate 6.45 TB/s): 64 sequences of 4096
-// slots, 32 / 8 heads of 128, 65 us = 4.4 TB/s (fcu_attn_decode over the fp32
-// cache 422 us); one sequence of 262000, 12 / 4 heads of 64, 28 us = 2.7 TB/s;
-// 16 x 2047 slots, 16 / 16 heads of 80, with weights, 27 us.  Instructions bound
-// it (issue 57 % busy, ALU pipe 56 %, tensor pipe 27 %, DRAM at 68 %), about a
-// thousand a tile: 3 for every 8 codes and operand, 15 a score; below some 50 MB
-// of cache its two launches and a few microseconds of start and merge.
+// slots, 32 / 8 heads of 128, 65 us = 4.4 TB/s (79 us on pages of 16, 81 on pages
+// of 100; fcu_attn_decode over the fp32 cache 422 us); one sequence of 262000,
+// 12 / 4 heads of 64, 26 us = 2.9 TB/s; 16 x 2047 slots, 16 / 16 heads of 80, with
+// weights, 26 us.  Instructions bound it (issue 57 % busy, ALU pipe 56 %, tensor
+// pipe 27 %, DRAM at 68 %), about a thousand a tile: 3 for every 8 codes and
+// operand, 15 a score; below some 50 MB of cache its two launches and a few
+// microseconds of start and merge.
 #include <cuda_fp16.h>
 
 #include "kv4.cuh"
@@ -320,6 +321,25 @@ __device__ __noinline__ void issue_scattered(const int32_t *table, int64_t block
   c.table = table, c.blocks = blocks, c.mb = mb, c.nKV = nKV, c.bs = bs, c.div_mul = div_mul, c.div_shift = div_shift;
   const int lane = threadIdx.x & 31;
   const uint32_t code_s = (uint32_t)__cvta_generic_to_shared(part), grid_s = code_s + C::kCodes;
+  if (cnt == C::kTile && C::kTile <= bs) {
+    // a full tile lies in one block or two: `cut` slots and the rest, whose row r1
+    // is that of the tile's first slot had it been there
+    const int blk = (int)block_index(c, j0), off = j0 - blk * bs, cut = bs - off;
+    const int64_t p0 = block_of(c, b, blk), p1 = cut < C::kTile ? block_of(c, b, blk + 1) : p0;
+    if (p0 >= 0 && p1 >= 0) {
+      const int64_t r0 = (p0 * nKV + h) * bs + off, r1 = (p1 * nKV + h) * bs - cut;
+      const uint8_t *s0 = codes + r0 * C::kRow + 16 * lane, *s1 = codes + r1 * C::kRow + 16 * lane;
+#pragma unroll
+      for (int i = 0; i < C::kTile * W / 32; i++) {
+        const int x = i * 32 + lane;
+        cp_async16(code_s + 16 * (W % 2 == 0 ? x - x % W + (x % W ^ swizzle<W>(x / W)) : x), (x < cut * W ? s0 : s1) + 512 * i, true);
+      }
+#pragma unroll
+      for (int i = 0; i < C::kTile / 32; i++)
+        cp_async4(grid_s + grid_at<C>(lane) + 16 * i, grids + (32 * i + lane < cut ? r0 : r1) + 32 * i + lane, true);
+      return;
+    }
+  }
   for (int x = lane; x < C::kTile; x += 32) {
     const uint32_t at = grid_at<C>(x);
     const int64_t row = x < cnt ? row_of(c, b, h, j0 + x) : -1;
