@@ -486,7 +486,8 @@ int fcu_attn_decode(fcu_ctx *ctx, const float *q, int64_t ld_q, const float *k_c
  * (table NULL: block b * max_blocks + j / block_size) at j % block_size.  A
  * table entry outside [0, blocks) is never followed: attention over such a
  * block and values of its slots are NaN, writes to it are dropped, and
- * fcu_kv4_evict leaves the whole sequence as it is. */
+ * fcu_kv4_evict leaves the whole sequence as it is.  A sequence has at most
+ * 2^30 slots (2^26 where it is evicted from), a cache at most 65535 kv heads. */
 typedef struct {
   void *k, *v, *kg, *vg;
   float *weight;
@@ -560,7 +561,7 @@ int64_t fcu_beam_work(fcu_ctx *ctx, int B, int W, int64_t V);
  * is not finite counts as -inf.  The W best, by score and then by lowest
  * w * V + token, give out_scores, tokens, parents (= w) and out_done (ended
  * before, or token is eos), [B, W] each, best first; none of them may overlap
- * another or an input.  1 <= W <= 32.  logits may hold -inf (a banned token); a NaN
+ * another or an input.  1 <= W <= 32, B * W at most 65535, V at most 2^30.  logits may hold -inf (a banned token); a NaN
  * or +inf makes all of its row's candidates -inf. */
 int fcu_beam_step(fcu_ctx *ctx, const float *logits, int64_t ld, const float *scores, const uint8_t *done, int B,
                   int W, int64_t V, int eos, float *out_scores, int32_t *tokens, int32_t *parents,
@@ -578,7 +579,7 @@ typedef struct {
  * they were before the call; slots past that stay.  A parent outside [0, W)
  * leaves its beam as it is, and so does a block outside [0, blocks).  Slots map
  * to blocks as in fcu_kv4; no two beams may share a block, and no two arrays
- * memory.  1 <= W <= 32, at most 8 arrays. */
+ * memory.  1 <= W <= 32, at most 8 arrays, 65535 layers and 65535 searches. */
 int fcu_cache_reorder(fcu_ctx *ctx, const fcu_cache_array *arrays, int n_arrays, int64_t layers, int64_t blocks,
                       const int32_t *table, int block_size, int max_blocks, const int32_t *parents,
                       const int32_t *lens, int B, int W);
