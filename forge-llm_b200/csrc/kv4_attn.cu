@@ -8,14 +8,19 @@
 // reading the cache: a slot of one kv head is 2 (dH / 2 + 4) bytes, and every
 // q head of the group uses it while it is on the chip.
 //
-// Both products run on mma.sync m16n8k16 with the codes as the 16-row operand,
-// fp16 operands and fp32 sums.  The codes are exact in fp16 without a
-// conversion: a nibble in the mantissa of a 16-bit half is a subnormal, so a
-// shift and an AND give two operands.  The other operand carries 22 bits, x = hi + lo, in columns 2i and 2i + 1 (four heads to
-// an 8-column tile), whose sums one thread holds side by side and adds in fp32;
-// a power of two keeps x in fp16's range.  (A tcgen05 tile would want the codes
-// expanded to 16 bits in shared memory first, four times the traffic of the
-// codes themselves; fed from registers the legacy pipe is fast enough.)
+// Both products run on mma.sync m16n8k32 in integers, the codes as the 16-row
+// operand of unsigned bytes: a nibble is one AND away from its place (a shift for
+// every other), and sums are exact.  The other operand carries fixed-point numbers
+// in signed digits of base 256, a head's first two in columns 2t and 2t + 1 (four
+// heads to an 8-column tile), so that one thread holds a head's sums side by side:
+// q in four digits where a CTA has up to 4 heads, in three (2^-23 of the head's
+// largest value) for 8, whose third ones share a tile; p step alike, on a scale of
+// the tile's own.  (fp16 operands of two parts each, codes moved to where their
+// subnormals keep their bits, took 65 us where this takes 61, with nine times the
+// error over 70001 slots, 6e-6, since the tensor core drops bits when it lines
+// products up.  A tcgen05 tile would want the codes expanded in shared memory first, at
+// least twice the traffic of the codes themselves; fed from registers the legacy
+// pipe is fast enough.)
 //
 // Work is cut by tiles of slots, not by sequence: the tiles of all (sequence,
 // kv head) segments in a row are dealt in equal runs to as many CTAs as the GPU
@@ -29,15 +34,11 @@
 // is always on its way and three fit on chip.
 //
 // Measured, whole calls on one B200 (copy rate 6.45 TB/s): 64 sequences of 4096
-// slots, 32 / 8 heads of 128, 65 us = 4.4 TB/s (79 us on pages of 16, 81 on pages
-// of 100; fcu_attn_decode over the fp32 cache 422 us); one sequence of 262000,
-// 12 / 4 heads of 64, 26 us = 2.9 TB/s; 16 x 2047 slots, 16 / 16 heads of 80, with
-// weights, 26 us.  Instructions bound it (issue 57 % busy, ALU pipe 56 %, tensor
-// pipe 27 %, DRAM at 68 %), about a thousand a tile: 3 for every 8 codes and
-// operand, 15 a score; below some 50 MB of cache its two launches and a few
-// microseconds of start and merge.
-#include <cuda_fp16.h>
-
+// slots, 32 / 8 heads of 128, 61 us = 4.7 TB/s (74 us on pages of 16 or 100;
+// fcu_attn_decode over the fp32 cache 422 us); one sequence of 262000, 12 / 4
+// heads of 64, 24 us = 3.1 TB/s; 16 x 2047 slots, 16 / 16 heads of 80, with
+// weights, 25 us.  Instructions bound it, and below some 50 MB of cache its two
+// launches and a few microseconds of start and merge.
 #include "kv4.cuh"
 
 namespace fcu {
@@ -243,40 +244,38 @@ __device__ __forceinline__ float ex2(float x) {
   return y;
 }
 
-// c += a b, and the same from zero
-__device__ __forceinline__ void mma(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-  asm(
-      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+// c += a b, and the same from zero.  A sum c is kept as the bits of the float
+// 1.5 2^23 + c: kMagic is zero, and sums below 2^22 are read with a subtraction.
+constexpr int kMagic = 0x4b400000;
+__device__ __forceinline__ void imma(int (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k32.row.col.s32.u8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+      : "+r"(c[0]), "+r"(c[1]), "+r"(c[2]), "+r"(c[3])
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
-__device__ __forceinline__ void mma0(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-  asm(
-      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
-      : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])
-      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.f));
+__device__ __forceinline__ void imma0(int (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k32.row.col.s32.u8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+      : "=r"(c[0]), "=r"(c[1]), "=r"(c[2]), "=r"(c[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "r"(kMagic));
+}
+__device__ __forceinline__ float sum_of(int c) { return __int_as_float(c) - 0x1.8p23f; }
+
+// x in signed digits of base 256, a byte each: four of |x| < 2^31 / 1.004 (G 1) or
+// the upper three bytes of |x| < 2^23 / 1.004 (G 2), and a sum over the four
+// digits' sums, the last of which G 2 does not have.
+template <int G>
+__device__ __forceinline__ uint32_t digits(float x) {
+  const uint32_t v = G == 1 ? __float2int_rn(x) : __float2int_rn(x) << 8;
+  return (v + 0x80808080u) ^ 0x80808080u;
+}
+template <int G>
+__device__ __forceinline__ float total(int c0, int c1, int c2, int c3) {
+  const float low = G == 1 ? fmaf(sum_of(c2), 0x1p8f, sum_of(c3)) : sum_of(c2) * 0x1p8f;
+  return fmaf(sum_of(c0), 0x1p24f, fmaf(sum_of(c1), 0x1p16f, low));
 }
 
-// Codes N (of 0..3) of the two 16-bit halves of x as fp16 operands: moved to bits
-// 6..9, where a subnormal's value is c 2^-18.  Where in the mantissa they sit
-// matters: the tensor core lines its products up by their exponent fields and
-// drops what falls below, so the zeros above a code are bits lost.  Errors against
-// 64 bits over sixteen sizes: 2e-7 to 6e-7 here, the same as for codes made
-// normal by an extra fp16 subtraction (20 % slower); 3e-7 to 7e-7 at bits 4..7
-// (one shift fewer, 2 % faster); 1e-6 to 1e-5 where they lie, at bits 0..3 and
-// 4..7 (10 % faster).
-constexpr int kCodeExp = 18;
-template <int N>
-__device__ __forceinline__ uint32_t codes(uint32_t x) {
-  return (N == 0 ? x << 6 : N == 1 ? x << 2 : N == 2 ? x >> 2 : x >> 6) & 0x03c003c0u;
-}
-
-// x as (hi, lo) fp16: its first 11 bits, which fp16 holds, and the rest rounded
-// to 11 (2^-22 of x at most is lost; below fp16's normal range 2^-25)
-__device__ __forceinline__ uint32_t split(float x) {
-  const float h = __uint_as_float(__float_as_uint(x) & 0xffffe000u);
-  const __half2 p = __floats2half2_rn(h, x - h);
-  return *reinterpret_cast<const uint32_t *>(&p);
+// Bytes b of four words (sel: b and b + 4 in its nibbles).
+__device__ __forceinline__ uint32_t bytes4(uint32_t x0, uint32_t x1, uint32_t x2, uint32_t x3, uint32_t sel) {
+  return __byte_perm(__byte_perm(x0, x1, sel), __byte_perm(x2, x3, sel), 0x5410);
 }
 
 // The 8 x 8 matrix of 16-bit elements whose row `lane / 4` the warp holds in
@@ -534,10 +533,10 @@ __global__ void __launch_bounds__(kThreads, Cfg<W, G>::kCtas) kv4_attn_kernel(At
     issue_k(t0 + warp, 0);
     issue_v(t0 + warp);
 
-    // scale * log2 e * q of head r / 2 (its hi part for even r, the remainder
-    // for odd r) against the eight elements of word t of every piece, in the
-    // order that the masks below take a code word apart
-    uint32_t qb[G][2 * W][2];
+    // scale * log2 e * q of head r / 2 against the eight elements of word t of every
+    // piece, even ones (the low nibbles) and odd ones: its first digit for even r,
+    // the second for odd r, and (qc) the third and fourth or each tile's third
+    uint32_t qb[G][W][2], qc[W][2];
     float qs[G], qf[G];      // for head t: sum of the scaled q in the units of the tile's sums; those units
 #pragma unroll
     for (int g = 0; g < G; g++) {
@@ -565,28 +564,31 @@ __global__ void __launch_bounds__(kThreads, Cfg<W, G>::kCtas) kv4_attn_kernel(At
       big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, 2)) * fabsf(sc);
       sum += __shfl_xor_sync(0xffffffffu, sum, 1);
       sum += __shfl_xor_sync(0xffffffffu, sum, 2);
-      // x * sc * up below 2^14, up a power of two; the codes carry 2^-kCodeExp
-      const int ex = min(240, max(27, (int)(__float_as_uint(big) >> 23)));
-      const float up = __uint_as_float((uint32_t)(267 - ex) << 23);
-      const float f = __uint_as_float((uint32_t)(ex + kCodeExp - 13) << 23);      // 2^kCodeExp / up
-      const float inv = __uint_as_float((uint32_t)(267 - kCodeExp - ex) << 23);   // its inverse
+      // x * sc * up is what digits() takes, up a power of two
+      const int ex = min(254, max(44, (int)(__float_as_uint(big * 1.004f) >> 23)));
+      const float up = __uint_as_float((uint32_t)((G == 1 ? 284 : 276) - ex) << 23);
+      const float f = __uint_as_float((uint32_t)(ex - 30) << 23);      // 2^-31 times what big is below
       const float sc_up = sc * up;
-      const uint32_t sel = r & 1 ? 0x7632 : 0x5410;
+      const uint32_t sel = r & 1 ? 0x62 : 0x73, sel2 = G == 1 && r & 1 ? 0x40 : 0x51;
 #pragma unroll
       for (int i = 0; i < W; i++) {
         uint32_t y[8];
 #pragma unroll
-        for (int e = 0; e < 8; e++) y[e] = split(x[8 * i + e] * sc_up);
-        qb[g][2 * i][0] = __byte_perm(y[0], y[4], sel);
-        qb[g][2 * i][1] = __byte_perm(y[2], y[6], sel);
-        qb[g][2 * i + 1][0] = __byte_perm(y[1], y[5], sel);
-        qb[g][2 * i + 1][1] = __byte_perm(y[3], y[7], sel);
+        for (int e = 0; e < 8; e++) {
+          y[e] = digits<G>(x[8 * i + e] * sc_up);
+        }
+        qb[g][i][0] = bytes4(y[0], y[2], y[4], y[6], sel);
+        qb[g][i][1] = bytes4(y[1], y[3], y[5], y[7], sel);
+        if (g == 0 || r & 1) {
+          qc[i][0] = bytes4(y[0], y[2], y[4], y[6], sel2);
+          qc[i][1] = bytes4(y[1], y[3], y[5], y[7], sel2);
+        }
       }
-      qs[g] = __shfl_sync(0xffffffffu, sum * sc * inv, 8 * t);
+      qs[g] = __shfl_sync(0xffffffffu, sum * sc * (G == 1 ? up : up * 0x1p8f), 8 * t);
       qf[g] = __shfl_sync(0xffffffffu, f, 8 * t);
     }
 
-    // the running maximum, in the units of the tile's sums and, for head t
+    // the running maximum (in the units of the scores' sums), for head t
     float m[G], l[G], z[G], o[G][4 * W];
 #pragma unroll
     for (int g = 0; g < G; g++) {
@@ -616,19 +618,19 @@ __global__ void __launch_bounds__(kThreads, Cfg<W, G>::kCtas) kv4_attn_kernel(At
           uint32_t w[KB][2][W];
 #pragma unroll
           for (int k = 0; k < KB; k++) rows16<W, false>(ks_s, off, k0 + k, w[k]);
-          float acc[KB][G][4];
+          int acc[KB][G][4], low[KB][4];
 #pragma unroll
           for (int i = 0; i < W; i++)
 #pragma unroll
             for (int k = 0; k < KB; k++) {
-              const uint32_t x0 = w[k][0][i], x1 = w[k][1][i];
-              const uint32_t lo[4] = {codes<0>(x0), codes<0>(x1), codes<2>(x0), codes<2>(x1)};
-              const uint32_t hi[4] = {codes<1>(x0), codes<1>(x1), codes<3>(x0), codes<3>(x1)};
+              const uint32_t x0 = w[k][0][i], x1 = w[k][1][i], m4 = 0x0f0f0f0fu;
+              const uint32_t cs[4] = {x0 & m4, x1 & m4, x0 >> 4 & m4, x1 >> 4 & m4};
+              if (i == 0) imma0(low[k], cs, qc[0][0], qc[0][1]);
+              else imma(low[k], cs, qc[i][0], qc[i][1]);
 #pragma unroll
               for (int g = 0; g < G; g++) {
-                if (i == 0) mma0(acc[k][g], lo, qb[g][0][0], qb[g][0][1]);
-                else mma(acc[k][g], lo, qb[g][2 * i][0], qb[g][2 * i][1]);
-                mma(acc[k][g], hi, qb[g][2 * i + 1][0], qb[g][2 * i + 1][1]);
+                if (i == 0) imma0(acc[k][g], cs, qb[g][0][0], qb[g][0][1]);
+                else imma(acc[k][g], cs, qb[g][i][0], qb[g][i][1]);
               }
             }
 #pragma unroll
@@ -638,7 +640,8 @@ __global__ void __launch_bounds__(kThreads, Cfg<W, G>::kCtas) kv4_attn_kernel(At
 #pragma unroll
               for (int e = 0; e < 2; e++) {
                 const uint32_t gd = gr[2 * (k0 + k) + e];
-                s[g][2 * (k0 + k) + e] = fmaf(acc[k][g][2 * e] + acc[k][g][2 * e + 1], grid_step(gd), qs[g] * grid_base(gd));
+                const float x = total<G>(acc[k][g][2 * e], acc[k][g][2 * e + 1], low[k][2 * e + (G == 1 ? 0 : g)], low[k][2 * e + 1]);
+                s[g][2 * (k0 + k) + e] = fmaf(x, grid_step(gd), qs[g] * grid_base(gd));
               }
         }
       }
@@ -681,35 +684,51 @@ __global__ void __launch_bounds__(kThreads, Cfg<W, G>::kCtas) kv4_attn_kernel(At
           for (int i = 0; i < 4 * W; i++) o[g][i] *= f;
         }
       }
-      // p_j step_j as (hi, lo) pairs, transposed into the operand's columns: the
-      // tile's steps are scaled by a power of two that brings the largest into
-      // [2^13, 2^14)
+      // p_j step_j in digits, those of slots r and 8 + r of sixteen side by side,
+      // transposed into the operand's columns.  A head's are scaled by a power of
+      // two that the tile's largest decides.
       asm volatile("cp.async.wait_group 1;");
       __syncwarp();
-      uint32_t pb[G][KS][2];
-      float down;
+      uint32_t pb[G][KS], pc[KS];
+      float down[G];
       {
         uint32_t gr[2 * KS];
-        float big = 0.f;
+        float big = 0.f, up[G];
         lds<2 * KS>(vbuf + C::kCodes + 4 * r * C::kGridStride, gr);
 #pragma unroll
         for (int i = 0; i < 2 * KS; i++) big = fmaxf(big, fabsf(grid_step(gr[i])));
-        const int ex = max(13, (int)(__reduce_max_sync(0xffffffffu, __float_as_uint(big)) >> 23));
-        const float up = __uint_as_float((uint32_t)(267 - ex) << 23);
-        down = __uint_as_float((uint32_t)min(254, ex + kCodeExp - 13) << 23);   // 2^kCodeExp / up
+        big = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(big)));
+#pragma unroll
+        for (int g = 0; g < G; g++) {
+          // (below 2^-60 of the largest so far a tile no longer counts)
+          const float most = fmaxf(ex2((top[g] - m[g]) * qf[g]), 0x1p-60f) * big * 1.004f;
+          const int ex = min(254, max(44, (int)(__float_as_uint(most) >> 23)));
+          up[g] = __uint_as_float((uint32_t)((G == 1 ? 284 : 276) - ex) << 23);
+          down[g] = __uint_as_float((uint32_t)(ex - 30) << 23);
+        }
         float tl[G], tz[G];
 #pragma unroll
         for (int g = 0; g < G; g++) tl[g] = tz[g] = 0.f;
 #pragma unroll
-        for (int i = 0; i < 2 * KS; i++) {
-          const float step = grid_step(gr[i]) * up, base = grid_base(gr[i]);
+        for (int k = 0; k < KS; k++) {
+          uint32_t y[G][2];
 #pragma unroll
-          for (int g = 0; g < G; g++) {
-            const float p = ex2((s[g][i] - m[g]) * qf[g]);
-            tl[g] += p;
-            tz[g] = fmaf(p, base, tz[g]);
-            pb[g][i / 2][i & 1] = transpose8(split(p * step));
+          for (int e = 0; e < 2; e++) {
+            const int i = 2 * k + e;
+            const float step = grid_step(gr[i]), base = fmaf(step, 0.f, grid_base(gr[i]));      // a step that is not finite: NaN
+#pragma unroll
+            for (int g = 0; g < G; g++) {
+              const float p = ex2((s[g][i] - m[g]) * qf[g]);
+              tl[g] += p;
+              tz[g] = fmaf(p, base, tz[g]);
+              y[g][e] = digits<G>(p * (step * up[g]));
+            }
           }
+#pragma unroll
+          for (int g = 0; g < G; g++) pb[g][k] = transpose8(__byte_perm(y[g][0], y[g][1], 0x6273));
+          pc[k] = transpose8(G == 1 ? __byte_perm(y[0][0], y[0][1], 0x4051)
+                                    : __byte_perm(__byte_perm(y[0][0], y[0][1], 0x5151),
+                                                  __byte_perm(y[G - 1][0], y[G - 1][1], 0x5151), 0x5410));
         }
 #pragma unroll
         for (int g = 0; g < G; g++) {
@@ -725,30 +744,37 @@ __global__ void __launch_bounds__(kThreads, Cfg<W, G>::kCtas) kv4_attn_kernel(At
       for (int k = 0; k < KS; k++) rows16<W, true>(vbuf_s, off, k, vw[k]);
 #pragma unroll
       for (int u = 0; u < W; u++) {
-        float acc[G][2][4];
+        int acc[G][2][4], low[2][4];
 #pragma unroll
-        for (int k = 0; k < KS; k++) {
-          const uint32_t x = vw[k][0][u], y = vw[k][1][u];
-          const uint32_t a0[4] = {codes<0>(x), codes<1>(x), codes<0>(y), codes<1>(y)};
-          const uint32_t a1[4] = {codes<2>(x), codes<3>(x), codes<2>(y), codes<3>(y)};
+        for (int k = 0; k < KS; k += 2) {
+          uint32_t cs[2][4];
 #pragma unroll
-          for (int g = 0; g < G; g++) {
-            if (k == 0) {
-              mma0(acc[g][0], a0, pb[g][0][0], pb[g][0][1]);
-              mma0(acc[g][1], a1, pb[g][0][0], pb[g][0][1]);
-            } else {
-              mma(acc[g][0], a0, pb[g][k][0], pb[g][k][1]);
-              mma(acc[g][1], a1, pb[g][k][0], pb[g][k][1]);
+          for (int e = 0; e < 2; e++) {
+            const uint32_t x = vw[k + e][0][u], y = vw[k + e][1][u], m4 = 0x0f0f0f0fu;
+            const uint32_t even = __byte_perm(x, y, 0x6240), odd = __byte_perm(x, y, 0x7351);
+            cs[0][2 * e] = even & m4, cs[0][2 * e + 1] = even >> 4 & m4;
+            cs[1][2 * e] = odd & m4, cs[1][2 * e + 1] = odd >> 4 & m4;
+          }
+#pragma unroll
+          for (int x = 0; x < 2; x++) {
+            if (k == 0) imma0(low[x], cs[x], pc[0], pc[1]);
+            else imma(low[x], cs[x], pc[k], pc[k + 1]);
+#pragma unroll
+            for (int g = 0; g < G; g++) {
+              if (k == 0) imma0(acc[g][x], cs[x], pb[g][0], pb[g][1]);
+              else imma(acc[g][x], cs[x], pb[g][k], pb[g][k + 1]);
             }
           }
         }
 #pragma unroll
         for (int g = 0; g < G; g++)
 #pragma unroll
-          for (int x = 0; x < 2; x++) {
-            o[g][4 * u + 2 * x] = fmaf(acc[g][x][0] + acc[g][x][1], down, o[g][4 * u + 2 * x]);
-            o[g][4 * u + 2 * x + 1] = fmaf(acc[g][x][2] + acc[g][x][3], down, o[g][4 * u + 2 * x + 1]);
-          }
+          for (int x = 0; x < 2; x++)
+#pragma unroll
+            for (int e = 0; e < 2; e++) {
+              const float v = total<G>(acc[g][x][2 * e], acc[g][x][2 * e + 1], low[x][2 * e + (G == 1 ? 0 : g)], low[x][2 * e + 1]);
+              o[g][4 * u + 2 * x + e] = fmaf(v, down[g], o[g][4 * u + 2 * x + e]);
+            }
       }
       __syncwarp();
       issue_v(tile + kWarps);
