@@ -14,8 +14,8 @@
 // in signed digits of base 256, a head's first two in columns 2t and 2t + 1 (four
 // heads to an 8-column tile), so that one thread holds a head's sums side by side:
 // q in four digits where a CTA has up to 4 heads, in three (2^-23 of the head's
-// largest value) for 8, whose third ones share a tile; p step alike, on a scale of
-// the tile's own.  (fp16 operands of two parts each, codes moved to where their
+// largest value) for 8, whose third ones share a tile; p step alike, of the largest
+// in the tile.  (fp16 operands of two parts each, codes moved to where their
 // subnormals keep their bits, took 65 us where this takes 61, with nine times the
 // error over 70001 slots, 6e-6, since the tensor core drops bits when it lines
 // products up.  A tcgen05 tile would want the codes expanded in shared memory first, at
@@ -686,54 +686,51 @@ __global__ void __launch_bounds__(kThreads, Cfg<W, G>::kCtas) kv4_attn_kernel(At
       }
       // p_j step_j in digits, those of slots r and 8 + r of sixteen side by side,
       // transposed into the operand's columns.  A head's are scaled by a power of
-      // two that the tile's largest decides.
+      // two that the largest of them in the tile decides.
       asm volatile("cp.async.wait_group 1;");
       __syncwarp();
       uint32_t pb[G][KS], pc[KS];
       float down[G];
       {
         uint32_t gr[2 * KS];
-        float big = 0.f, up[G];
         lds<2 * KS>(vbuf + C::kCodes + 4 * r * C::kGridStride, gr);
+        float tl[G], tz[G], most[G], up[G];
 #pragma unroll
-        for (int i = 0; i < 2 * KS; i++) big = fmaxf(big, fabsf(grid_step(gr[i])));
-        big = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(big)));
+        for (int g = 0; g < G; g++) tl[g] = tz[g] = most[g] = 0.f;
 #pragma unroll
-        for (int g = 0; g < G; g++) {
-          // (below 2^-60 of the largest so far a tile no longer counts)
-          const float most = fmaxf(ex2((top[g] - m[g]) * qf[g]), 0x1p-60f) * big * 1.004f;
-          const int ex = min(254, max(44, (int)(__float_as_uint(most) >> 23)));
-          up[g] = __uint_as_float((uint32_t)((G == 1 ? 284 : 276) - ex) << 23);
-          down[g] = __uint_as_float((uint32_t)(ex - 30) << 23);
-        }
-        float tl[G], tz[G];
+        for (int i = 0; i < 2 * KS; i++) {
+          const float step = grid_step(gr[i]), base = fmaf(step, 0.f, grid_base(gr[i]));      // a step that is not finite: NaN
 #pragma unroll
-        for (int g = 0; g < G; g++) tl[g] = tz[g] = 0.f;
-#pragma unroll
-        for (int k = 0; k < KS; k++) {
-          uint32_t y[G][2];
-#pragma unroll
-          for (int e = 0; e < 2; e++) {
-            const int i = 2 * k + e;
-            const float step = grid_step(gr[i]), base = fmaf(step, 0.f, grid_base(gr[i]));      // a step that is not finite: NaN
-#pragma unroll
-            for (int g = 0; g < G; g++) {
-              const float p = ex2((s[g][i] - m[g]) * qf[g]);
-              tl[g] += p;
-              tz[g] = fmaf(p, base, tz[g]);
-              y[g][e] = digits<G>(p * (step * up[g]));
-            }
+          for (int g = 0; g < G; g++) {
+            const float p = ex2((s[g][i] - m[g]) * qf[g]);
+            tl[g] += p;
+            tz[g] = fmaf(p, base, tz[g]);
+            s[g][i] = p * step;
+            most[g] = fmaxf(most[g], fabsf(s[g][i]));
           }
-#pragma unroll
-          for (int g = 0; g < G; g++) pb[g][k] = transpose8(__byte_perm(y[g][0], y[g][1], 0x6273));
-          pc[k] = transpose8(G == 1 ? __byte_perm(y[0][0], y[0][1], 0x4051)
-                                    : __byte_perm(__byte_perm(y[0][0], y[0][1], 0x5151),
-                                                  __byte_perm(y[G - 1][0], y[G - 1][1], 0x5151), 0x5410));
         }
 #pragma unroll
         for (int g = 0; g < G; g++) {
           l[g] += tl[g];
           z[g] += tz[g];
+#pragma unroll
+          for (int x = 4; x < 32; x <<= 1) most[g] = fmaxf(most[g], __shfl_xor_sync(0xffffffffu, most[g], x));
+          const int ex = min(254, max(44, (int)(__float_as_uint(most[g] * 1.004f) >> 23)));
+          up[g] = __uint_as_float((uint32_t)((G == 1 ? 284 : 276) - ex) << 23);
+          down[g] = __uint_as_float((uint32_t)(ex - 30) << 23);
+        }
+#pragma unroll
+        for (int k = 0; k < KS; k++) {
+          uint32_t y[G][2];
+#pragma unroll
+          for (int g = 0; g < G; g++) {
+            y[g][0] = digits<G>(s[g][2 * k] * up[g]);
+            y[g][1] = digits<G>(s[g][2 * k + 1] * up[g]);
+            pb[g][k] = transpose8(__byte_perm(y[g][0], y[g][1], 0x6273));
+          }
+          pc[k] = transpose8(G == 1 ? __byte_perm(y[0][0], y[0][1], 0x4051)
+                                    : __byte_perm(__byte_perm(y[0][0], y[0][1], 0x5151),
+                                                  __byte_perm(y[G - 1][0], y[G - 1][1], 0x5151), 0x5410));
         }
       }
 

@@ -167,6 +167,23 @@ def test_attention_over_unequal_rows():
     check_attention(c, q * 1e18, [333, 60])
 
 
+@pytest.mark.parametrize("nH,dH", [(4, 64), (8, 64), (3, 128), (10, 96), (2, 24)])
+def test_attention_with_large_values_of_little_weight(nH, dH):
+    """Every 32nd slot holds values 2^18 times the others' with weights of about
+    e^-19: what is kept of the others' must not go by either alone."""
+    seen = []
+
+    def rows(x, rng):
+        if seen:
+            x[:, :, 7::32] *= 2.0 ** 18
+        else:
+            x[:, :, 7::32] = -3 * np.sqrt(64 / dH)
+        seen.append(1)
+    c = Cache(2, 512, 1, dH, 0, seed=13, rows=rows)
+    q = np.abs(np.random.default_rng(14).standard_normal((2, nH, dH))).astype(np.float32)
+    check_attention(c, q, [512, 75])
+
+
 def test_slots_past_the_length_are_not_read():
     c = Cache(3, 256, 2, 64, 32, seed=4)
     lens = [100, 0, 33]
