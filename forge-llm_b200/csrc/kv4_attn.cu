@@ -37,8 +37,10 @@
 // slots, 32 / 8 heads of 128, 61 us = 4.7 TB/s (74 us on pages of 16 or 100;
 // fcu_attn_decode over the fp32 cache 422 us); one sequence of 262000, 12 / 4
 // heads of 64, 24 us = 3.1 TB/s; 16 x 2047 slots, 16 / 16 heads of 80, with
-// weights, 25 us.  Instructions bound it, and below some 50 MB of cache its two
-// launches and a few microseconds of start and merge.
+// weights, 25 us.  Nearest its limit is issue, 55 % busy with the 11 warps per SM
+// that registers leave (about 960 instructions a tile of 64 slots; ALU pipe 42 %,
+// tensor pipe 29 %, DRAM at 73 % of the copy rate); below some 50 MB of cache its
+// two launches and a few microseconds of start and merge.
 #include "kv4.cuh"
 
 namespace fcu {
@@ -612,37 +614,31 @@ __global__ void __launch_bounds__(kThreads, Cfg<W, G>::kCtas) kv4_attn_kernel(At
         const uint32_t ks_s = kbuf_s + (uint32_t)(ks - kbuf);
         uint32_t gr[2 * KS];
         lds<2 * KS>(ks + C::kCodes + 4 * r * C::kGridStride, gr);
-        constexpr int KB = KS < 2 ? KS : 2;   // row tiles whose chains of sums run side by side
 #pragma unroll
-        for (int k0 = 0; k0 < KS; k0 += KB) {
-          uint32_t w[KB][2][W];
+        for (int k = 0; k < KS; k++) {      // (two at a time, side by side: 1 % slower)
+          uint32_t w[2][W];
+          rows16<W, false>(ks_s, off, k, w);
+          int acc[G][4], low[4];
 #pragma unroll
-          for (int k = 0; k < KB; k++) rows16<W, false>(ks_s, off, k0 + k, w[k]);
-          int acc[KB][G][4], low[KB][4];
+          for (int i = 0; i < W; i++) {
+            const uint32_t x0 = w[0][i], x1 = w[1][i], m4 = 0x0f0f0f0fu;
+            const uint32_t cs[4] = {x0 & m4, x1 & m4, x0 >> 4 & m4, x1 >> 4 & m4};
+            if (i == 0) imma0(low, cs, qc[0][0], qc[0][1]);
+            else imma(low, cs, qc[i][0], qc[i][1]);
 #pragma unroll
-          for (int i = 0; i < W; i++)
-#pragma unroll
-            for (int k = 0; k < KB; k++) {
-              const uint32_t x0 = w[k][0][i], x1 = w[k][1][i], m4 = 0x0f0f0f0fu;
-              const uint32_t cs[4] = {x0 & m4, x1 & m4, x0 >> 4 & m4, x1 >> 4 & m4};
-              if (i == 0) imma0(low[k], cs, qc[0][0], qc[0][1]);
-              else imma(low[k], cs, qc[i][0], qc[i][1]);
-#pragma unroll
-              for (int g = 0; g < G; g++) {
-                if (i == 0) imma0(acc[k][g], cs, qb[g][0][0], qb[g][0][1]);
-                else imma(acc[k][g], cs, qb[g][i][0], qb[g][i][1]);
-              }
+            for (int g = 0; g < G; g++) {
+              if (i == 0) imma0(acc[g], cs, qb[g][0][0], qb[g][0][1]);
+              else imma(acc[g], cs, qb[g][i][0], qb[g][i][1]);
             }
+          }
 #pragma unroll
-          for (int k = 0; k < KB; k++)
+          for (int g = 0; g < G; g++)
 #pragma unroll
-            for (int g = 0; g < G; g++)
-#pragma unroll
-              for (int e = 0; e < 2; e++) {
-                const uint32_t gd = gr[2 * (k0 + k) + e];
-                const float x = total<G>(acc[k][g][2 * e], acc[k][g][2 * e + 1], low[k][2 * e + (G == 1 ? 0 : g)], low[k][2 * e + 1]);
-                s[g][2 * (k0 + k) + e] = fmaf(x, grid_step(gd), qs[g] * grid_base(gd));
-              }
+            for (int e = 0; e < 2; e++) {
+              const uint32_t gd = gr[2 * k + e];
+              const float x = total<G>(acc[g][2 * e], acc[g][2 * e + 1], low[2 * e + (G == 1 ? 0 : g)], low[2 * e + 1]);
+              s[g][2 * k + e] = fmaf(x, grid_step(gd), qs[g] * grid_base(gd));
+            }
         }
       }
       if (cnt < TP) {
