@@ -570,14 +570,13 @@ __global__ void __launch_bounds__(kThreads, Cfg<W, G>::kCtas) kv4_attn_kernel(At
       const int ex = min(254, max(44, (int)(__float_as_uint(big * 1.004f) >> 23)));
       const float up = __uint_as_float((uint32_t)((G == 1 ? 284 : 276) - ex) << 23);
       const float f = __uint_as_float((uint32_t)(ex - 30) << 23);      // 2^-31 times what big is below
-      const float sc_up = sc * up;
       const uint32_t sel = r & 1 ? 0x62 : 0x73, sel2 = G == 1 && r & 1 ? 0x40 : 0x51;
 #pragma unroll
       for (int i = 0; i < W; i++) {
         uint32_t y[8];
 #pragma unroll
         for (int e = 0; e < 8; e++) {
-          y[e] = digits<G>(x[8 * i + e] * sc_up);
+          y[e] = digits<G>(x[8 * i + e] * sc * up);
         }
         qb[g][i][0] = bytes4(y[0], y[2], y[4], y[6], sel);
         qb[g][i][1] = bytes4(y[1], y[3], y[5], y[7], sel);

@@ -184,6 +184,30 @@ def test_attention_with_large_values_of_little_weight(nH, dH):
     check_attention(c, q, [512, 75])
 
 
+@pytest.mark.parametrize("nH", [8, 16])
+def test_attention_with_extreme_queries(nH):
+    """Queries and scales whose product is ordinary, heads that are not finite
+    beside ones that are, and grids that run downwards."""
+    c = Cache(2, 200, 2, 64, 64, seed=15)
+    q = np.random.default_rng(16).standard_normal((2, nH, 64)).astype(np.float32)
+    for big in (1e30, 1e-30, 2.0 ** 90):
+        check_attention(c, (q * np.float32(big)), [200, 77], scale=0.125 / big)
+    check_attention(c, q * np.float32(1e-36), [200, 77])
+    bad = q.copy()
+    bad[0, 1, 5] = np.nan
+    bad[1, nH - 1, 63] = np.inf
+    bad[1, 2, 0] = -np.inf
+    out = F().kv4Attention(dev(bad), *c.args(), dev(np.array([200, 77], np.int32)), table=c.dtable).cpu().numpy()
+    hit = np.isnan(out).all(-1)
+    assert hit[0, 1] and hit[1, nH - 1] and hit[1, 2] and hit.sum() == 3
+    good = check_attention(c, q, [200, 77])
+    assert np.array_equal(out[~hit], good[~hit])
+    c.step = tuple(-x for x in c.step)
+    c.kg, c.vg = [dev(np.concatenate([x, b], -1).astype(np.float32), BF) for x, b in zip(c.step, c.base)]
+    c.bound = lambda w: np.abs(c.base[w]) + 15 * np.abs(c.step[w])
+    check_attention(c, q, [200, 77])
+
+
 def test_slots_past_the_length_are_not_read():
     c = Cache(3, 256, 2, 64, 32, seed=4)
     lens = [100, 0, 33]
