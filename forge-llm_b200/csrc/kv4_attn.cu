@@ -34,13 +34,13 @@
 // is always on its way and three fit on chip.
 //
 // Measured, whole calls on one B200 (copy rate 6.45 TB/s): 64 sequences of 4096
-// slots, 32 / 8 heads of 128, 61 us = 4.7 TB/s (74 us on pages of 16 or 100;
+// slots, 32 / 8 heads of 128, 61 us = 4.7 TB/s (70 us on pages of 16, 73 of 100;
 // fcu_attn_decode over the fp32 cache 422 us); one sequence of 262000, 12 / 4
 // heads of 64, 24 us = 3.1 TB/s; 16 x 2047 slots, 16 / 16 heads of 80, with
-// weights, 25 us.  Nearest its limit is issue, 55 % busy with the 11 warps per SM
-// that registers leave (about 960 instructions a tile of 64 slots; ALU pipe 42 %,
-// tensor pipe 29 %, DRAM at 73 % of the copy rate); below some 50 MB of cache its
-// two launches and a few microseconds of start and merge.
+// weights, 25 us.  No pipe is full: issue 56 % busy (about 960 instructions a tile
+// of 64 slots), ALU pipe 44 %, tensor pipe 29 %, DRAM at 73 % of the copy rate,
+// the same with 11 and with 14 warps per SM; below some 50 MB of cache its two
+// launches and a few microseconds of start and merge.
 #include "kv4.cuh"
 
 namespace fcu {
@@ -66,8 +66,9 @@ struct Cfg {
   static constexpr int kMerge = kWarps * kHeads * (32 * W + 4) * 4;   // the warps' o, m, l at a segment's end
   static constexpr int kSmem = kRing > kMerge ? kRing : kMerge;
   // resident per SM: by registers, and by shared memory (228 KB, 1 KB and the
-  // static arrays of each CTA aside)
-  static constexpr int kByRegs = G == 1 ? (W <= 3 ? 4 : 3) : (W <= 4 ? 3 : 2);
+  // static arrays of each CTA aside).  (One tile of heads over W 4: with 4 a batch
+  // of 64 x 4096 on pages of 16 takes 70 us, with 3 73; without pages 61 both.)
+  static constexpr int kByRegs = G == 1 ? (W <= 4 ? 4 : 3) : (W <= 4 ? 3 : 2);
   static constexpr int kBySmem = 228 * 1024 / (kSmem + 3 * 1024);
   static constexpr int kCtas = kByRegs < kBySmem ? kByRegs : kBySmem;
 };
