@@ -34,11 +34,11 @@ EOS = 2
 
 
 def _fw():
-    """The framework's package, found once, as a program imports it."""
-    if "forgellm" not in sys.modules:
-        sys.path.insert(0, os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "forge-llm_b200"))
-        import forgellm
-    return sys.modules["forgellm"]
+    root = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "forge-llm_b200")
+    if root not in sys.path:
+        sys.path.insert(0, root)
+    import forgellm
+    return forgellm
 
 
 # ------------------------------------------------------------------ the cases
