@@ -2,6 +2,8 @@
 // (fcu_beam_step) and the reordering of the beams' caches after it
 // (fcu_cache_reorder).  The reference samples one sequence on the host
 // (src/L8/sampling.js:28-96) and has no beam search.
+#include <float.h>
+
 #include "common.cuh"
 
 namespace fcu {
@@ -127,7 +129,9 @@ __global__ void __launch_bounds__(kBeamThreads, 4) beam_rows_kernel(BeamArgs a) 
   const float *x = a.logits + row * a.ld;
   // tiles start where a 16-byte line does: at most three tokens before v0
   const int skew = (int)(((uintptr_t)(x + v0) >> 2) & 3);
-  float M = -INFINITY, s = 0.f;              // this lane's
+  // This lane's.  M starts at the type's lowest value: terms of -inf are 0 from there
+  // on and a NaN is one, wherever it lies, so that no sum has to be left out.
+  float M = -FLT_MAX, s = 0.f;
   uint32_t *mine = found[warp];              // tokens
   int n = 0;                                 // in it
   float least = -INFINITY;                   // no smaller logit is among the slice's W best
@@ -175,17 +179,15 @@ __global__ void __launch_bounds__(kBeamThreads, 4) beam_rows_kernel(BeamArgs a) 
     for (int i = 0; i < 4; i++)
       f[4 * i] = next[i].x, f[4 * i + 1] = next[i].y, f[4 * i + 2] = next[i].z, f[4 * i + 3] = next[i].w;
     fetch(t0 + kTile * kBeamWarps);
-    float top = f[0];
+    float top = -INFINITY;                   // (fmaxf passes a NaN over)
 #pragma unroll
-    for (int i = 1; i < 16; i++) top = fmaxf(top, f[i]);
+    for (int i = 0; i < 16; i++) top = fmaxf(top, f[i]);
     const float M1 = fmaxf(M, top * kLog2e);
-    if (M1 > -INFINITY) {
-      float ts = 0.f;
+    float ts = 0.f;
 #pragma unroll
-      for (int i = 0; i < 16; i++) ts += beam_ex2(fmaf(f[i], kLog2e, -M1));
-      s = s * beam_ex2(M - M1) + ts;
-      M = M1;
-    }
+    for (int i = 0; i < 16; i++) ts += beam_ex2(fmaf(f[i], kLog2e, -M1));
+    s = s * beam_ex2(M - M1) + ts;
+    M = M1;
     most = fmaxf(most, top);
     const uint32_t bits = nth(order_bits(most), share);
     if (lane == 0) *(volatile uint32_t *)&reached[warp] = bits;
@@ -235,17 +237,16 @@ __global__ void __launch_bounds__(kBeamThreads, 4) beam_rows_kernel(BeamArgs a) 
   for (int o = 16; o > 0; o >>= 1) {
     const float oM = __shfl_xor_sync(0xffffffffu, M, o), os = __shfl_xor_sync(0xffffffffu, s, o);
     const float M1 = fmaxf(M, oM);
-    if (M1 > -INFINITY) s = s * beam_ex2(M - M1) + os * beam_ex2(oM - M1);
+    s = s * beam_ex2(M - M1) + os * beam_ex2(oM - M1);
     M = M1;
   }
   if (lane == 0) red_m[warp] = M, red_s[warp] = s;
   __syncthreads();
   const int64_t at = row * a.slices + blockIdx.x;
   if (threadIdx.x == 0) {
-    float M1 = -INFINITY, S = 0.f;
-    for (int w = 0; w < kBeamWarps; w++) M1 = fmaxf(M1, red_m[w]);
-    if (M1 > -INFINITY)
-      for (int w = 0; w < kBeamWarps; w++) S += red_s[w] * beam_ex2(red_m[w] - M1);
+    float M1 = red_m[0], S = 0.f;
+    for (int w = 1; w < kBeamWarps; w++) M1 = fmaxf(M1, red_m[w]);
+    for (int w = 0; w < kBeamWarps; w++) S += red_s[w] * beam_ex2(red_m[w] - M1);
     a.sums[at] = make_float2(M1, S);
   }
   // the warps' lists are sorted and share no key: one's rank is its own place
@@ -276,16 +277,17 @@ __global__ void __launch_bounds__(kBeamThreads) beam_merge_kernel(BeamArgs a) {
   pdl_wait();
   for (int i = tid; i < N; i += kBeamThreads) raw[i] = a.best[b * N + i];
   for (int w = tid >> 5; w < W; w += kBeamWarps) {
-    float M = -INFINITY, S = 0.f;
+    float M = -FLT_MAX, S = 0.f;
     for (int i = lane; i < a.slices; i += 32) {
       const float2 x = a.sums[(b * W + w) * a.slices + i];
       const float M1 = fmaxf(M, x.x);
-      if (M1 > -INFINITY) S = S * beam_ex2(M - M1) + x.y * beam_ex2(x.x - M1);
+      S = S * beam_ex2(M - M1) + x.y * beam_ex2(x.x - M1);
       M = M1;
     }
     const float top = warp_max(M);
-    S = warp_sum(top > -INFINITY ? S * beam_ex2(M - top) : 0.f);
-    // 2^M S in units of kLog2e's fp32 value: what the terms were raised with
+    S = warp_sum(S * beam_ex2(M - top));
+    // 2^M S in units of kLog2e's fp32 value: what the terms were raised with (not
+    // finite where a logit was NaN or +inf, or all were -inf)
     if (lane == 0) lse[w] = ((double)top + log2((double)S)) / (double)kLog2e;
   }
   __syncthreads();

@@ -112,6 +112,30 @@ def test_beam_step_banned_and_unusable_rows():
     check_beam(x, scores, np.zeros((4, 4), bool), 2)
 
 
+@pytest.mark.parametrize("V", [64, 65, 513, 2049, 9001])
+def test_beam_step_a_nan_wherever_it_lies(V):
+    """One NaN makes its beam unusable, whatever the logits beside it are: alone at
+    the end, with its whole 16-byte piece, beside banned tokens only, in a run of
+    NaN at the start, on rows that start at any 4 bytes."""
+    rng = np.random.default_rng(V)
+    none = np.zeros((4, 4), bool)
+    for pad in (0, 1, 2, 3):
+        x = rng.standard_normal((4, 4, V)).astype(np.float32)
+        x[0, 0, V - 1] = np.nan
+        x[0, 2, :4] = np.nan
+        x[1, 0, :] = -np.inf
+        x[1, 0, V // 2] = np.nan
+        x[1, 1, :64] = -np.inf
+        x[1, 1, 17] = np.nan
+        x[2, 1, :min(512, V - 1)] = np.nan
+        x[2, 3, 60] = np.nan
+        x[2, 3, 61:] = -np.inf
+        x[3, 0, V // 2:] = np.nan
+        x[3, 1, ::2] = -np.inf
+        x[3, 1, 1::2] = np.where(np.arange(1, V, 2) < V // 2, np.nan, 1.0)
+        check_beam(x, -rng.random((4, 4)), none, 2, pad=pad)
+
+
 @pytest.mark.parametrize("L,B,W,heads,bs,mb,unit,table", [
     (2, 2, 4, 2, 16, 4, 32, True), (1, 3, 2, 1, 100, 1, 768, False), (3, 1, 5, 3, 7, 5, 4, True),
     (1, 2, 32, 2, 5, 3, 12, False), (2, 1, 3, 1, 1, 40, 20, True), (1, 4, 8, 4, 64, 2, 16, True)])
