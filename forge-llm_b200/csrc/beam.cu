@@ -60,16 +60,18 @@ struct BeamArgs {
   const uint8_t *done;
   int V, B, W, eos, slices;
   int slice;             // logits per slice
-  float2 *sums;          // [rows][slices]: M, the maximum times kLog2e, and sum of 2^(x kLog2e - M)
+  float2 *sums;          // [rows][slices]: M, the maximum, and the sum of exp(x - M)
   Key *best;             // [rows][slices][W]
   float *out_scores;
   int32_t *tokens, *parents;
   uint8_t *out_done;
 };
 
-__device__ __forceinline__ float beam_ex2(float x) {
+// e^(x - m).  The difference is taken first: x log2 e leaves fp32 for finite x
+// (masks of the type's lowest value among them).
+__device__ __forceinline__ float beam_exp(float x, float m) {
   float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"((x - m) * kLog2e));
   return y;
 }
 
@@ -182,11 +184,11 @@ __global__ void __launch_bounds__(kBeamThreads, 4) beam_rows_kernel(BeamArgs a) 
     float top = -INFINITY;                   // (fmaxf passes a NaN over)
 #pragma unroll
     for (int i = 0; i < 16; i++) top = fmaxf(top, f[i]);
-    const float M1 = fmaxf(M, top * kLog2e);
+    const float M1 = fmaxf(M, top);
     float ts = 0.f;
 #pragma unroll
-    for (int i = 0; i < 16; i++) ts += beam_ex2(fmaf(f[i], kLog2e, -M1));
-    s = s * beam_ex2(M - M1) + ts;
+    for (int i = 0; i < 16; i++) ts += beam_exp(f[i], M1);
+    s = s * beam_exp(M, M1) + ts;
     M = M1;
     most = fmaxf(most, top);
     const uint32_t bits = nth(order_bits(most), share);
@@ -237,7 +239,7 @@ __global__ void __launch_bounds__(kBeamThreads, 4) beam_rows_kernel(BeamArgs a) 
   for (int o = 16; o > 0; o >>= 1) {
     const float oM = __shfl_xor_sync(0xffffffffu, M, o), os = __shfl_xor_sync(0xffffffffu, s, o);
     const float M1 = fmaxf(M, oM);
-    s = s * beam_ex2(M - M1) + os * beam_ex2(oM - M1);
+    s = s * beam_exp(M, M1) + os * beam_exp(oM, M1);
     M = M1;
   }
   if (lane == 0) red_m[warp] = M, red_s[warp] = s;
@@ -246,7 +248,7 @@ __global__ void __launch_bounds__(kBeamThreads, 4) beam_rows_kernel(BeamArgs a) 
   if (threadIdx.x == 0) {
     float M1 = red_m[0], S = 0.f;
     for (int w = 1; w < kBeamWarps; w++) M1 = fmaxf(M1, red_m[w]);
-    for (int w = 0; w < kBeamWarps; w++) S += red_s[w] * beam_ex2(red_m[w] - M1);
+    for (int w = 0; w < kBeamWarps; w++) S += red_s[w] * beam_exp(red_m[w], M1);
     a.sums[at] = make_float2(M1, S);
   }
   // the warps' lists are sorted and share no key: one's rank is its own place
@@ -270,7 +272,8 @@ __global__ void __launch_bounds__(kBeamThreads) beam_merge_kernel(BeamArgs a) {
   __shared__ double score[kMaxW][kMaxW];
   __shared__ int token[kMaxW][kMaxW];                  // -1: no candidate
   __shared__ uint8_t order[kMaxW][kMaxW];              // a row's candidates, best first
-  __shared__ double lse[kMaxW];
+  __shared__ float top_s[kMaxW];                       // a row's largest logit
+  __shared__ double log_s[kMaxW];                      // and the log of its sum of exp(x - the largest)
   const int tid = threadIdx.x, lane = tid & 31, W = a.W, per = a.slices * W, N = W * per;
   const int64_t b = blockIdx.x;
   for (int i = tid; i < W * W; i += kBeamThreads) best[i / W][i % W] = 0;
@@ -281,14 +284,13 @@ __global__ void __launch_bounds__(kBeamThreads) beam_merge_kernel(BeamArgs a) {
     for (int i = lane; i < a.slices; i += 32) {
       const float2 x = a.sums[(b * W + w) * a.slices + i];
       const float M1 = fmaxf(M, x.x);
-      S = S * beam_ex2(M - M1) + x.y * beam_ex2(x.x - M1);
+      S = S * beam_exp(M, M1) + x.y * beam_exp(x.x, M1);
       M = M1;
     }
     const float top = warp_max(M);
-    S = warp_sum(S * beam_ex2(M - top));
-    // 2^M S in units of kLog2e's fp32 value: what the terms were raised with (not
-    // finite where a logit was NaN or +inf, or all were -inf)
-    if (lane == 0) lse[w] = ((double)top + log2((double)S)) / (double)kLog2e;
+    S = warp_sum(S * beam_exp(M, top));
+    // (not finite where a logit was NaN or +inf, or all were -inf)
+    if (lane == 0) top_s[w] = top, log_s[w] = log((double)S);
   }
   __syncthreads();
   // A row's W best of its slices' sorted lists.  Few lists: a key's rank is its
@@ -329,7 +331,7 @@ __global__ void __launch_bounds__(kBeamThreads) beam_merge_kernel(BeamArgs a) {
     const double cum = a.scores[b * W + w];
     const bool done = a.done[b * W + w] != 0;
     // a beam with nothing finite to offer stands for its lowest tokens
-    const bool dead = !isfinite(cum) || (!done && !isfinite(lse[w]));
+    const bool dead = !isfinite(cum) || (!done && !isfinite(log_s[w]));
     double v = -INFINITY;
     int tok = r < a.V ? r : -1;
     if (done && !dead) {
@@ -339,7 +341,7 @@ __global__ void __launch_bounds__(kBeamThreads) beam_merge_kernel(BeamArgs a) {
     } else if (!dead) {
       const Key k = best[w][r];
       tok = k ? (int)(0xffffffffu - (uint32_t)k) : -1;
-      v = cum + ((double)key_logit(k) - lse[w]);
+      v = cum + (((double)key_logit(k) - top_s[w]) - log_s[w]);
       if (!isfinite(v)) v = -INFINITY;
     }
     score[w][r] = v + 0.0;

@@ -556,8 +556,8 @@ int64_t fcu_beam_work(fcu_ctx *ctx, int B, int W, int64_t V);
  * of logits ([V] floats, rows ld floats apart) belongs to beam w of sequence b,
  * whose score is scores[b * W + w]; done (bytes, 0 or 1) marks the beams that
  * have ended.  Candidate (w, token) of a sequence scores
- *   scores[w] + logits[w][token] - log sum exp logits[w]
- * in double; a beam that has ended offers (w, eos) at scores[w] alone; whatever
+ *   scores[w] + ((logits[w][token] - m) - log sum exp(logits[w] - m)),  m = max logits[w]
+ * in double (the sum itself in fp32); a beam that has ended offers (w, eos) at scores[w] alone; whatever
  * is not finite counts as -inf.  The W best, by score and then by lowest
  * w * V + token, give out_scores, tokens, parents (= w) and out_done (ended
  * before, or token is eos), [B, W] each, best first; none of them may overlap

@@ -136,6 +136,35 @@ def test_beam_step_a_nan_wherever_it_lies(V):
         check_beam(x, -rng.random((4, 4)), none, 2, pad=pad)
 
 
+def test_beam_step_logits_at_the_ends_of_their_type():
+    """Tokens and whole rows masked with the type's lowest value, and rows of its
+    largest: all of them finite, so their log-softmax is (a row of equal logits
+    offers each token at its score - log V)."""
+    top = float(np.finfo(np.float32).max)
+    rng = np.random.default_rng(3)
+    for V in (4, 70, 5000):
+        x = rng.standard_normal((5, 4, V)).astype(np.float32)
+        x[0, :, 3:] = -top                      # tokens of every beam
+        x[1, :3] = -top                         # whole beams
+        x[2] = -top                             # all of them
+        x[3, 0] = top
+        x[3, 1] = np.float32(-3e38)
+        x[3, 2, 1:] = -top
+        x[4, 0] = np.where(np.arange(V) == 2, np.float32(2.5e38), np.float32(1e38))
+        x[4, 1] = np.where(np.arange(V) % 3 == 1, -np.float32(top), -np.inf)
+        done = np.zeros((5, 4), bool)
+        for order in (1, -1):
+            scores = -np.arange(4.0)[::order] * np.ones((5, 1)) / 8
+            got = F().beamStep(dev(x.reshape(20, V)), dev(scores.astype(np.float32)).view(-1), dev(done).view(-1), 4, 2)
+            s, t, p, d = [g.cpu().numpy() for g in got]
+            # a log-softmax does not change with the row's offset; in 64 bits it is lost beside one of 2^128
+            y = x.astype(np.float64)
+            y -= y.max(-1, keepdims=True)
+            ws, wt, wp, wd = R.beam(y, scores, done, 4, 2)
+            assert np.array_equal(t, wt) and np.array_equal(p, wp) and np.array_equal(d, wd), (V, order)
+            assert (np.abs(s - ws) <= 2.0 ** -23 * np.abs(ws) + 2.0 ** -18).all(), (V, order)
+
+
 @pytest.mark.parametrize("L,B,W,heads,bs,mb,unit,table", [
     (2, 2, 4, 2, 16, 4, 32, True), (1, 3, 2, 1, 100, 1, 768, False), (3, 1, 5, 3, 7, 5, 4, True),
     (1, 2, 32, 2, 5, 3, 12, False), (2, 1, 3, 1, 1, 40, 20, True), (1, 4, 8, 4, 64, 2, 16, True)])
