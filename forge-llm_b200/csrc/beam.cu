@@ -20,7 +20,8 @@ namespace {
 // warp's list is cut down to its W best when it is full and at the end.
 // beam_merge, one CTA per sequence, turns the slices' sums into each row's
 // log-sum-exp and picks the W best of the W rows' W best.  Within a row the
-// candidates order as the logits do, so W per slice are enough.  The bound is
+// candidates order as the logits do, so W per slice are enough (a row whose scores
+// tie past its W-th best logit is read once more).  The bound is
 // reading the logits (HBM): 32 x 8 rows of 100003, 102 MB, take 34 us, 27 of
 // them beam_rows (3.8 TB/s, issue slots 55 % busy; 43 us with sorted lists kept
 // in registers, a bound per warp; 38 with three tiles of a warp in shared memory
@@ -30,6 +31,7 @@ constexpr int kBeamWarps = kBeamThreads / 32;
 constexpr int kMaxW = 32;
 constexpr int kTile = 512;                          // logits a warp takes at a time
 constexpr int kMaxSlices = 64;
+constexpr int kAgain = 8;                           // loads in flight of a lane that reads a tied row again
 constexpr int kFound = 64;                          // tokens a warp lists: kMaxW and 32 more at least
 constexpr float kLog2e = 1.4426950408889634f;
 
@@ -274,6 +276,7 @@ __global__ void __launch_bounds__(kBeamThreads) beam_merge_kernel(BeamArgs a) {
   __shared__ uint8_t order[kMaxW][kMaxW];              // a row's candidates, best first
   __shared__ float top_s[kMaxW];                       // a row's largest logit
   __shared__ double log_s[kMaxW];                      // and the log of its sum of exp(x - the largest)
+  __shared__ bool tied[kMaxW];                         // a logit below the W-th best scores what that one does
   const int tid = threadIdx.x, lane = tid & 31, W = a.W, per = a.slices * W, N = W * per;
   const int64_t b = blockIdx.x;
   for (int i = tid; i < W * W; i += kBeamThreads) best[i / W][i % W] = 0;
@@ -326,9 +329,11 @@ __global__ void __launch_bounds__(kBeamThreads) beam_merge_kernel(BeamArgs a) {
     }
   }
   __syncthreads();
+  auto value = [&](int w, double cum, float logit) { return cum + (((double)logit - top_s[w]) - log_s[w]) + 0.0; };
   for (int i = tid; i < W * W; i += kBeamThreads) {
     const int w = i / W, r = i - w * W;
     const double cum = a.scores[b * W + w];
+    bool more = false;
     const bool done = a.done[b * W + w] != 0;
     // a beam with nothing finite to offer stands for its lowest tokens
     const bool dead = !isfinite(cum) || (!done && !isfinite(log_s[w]));
@@ -341,11 +346,41 @@ __global__ void __launch_bounds__(kBeamThreads) beam_merge_kernel(BeamArgs a) {
     } else if (!dead) {
       const Key k = best[w][r];
       tok = k ? (int)(0xffffffffu - (uint32_t)k) : -1;
-      v = cum + (((double)key_logit(k) - top_s[w]) - log_s[w]);
+      v = value(w, cum, key_logit(k));
       if (!isfinite(v)) v = -INFINITY;
+      const uint32_t u = (uint32_t)(k >> 32), below = u == order_bits(0.f) ? u - 2 : u - 1;   // (u - 1 there: -0)
+      more = r == W - 1 && k && v > -INFINITY && value(w, cum, bits_float(below)) == v;
     }
     score[w][r] = v + 0.0;
     token[w][r] = tok;
+    if (r == W - 1) tied[w] = more;
+  }
+  __syncthreads();
+  // Where the beam's score or its log-sum-exp swallows the difference of two logits
+  // (a score of -1e30, logits of 1e-20), tokens that the row's W best logits do not
+  // hold may tie with the last of those: the lowest of all that score as it does
+  // take its place and those of its equals in the list.
+  for (int w = tid >> 5; w < W; w += kBeamWarps) {
+    if (!tied[w]) continue;
+    const float *x = a.logits + (b * W + w) * a.ld;
+    const double cum = a.scores[b * W + w], last = score[w][W - 1];
+    int at = __popc(__ballot_sync(0xffffffffu, lane < W && score[w][lane] > last));
+    for (int t0 = 0; t0 < a.V && at < W; t0 += 32 * kAgain) {
+      float f[kAgain];
+#pragma unroll
+      for (int i = 0; i < kAgain; i++) {
+        const int t = t0 + 32 * i + lane;
+        f[i] = t < a.V ? x[t] : -INFINITY;
+      }
+#pragma unroll
+      for (int i = 0; i < kAgain; i++) {
+        const bool hit = value(w, cum, f[i]) == last;
+        const uint32_t who = __ballot_sync(0xffffffffu, hit);
+        const int place = at + __popc(who & ((1u << lane) - 1));
+        if (hit && place < W) token[w][place] = t0 + 32 * i + lane;
+        at += __popc(who);
+      }
+    }
   }
   __syncthreads();
   // A row's scores fall as its logits do, but where the beam's score swallows the

@@ -165,6 +165,29 @@ def test_beam_step_logits_at_the_ends_of_their_type():
             assert (np.abs(s - ws) <= 2.0 ** -23 * np.abs(ws) + 2.0 ** -18).all(), (V, order)
 
 
+def test_beam_step_ties_that_doubles_make():
+    """Logits that differ where their scores do not: below a score of -1e30, and
+    tiny ones beside a log-sum-exp of about 8.  The lowest tokens are first, those
+    that are not among the largest logits too."""
+    rng = np.random.default_rng(21)
+    done = np.zeros((4, 4), bool)
+    for V in (3, 40, 3000):
+        x = rng.standard_normal((4, 4, V)).astype(np.float32)
+        x[1] = rng.random((4, V)).astype(np.float32) * np.float32(1e-20)
+        x[2] = np.where(rng.random((4, V)) < 0.2, 1.0, x[1])
+        x[2, 0, 0] = -np.inf
+        x[3, 1] = -np.arange(V, dtype=np.float32)[::-1]
+        scores = np.array([[-1e30] * 4, [0, -1, -2, -3], [-0.5, 0, -1, -2], [-1e25, -1e20, -1e30, -1e30]])
+        check_beam(x, scores, done, 2)
+        x[0, :, 0] = np.nan
+        x[0, 2] = -np.inf
+        x[0, 2, 1:] = 0
+        check_beam(x, scores, done, 2, pad=2)
+        d = done.copy()
+        d[:, 0] = True
+        check_beam(x, scores, d, 1)
+
+
 @pytest.mark.parametrize("L,B,W,heads,bs,mb,unit,table", [
     (2, 2, 4, 2, 16, 4, 32, True), (1, 3, 2, 1, 100, 1, 768, False), (3, 1, 5, 3, 7, 5, 4, True),
     (1, 2, 32, 2, 5, 3, 12, False), (2, 1, 3, 1, 1, 40, 20, True), (1, 4, 8, 4, 64, 2, 16, True)])
