@@ -51,6 +51,8 @@ constexpr int kThreads = 128;
 constexpr int kWarps = kThreads / 32;
 constexpr int kKBufs = 2;      // k tiles on chip, one of them on its way
 constexpr float kLog2e = 1.4426950408889634f;
+// Powers of two of the scores' scale (kv4_attn_kernel).
+constexpr int kDown = 44, kLeastUnit = -126, kMostUnit = 127;
 
 // W: a row is W 16-byte units (dP = 32 W elements).  G: tiles of four q heads.
 template <int W, int G>
@@ -262,18 +264,24 @@ __device__ __forceinline__ void imma0(int (&c)[4], const uint32_t (&a)[4], uint3
 }
 __device__ __forceinline__ float sum_of(int c) { return __int_as_float(c) - 0x1.8p23f; }
 
+// 2^e for e in -126 .. 127, and the largest power of two in a float (-127: 2^-126
+// or below; 128: not finite).
+__device__ __forceinline__ float exp2i(int e) { return __uint_as_float((uint32_t)(e + 127) << 23); }
+__device__ __forceinline__ int exponent(float x) { return (int)(__float_as_uint(x) >> 23 & 255) - 127; }
+
 // x in signed digits of base 256, a byte each: four of |x| < 2^31 / 1.004 (G 1) or
-// the upper three bytes of |x| < 2^23 / 1.004 (G 2), and a sum over the four
-// digits' sums, the last of which G 2 does not have.
+// the upper three bytes of |x| < 2^23 / 1.004 (G 2), and 2^-DOWN times a sum over
+// the four digits' sums, the last of which G 2 does not have.
 template <int G>
 __device__ __forceinline__ uint32_t digits(float x) {
   const uint32_t v = G == 1 ? __float2int_rn(x) : __float2int_rn(x) << 8;
   return (v + 0x80808080u) ^ 0x80808080u;
 }
-template <int G>
+template <int G, int DOWN>
 __device__ __forceinline__ float total(int c0, int c1, int c2, int c3) {
-  const float low = G == 1 ? fmaf(sum_of(c2), 0x1p8f, sum_of(c3)) : sum_of(c2) * 0x1p8f;
-  return fmaf(sum_of(c0), 0x1p24f, fmaf(sum_of(c1), 0x1p16f, low));
+  float low = sum_of(c2) * exp2i(8 - DOWN);
+  if (G == 1) low = fmaf(sum_of(c2), exp2i(8 - DOWN), fmaf(__int_as_float(c3), exp2i(-DOWN), -0x1.8p23f * exp2i(-DOWN)));
+  return fmaf(sum_of(c0), exp2i(24 - DOWN), fmaf(sum_of(c1), exp2i(16 - DOWN), low));
 }
 
 // Bytes b of four words (sel: b and b + 4 in its nibbles).
@@ -540,13 +548,17 @@ __global__ void __launch_bounds__(kThreads, Cfg<W, G>::kCtas) kv4_attn_kernel(At
     // piece, even ones (the low nibbles) and odd ones: its first digit for even r,
     // the second for odd r, and (qc) the third and fourth or each tile's third
     uint32_t qb[G][W][2], qc[W][2];
-    float qs[G], qf[G];      // for head t: sum of the scaled q in the units of the tile's sums; those units
+    // For head t: its scaled q lie below 2^qe, and their digits stand for 2^(31 - qe) times
+    // them.  A sum of codes times digits, below 2^43, is brought down by 2^-kDown before it
+    // meets the row's grid, so that no row that the cache holds takes a score out of fp32;
+    // scores are kept over unit(), the rest of that scale.  qs: the sum of the scaled q, alike.
+    float qs[G];
+    int qe[G];
 #pragma unroll
     for (int g = 0; g < G; g++) {
       const int head = 4 * g + (r >> 1);
       const float *q = a.q + at.b * a.ld_q + (int64_t)(h0 + head) * c.dH;
-      const float sc = a.scale * kLog2e;
-      float x[8 * W], big = 0.f, sum = 0.f;
+      float x[8 * W], big = 0.f;
 #pragma unroll
       for (int i = 0; i < 8 * W; i += 4) {
         const int d = 32 * (i / 8) + 8 * t + i % 8;
@@ -559,25 +571,26 @@ __global__ void __launch_bounds__(kThreads, Cfg<W, G>::kCtas) kv4_attn_kernel(At
         }
       }
 #pragma unroll
-      for (int i = 0; i < 8 * W; i++) {
-        big = fmaxf(big, fabsf(x[i]));
-        sum += x[i];
-      }
+      for (int i = 0; i < 8 * W; i++) big = fmaxf(big, fabsf(x[i]));
       big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, 1));
-      big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, 2)) * fabsf(sc);
-      sum += __shfl_xor_sync(0xffffffffu, sum, 1);
-      sum += __shfl_xor_sync(0xffffffffu, sum, 2);
-      // x * sc * up is what digits() takes, up a power of two
-      const int ex = min(254, max(44, (int)(__float_as_uint(big * 1.004f) >> 23)));
-      const float up = __uint_as_float((uint32_t)((G == 1 ? 284 : 276) - ex) << 23);
-      const float f = __uint_as_float((uint32_t)(ex - 30) << 23);      // 2^-31 times what big is below
+      big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, 2));
+      // scale log2 e x = (x 2^-e0) sc 2^(e0 + e1): both factors are near 1, whatever q and scale are
+      const int e0 = min(126, exponent(big)), e1 = min(126, exponent(a.scale));
+      const float near1 = exp2i(-e0), sc = a.scale * exp2i(-e1) * kLog2e;
+      const int e2 = min(8, max(-64, exponent(big * near1 * fabsf(sc) * 1.004f) + 1));
+      // (below what unit() can be, of use beside keys of 2^100 and more only: fewer digits)
+      const int lost = min(64, max(0, kLeastUnit + 31 - kDown - (e0 + e1 + e2)));
+      const float up = sc * exp2i((G == 1 ? 31 : 23) - e2 - lost);
+      float sum = 0.f;
       const uint32_t sel = r & 1 ? 0x62 : 0x73, sel2 = G == 1 && r & 1 ? 0x40 : 0x51;
 #pragma unroll
       for (int i = 0; i < W; i++) {
         uint32_t y[8];
 #pragma unroll
         for (int e = 0; e < 8; e++) {
-          y[e] = digits<G>(x[8 * i + e] * sc * up);
+          const float z = x[8 * i + e] * near1 * up;
+          sum += z;
+          y[e] = digits<G>(z);
         }
         qb[g][i][0] = bytes4(y[0], y[2], y[4], y[6], sel);
         qb[g][i][1] = bytes4(y[1], y[3], y[5], y[7], sel);
@@ -586,11 +599,14 @@ __global__ void __launch_bounds__(kThreads, Cfg<W, G>::kCtas) kv4_attn_kernel(At
           qc[i][1] = bytes4(y[1], y[3], y[5], y[7], sel2);
         }
       }
-      qs[g] = __shfl_sync(0xffffffffu, sum * sc * (G == 1 ? up : up * 0x1p8f), 8 * t);
-      qf[g] = __shfl_sync(0xffffffffu, f, 8 * t);
+      sum += __shfl_xor_sync(0xffffffffu, sum, 1);
+      sum += __shfl_xor_sync(0xffffffffu, sum, 2);
+      qs[g] = __shfl_sync(0xffffffffu, sum * exp2i((G == 1 ? 0 : 8) - kDown), 8 * t);
+      qe[g] = __shfl_sync(0xffffffffu, max(e0 + e1 + e2 + lost, kLeastUnit + 31 - kDown), 8 * t);
     }
+    auto unit = [&](int g) { return exp2i(min(qe[g] + kDown - 31, kMostUnit)); };
 
-    // the running maximum (in the units of the scores' sums), for head t
+    // the running maximum (over unit(), as the scores), for head t
     float m[G], l[G], z[G], o[G][4 * W];
 #pragma unroll
     for (int g = 0; g < G; g++) {
@@ -636,11 +652,16 @@ __global__ void __launch_bounds__(kThreads, Cfg<W, G>::kCtas) kv4_attn_kernel(At
 #pragma unroll
             for (int e = 0; e < 2; e++) {
               const uint32_t gd = gr[2 * k + e];
-              const float x = total<G>(acc[g][2 * e], acc[g][2 * e + 1], low[2 * e + (G == 1 ? 0 : g)], low[2 * e + 1]);
+              const float x = total<G, kDown>(acc[g][2 * e], acc[g][2 * e + 1], low[2 * e + (G == 1 ? 0 : g)], low[2 * e + 1]);
               s[g][2 * k + e] = fmaf(x, grid_step(gd), qs[g] * grid_base(gd));
             }
         }
       }
+#pragma unroll
+      for (int g = 0; g < G; g++)
+        if (qe[g] + kDown - 31 > kMostUnit)      // scaled q of 2^114 and more
+#pragma unroll
+          for (int i = 0; i < 2 * KS; i++) s[g][i] *= exp2i(min(127, qe[g] + kDown - 31 - kMostUnit));
       if (cnt < TP) {
 #pragma unroll
         for (int i = 0; i < 2 * KS; i++)
@@ -655,7 +676,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<W, G>::kCtas) kv4_attn_kernel(At
             float *sc = a.scores + (at.b * a.nH + h0 + 4 * g + t) * c.cap + j0 + r;
 #pragma unroll
             for (int i = 0; i < 2 * KS; i++)
-              if (8 * i + r < cnt) sc[8 * i] = s[g][i] * qf[g];
+              if (8 * i + r < cnt) sc[8 * i] = s[g][i] * unit(g);
           }
       }
       float top[G];
@@ -672,7 +693,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<W, G>::kCtas) kv4_attn_kernel(At
       if (__any_sync(0xffffffffu, grows)) {
 #pragma unroll
         for (int g = 0; g < G; g++) {
-          const float m1 = fmaxf(m[g], top[g]), f = m1 > m[g] ? ex2((m[g] - m1) * qf[g]) : 1.f;
+          const float m1 = fmaxf(m[g], top[g]), f = m1 > m[g] ? ex2((m[g] - m1) * unit(g)) : 1.f;
           m[g] = m1;
           l[g] *= f;
           z[g] *= f;
@@ -690,9 +711,9 @@ __global__ void __launch_bounds__(kThreads, Cfg<W, G>::kCtas) kv4_attn_kernel(At
       {
         uint32_t gr[2 * KS];
         lds<2 * KS>(vbuf + C::kCodes + 4 * r * C::kGridStride, gr);
-        float tl[G], tz[G], most[G], up[G];
+        float tl[G], tz[G], most[G], up[G], qf[G];
 #pragma unroll
-        for (int g = 0; g < G; g++) tl[g] = tz[g] = most[g] = 0.f;
+        for (int g = 0; g < G; g++) tl[g] = tz[g] = most[g] = 0.f, qf[g] = unit(g);
 #pragma unroll
         for (int i = 0; i < 2 * KS; i++) {
           const float step = grid_step(gr[i]), base = fmaf(step, 0.f, grid_base(gr[i]));      // a step that is not finite: NaN
@@ -765,7 +786,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<W, G>::kCtas) kv4_attn_kernel(At
           for (int x = 0; x < 2; x++)
 #pragma unroll
             for (int e = 0; e < 2; e++) {
-              const float v = total<G>(acc[g][x][2 * e], acc[g][x][2 * e + 1], low[x][2 * e + (G == 1 ? 0 : g)], low[x][2 * e + 1]);
+              const float v = total<G, 0>(acc[g][x][2 * e], acc[g][x][2 * e + 1], low[x][2 * e + (G == 1 ? 0 : g)], low[x][2 * e + 1]);
               o[g][4 * u + 2 * x + e] = fmaf(v, down[g], o[g][4 * u + 2 * x + e]);
             }
       }
@@ -789,7 +810,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<W, G>::kCtas) kv4_attn_kernel(At
       for (int i = 0; i < W; i++)
         *reinterpret_cast<float4 *>(mine + 32 * i + 4 * r) =
             make_float4(o[g][4 * i] + z[g], o[g][4 * i + 1] + z[g], o[g][4 * i + 2] + z[g], o[g][4 * i + 3] + z[g]);
-      if (r == 0) *reinterpret_cast<float2 *>(mine + dP) = make_float2(m[g] * qf[g], l[g]);   // log2 units from here on
+      if (r == 0) *reinterpret_cast<float2 *>(mine + dP) = make_float2(m[g] * unit(g), l[g]);   // log2 units from here on
     }
     __syncthreads();
     const bool whole = a.whole || (t0 == 0 && t1 == at.tiles);

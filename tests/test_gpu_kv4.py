@@ -208,6 +208,58 @@ def test_attention_with_extreme_queries(nH):
     check_attention(c, q, [200, 77])
 
 
+@pytest.mark.parametrize("nH,dH", [(4, 128), (16, 64), (6, 256)])
+@pytest.mark.parametrize("size", [2.0 ** 92, 2.0 ** 100, 2.0 ** 115, 2.0 ** 120])
+def test_attention_over_keys_of_any_size(nH, dH, size):
+    """Keys up to what the cache holds as finite: with queries that make the scores
+    ordinary, and with ones that make them large (one slot takes all, or equal
+    rows share)."""
+    def rows(x, rng):
+        if not seen:
+            x *= np.float32(size)
+        seen.append(1)
+    seen = []
+    c = Cache(2, 200, 2, dH, 64, seed=17, rows=rows)
+    q = np.random.default_rng(18).standard_normal((2, nH, dH)).astype(np.float32)
+    check_attention(c, q * np.float32(1 / size), [200, 77])
+    check_attention(c, q, [200, 77], scale=0.125 / size)
+    check_attention(c, q * np.float32(2.0 ** 14), [200, 77], scale=2.0 ** -17 / size)
+    # scores of the keys' own size: a query along the unit vector e picks the slot of the
+    # largest element e, and the largest two are further apart than any rounding
+    K = [np.concatenate([c.rows(0, b, h, n) for h in range(2)], 1).reshape(n, 2, dH) for b, n in ((0, 200), (1, 77))]
+    one = np.zeros((2, nH, dH), np.float32)
+    want = np.zeros((2, nH, dH))
+    for b in range(2):
+        for h in range(nH):
+            kv = h // (nH // 2)
+            col = K[b][:, kv]
+            top = np.sort(col, 0)
+            e = int(np.argmax(top[-1] - top[-2]))
+            assert top[-1, e] - top[-2, e] > size * 2.0 ** -10
+            one[b, h, e] = 1
+            want[b, h] = c.rows(1, b, kv, len(col))[int(np.argmax(col[:, e]))]
+    got = F().kv4Attention(dev(one), *c.args(), dev(np.array([200, 77], np.int32)), scale=1.0, table=c.dtable)
+    assert np.abs(got.cpu().numpy() - want).max() <= 2.0 ** -19 * np.abs(want).max()
+
+
+def test_attention_with_queries_whose_sum_leaves_fp32():
+    """Finite queries of one sign: their sum, which meets the rows' base, passes
+    2^128, their scaled sum does not; and queries so large that only tiny keys
+    make ordinary scores of them."""
+    c = Cache(2, 200, 2, 64, 64, seed=19)
+    q = np.abs(np.random.default_rng(20).standard_normal((2, 8, 64))).astype(np.float32) + 1
+    check_attention(c, q * np.float32(2.0 ** 124), [200, 77], scale=2.0 ** -128)
+    tiny = []
+
+    def rows(x, rng):
+        if not tiny:
+            x *= np.float32(2.0 ** -112)      # the keys
+        tiny.append(1)
+    c = Cache(2, 200, 2, 64, 64, seed=19, rows=rows)
+    check_attention(c, q * np.float32(2.0 ** 109), [200, 77])
+    check_attention(c, q * np.float32(2.0 ** 100), [200, 77], scale=2.0 ** 8)
+
+
 def test_slots_past_the_length_are_not_read():
     c = Cache(3, 256, 2, 64, 32, seed=4)
     lens = [100, 0, 33]
