@@ -2,15 +2,18 @@
 // (fcu_kv4_attn; layout in kv4.cuh).
 //
 //   s_j = scale (step_j q.c_j + base_j sum q),  p = softmax(s)
-//   o_e = sum_j p_j step_j c_je + sum_j p_j base_j
+//   o_e = sum_j p_j step_j (c_je - 8) + sum_j p_j (base_j + 8 step_j)
+//
+// (The middle of a row's grid is near the middle of its values.  About base, the two
+// sums of o cancel to a small part of either where many slots share the weight.)
 //
 // One pass over the cache with a running maximum and sum.  The bound is
 // reading the cache: a slot of one kv head is 2 (dH / 2 + 4) bytes, and every
 // q head of the group uses it while it is on the chip.
 //
 // Both products run on mma.sync m16n8k32 in integers, the codes as the 16-row
-// operand of unsigned bytes: a nibble is one AND away from its place (a shift for
-// every other), and sums are exact.  The other operand carries fixed-point numbers
+// operand of bytes: a nibble is one AND (for v one LOP3) away from its place, a
+// shift for every other, and sums are exact.  The other operand carries fixed-point numbers
 // in signed digits of base 256, a head's first two in columns 2t and 2t + 1 (four
 // heads to an 8-column tile), so that one thread holds a head's sums side by side:
 // q in four digits where a CTA has up to 4 heads, in three (2^-23 of the head's
@@ -252,16 +255,29 @@ __device__ __forceinline__ float ex2(float x) {
 // c += a b, and the same from zero.  A sum c is kept as the bits of the float
 // 1.5 2^23 + c: kMagic is zero, and sums below 2^22 are read with a subtraction.
 constexpr int kMagic = 0x4b400000;
+// SIGNED: a's bytes are.
+#define FCU_IMMA "mma.sync.aligned.m16n8k32.row.col.s32."
+template <bool SIGNED>
 __device__ __forceinline__ void imma(int (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-  asm("mma.sync.aligned.m16n8k32.row.col.s32.u8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-      : "+r"(c[0]), "+r"(c[1]), "+r"(c[2]), "+r"(c[3])
-      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+#define FCU_CASE(T)                                                                       \
+  asm(FCU_IMMA T ".s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"          \
+      : "+r"(c[0]), "+r"(c[1]), "+r"(c[2]), "+r"(c[3])                                    \
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1))
+  if constexpr (SIGNED) FCU_CASE("s8");
+  else FCU_CASE("u8");
+#undef FCU_CASE
 }
+template <bool SIGNED>
 __device__ __forceinline__ void imma0(int (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-  asm("mma.sync.aligned.m16n8k32.row.col.s32.u8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
-      : "=r"(c[0]), "=r"(c[1]), "=r"(c[2]), "=r"(c[3])
-      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "r"(kMagic));
+#define FCU_CASE(T)                                                                       \
+  asm(FCU_IMMA T ".s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"      \
+      : "=r"(c[0]), "=r"(c[1]), "=r"(c[2]), "=r"(c[3])                                    \
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "r"(kMagic))
+  if constexpr (SIGNED) FCU_CASE("s8");
+  else FCU_CASE("u8");
+#undef FCU_CASE
 }
+#undef FCU_IMMA
 __device__ __forceinline__ float sum_of(int c) { return __int_as_float(c) - 0x1.8p23f; }
 
 // 2^e for e in -126 .. 127, and the largest power of two in a float (-127: 2^-126
@@ -282,6 +298,14 @@ __device__ __forceinline__ float total(int c0, int c1, int c2, int c3) {
   float low = sum_of(c2) * exp2i(8 - DOWN);
   if (G == 1) low = fmaf(sum_of(c2), exp2i(8 - DOWN), fmaf(__int_as_float(c3), exp2i(-DOWN), -0x1.8p23f * exp2i(-DOWN)));
   return fmaf(sum_of(c0), exp2i(24 - DOWN), fmaf(sum_of(c1), exp2i(16 - DOWN), low));
+}
+
+// 16 (c - 8) in each byte, c the code in its upper nibble: (x & 0xf0..) ^ 0x80.. in one
+// instruction, which the compiler makes two of (64 x 4096 slots 65.6 us, so 63.3).
+__device__ __forceinline__ uint32_t middle(uint32_t x) {
+  uint32_t y;
+  asm("lop3.b32 %0, %1, %2, %3, 0x6a;" : "=r"(y) : "r"(x), "r"(0xf0f0f0f0u), "r"(0x80808080u));
+  return y;
 }
 
 // Bytes b of four words (sel: b and b + 4 in its nibbles).
@@ -639,12 +663,12 @@ __global__ void __launch_bounds__(kThreads, Cfg<W, G>::kCtas) kv4_attn_kernel(At
           for (int i = 0; i < W; i++) {
             const uint32_t x0 = w[0][i], x1 = w[1][i], m4 = 0x0f0f0f0fu;
             const uint32_t cs[4] = {x0 & m4, x1 & m4, x0 >> 4 & m4, x1 >> 4 & m4};
-            if (i == 0) imma0(low, cs, qc[0][0], qc[0][1]);
-            else imma(low, cs, qc[i][0], qc[i][1]);
+            if (i == 0) imma0<false>(low, cs, qc[0][0], qc[0][1]);
+            else imma<false>(low, cs, qc[i][0], qc[i][1]);
 #pragma unroll
             for (int g = 0; g < G; g++) {
-              if (i == 0) imma0(acc[g], cs, qb[g][0][0], qb[g][0][1]);
-              else imma(acc[g], cs, qb[g][i][0], qb[g][i][1]);
+              if (i == 0) imma0<false>(acc[g], cs, qb[g][0][0], qb[g][0][1]);
+              else imma<false>(acc[g], cs, qb[g][i][0], qb[g][i][1]);
             }
           }
 #pragma unroll
@@ -716,12 +740,12 @@ __global__ void __launch_bounds__(kThreads, Cfg<W, G>::kCtas) kv4_attn_kernel(At
         for (int g = 0; g < G; g++) tl[g] = tz[g] = most[g] = 0.f, qf[g] = unit(g);
 #pragma unroll
         for (int i = 0; i < 2 * KS; i++) {
-          const float step = grid_step(gr[i]), base = fmaf(step, 0.f, grid_base(gr[i]));      // a step that is not finite: NaN
+          const float step = grid_step(gr[i]), mid = fmaf(step, 8.f, grid_base(gr[i]));
 #pragma unroll
           for (int g = 0; g < G; g++) {
             const float p = ex2((s[g][i] - m[g]) * qf[g]);
             tl[g] += p;
-            tz[g] = fmaf(p, base, tz[g]);
+            tz[g] = fmaf(p, mid, tz[g]);
             s[g][i] = p * step;
             most[g] = fmaxf(most[g], fabsf(s[g][i]));
           }
@@ -734,7 +758,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<W, G>::kCtas) kv4_attn_kernel(At
           for (int x = 4; x < 32; x <<= 1) most[g] = fmaxf(most[g], __shfl_xor_sync(0xffffffffu, most[g], x));
           const int ex = min(254, max(44, (int)(__float_as_uint(most[g] * 1.004f) >> 23)));
           up[g] = __uint_as_float((uint32_t)((G == 1 ? 284 : 276) - ex) << 23);
-          down[g] = __uint_as_float((uint32_t)(ex - 30) << 23);
+          down[g] = __uint_as_float((uint32_t)(ex - 34) << 23);      // (a sixteenth for middle()'s 16)
         }
 #pragma unroll
         for (int k = 0; k < KS; k++) {
@@ -764,19 +788,19 @@ __global__ void __launch_bounds__(kThreads, Cfg<W, G>::kCtas) kv4_attn_kernel(At
           uint32_t cs[2][4];
 #pragma unroll
           for (int e = 0; e < 2; e++) {
-            const uint32_t x = vw[k + e][0][u], y = vw[k + e][1][u], m4 = 0x0f0f0f0fu;
+            const uint32_t x = vw[k + e][0][u], y = vw[k + e][1][u];
             const uint32_t even = __byte_perm(x, y, 0x6240), odd = __byte_perm(x, y, 0x7351);
-            cs[0][2 * e] = even & m4, cs[0][2 * e + 1] = even >> 4 & m4;
-            cs[1][2 * e] = odd & m4, cs[1][2 * e + 1] = odd >> 4 & m4;
+            cs[0][2 * e] = middle(even << 4), cs[0][2 * e + 1] = middle(even);
+            cs[1][2 * e] = middle(odd << 4), cs[1][2 * e + 1] = middle(odd);
           }
 #pragma unroll
           for (int x = 0; x < 2; x++) {
-            if (k == 0) imma0(low[x], cs[x], pc[0], pc[1]);
-            else imma(low[x], cs[x], pc[k], pc[k + 1]);
+            if (k == 0) imma0<true>(low[x], cs[x], pc[0], pc[1]);
+            else imma<true>(low[x], cs[x], pc[k], pc[k + 1]);
 #pragma unroll
             for (int g = 0; g < G; g++) {
-              if (k == 0) imma0(acc[g][x], cs[x], pb[g][0], pb[g][1]);
-              else imma(acc[g][x], cs[x], pb[g][k], pb[g][k + 1]);
+              if (k == 0) imma0<true>(acc[g][x], cs[x], pb[g][0], pb[g][1]);
+              else imma<true>(acc[g][x], cs[x], pb[g][k], pb[g][k + 1]);
             }
           }
         }

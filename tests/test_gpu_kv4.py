@@ -152,6 +152,16 @@ def test_attention_with_sharp_and_flat_scores():
     check_attention(c, q, [700, 64, 130], scale=-0.3)
 
 
+@pytest.mark.parametrize("nH,nKV,dH,n,size", [(12, 4, 72, 333, 0.05), (8, 2, 128, 3000, 0.05), (16, 2, 64, 3000, 0.01),
+                                              (4, 1, 64, 30000, 0.3)])
+@pytest.mark.parametrize("seed", range(3))
+def test_attention_with_nearly_equal_weights(nH, nKV, dH, n, size, seed):
+    """The mean of many rows is far smaller than the rows and than their grids' bases."""
+    c = Cache(2, n, nKV, dH, 0, seed=seed)
+    q = np.random.default_rng(seed + 50).standard_normal((2, nH, dH)).astype(np.float32) * np.float32(size)
+    check_attention(c, q, [n, n // 3])
+
+
 def test_attention_over_unequal_rows():
     """Constant rows (step 0), rows far from zero, tiny and large rows."""
     def rows(x, rng):
