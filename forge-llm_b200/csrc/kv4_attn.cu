@@ -55,7 +55,7 @@ constexpr int kWarps = kThreads / 32;
 constexpr int kKBufs = 2;      // k tiles on chip, one of them on its way
 constexpr float kLog2e = 1.4426950408889634f;
 // Powers of two of the scores' scale (kv4_attn_kernel).
-constexpr int kDown = 44, kLeastUnit = -126, kMostUnit = 127;
+constexpr int kDown = 40, kLeastUnit = -126, kMostUnit = 127;
 
 // W: a row is W 16-byte units (dP = 32 W elements).  G: tiles of four q heads.
 template <int W, int G>
@@ -253,8 +253,9 @@ __device__ __forceinline__ float ex2(float x) {
 }
 
 // c += a b, and the same from zero.  A sum c is kept as the bits of the float
-// 1.5 2^23 + c: kMagic is zero, and sums below 2^22 are read with a subtraction.
-constexpr int kMagic = 0x4b400000;
+// (1.5 2^23 + c) 2^-kDown: kMagic is zero, and of sums below 2^22 one subtraction
+// makes c 2^-kDown.
+constexpr int kMagic = 0x4b400000 - (kDown << 23);
 // SIGNED: a's bytes are.
 #define FCU_IMMA "mma.sync.aligned.m16n8k32.row.col.s32."
 template <bool SIGNED>
@@ -278,7 +279,7 @@ __device__ __forceinline__ void imma0(int (&c)[4], const uint32_t (&a)[4], uint3
 #undef FCU_CASE
 }
 #undef FCU_IMMA
-__device__ __forceinline__ float sum_of(int c) { return __int_as_float(c) - 0x1.8p23f; }
+__device__ __forceinline__ float sum_of(int c) { return __int_as_float(c) - __int_as_float(kMagic); }
 
 // 2^e for e in -126 .. 127, and the largest power of two in a float (-127: 2^-126
 // or below; 128: not finite).
@@ -286,19 +287,21 @@ __device__ __forceinline__ float exp2i(int e) { return __uint_as_float((uint32_t
 __device__ __forceinline__ int exponent(float x) { return (int)(__float_as_uint(x) >> 23 & 255) - 127; }
 
 // x in signed digits of base 256, a byte each: four of |x| < 2^31 / 1.004 (G 1) or
-// the upper three bytes of |x| < 2^23 / 1.004 (G 2), and 2^-DOWN times a sum over
+// the upper three bytes of |x| < 2^23 / 1.004 (G 2), and 2^-kDown times a sum over
 // the four digits' sums, the last of which G 2 does not have.
 template <int G>
 __device__ __forceinline__ uint32_t digits(float x) {
   const uint32_t v = G == 1 ? __float2int_rn(x) : __float2int_rn(x) << 8;
   return (v + 0x80808080u) ^ 0x80808080u;
 }
-template <int G, int DOWN>
+template <int G>
 __device__ __forceinline__ float total(int c0, int c1, int c2, int c3) {
-  float low = sum_of(c2) * exp2i(8 - DOWN);
-  if (G == 1) low = fmaf(sum_of(c2), exp2i(8 - DOWN), fmaf(__int_as_float(c3), exp2i(-DOWN), -0x1.8p23f * exp2i(-DOWN)));
-  return fmaf(sum_of(c0), exp2i(24 - DOWN), fmaf(sum_of(c1), exp2i(16 - DOWN), low));
+  const float low = G == 1 ? fmaf(sum_of(c2), 0x1p8f, sum_of(c3)) : sum_of(c2) * 0x1p8f;
+  return fmaf(sum_of(c0), 0x1p24f, fmaf(sum_of(c1), 0x1p16f, low));
 }
+
+// Powers of two by which the output's sums over n slots are kept down: 5 to 35.
+__device__ __forceinline__ int spare_of(int n) { return 36 - __clz(n); }
 
 // 16 (c - 8) in each byte, c the code in its upper nibble: (x & 0xf0..) ^ 0x80.. in one
 // instruction, which the compiler makes two of (64 x 4096 slots 65.6 us, so 63.3).
@@ -630,6 +633,8 @@ __global__ void __launch_bounds__(kThreads, Cfg<W, G>::kCtas) kv4_attn_kernel(At
     }
     auto unit = [&](int g) { return exp2i(min(qe[g] + kDown - 31, kMostUnit)); };
 
+    // o and z are kept in 2^spare: sums of n weights' values stay below those of the values
+    const int spare = spare_of(n);
     // the running maximum (over unit(), as the scores), for head t
     float m[G], l[G], z[G], o[G][4 * W];
 #pragma unroll
@@ -676,14 +681,14 @@ __global__ void __launch_bounds__(kThreads, Cfg<W, G>::kCtas) kv4_attn_kernel(At
 #pragma unroll
             for (int e = 0; e < 2; e++) {
               const uint32_t gd = gr[2 * k + e];
-              const float x = total<G, kDown>(acc[g][2 * e], acc[g][2 * e + 1], low[2 * e + (G == 1 ? 0 : g)], low[2 * e + 1]);
+              const float x = total<G>(acc[g][2 * e], acc[g][2 * e + 1], low[2 * e + (G == 1 ? 0 : g)], low[2 * e + 1]);
               s[g][2 * k + e] = fmaf(x, grid_step(gd), qs[g] * grid_base(gd));
             }
         }
       }
 #pragma unroll
       for (int g = 0; g < G; g++)
-        if (qe[g] + kDown - 31 > kMostUnit)      // scaled q of 2^114 and more
+        if (qe[g] + kDown - 31 > kMostUnit)      // scaled q of 2^118 and more
 #pragma unroll
           for (int i = 0; i < 2 * KS; i++) s[g][i] *= exp2i(min(127, qe[g] + kDown - 31 - kMostUnit));
       if (cnt < TP) {
@@ -753,12 +758,12 @@ __global__ void __launch_bounds__(kThreads, Cfg<W, G>::kCtas) kv4_attn_kernel(At
 #pragma unroll
         for (int g = 0; g < G; g++) {
           l[g] += tl[g];
-          z[g] += tz[g];
+          z[g] = fmaf(tz[g], exp2i(-spare), z[g]);
 #pragma unroll
           for (int x = 4; x < 32; x <<= 1) most[g] = fmaxf(most[g], __shfl_xor_sync(0xffffffffu, most[g], x));
-          const int ex = min(254, max(44, (int)(__float_as_uint(most[g] * 1.004f) >> 23)));
+          const int ex = min(252, max(31, (int)(__float_as_uint(most[g] * 1.004f) >> 23)));
           up[g] = __uint_as_float((uint32_t)((G == 1 ? 284 : 276) - ex) << 23);
-          down[g] = __uint_as_float((uint32_t)(ex - 34) << 23);      // (a sixteenth for middle()'s 16)
+          down[g] = __uint_as_float((uint32_t)(ex + kDown - 34 - spare) << 23);      // (a sixteenth for middle()'s 16)
         }
 #pragma unroll
         for (int k = 0; k < KS; k++) {
@@ -810,7 +815,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<W, G>::kCtas) kv4_attn_kernel(At
           for (int x = 0; x < 2; x++)
 #pragma unroll
             for (int e = 0; e < 2; e++) {
-              const float v = total<G, 0>(acc[g][x][2 * e], acc[g][x][2 * e + 1], low[x][2 * e + (G == 1 ? 0 : g)], low[x][2 * e + 1]);
+              const float v = total<G>(acc[g][x][2 * e], acc[g][x][2 * e + 1], low[x][2 * e + (G == 1 ? 0 : g)], low[x][2 * e + 1]);
               o[g][4 * u + 2 * x + e] = fmaf(v, down[g], o[g][4 * u + 2 * x + e]);
             }
       }
@@ -834,7 +839,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<W, G>::kCtas) kv4_attn_kernel(At
       for (int i = 0; i < W; i++)
         *reinterpret_cast<float4 *>(mine + 32 * i + 4 * r) =
             make_float4(o[g][4 * i] + z[g], o[g][4 * i + 1] + z[g], o[g][4 * i + 2] + z[g], o[g][4 * i + 3] + z[g]);
-      if (r == 0) *reinterpret_cast<float2 *>(mine + dP) = make_float2(m[g] * unit(g), l[g]);   // log2 units from here on
+      if (r == 0) *reinterpret_cast<float2 *>(mine + dP) = make_float2(m[g] * unit(g), l[g] * exp2i(-spare));   // log2 units from here on
     }
     __syncthreads();
     const bool whole = a.whole || (t0 == 0 && t1 == at.tiles);
@@ -1062,7 +1067,7 @@ __global__ void __launch_bounds__(kFinishThreads) kv4_attn_finish_kernel(AttnArg
     }
     if (lane == 0) {
       m_s[hd] = x.x;
-      il_s[hd] = 1.f / x.y;
+      il_s[hd] = exp2i(-spare_of((int)n)) / x.y;      // (l is kept as o is)
     }
   }
   __syncthreads();

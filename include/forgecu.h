@@ -530,7 +530,8 @@ int64_t fcu_kv4_attn_work(fcu_ctx *ctx, const fcu_kv4 *cache, int B, int nH);
  * slot's weight grows by its p summed over the q heads of its kv head; sequences
  * may then share no block among their first seq_lens slots.  Finite q and rows may
  * have any size that leaves |scale q_e k^_e| summed over e below 2^127 (a head past
- * that is NaN where its scores leave fp32).  nH / nKV <= 16, B at
+ * that is NaN where its scores leave fp32), rows of v up to 2^122; below 2^-80
+ * an output's error is absolute, 2^-100.  nH / nKV <= 16, B at
  * most 65535, out overlaps no part of q.  `work` is the caller's (fcu_kv4_attn_work bytes, 16-byte
  * aligned) and may be reused once the call's work on the stream is done: two
  * calls that may run at the same time, or graphs of them, have one each. */

@@ -270,6 +270,26 @@ def test_attention_with_queries_whose_sum_leaves_fp32():
     check_attention(c, q * np.float32(2.0 ** 100), [200, 77], scale=2.0 ** 8)
 
 
+@pytest.mark.parametrize("nH,dH,n", [(4, 64, 200), (8, 128, 3000), (1, 16, 70001)])
+def test_attention_over_values_near_the_largest(nH, dH, n):
+    """Values near 2^122 under weights that are nearly equal: their mean is in the type,
+    their sum is not; with small ones beside them."""
+    seen = []
+
+    def rows(x, rng):
+        if seen:
+            x[:] = 2.0 ** 122 * (0.8 + 0.19 * rng.random(x.shape))
+            x[:, :, 3::5] *= -0.5
+            x[:, :, 4::7] *= 2.0 ** -110
+        else:
+            x *= 0.05
+        seen.append(1)
+    c = Cache(2, n, 1, dH, 0, seed=22, rows=rows)
+    q = np.random.default_rng(23).standard_normal((2, nH, dH)).astype(np.float32)
+    check_attention(c, q, [n, n // 3], weight=np.zeros((2, 1, n), np.float32))
+    check_attention(c, q, [n, 1])
+
+
 def test_slots_past_the_length_are_not_read():
     c = Cache(3, 256, 2, 64, 32, seed=4)
     lens = [100, 0, 33]
