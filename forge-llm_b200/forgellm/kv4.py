@@ -379,7 +379,8 @@ class QuantKVCache(KVCache):
     `table` and `physBlocks` as in PagedKVCache).  Transformer.forward and
     forwardBatch take it in their place.  track=True keeps every slot's attention
     weight and position, which evict() goes by; after an eviction a position no
-    longer names its slot: sequence b's next token goes to slot lens[b]."""
+    longer names its slot: sequence b's next token goes to slot lens[b], and only
+    tokens that came after it may be written again."""
 
     def __init__(self, nLayers: int, maxSeq: int, nKvHeads: int, dHead: int, batch: int = 1,
                  blockSize: int | None = None, table=None, physBlocks: int | None = None, track: bool = False):
@@ -413,16 +414,20 @@ class QuantKVCache(KVCache):
         self.len = 0
         self.lens = np.zeros(self.batch, np.int32)       # slots in use
         self.dropped = np.zeros(self.batch, np.int32)    # tokens evicted so far
+        self.kept = np.zeros(self.batch, np.int32)       # slots that the last eviction left, in no order of position
 
     def slotOf(self, pos: int, seq: int = 0) -> int:
-        """The slot that position `pos` of a sequence is written to: its next one
-        or, while nothing was evicted, any."""
+        """The slot that position `pos` of a sequence is written to: its next one, one
+        written since the last eviction or, while nothing was evicted, any."""
         s = int(pos) - int(self.dropped[seq])
         if s < 0 or s >= self.max_blocks * self.block_size:
             raise ValueError(f"QuantKVCache: no slot for position {pos} ({self.dropped[seq]} tokens evicted, "
                              f"{self.max_blocks * self.block_size} slots)")
-        if self.dropped[seq] and s < self.lens[seq]:
+        if self.dropped[seq] and s < self.kept[seq]:
             raise ValueError(f"QuantKVCache: position {pos} may have been evicted")
+        if self.dropped[seq] and s > self.lens[seq]:
+            raise ValueError(f"QuantKVCache: position {pos} is not next ({self.lens[seq] + self.dropped[seq]} is), and "
+                             "the slots between hold evicted tokens")
         return s
 
     def _used(self, seq: int, slot: int) -> None:
@@ -486,6 +491,7 @@ class QuantKVCache(KVCache):
         lens = torch.from_numpy(self.lens.copy()).to(self.k.device)
         kv4Evict(self.k, self.kg, self.v, self.vg, self.weight, self.pos, lens, budget, recent, table=self.table)
         new = np.minimum(self.lens, budget).astype(np.int32)
+        self.kept = np.where(new < self.lens, new, self.kept)
         self.dropped += self.lens - new
         self.lens, self.len = new, int(new.max())
 
@@ -497,7 +503,7 @@ class QuantKVCache(KVCache):
         _reorder(self, [t for t in (self.k, self.kg, self.v, self.vg, self.weight, self.pos) if t is not None], p,
                  self.lens)
         src = (np.arange(p.shape[0])[:, None] * p.shape[1] + p).reshape(-1)
-        self.lens, self.dropped = self.lens[src].copy(), self.dropped[src].copy()
+        self.lens, self.dropped, self.kept = self.lens[src].copy(), self.dropped[src].copy(), self.kept[src].copy()
         self.len = int(self.lens.max(initial=0))
 
     def bytes(self) -> int:

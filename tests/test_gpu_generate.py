@@ -315,6 +315,43 @@ def test_put_writes_a_row_of_one_sequence(model):
     assert int(c.pos[1, 2 * 4 + 1, 0, 1]) == 9 and int((c.pos != 0).sum()) == 2
 
 
+def test_put_after_an_eviction():
+    """Rows put layer by layer go on after an eviction: every layer's row of a new
+    position goes to one slot, a position since then may be put again, an evicted
+    one and one that would leave stale slots between may not."""
+    c = F().QuantKVCache(3, 32, 2, 64, batch=2, blockSize=8, track=True)
+    rng = np.random.default_rng(2)
+    rows = rng.standard_normal((30, 3, 2, 128)).astype(np.float32)
+    put = lambda p: [c.put(l, p, *rows[p, l], seq=1) for l in range(3)]  # noqa: E731
+    for p in range(20):
+        put(p)
+    c.evict(6, 6)                             # the newest six stay
+    assert c.lens.tolist() == [0, 6] and c.dropped.tolist() == [0, 14]
+    for p in (20, 21, 21, 20, 22):
+        put(p)
+    assert c.lens.tolist() == [0, 9] and c.len == 9
+    blk = torch.arange(4, 8, device="cuda")
+    pos = c.pos[:, blk].movedim(2, 1).flatten(2)[:, :, :9].cpu().numpy()      # [layers, heads, slots]
+    assert (np.sort(pos, -1) == np.arange(14, 23)).all() and (pos[:, :, 6:] == [20, 21, 22]).all()
+    for l in range(3):
+        for p, slot in ((20, 6), (21, 7), (22, 8)):
+            want = R.values(*R.quantize(rows[p, l, 0].reshape(2, 64))).ravel()
+            assert np.array_equal(c.sliceK(l, slot, 1).cpu().numpy(), want)
+    for p in (0, 13, 19, 24, 29):
+        with pytest.raises(ValueError):
+            c.put(0, p, *rows[p, 0], seq=1)
+    c.reorder([[1, 1]])
+    put(23)
+    c.put(0, 22, *rows[22, 0], seq=0)
+    for p in (19, 24):
+        with pytest.raises(ValueError):
+            c.put(0, p, *rows[p, 0], seq=0)
+    assert c.lens.tolist() == [9, 10]
+    c.reset()
+    put(3)
+    assert c.lens.tolist() == [0, 4]
+
+
 def reference_search(tr, cfg, prompt, W, n, eos, cache_of):
     """Beam search that recomputes every hypothesis from its tokens."""
     def logits_of(text):
