@@ -49,20 +49,40 @@ def _need(ok, what: str) -> None:
 class _Contexts(threading.local):
     """This thread's contexts by device.  (The package's own is one per device: a
     thread that binds it to its stream would take along a call that another has
-    begun, and the kernels of one call would run on two streams.)"""
+    begun, and the kernels of one call would run on two streams.)  A thread that
+    ends leaves them to the next one that needs some, so there are as many as
+    threads have been in these calls at once."""
 
     def __init__(self):
-        self.of = {}
+        self.of = _Held()
 
 
+class _Held(dict):
+    def __del__(self):
+        if _FREE is not None:           # (the interpreter is not on its way out)
+            for dev, c in self.items():
+                _FREE.setdefault(dev, []).append(c)
+
+
+_FREE: dict = {}                        # contexts of no thread, by device
 _CONTEXTS = _Contexts()
+
+
+def _context(dev: int):
+    """A context of device `dev` that no thread holds.  (No lock: a collection that
+    ends another thread's dict may run inside any of these operations, and each of
+    them is one step to other threads.)"""
+    try:
+        return _FREE[dev].pop()
+    except (KeyError, IndexError):
+        return Context(dev)
 
 
 def _on(dev: int):
     """This thread's fcu_ctx of the current device `dev`, bound to its current stream."""
     c = _CONTEXTS.of.get(dev)
     if c is None:
-        c = _CONTEXTS.of[dev] = Context(dev)
+        c = _CONTEXTS.of[dev] = _context(dev)
     c.bind_stream(torch._C._cuda_getCurrentRawStream(dev))
     return c.handle
 

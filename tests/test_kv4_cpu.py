@@ -181,6 +181,61 @@ def test_every_thread_has_a_context_of_its_own(monkeypatch):
     assert len({id(h) for s in seen.values() for h in s[:3]}) == 6
 
 
+def test_a_finished_threads_contexts_are_used_again(monkeypatch):
+    """Many short threads make as many contexts as are held at once, each bound to its
+    holder's stream."""
+    torch = pytest.importorskip("torch")
+    import gc
+    import threading
+    from forgellm import kv4
+
+    class Fake:
+        made = []
+
+        def __init__(self, device):
+            self.handle, self.stream, self.device = object(), None, device
+            self.made.append(self)
+
+        def bind_stream(self, s):
+            self.stream = s
+
+    streams = threading.local()
+    monkeypatch.setattr(kv4, "Context", Fake)
+    monkeypatch.setattr(kv4, "_FREE", {}, raising=False)
+    monkeypatch.setattr(kv4, "_CONTEXTS", kv4._Contexts())
+    monkeypatch.setattr(torch._C, "_cuda_getCurrentRawStream", lambda d: streams.now, raising=False)
+    wrong = []
+
+    def work(i, gate=None):
+        streams.now = i
+        for dev in (0, 1, 0):
+            h = kv4._on(dev)
+            c = kv4._CONTEXTS.of[dev]
+            if c.handle is not h or c.stream != i or c.device != dev:
+                wrong.append(i)
+            if gate:
+                gate.wait(10)
+                if c.stream != i:
+                    wrong.append(i)
+
+    def run(n, gate=None):
+        threads = [threading.Thread(target=work, args=(i, gate)) for i in range(n)]
+        for t in threads:
+            t.start()
+        for t in threads:
+            t.join()
+        gc.collect()
+
+    for _ in range(20):
+        run(1)
+    assert len(Fake.made) == 2 and not wrong
+    run(5, threading.Barrier(5))
+    assert len(Fake.made) == 10 and not wrong
+    for _ in range(10):
+        run(5)
+    assert len(Fake.made) == 10 and not wrong
+
+
 # ------------------------------------------------------------------ the restatements themselves
 def test_reference_quantizer_bound():
     """|x - x^| <= step / 2 inside the grid; the ends add the roundings of base and
