@@ -242,9 +242,9 @@ __global__ void __launch_bounds__(kPutThreads, 4) kv4_put_kernel(PutArgs a) {
       const float base = __bfloat162float(base_b);
       // step = bf16(fp32((hi - base) / 15)): the product below is within 4 units
       // of its last place of that fp32 value, so it rounds to the same bf16 unless
-      // it is that near the middle of two
+      // it is that near the middle of two (or hi - base near the ends of fp32)
       float q15 = fmaxf(hi - base, 0.f) * (1.0f / 15.0f);
-      if (abs((int)(__float_as_uint(q15) & 0xffffu) - 0x8000) <= 16 || q15 < 1e-30f) {
+      if (abs((int)(__float_as_uint(q15) & 0xffffu) - 0x8000) <= 16 || !(q15 >= 1e-30f && q15 < 0x1p123f)) {
         const double range = (double)hi - (double)base;
         q15 = (float)((range > 0 ? range : 0.0) / 15.0);
       }

@@ -503,6 +503,28 @@ def test_put_of_unusual_rows():
     assert np.array_equal(V.cpu().numpy()[:, 0, 0], want[::-1], equal_nan=True)
 
 
+def test_put_of_rows_as_wide_as_the_cache_takes():
+    """From just above -2^127 to just below 2^127: the difference of the ends rounds to
+    2^128 in fp32, the grid's step is finite."""
+    fw = F()
+    dH, top = 32, np.nextafter(np.float32(2.0 ** 127), np.float32(0))
+    rows = (np.random.default_rng(3).uniform(-1, 1, (6, dH)) * 2.0 ** 126).astype(np.float32)
+    for i, (lo, hi) in enumerate(((-top, top), (-top, 0), (0, top), (-top * 0.99, top), (-top, top * 0.99), (-2.0 ** 126, top))):
+        rows[i, 5], rows[i, 9] = lo, hi
+    n = len(rows)
+    k = torch.zeros(n, 1, 1, 16, dtype=U8, device="cuda")
+    kg = torch.zeros(n, 1, 1, 2, dtype=BF, device="cuda")
+    v, vg = torch.zeros_like(k), torch.zeros_like(kg)
+    z = torch.zeros(n, dtype=I32, device="cuda")
+    fw.kv4Put(dev(np.concatenate([rows, rows], 1)), 0, z, z, k, kg, v, vg, theta=0.0)
+    K, _ = fw.kv4Values(k, kg, v, vg, dH, z, 1)
+    code, step, base = R.quantize(rows)
+    assert np.isfinite(step).all()
+    assert np.array_equal(k.cpu().numpy()[:, 0, 0], R.pack(code, 16))
+    with np.errstate(over="ignore"):
+        assert np.array_equal(K.cpu().numpy()[:, 0, 0], R.values(code, step, base))
+
+
 def test_put_outside_the_cache_changes_nothing():
     fw = F()
     x, c, _, _, d = put_case(5, 2, 2, 2, 64, 16, 1e4, seed=4)
