@@ -948,7 +948,7 @@ __global__ void __launch_bounds__(kFinishThreads) kv4_attn_finish_kernel(AttnArg
     const int run0 = (int)blockIdx.x - lane;
     if (lane < kMaxHeads && run0 >= 0) cut = a.cuts[run0];
     // (nothing is written elsewhere whatever another call made of the workspace)
-    if (cut.heads < 0 || cut.heads > kMaxHeads || cut.bh < 0 || cut.bh + cut.heads > a.B * a.nH) cut.pieces = 0;
+    if (cut.heads < 0 || cut.heads > kMaxHeads || cut.bh < 0 || cut.bh + cut.heads > (int64_t)a.B * a.nH) cut.pieces = 0;
     const bool mine = lane == 0 ? cut.pieces > 0 : cut.pieces > kFewPieces && lane < cut.heads;
     const uint32_t who = __ballot_sync(0xffffffffu, mine);
     if (!who) return;

@@ -371,6 +371,30 @@ def test_attention_past_four_gigabytes_of_codes():
     check_attention(c, q, [1000], got=got)
 
 
+def test_attention_of_more_heads_than_an_int_counts():
+    """65535 sequences of 32784 q heads of 2 (2^31 of them and more, 17 GB of q), all
+    but the first empty, whose segments the runs' ends cut."""
+    B, nKV, dH, n = 65535, 2049, 2, 13 * 128
+    c = Cache(1, n, nKV, dH, n, seed=24, shuffle=False)
+    nH = 16 * nKV
+    q = torch.zeros(B, nH, dH, device="cuda")
+    q0 = np.random.default_rng(25).standard_normal((nH, dH)).astype(np.float32)
+    q[0] = dev(q0)
+    lens = torch.zeros(B, dtype=I32, device="cuda")
+    lens[0] = n
+    out = torch.full((B, nH, dH), float("nan"), device="cuda")
+    F().kv4Attention(q, *c.args(), lens, table=torch.zeros(B, 1, dtype=I32, device="cuda"), out=out)
+    got = out[0].cpu().numpy()
+    assert float(out[1:].abs().max()) == 0
+    K, V = [np.stack([c.rows(w, 0, h, n) for h in range(nKV)]) for w in range(2)]
+    s = np.einsum("hgd,hnd->hgn", q0.reshape(nKV, 16, dH).astype(np.float64), K) / math.sqrt(dH)
+    p = np.exp(s - s.max(-1, keepdims=True))
+    want = np.einsum("hgn,hnd->hgd", p / p.sum(-1, keepdims=True), V).reshape(nH, dH)
+    assert np.abs(got - want).max() <= tolerance(c, q0[None], 1 / math.sqrt(dH))
+    del q, out
+    torch.cuda.empty_cache()
+
+
 def test_a_long_sequence():
     c = Cache(1, 70001, 1, 32, 0, seed=8)
     q = np.random.default_rng(10).standard_normal((1, 4, 32)).astype(np.float32)
