@@ -251,7 +251,7 @@ class Transformer:
                 wqkv=self._ql(L["wqkv"], c.qkvOut, c.dim), wo=self._ql(L["wo"], c.dim, c.dim),
                 gate=self._ql(L["ffn_gate"], c.hidden, c.dim), up=self._ql(L["ffn_up"], c.hidden, c.dim),
                 down=self._ql(L["ffn_down"], c.dim, c.hidden)))
-        self._bufs = {}
+        self._bufs, self._graphs = {}, {}       # (a graph holds the weights and buffers that it was captured with)
         return self
 
     def _buffers(self, B):
@@ -305,7 +305,7 @@ class Transformer:
             return self._step(B, cache)
         from ._lib import lib
         import ctypes
-        graphs = self.__dict__.setdefault("_graphs", {})
+        graphs = self._graphs
         key = (B, id(cache))
         scr = ctypes.c_size_t(0)
         lib().fcu_ctx_scratch_bytes(ctx().handle, ctypes.byref(scr))

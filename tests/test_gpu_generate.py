@@ -428,6 +428,24 @@ def test_search_with_eviction(model):
     assert np.isfinite(w) and w > 0
 
 
+def test_weights_loaded_again(model):
+    """Graphs of a step go with the weights that they were captured with."""
+    from forgellm.train import init_weights_flat
+    import oracle as O
+    cfg, _ = model
+    fw = F()
+    ocfg = O.Config(**{k: v for k, v in CFG.items() if k != "maxSeq"})
+    tr = fw.Transformer(cfg)
+    c = fw.QuantKVCache(cfg.nLayers, 32, cfg.nKvHeads, cfg.dHead, batch=2)
+    for seed in (11, 12):
+        tr.loadWeights(O.unflatten_weights(ocfg, init_weights_flat(cfg, seed)))
+        out = []
+        for graph in (True, False):
+            c.reset()
+            out.append(torch.stack([tr.forwardBatch([3 + p, 40 - p], [p, p], c, graph=graph).clone() for p in range(4)]))
+        assert torch.equal(*out), seed
+
+
 def test_reorder_of_a_paged_cache_with_spare_blocks():
     """Without a table the beams' blocks are the first of a larger pool."""
     fw = F()
