@@ -22,10 +22,10 @@ namespace {
 // log-sum-exp and picks the W best of the W rows' W best.  Within a row the
 // candidates order as the logits do, so W per slice are enough (a row whose scores
 // tie past its W-th best logit is read once more).  The bound is
-// reading the logits (HBM): 32 x 8 rows of 100003, 102 MB, take 34 us, 27 of
-// them beam_rows (3.8 TB/s, issue slots 55 % busy; 43 us with sorted lists kept
-// in registers, a bound per warp; 38 with three tiles of a warp in shared memory
-// in place of one ahead in registers); 4 rows of 32000 take 10 us, all latency.
+// reading the logits (HBM): 32 x 8 rows of 100003, 102 MB, take 30 us, 27 of
+// them beam_rows (3.8 TB/s, issue slots 58 % busy; 9 us more with sorted lists kept
+// in registers, a bound per warp; 4 more with three tiles of a warp in shared memory
+// in place of one ahead in registers); 4 rows of 32000 take 9 us, all latency.
 constexpr int kBeamThreads = 256;
 constexpr int kBeamWarps = kBeamThreads / 32;
 constexpr int kMaxW = 32;
@@ -298,9 +298,9 @@ __global__ void __launch_bounds__(kBeamThreads) beam_merge_kernel(BeamArgs a) {
   __syncthreads();
   // A row's W best of its slices' sorted lists.  Few lists: a key's rank is its
   // own place plus what every other list has above it.  Many: W times the largest
-  // of their heads, of which a lane has up to two.  (Whole steps: 2
-  // lists of 8 34.2 us by rank, 36.9 by heads; 2 of 32 79.5 and 98.5; 16 of 4 12.3
-  // and 10.3.)
+  // of their heads, of which a lane has up to two.  (Whole steps by rank and by heads:
+  // 2 lists of 8 29.7 and 31.7 us, 2 of 32 71.0 and 86.9; 5 of 8 14.8 and 12.5, 8 of 32
+  // 168 and 45.8, 16 of 4 10.9 and 8.8.)
   if (a.slices <= 2) {
     for (int i = tid; i < N; i += kBeamThreads) {
       const int w = i / per, mine = (i - w * per) / W;
@@ -424,8 +424,9 @@ __global__ void __launch_bounds__(kBeamThreads) beam_merge_kernel(BeamArgs a) {
   }
 }
 
-// Slices per row: enough warps for about 24 on each SM, none of them with less
-// than a tile, and few enough that the merge ranks at most 256 survivors a row.
+// Slices per row: enough warps for about 24 on each SM; of more than 1024 logits each
+// (about 2048 in long rows), so that three or four of a CTA's eight warps have a tile at
+// least; and few enough that the merge ranks at most 256 survivors a row.
 int beam_slices(int num_sms, int B, int W, int64_t V) {
   const int64_t rows = (int64_t)B * W > 0 ? (int64_t)B * W : 1;
   int64_t s = ((int64_t)num_sms * 24 / kBeamWarps + rows - 1) / rows;
@@ -462,7 +463,8 @@ __device__ __forceinline__ void re_load(uint32_t dst, const uint8_t *src, int n,
   if (wide && n == 16) {
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src));
   } else {
-    for (int i = 0; i < n; i += 4) asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(dst + i), "l"(src + i));
+    for (int i = 0; i < n; i += 4)
+      asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(dst + i), "l"(src + i));
   }
 }
 __device__ __forceinline__ void re_store(uint8_t *dst, const uint4 *src, int n, bool wide) {
@@ -646,7 +648,8 @@ int fcu_cache_reorder(fcu_ctx *ctx, const fcu_cache_array *arrays, int n_arrays,
   const int depth = W <= 4 ? 4 : W <= 8 ? 2 : 1;
   int64_t most = 0;
   for (int i = 0; i < n_arrays; i++) {
-    FCU_REQUIRE(arrays[i].base && ((uintptr_t)arrays[i].base & 15) == 0, "fcu_cache_reorder: array %d is null or not 16-byte aligned", i);
+    FCU_REQUIRE(arrays[i].base && ((uintptr_t)arrays[i].base & 15) == 0,
+                "fcu_cache_reorder: array %d is null or not 16-byte aligned", i);
     FCU_REQUIRE(arrays[i].heads > 0 && arrays[i].heads <= 65535 && arrays[i].unit > 0 && arrays[i].unit % 4 == 0 &&
                     arrays[i].unit <= 1 << 24 && (int64_t)block_size * arrays[i].unit <= (int64_t)1 << 34,
                 "fcu_cache_reorder: array %d of %lld heads, %lld bytes a slot", i, (long long)arrays[i].heads,
@@ -658,7 +661,8 @@ int fcu_cache_reorder(fcu_ctx *ctx, const fcu_cache_array *arrays, int n_arrays,
     const double bytes = (double)layers * blocks * block_size;
     for (int j = 0; j < i; j++) {
       const uintptr_t p = (uintptr_t)a.base[i], q = (uintptr_t)a.base[j];
-      FCU_REQUIRE(p < q ? (double)(q - p) >= bytes * a.heads[i] * a.unit[i] : (double)(p - q) >= bytes * a.heads[j] * a.unit[j],
+      const double first = p < q ? bytes * a.heads[i] * a.unit[i] : bytes * a.heads[j] * a.unit[j];
+      FCU_REQUIRE((double)(p < q ? q - p : p - q) >= first,
                   "fcu_cache_reorder: arrays %d and %d overlap", j, i);
     }
     const int64_t chunk = 512 * depth, steps = ((int64_t)block_size * arrays[i].unit + chunk - 1) / chunk;
@@ -688,7 +692,8 @@ int fcu_cache_reorder(fcu_ctx *ctx, const fcu_cache_array *arrays, int n_arrays,
                                         kMaxW * kReThreads * 16));
     set[ctx->device & 63] = true;
   }
-  void (*kernel)(ReArgs) = depth == 4 ? cache_reorder_kernel<4> : depth == 2 ? cache_reorder_kernel<2> : cache_reorder_kernel<1>;
+  void (*kernel)(ReArgs) = cache_reorder_kernel<1>;
+  if (depth > 1) kernel = depth == 4 ? cache_reorder_kernel<4> : cache_reorder_kernel<2>;
   FCU_CHECK_CUDA(launch_pdl(kernel, dim3((unsigned)gx, B, (unsigned)layers), dim3(kReThreads), smem,
                             ctx->stream, a));
   note_launch();

@@ -16,8 +16,8 @@ int view(const char *who, const fcu_kv4 *in, int64_t B, bool need_values, Cache 
               "%s: bad cache geometry", who);
   const int64_t cap = (int64_t)in->max_blocks * in->block_size;
   FCU_REQUIRE(cap <= 1 << 30, "%s: %lld slots per sequence (at most 2^30)", who, (long long)cap);
-  FCU_REQUIRE(in->table || B * in->max_blocks <= in->blocks, "%s: %lld sequences of %d blocks in a cache of %lld blocks",
-              who, (long long)B, in->max_blocks, (long long)in->blocks);
+  FCU_REQUIRE(in->table || B * in->max_blocks <= in->blocks,
+              "%s: %lld sequences of %d blocks in a cache of %lld blocks", who, (long long)B, in->max_blocks, (long long)in->blocks);
   // row indexes, and a row's byte offset, stay far inside 64 bits
   FCU_REQUIRE(in->blocks <= (int64_t)1 << 40 && in->layers <= 1 << 20 &&
                   (double)in->layers * in->blocks * in->n_kv * in->block_size <= 1e15,
@@ -259,7 +259,8 @@ __global__ void __launch_bounds__(kPutThreads, 4) kv4_put_kernel(PutArgs a) {
         float near = 1.f;
 #pragma unroll
         for (int u = 0; u < 8; u++) {
-          const float q = fminf(fmaxf((x[u] - base) * inv, 0.f), 15.f), m = q + 0x1.8p23f;   // m: q rounded, ties to even
+          const float q = fminf(fmaxf((x[u] - base) * inv, 0.f), 15.f);
+          const float m = q + 0x1.8p23f;      // q rounded, ties to even
           near = fminf(near, fabsf(fabsf(q - (m - 0x1.8p23f)) - 0.5f));
           if (e0 + u < dH) word |= (__float_as_uint(m) & 15u) << (4 * u);
         }
@@ -367,8 +368,15 @@ constexpr int kEvWarps = kEvThreads / 32;
 constexpr int kEvBins = 2048;
 constexpr int kEvBatch = 2;                   // loads of a thread in flight, of four slots each where they line up
 constexpr int kEvPieces = 4;
-constexpr int kEvInline = 512;                // moves of one head that the selecting CTA makes itself
-constexpr int kEvFew = kEvThreads;            // keys that are ranked directly
+// Moves of one head that the selecting CTA makes itself.  Calls on 384 heads of 64 cut in
+// half, moves here and in kv4_move_kernel: 300 moves 9.7 and 12.5 us, 500 10.7 and 13.3,
+// 1000 13.5 and 17.2, 2000 17.3 and 23.0 (32 heads of 128, 1000 moves: 8.5 and 10.9).
+// kv4_move_kernel was taken for 512 heads of 128 with 2000 moves each, where a CTA's moves
+// wait for its selection; the limit has room below that.
+constexpr int kEvInline = 512;
+// Keys that are ranked directly, one to a thread at most (64 in place of 512: 512 heads cut
+// from 16001 to 2048 slots 52.9 us, so 51.5; from 4001 to 1000 25.5 and 25.1).
+constexpr int kEvFew = kEvThreads;
 constexpr int kEvSmemSlots = 40 * 1024;   // keys of one head kept in shared memory
 
 struct EvArgs {
@@ -447,9 +455,10 @@ __device__ __forceinline__ void load_slots(T (&x)[G], const T *p, bool on, T oth
 // weights and positions.
 // VEC: four slots of a head are 16 aligned bytes of weight and pos.  CTAS:
 // resident per SM, by registers: 3 while a head's keys are short, since then a
-// few hundred heads run at once (12 x 8 x 4 heads of 1025 slots: 14.3 us, 18.4
-// with 2); with long ones shared memory leaves no more anyway and the registers
-// are worth more (4 x 16 x 8 heads of 16001 slots: 155 us, 177 with 3).
+// few hundred heads run at once (12 x 8 x 4 heads of 1025 slots 9.3 us, 11.7 with 2; of
+// 8000, 17.6 and 20.5; 4 x 16 x 8 heads of 8000 24.7 and 25.6); with long ones shared
+// memory leaves no more anyway and the registers are worth more (4 x 16 x 8 heads of
+// 16001 slots cut to 2048, before the moves had a kernel: 155 us, 177 with 3).
 template <bool SMEM, bool VEC, int CTAS>
 __global__ void __launch_bounds__(kEvThreads, CTAS) kv4_evict_kernel(EvArgs a) {
   pdl_trigger();
@@ -700,7 +709,7 @@ __global__ void __launch_bounds__(kEvThreads, CTAS) kv4_evict_kernel(EvArgs a) {
 // slowest): a warp takes 32 of a head's, a lane finds one's rows, and the lanes
 // then copy the rows' 16-byte pieces side by side.  Sources lie past the budget
 // and destinations below it, so loads may pass stores.  Bound by HBM: 512 heads'
-// 950,000 rows of head dim 128 cut from 16001 to 2048, 80 us at 5.4 TB/s of DRAM
+// 950,000 rows of head dim 128 cut from 16001 to 2048, 75 us at 5.8 TB/s of DRAM
 // traffic, of which 60 % is asked for: a row's four 4-byte fields each pull 64
 // bytes.
 constexpr int kMvThreads = 256;
@@ -887,14 +896,16 @@ int fcu_kv4_evict(fcu_ctx *ctx, const fcu_kv4 *cache, const int32_t *seq_lens, i
     a.from = a.to + heads * w.most;
   }
   const bool vec = a.c.bs % 4 == 0 && (((uintptr_t)a.c.weight | (uintptr_t)a.c.pos) & 15) == 0;
-  void (*kernel)(EvArgs) = w.keys ? (vec ? kv4_evict_kernel<false, true, 2> : kv4_evict_kernel<false, false, 2>)
-                           : a.c.cap <= 8192 ? (vec ? kv4_evict_kernel<true, true, 3> : kv4_evict_kernel<true, false, 3>)
-                                             : (vec ? kv4_evict_kernel<true, true, 2> : kv4_evict_kernel<true, false, 2>);
+  void (*kernel)(EvArgs);
+  if (w.keys) kernel = vec ? kv4_evict_kernel<false, true, 2> : kv4_evict_kernel<false, false, 2>;
+  else if (a.c.cap <= 8192) kernel = vec ? kv4_evict_kernel<true, true, 3> : kv4_evict_kernel<true, false, 3>;
+  else kernel = vec ? kv4_evict_kernel<true, true, 2> : kv4_evict_kernel<true, false, 2>;
   static bool set[64] = {false};
   if (!set[ctx->device & 63]) {
     const int most = ev_at(kEvSmemSlots) * 4;
-    FCU_CHECK_CUDA(cudaFuncSetAttribute(kv4_evict_kernel<true, true, 2>, cudaFuncAttributeMaxDynamicSharedMemorySize, most));
-    FCU_CHECK_CUDA(cudaFuncSetAttribute(kv4_evict_kernel<true, false, 2>, cudaFuncAttributeMaxDynamicSharedMemorySize, most));
+    const cudaFuncAttribute smem = cudaFuncAttributeMaxDynamicSharedMemorySize;
+    FCU_CHECK_CUDA(cudaFuncSetAttribute(kv4_evict_kernel<true, true, 2>, smem, most));
+    FCU_CHECK_CUDA(cudaFuncSetAttribute(kv4_evict_kernel<true, false, 2>, smem, most));
     set[ctx->device & 63] = true;
   }
   const cudaError_t e = launch_pdl(kernel, dim3((unsigned)heads), dim3(kEvThreads),

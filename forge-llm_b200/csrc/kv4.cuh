@@ -2,7 +2,7 @@
 //
 // A row is one kv head of one slot: dH values x as codes c in 0..15 on the
 // row's own grid, x^ = base + step * c (step, base in bf16).  Element e sits in
-// nibble e & 1 of byte e / 2; a row is padded to kv4_pad(dH) elements so that
+// nibble e & 1 of byte e / 2; a row is padded to pad(dH) elements so that
 // it is a whole number of 16-byte units.  Row (layer, block, head, slot in
 // block) has index ((layer * blocks + block) * nKV + head) * block_size + slot:
 // the slots of one head of one block are contiguous, which is what a kernel
@@ -19,8 +19,8 @@ namespace kv4 {
 constexpr int kMaxDh = 256;
 constexpr int kMaxGroup = 16;   // q heads per kv head
 
-// Elements a row of dH values is stored as: the head dims the attention
-// kernel is built for (a quarter warp reads a row as whole 32-bit words).
+// Elements a row of dH values is stored as: the widths that the kernels are built for,
+// whole 16-byte pieces.
 __host__ __device__ inline int pad(int dH) {
   return dH <= 32 ? 32 : dH <= 64 ? 64 : dH <= 96 ? 96 : dH <= 128 ? 128 : dH <= 192 ? 192 : 256;
 }

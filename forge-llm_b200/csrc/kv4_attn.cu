@@ -36,14 +36,15 @@
 // ahead and v as soon as the last one's has been used, so that one part per warp
 // is always on its way and three fit on chip.
 //
-// Measured, whole calls on one B200 (copy rate 6.45 TB/s): 64 sequences of 4096
-// slots, 32 / 8 heads of 128, 61 us = 4.7 TB/s (70 us on pages of 16, 73 of 100;
-// fcu_attn_decode over the fp32 cache 422 us); one sequence of 262000, 12 / 4
-// heads of 64, 24 us = 3.1 TB/s; 16 x 2047 slots, 16 / 16 heads of 80, with
-// weights, 25 us.  No pipe is full: issue 56 % busy (about 960 instructions a tile
-// of 64 slots), ALU pipe 44 %, tensor pipe 29 %, DRAM at 73 % of the copy rate,
-// the same with 11 and with 14 warps per SM; below some 50 MB of cache its two
-// launches and a few microseconds of start and merge.
+// Measured on one B200 (copy rate 6.45 TB/s; replayed): 64 sequences of 4096
+// slots, 32 / 8 heads of 128, 57 us = 5.1 TB/s (68 us on pages of 16, 73 of 100;
+// 8 q heads per kv head 83, 16 146; fcu_attn_decode over the fp32 cache 422 us); one
+// sequence of 262000, 12 / 4 heads of 64, 25 us = 3.0 TB/s; 16 x 2047 slots, 16 / 16
+// heads of 80, with weights, 25 us.  No pipe is full at 64 x 4096: issue 60 % busy
+// (about 1030 instructions a tile of 64 slots), ALU pipe 43 %, tensor pipe 30 %, DRAM at
+// 78 % of the copy rate; 11 and 14 warps per SM took the same time.  What bounds it then
+// is not known.  Below some 50 MB of cache it is two launches and a few microseconds
+// of start and merge.
 #include "kv4.cuh"
 
 namespace fcu {
@@ -351,9 +352,9 @@ __device__ __forceinline__ uint32_t grid_at(int x) {
 // issue() for blocks that sixteen slots may straddle.  (Not inlined, and so the
 // cache's geometry goes by value: a reference would put all of it on the stack.)
 template <class C, int W>
-__device__ __noinline__ void issue_scattered(const int32_t *table, int64_t blocks, int mb, int nKV, int bs, uint32_t div_mul,
-                                             int div_shift, const uint8_t *codes, const uint32_t *grids, int64_t b, int h,
-                                             int j0, int cnt, uint8_t *part) {
+__device__ __noinline__ void issue_scattered(const int32_t *table, int64_t blocks, int mb, int nKV, int bs,
+                                             uint32_t div_mul, int div_shift, const uint8_t *codes,
+                                             const uint32_t *grids, int64_t b, int h, int j0, int cnt, uint8_t *part) {
   Cache c;
   c.table = table, c.blocks = blocks, c.mb = mb, c.nKV = nKV, c.bs = bs, c.div_mul = div_mul, c.div_shift = div_shift;
   const int lane = threadIdx.x & 31;
@@ -369,7 +370,8 @@ __device__ __noinline__ void issue_scattered(const int32_t *table, int64_t block
 #pragma unroll
       for (int i = 0; i < C::kTile * W / 32; i++) {
         const int x = i * 32 + lane;
-        cp_async16(code_s + 16 * (W % 2 == 0 ? x - x % W + (x % W ^ swizzle<W>(x / W)) : x), (x < cut * W ? s0 : s1) + 512 * i, true);
+        cp_async16(code_s + 16 * (W % 2 == 0 ? x - x % W + (x % W ^ swizzle<W>(x / W)) : x),
+                   (x < cut * W ? s0 : s1) + 512 * i, true);
       }
 #pragma unroll
       for (int i = 0; i < C::kTile / 32; i++)
@@ -396,8 +398,8 @@ __device__ __noinline__ void issue_scattered(const int32_t *table, int64_t block
 // have NaN grids.  flat: the row of slot 0 where all slots lie in one block, else
 // -1.
 template <class C, int W>
-__device__ __forceinline__ void issue(const Cache &c, const uint8_t *codes, const uint32_t *grids, int64_t flat, int64_t b,
-                                      int h, int j0, int cnt, uint8_t *part) {
+__device__ __forceinline__ void issue(const Cache &c, const uint8_t *codes, const uint32_t *grids, int64_t flat,
+                                      int64_t b, int h, int j0, int cnt, uint8_t *part) {
   const int lane = threadIdx.x & 31;
   const uint32_t code_s = (uint32_t)__cvta_generic_to_shared(part), grid_s = code_s + C::kCodes;
   int64_t row = flat + j0;             // where a full tile's rows are contiguous; -1: they are not
@@ -426,12 +428,14 @@ __device__ __forceinline__ void issue(const Cache &c, const uint8_t *codes, cons
       const uint8_t *p = codes + first * C::kRow;
 #pragma unroll
       for (int k = 0; k < C::kTile / 16; k++) {
-        const uint8_t *src = reinterpret_cast<const uint8_t *>(__shfl_sync(0xffffffffu, reinterpret_cast<uint64_t>(p), k)) + 16 * lane;
+        const uint64_t at = __shfl_sync(0xffffffffu, reinterpret_cast<uint64_t>(p), k);
+        const uint8_t *src = reinterpret_cast<const uint8_t *>(at) + 16 * lane;
 #pragma unroll
         for (int i = 0; i < (W + 1) / 2; i++) {
           const int x = i * 32 + lane;
           if (32 * i + 32 <= 16 * W || lane < 16)
-            cp_async16(code_s + 16 * (16 * W * k + (W % 2 == 0 ? x - x % W + (x % W ^ swizzle<W>(x / W)) : x)), src + 512 * i, true);
+            cp_async16(code_s + 16 * (16 * W * k + (W % 2 == 0 ? x - x % W + (x % W ^ swizzle<W>(x / W)) : x)),
+                       src + 512 * i, true);
         }
       }
 #pragma unroll
@@ -459,7 +463,8 @@ __device__ __forceinline__ void issue(const Cache &c, const uint8_t *codes, cons
                  on ? codes + row * C::kRow + 16 * (x - (j & ~15) * W) : codes, on);
     }
   } else {
-    issue_scattered<C, W>(c.table, c.blocks, c.mb, c.nKV, c.bs, c.div_mul, c.div_shift, codes, grids, b, h, j0, cnt, part);
+    issue_scattered<C, W>(c.table, c.blocks, c.mb, c.nKV, c.bs, c.div_mul, c.div_shift, codes, grids, b, h, j0, cnt,
+                          part);
   }
 }
 
@@ -477,7 +482,8 @@ __device__ __forceinline__ void ldsm4(uint32_t p, uint32_t &a, uint32_t &b, uint
 template <bool T>
 __device__ __forceinline__ void ldsm2(uint32_t p, uint32_t &a, uint32_t &b) {
   if constexpr (T)
-    asm volatile("ldmatrix.sync.aligned.m8n8.x2.trans.shared.b16 {%0,%1}, [%2];" : "=r"(a), "=r"(b) : "r"(p) : "memory");
+    asm volatile("ldmatrix.sync.aligned.m8n8.x2.trans.shared.b16 {%0,%1}, [%2];"
+                 : "=r"(a), "=r"(b) : "r"(p) : "memory");
   else
     asm volatile("ldmatrix.sync.aligned.m8n8.x2.shared.b16 {%0,%1}, [%2];" : "=r"(a), "=r"(b) : "r"(p) : "memory");
 }
@@ -487,7 +493,8 @@ __device__ __forceinline__ void ldsm2(uint32_t p, uint32_t &a, uint32_t &b) {
 template <int W, bool T>
 __device__ __forceinline__ void rows16(uint32_t codes, const uint32_t (&off)[(W + 1) / 2], int k, uint32_t (&w)[2][W]) {
 #pragma unroll
-  for (int c = 0; c + 1 < W; c += 2) ldsm4<T>(codes + off[c / 2] + 16 * k * 16 * W, w[0][c], w[1][c], w[0][c + 1], w[1][c + 1]);
+  for (int c = 0; c + 1 < W; c += 2)
+    ldsm4<T>(codes + off[c / 2] + 16 * k * 16 * W, w[0][c], w[1][c], w[0][c + 1], w[1][c + 1]);
   if constexpr (W % 2) ldsm2<T>(codes + off[W / 2] + 16 * k * 16 * W, w[0][W - 1], w[1][W - 1]);
 }
 
@@ -590,7 +597,8 @@ __global__ void __launch_bounds__(kThreads, Cfg<W, G>::kCtas) kv4_attn_kernel(At
       for (int i = 0; i < 8 * W; i += 4) {
         const int d = 32 * (i / 8) + 8 * t + i % 8;
         if (a.vec) {
-          const float4 f = head < heads && d < c.dH ? *reinterpret_cast<const float4 *>(q + d) : float4{0.f, 0.f, 0.f, 0.f};
+          float4 f = {0.f, 0.f, 0.f, 0.f};
+          if (head < heads && d < c.dH) f = *reinterpret_cast<const float4 *>(q + d);
           x[i] = f.x, x[i + 1] = f.y, x[i + 2] = f.z, x[i + 3] = f.w;
         } else {
 #pragma unroll
@@ -815,7 +823,8 @@ __global__ void __launch_bounds__(kThreads, Cfg<W, G>::kCtas) kv4_attn_kernel(At
           for (int x = 0; x < 2; x++)
 #pragma unroll
             for (int e = 0; e < 2; e++) {
-              const float v = total<G>(acc[g][x][2 * e], acc[g][x][2 * e + 1], low[x][2 * e + (G == 1 ? 0 : g)], low[x][2 * e + 1]);
+              const float v = total<G>(acc[g][x][2 * e], acc[g][x][2 * e + 1], low[x][2 * e + (G == 1 ? 0 : g)],
+                                       low[x][2 * e + 1]);
               o[g][4 * u + 2 * x + e] = fmaf(v, down[g], o[g][4 * u + 2 * x + e]);
             }
       }
@@ -839,7 +848,8 @@ __global__ void __launch_bounds__(kThreads, Cfg<W, G>::kCtas) kv4_attn_kernel(At
       for (int i = 0; i < W; i++)
         *reinterpret_cast<float4 *>(mine + 32 * i + 4 * r) =
             make_float4(o[g][4 * i] + z[g], o[g][4 * i + 1] + z[g], o[g][4 * i + 2] + z[g], o[g][4 * i + 3] + z[g]);
-      if (r == 0) *reinterpret_cast<float2 *>(mine + dP) = make_float2(m[g] * unit(g), l[g] * exp2i(-spare));   // log2 units from here on
+      // (m in log2 units from here on)
+      if (r == 0) *reinterpret_cast<float2 *>(mine + dP) = make_float2(m[g] * unit(g), l[g] * exp2i(-spare));
     }
     __syncthreads();
     const bool whole = a.whole || (t0 == 0 && t1 == at.tiles);
@@ -931,6 +941,9 @@ struct Pieces {
 // pieces has as many runs to itself, and block i + d takes its d-th head, all
 // warps together.  Where weights are kept the other blocks add them up,
 // weight_j += sum over the group's q heads of p_j, kWtSlots slots each.
+// (kFewPieces is at least kMaxHeads, so that the blocks are the segment's own.  32768
+// slots, a warp to a head and all warps to one: 18 pieces a segment 36.7 and 34.2 us, 37
+// pieces 28.5 and 24.5; 9 pieces 35.4 and 34.8.)
 constexpr int kFewPieces = 12;
 constexpr int kFinishThreads = 256;
 constexpr int kFinishWarps = kFinishThreads / 32;
@@ -948,7 +961,8 @@ __global__ void __launch_bounds__(kFinishThreads) kv4_attn_finish_kernel(AttnArg
     const int run0 = (int)blockIdx.x - lane;
     if (lane < kMaxHeads && run0 >= 0) cut = a.cuts[run0];
     // (nothing is written elsewhere whatever another call made of the workspace)
-    if (cut.heads < 0 || cut.heads > kMaxHeads || cut.bh < 0 || cut.bh + cut.heads > (int64_t)a.B * a.nH) cut.pieces = 0;
+    if (cut.heads < 0 || cut.heads > kMaxHeads || cut.bh < 0 || cut.bh + cut.heads > (int64_t)a.B * a.nH)
+      cut.pieces = 0;
     const bool mine = lane == 0 ? cut.pieces > 0 : cut.pieces > kFewPieces && lane < cut.heads;
     const uint32_t who = __ballot_sync(0xffffffffu, mine);
     if (!who) return;
@@ -1082,7 +1096,8 @@ __global__ void __launch_bounds__(kFinishThreads) kv4_attn_finish_kernel(AttnArg
       }
   }
   if (VEC && row[3] >= 0) {
-    *reinterpret_cast<float4 *>(c.weight + row[0]) = make_float4(old[0] + w[0], old[1] + w[1], old[2] + w[2], old[3] + w[3]);
+    *reinterpret_cast<float4 *>(c.weight + row[0]) =
+        make_float4(old[0] + w[0], old[1] + w[1], old[2] + w[2], old[3] + w[3]);
   } else {
 #pragma unroll
     for (int k = 0; k < kPer; k++)
@@ -1117,8 +1132,10 @@ int checked(const char *who, const fcu_kv4 *cache, int B, int nH, bool arrays, C
 // CTAs of the main kernel: all that are resident, or one per tile if the cache
 // cannot hold that many.  A cache of at most kWholeTiles tiles per sequence
 // whose segments are all resident at once gives each a CTA of its own: its two
-// steps per warp cost less than the second kernel that would merge pieces (one
-// sequence of 37 slots in a cache of 1024: 12 us a call, 18 with the merge).
+// steps per warp cost less than the second kernel that would merge pieces.  (Full caches
+// of 8 tiles, whole and merged: 1 x 1024 slots of 12 / 4 heads of 64 6.1 and 7.1 us, 1 x
+// 512 of 32 / 8 heads of 128 6.4 and 7.3, 16 x 512 9.3 and 10.5, 64 x 512 13.5 and 21.8.
+// Of 16 tiles: 8.7 and 7.1, 9.0 and 8.4, 14.5 and 12.9, but 20.2 and 25.8.)
 constexpr int kWholeTiles = 8;
 template <int W, int G>
 void plan_ctas(const fcu_ctx *ctx, const Cache &c, int B, Heads *p) {
@@ -1139,10 +1156,12 @@ int launch(fcu_ctx *ctx, const AttnArgs &a) {
   }
   FCU_CHECK_CUDA(launch_pdl(kv4_attn_kernel<W, G>, dim3(a.ctas), dim3(kThreads), C::kSmem, ctx->stream, a));
   note_launch();
-  const int64_t blocks = (a.whole ? 0 : a.ctas - 1) + (a.scores ? (int64_t)a.B * a.c.nKV * ((a.c.cap + kWtSlots - 1) / kWtSlots) : 0);
+  const int64_t sums = a.scores ? (int64_t)a.B * a.c.nKV * ((a.c.cap + kWtSlots - 1) / kWtSlots) : 0;
+  const int64_t blocks = (a.whole ? 0 : a.ctas - 1) + sums;
   if (blocks > 0) {
     const bool vec = a.scores && a.c.cap % 4 == 0 && a.c.bs % 4 == 0 && ((uintptr_t)a.c.weight & 15) == 0;
-    FCU_CHECK_CUDA(launch_pdl(vec ? kv4_attn_finish_kernel<W, true> : kv4_attn_finish_kernel<W, false>, dim3((unsigned)blocks), dim3(kFinishThreads), 0, ctx->stream, a));
+    FCU_CHECK_CUDA(launch_pdl(vec ? kv4_attn_finish_kernel<W, true> : kv4_attn_finish_kernel<W, false>,
+                              dim3((unsigned)blocks), dim3(kFinishThreads), 0, ctx->stream, a));
     note_launch();
   }
   return FCU_OK;
@@ -1215,7 +1234,8 @@ int fcu_kv4_attn(fcu_ctx *ctx, const float *q, int64_t ld_q, const fcu_kv4 *cach
   a.vec = ld_q % 4 == 0 && a.c.dH % 4 == 0 && ((uintptr_t)q & 15) == 0;
   a.scale = (float)scale;
   a.out = out;
-  FCU_REQUIRE(!a.c.weight || (double)B * a.c.nKV * (a.c.cap / kWtSlots + 1) < 1e9, "fcu_kv4_attn: the cache is too large");
+  FCU_REQUIRE(!a.c.weight || (double)B * a.c.nKV * (a.c.cap / kWtSlots + 1) < 1e9,
+              "fcu_kv4_attn: the cache is too large");
   const int64_t need = 4 * work_floats(a.c, B, nH, p);
   FCU_REQUIRE(need == 0 || (work && work_bytes >= need && ((uintptr_t)work & 15) == 0),
               "fcu_kv4_attn: workspace of %lld bytes, %lld needed", (long long)work_bytes, (long long)need);

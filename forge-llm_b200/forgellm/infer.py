@@ -224,7 +224,8 @@ class Transformer:
     ffn_up, ffn_down}, optional wcls) with fp32 arrays or QuantLinear values.
     forward(token, pos, cache) is one decode step of one sequence;
     forwardBatch(tokens, positions, cache) steps cache.batch sequences at once
-    (each at its own position) and returns logits [B, vocab]."""
+    (each at its own position) and returns logits [B, vocab].  Steps share the
+    model's buffers: one thread at a time."""
 
     def __init__(self, config):
         from .train import Config

@@ -13,8 +13,10 @@ reference has no counterpart: its caches are fp32 and it samples one sequence.
 
 All tensors are on the current CUDA device and every call runs on its current
 stream.  A call that finds them anywhere else, or of another type, shape or
-stride than it takes, raises ValueError before anything is launched.  Host
-threads may call at the same time, each on streams of its own.
+stride than it takes, raises ValueError before anything is launched, and one
+that the library refuses (head counts, overlapping tensors, sizes past its
+limits) ForgeCUError.  Host threads may call these functions at the same time,
+each on streams of its own; a Transformer's steps are one thread's at a time.
 """
 from __future__ import annotations
 
@@ -255,7 +257,8 @@ def kv4Attention(q, k, kg, v, vg, lens, scale: float | None = None, table=None, 
     0 gives zeros), grouped heads as in attentionDecode.  scale: 1 / sqrt(dHead)
     unless given.  With `weight`, every slot's attention weight, summed over its
     kv head's q heads, is added to it; the sequences may then share no block among
-    those slots.  `out` may not overlap q."""
+    those slots, and the call takes 4 B nHeads (slots of a sequence's blocks) bytes of
+    workspace.  `out` may not overlap q."""
     dev = _device()
     if not (isinstance(q, torch.Tensor) and q.dtype is _F32 and q.ndim == 3):
         raise ValueError("q: a float32 [B, nHeads, dHead] is needed")
@@ -291,7 +294,8 @@ def kv4Evict(k, kg, v, vg, weight, pos, lens, budget: int, recent: int, table=No
     """Cuts every head of every layer (arrays with a leading layer dimension)
     of sequences longer than `budget` down to it: the slots of the `recent`
     newest positions and those of largest weight stay (ties: the lowest slot),
-    moved into the freed slots.  No two sequences may share a block.  Returns the new lengths, min(lens, budget)."""
+    moved into the freed slots.  No two sequences may share a block.  Returns the
+    new lengths, min(lens, budget)."""
     dev = _device()
     _check("lens", lens, _I32, dev)
     B = lens.numel()

@@ -519,9 +519,11 @@ int fcu_kv4_put(fcu_ctx *ctx, float *qkv, int64_t ld_qkv, int B, int T, int nH, 
  * the values of slot start[b] + t of head h.  A slot outside the sequence's
  * capacity gives NaN. */
 int fcu_kv4_values(fcu_ctx *ctx, const fcu_kv4 *cache, const int32_t *start, int B, int T, float *K, float *V);
-/* Bytes of workspace fcu_kv4_attn needs for B sequences of nH q heads (it
- * depends on whether the cache keeps weights); 0 if none, -1 for arguments
- * that fcu_kv4_attn would refuse. */
+/* Bytes of workspace fcu_kv4_attn needs for B sequences of nH q heads; 0 if
+ * none, -1 for arguments that fcu_kv4_attn would refuse.  A few MB for the
+ * pieces of cut segments; where the cache keeps weights, 4 B nH (capacity + 2)
+ * bytes more for the scores: by the sequences' capacity, not their lengths
+ * (64 sequences of 32 heads and 65536 slots: 537 MB). */
 int64_t fcu_kv4_attn_work(fcu_ctx *ctx, const fcu_kv4 *cache, int B, int nH);
 /* out[b, h, :] = sum_j p_j v^_j over slots j < seq_lens[b] (device; clamped to
  * the capacity), p = softmax_j(scale * q_bh . k^_j), kv head h / (nH / nKV):
@@ -532,9 +534,10 @@ int64_t fcu_kv4_attn_work(fcu_ctx *ctx, const fcu_kv4 *cache, int B, int nH);
  * have any size that leaves |scale q_e k^_e| summed over e below 2^127 (a head past
  * that is NaN where its scores leave fp32), rows of v up to 2^122; below 2^-80
  * an output's error is absolute, 2^-100.  nH / nKV <= 16, B at
- * most 65535, out overlaps no part of q.  `work` is the caller's (fcu_kv4_attn_work bytes, 16-byte
- * aligned) and may be reused once the call's work on the stream is done: two
- * calls that may run at the same time, or graphs of them, have one each. */
+ * most 65535, out overlaps no part of q.  `work` is the caller's
+ * (fcu_kv4_attn_work bytes, 16-byte aligned) and may be reused once the call's work
+ * on the stream is done: two calls that may run at the same time, or graphs of
+ * them, have one each. */
 int fcu_kv4_attn(fcu_ctx *ctx, const float *q, int64_t ld_q, const fcu_kv4 *cache, const int32_t *seq_lens, int B,
                  int nH, double scale, float *out, void *work, int64_t work_bytes);
 /* Bytes of workspace fcu_kv4_evict needs; 0 if none, -1 for bad arguments. */
@@ -564,8 +567,9 @@ int64_t fcu_beam_work(fcu_ctx *ctx, int B, int W, int64_t V);
  * is not finite counts as -inf.  The W best, by score and then by lowest
  * w * V + token, give out_scores, tokens, parents (= w) and out_done (ended
  * before, or token is eos), [B, W] each, best first; none of them may overlap
- * another or an input.  1 <= W <= 32, B * W at most 65535, V at most 2^30.  logits may hold -inf (a banned token); a NaN
- * or +inf makes all of its row's candidates -inf. */
+ * another or an input.  1 <= W <= 32, B * W at most 65535, V at most 2^30.  logits
+ * may hold -inf (a banned token); a NaN or +inf makes all of its row's candidates
+ * -inf. */
 int fcu_beam_step(fcu_ctx *ctx, const float *logits, int64_t ld, const float *scores, const uint8_t *done, int B,
                   int W, int64_t V, int eos, float *out_scores, int32_t *tokens, int32_t *parents,
                   uint8_t *out_done, void *work, int64_t work_bytes);
