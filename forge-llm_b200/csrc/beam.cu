@@ -31,7 +31,7 @@ constexpr int kBeamWarps = kBeamThreads / 32;
 constexpr int kMaxW = 32;
 constexpr int kTile = 512;                          // logits a warp takes at a time
 constexpr int kMaxSlices = 64;
-constexpr int kAgain = 8;                           // loads in flight of a lane that reads a tied row again
+constexpr int kAgain = 32;                          // loads in flight of a lane that reads a tied row again
 constexpr int kFound = 64;                          // tokens a warp lists: kMaxW and 32 more at least
 constexpr float kLog2e = 1.4426950408889634f;
 
@@ -277,6 +277,7 @@ __global__ void __launch_bounds__(kBeamThreads) beam_merge_kernel(BeamArgs a) {
   __shared__ float top_s[kMaxW];                       // a row's largest logit
   __shared__ double log_s[kMaxW];                      // and the log of its sum of exp(x - the largest)
   __shared__ bool tied[kMaxW];                         // a logit below the W-th best scores what that one does
+  __shared__ int again[kBeamWarps][kMaxW], agains[kBeamWarps];
   const int tid = threadIdx.x, lane = tid & 31, W = a.W, per = a.slices * W, N = W * per;
   const int64_t b = blockIdx.x;
   for (int i = tid; i < W * W; i += kBeamThreads) best[i / W][i % W] = 0;
@@ -359,30 +360,56 @@ __global__ void __launch_bounds__(kBeamThreads) beam_merge_kernel(BeamArgs a) {
   // Where the beam's score or its log-sum-exp swallows the difference of two logits
   // (a score of -1e30, logits of 1e-20), tokens that the row's W best logits do not
   // hold may tie with the last of those: the lowest of all that score as it does
-  // take its place and those of its equals in the list.
-  for (int w = tid >> 5; w < W; w += kBeamWarps) {
-    if (!tied[w]) continue;
+  // take its place and those of its equals in the list, if any of those are chosen.  A
+  // warp looks through an eighth of the row.  (One beam over logits less their maximum,
+  // whose best is 0, is such a row: 32 x 1 x 100003 42 us, 11 without, 196 with one warp
+  // to a row; 1 x 1 x 32000 13.7, 6.9 and 30.7.)
+  for (uint32_t m = __ballot_sync(0xffffffffu, lane < W && tied[lane]); m; m &= m - 1) {
+    const int w = __ffs(m) - 1;
+    const double last = score[w][W - 1];
+    int above = 0;                                     // candidates before the first of them
+    for (int i0 = 0; i0 < W * W; i0 += kBeamThreads) {
+      const int i = i0 + tid, x = i / W;
+      above += __syncthreads_count(i < W * W && token[x][i % W] >= 0 &&
+                                   (score[x][i % W] > last || (score[x][i % W] == last && x < w)));
+    }
+    if (above >= W) continue;                          // none of them is chosen
     const float *x = a.logits + (b * W + w) * a.ld;
-    const double cum = a.scores[b * W + w], last = score[w][W - 1];
-    int at = __popc(__ballot_sync(0xffffffffu, lane < W && score[w][lane] > last));
-    for (int t0 = 0; t0 < a.V && at < W; t0 += 32 * kAgain) {
+    const double cum = a.scores[b * W + w];
+    const int first = __popc(__ballot_sync(0xffffffffu, lane < W && score[w][lane < W ? lane : 0] > last));
+    // no logit below `low` scores `last`: value() rounds by far less than 2^-50 of its terms
+    const float best_w = key_logit(best[w][W - 1]);
+    const double off = 0x1p-50 * (fabs(cum) + fabs((double)top_s[w]) + fabs((double)best_w) + fabs(log_s[w]));
+    const float low = __double2float_rd((double)best_w - off);
+    const int part = (a.V + kBeamWarps - 1) / kBeamWarps, v0 = (tid >> 5) * part, v1 = min(a.V, v0 + part);
+    int n = 0;
+    for (int t0 = v0; t0 < v1 && n < W - first; t0 += 32 * kAgain) {
       float f[kAgain];
 #pragma unroll
       for (int i = 0; i < kAgain; i++) {
         const int t = t0 + 32 * i + lane;
-        f[i] = t < a.V ? x[t] : -INFINITY;
+        f[i] = t < v1 ? x[t] : -INFINITY;
       }
+      bool any = false;
+#pragma unroll
+      for (int i = 0; i < kAgain; i++) any |= f[i] >= low;
+      if (!__any_sync(0xffffffffu, any)) continue;
 #pragma unroll
       for (int i = 0; i < kAgain; i++) {
-        const bool hit = value(w, cum, f[i]) == last;
+        const bool hit = f[i] >= low && value(w, cum, f[i]) == last;
         const uint32_t who = __ballot_sync(0xffffffffu, hit);
-        const int place = at + __popc(who & ((1u << lane) - 1));
-        if (hit && place < W) token[w][place] = t0 + 32 * i + lane;
-        at += __popc(who);
+        const int place = n + __popc(who & ((1u << lane) - 1));
+        if (hit && place < W - first) again[tid >> 5][place] = t0 + 32 * i + lane;
+        n += __popc(who);
       }
     }
+    if (lane == 0) agains[tid >> 5] = min(n, W - first);
+    __syncthreads();
+    int at = first;
+    for (int i = 0; i < (tid >> 5); i++) at += agains[i];
+    if (lane < agains[tid >> 5] && at + lane < W) token[w][at + lane] = again[tid >> 5][lane];
+    __syncthreads();
   }
-  __syncthreads();
   // A row's scores fall as its logits do, but where the beam's score swallows the
   // difference of two logits they tie, and the lower token is first.  (Those of
   // -inf are in order: equal logits or none.)

@@ -188,6 +188,27 @@ def test_beam_step_ties_that_doubles_make():
         check_beam(x, scores, d, 1)
 
 
+@pytest.mark.parametrize("W", [1, 4, 9])
+@pytest.mark.parametrize("V", [40, 3001, 20000])
+def test_beam_step_ties_spread_over_a_row(W, V):
+    """A few tokens that tie in double lie anywhere in a row, the largest of them last;
+    some larger ones are before them; other beams take all or a part of the places."""
+    rng = np.random.default_rng(100 * W + V)
+    B = 12
+    x = (-4 - rng.random((B, W, V))).astype(np.float32)
+    for b in range(B):
+        for w in range(W):
+            at = np.sort(rng.choice(V, 14, replace=False))
+            x[b, w, at] = np.arange(1, 15, dtype=np.float32) * np.float32(1e-21)      # rises with the token
+            larger = b % 4
+            x[b, w, rng.choice(at, larger, replace=False)] = 1 + np.arange(larger)
+    x[7] -= x[7].max(-1, keepdims=True)
+    scores = np.where(np.arange(B)[:, None] % 3 == 0, -np.arange(W) * 0.01, -np.arange(W) * 3.0)
+    done = np.zeros((B, W), bool)
+    check_beam(x, scores, done, 2)
+    check_beam(x, scores[:, ::-1].copy(), done, 2, pad=3)
+
+
 @pytest.mark.parametrize("L,B,W,heads,bs,mb,unit,table", [
     (2, 2, 4, 2, 16, 4, 32, True), (1, 3, 2, 1, 100, 1, 768, False), (3, 1, 5, 3, 7, 5, 4, True),
     (1, 2, 32, 2, 5, 3, 12, False), (2, 1, 3, 1, 1, 40, 20, True), (1, 4, 8, 4, 64, 2, 16, True)])
