@@ -55,18 +55,24 @@ class _Contexts(threading.local):
     ends leaves them to the next one that needs some, so there are as many as
     threads have been in these calls at once."""
 
+    __slots__ = ("free",)               # (one for all threads, as slots of a threading.local are)
+
     def __init__(self):
-        self.of = _Held()
+        if not hasattr(self, "free"):
+            self.free = {}              # contexts of no thread, by device
+        self.of = _Held(self.free)
 
 
 class _Held(dict):
+    def __init__(self, free):
+        super().__init__()
+        self.free = free
+
     def __del__(self):
-        if _FREE is not None:           # (the interpreter is not on its way out)
-            for dev, c in self.items():
-                _FREE.setdefault(dev, []).append(c)
+        for dev, c in self.items():
+            self.free.setdefault(dev, []).append(c)
 
 
-_FREE: dict = {}                        # contexts of no thread, by device
 _CONTEXTS = _Contexts()
 
 
@@ -75,7 +81,7 @@ def _context(dev: int):
     ends another thread's dict may run inside any of these operations, and each of
     them is one step to other threads.)"""
     try:
-        return _FREE[dev].pop()
+        return _CONTEXTS.free[dev].pop()
     except (KeyError, IndexError):
         return Context(dev)
 

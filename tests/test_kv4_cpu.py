@@ -201,7 +201,6 @@ def test_a_finished_threads_contexts_are_used_again(monkeypatch):
 
     streams = threading.local()
     monkeypatch.setattr(kv4, "Context", Fake)
-    monkeypatch.setattr(kv4, "_FREE", {}, raising=False)
     monkeypatch.setattr(kv4, "_CONTEXTS", kv4._Contexts())
     monkeypatch.setattr(torch._C, "_cuda_getCurrentRawStream", lambda d: streams.now, raising=False)
     wrong = []
@@ -234,6 +233,9 @@ def test_a_finished_threads_contexts_are_used_again(monkeypatch):
     for _ in range(10):
         run(5)
     assert len(Fake.made) == 10 and not wrong
+    # they are this _Contexts' alone
+    monkeypatch.undo()
+    assert not any(isinstance(c, Fake) for cs in kv4._CONTEXTS.free.values() for c in cs)
 
 
 # ------------------------------------------------------------------ the restatements themselves
